@@ -38,6 +38,7 @@ extern "C" {
 #define MZB_ERR_TIMEOUT (-4)     /* a bounded device-side wait gave up */
 #define MZB_ERR_ALIGN (-5)       /* pointer not 16-byte aligned where required */
 #define MZB_ERR_BOUND (-6)       /* a device-side error-bound check failed */
+#define MZB_ERR_PAGES (-7)       /* a position past its page table, a page id outside the pool, no free page */
 
 /* element type codes */
 #define MZB_F32 0
@@ -265,6 +266,68 @@ MZB_API int mzb_kv_unpack_fp8(const uint8_t* codes, const uint8_t* scales, void*
 MZB_API int mzb_kv_pack_fp4(const void* x, uint8_t* codes, uint8_t* scales, int64_t rows, int D, void* stream);
 MZB_API int mzb_kv_unpack_fp4(const uint8_t* codes, const uint8_t* scales, void* out, int64_t rows, int D,
                               void* stream);
+
+/* ------------------------------------------------------------------ dense attention, grouped heads
+ * No counterpart in the reference's kernels (full-attention layers of a served model).
+ * mzb_gqa_prefill -- packed prompts.  q [Tq, Hq, D], k / v [Tk, Hkv, D] bf16 or f16 with the
+ *   given token and head strides in elements (the last dimension is dense; pointers and
+ *   strides 16-byte aligned), sequence b = rows cu_q[b] .. cu_q[b+1] of q and cu_k[b] ..
+ *   cu_k[b+1] of k / v (int32 [B+1], ascending from 0).  Row i of a sequence of nq tokens and
+ *   nk keys sees the keys j <= i + nk - nq (causal) or all; head h reads K / V head
+ *   h / (Hq / Hkv).  o [Tq, Hq, D] and lse fp32 [Tq, Hq] (natural log) dense; a row that sees
+ *   no key has o = 0 and lse = -inf.  Hq / Hkv at most 128; D in {64, 96, 128}.
+ * mzb_gqa_decode -- one token per sequence over a paged cache.  q [B, Hq, D]; k_pages /
+ *   v_pages [P, Hkv, page, D] by their page, head and token strides in elements; key t of
+ *   sequence b is slot t % page of page page_table[b, t / page], t < min(seq_lens[b], W * page).
+ *   Entries past a sequence's length are never used (ids outside [0, P) are clamped).
+ *   ws: mzb_gqa_decode_ws(...) floats.  page in {16, 32, 64, 128}.
+ */
+MZB_API int mzb_gqa_prefill(const void* q, const void* k, const void* v, const int32_t* cu_q, const int32_t* cu_k,
+                            void* o, float* lse, int64_t Tq, int64_t Tk, int B, int Hq, int Hkv, int D, int dtype,
+                            int64_t sq_t, int64_t sq_h, int64_t sk_t, int64_t sk_h, int64_t sv_t, int64_t sv_h,
+                            int causal, float softmax_scale, int* err, void* stream);
+MZB_API int64_t mzb_gqa_decode_ws(int B, int Hq, int Hkv, int D, int W, int page);
+MZB_API int mzb_gqa_decode(const void* q, const void* k_pages, const void* v_pages, const int32_t* page_table,
+                           const int32_t* seq_lens, void* o, float* lse, float* ws, int B, int Hq, int Hkv, int D,
+                           int dtype, int page, int64_t P, int W, int64_t sq_b, int64_t sq_h, int64_t sk_p,
+                           int64_t sk_h, int64_t sk_t, int64_t sv_p, int64_t sv_h, int64_t sv_t,
+                           float softmax_scale, int* err, void* stream);
+
+/* ------------------------------------------------------------------ pages of a K / V cache
+ * No counterpart in the reference.  State: page_table int32 [S, W] (-1 = no page), seq_lens
+ * int32 [S], refs int32 [P] (tables that name the page; 0 = free).  What cannot be done is left
+ * out and sets *err = MZB_ERR_PAGES; new pages are the lowest free ids.
+ * mzb_kv_append  -- row i of sequence b (rows cu[b] .. cu[b+1]; cu NULL: row b) of k, v goes to
+ *   position starts[b] + i.  strides: 10 byte strides: k token, head; v token, head; k_pages page,
+ *   head, token; v_pages page, head, token.  Rows of row_bytes (a multiple of 16) bytes.
+ * mzb_kv_reserve -- sequence b grows by n_new[b] tokens (all or none): pages are taken in
+ *   (sequence, position) order, seq_lens is raised, starts[b] is the old length.  ws: P ints.
+ * mzb_kv_free    -- the sequences seqs[0..n): refs - 1 for their pages, entries -1, length 0.
+ * mzb_kv_fork    -- dst[i] becomes a copy of src[i]: what dst held is released, full pages are
+ *   shared (refs + 1), a partly filled last page gets a page of its own.  dst distinct and
+ *   disjoint from src (other pairs are left out, as an error).  ws: 3 n + S ints; its first 2 n
+ *   are then the pages to copy: sources [n], destinations [n] (-1: none).
+ * mzb_kv_compact -- n = pages with refs > 0; the i-th of them at an id >= n moves to the i-th
+ *   free id below n.  new_table, new_refs: the state after it.  ws: 3 P + 1 ints: sources [P],
+ *   destinations [P], the map [P], the number of moves.
+ * mzb_kv_copy_pages -- page src[i] to page dst[i] (both -1: none) in n_pools pools of P pages
+ *   (page_bytes, page_strides: host arrays; multiples of 16 bytes); count (device, may be
+ *   NULL): the number of pairs, at most n.  No destination may be a source or named twice.
+ */
+MZB_API int mzb_kv_append(const void* k, const void* v, void* k_pages, void* v_pages, const int32_t* page_table,
+                          const int32_t* starts, const int32_t* cu, int64_t T, int B, int Hkv, int row_bytes,
+                          int page, int64_t P, int W, const int64_t* strides, int* err, void* stream);
+MZB_API int mzb_kv_reserve(int32_t* page_table, int32_t* seq_lens, int32_t* refs, const int32_t* n_new,
+                           int32_t* starts, int32_t* ws, int B, int W, int64_t P, int page, int* err, void* stream);
+MZB_API int mzb_kv_free(int32_t* page_table, int32_t* seq_lens, int32_t* refs, const int32_t* seqs, int64_t n,
+                        int64_t S, int W, int64_t P, int* err, void* stream);
+MZB_API int mzb_kv_fork(int32_t* page_table, int32_t* seq_lens, int32_t* refs, const int32_t* src, const int32_t* dst,
+                        int n, int32_t* ws, int64_t S, int W, int64_t P, int page, int* err, void* stream);
+MZB_API int mzb_kv_compact(const int32_t* page_table, const int32_t* refs, int32_t* new_table, int32_t* new_refs,
+                           int32_t* ws, int64_t entries, int64_t P, int* err, void* stream);
+MZB_API int mzb_kv_copy_pages(void* const* pools, const int64_t* page_bytes, const int64_t* page_strides, int n_pools,
+                              const int32_t* src, const int32_t* dst, const int32_t* count, int64_t n, int64_t P,
+                              int* err, void* stream);
 
 /* Self-test of the bounded device waits (no counterpart in the reference: it checks this
  * library's own failure path).  One thread waits on an mbarrier nothing arrives on; after

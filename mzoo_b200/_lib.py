@@ -21,6 +21,7 @@ MZB_ERR_LAUNCH = -3
 MZB_ERR_TIMEOUT = -4
 MZB_ERR_ALIGN = -5
 MZB_ERR_BOUND = -6
+MZB_ERR_PAGES = -7
 
 DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
@@ -60,8 +61,19 @@ SIGNATURES = {
     "mzb_kv_unpack_fp8": [_P, _P, _P, _I64, _I32, _P],
     "mzb_kv_pack_fp4": [_P, _P, _P, _I64, _I32, _P],
     "mzb_kv_unpack_fp4": [_P, _P, _P, _I64, _I32, _P],
+    "mzb_gqa_prefill": [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I32, _I32, _I32, _I32, _I32, _I64, _I64, _I64, _I64,
+                        _I64, _I64, _I32, _F32, _P, _P],
+    "mzb_gqa_decode_ws": [_I32, _I32, _I32, _I32, _I32, _I32],
+    "mzb_gqa_decode": [_P, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _I64, _I32, _I64, _I64,
+                       _I64, _I64, _I64, _I64, _I64, _I64, _F32, _P, _P],
+    "mzb_kv_append": [_P, _P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _I64, _I32, _P, _P, _P],
+    "mzb_kv_reserve": [_P, _P, _P, _P, _P, _P, _I32, _I32, _I64, _I32, _P, _P],
+    "mzb_kv_free": [_P, _P, _P, _P, _I64, _I64, _I32, _I64, _P, _P],
+    "mzb_kv_fork": [_P, _P, _P, _P, _P, _I32, _P, _I64, _I32, _I64, _I32, _P, _P],
+    "mzb_kv_compact": [_P, _P, _P, _P, _P, _I64, _I64, _P, _P],
+    "mzb_kv_copy_pages": [_P, _P, _P, _I32, _P, _P, _P, _I64, _I64, _P, _P],
 }
-_RESTYPE = {"mzb_last_error": ctypes.c_char_p}
+_RESTYPE = {"mzb_last_error": ctypes.c_char_p, "mzb_gqa_decode_ws": _I64}
 
 _lib = None
 

@@ -1,0 +1,487 @@
+// Pages of a K / V cache: writing new rows into their pages, taking, sharing (fork),
+// releasing and compacting pages.  No counterpart in the reference.
+//
+// The state is on the device and is changed on the caller's stream, so a serving step needs
+// no host read: page_table int32 [S, W] (-1 = no page), seq_lens int32 [S], refs int32 [P]
+// (how many tables name the page; 0 = free).  New pages are always the lowest free ids, in
+// the order of the sequences that ask, so equal inputs give equal tables.  What cannot be
+// done (a position past the table, a page id outside the pool, no free page) is left out and
+// recorded as MZB_ERR_PAGES in the error word.
+#include "common.cuh"
+
+namespace mzb {
+namespace pages {
+
+constexpr int NT = 1024;  // threads of the single-block planning kernels
+
+// ---------------------------------------------------------------- block-wide helpers
+
+// Exclusive prefix sum of one value per thread over a block of NT threads, and the total.
+__device__ __forceinline__ int block_scan(int v, int* warp_sums, int& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, d);
+    if (lane >= d) x += y;
+  }
+  __syncthreads();  // the previous call's readers are done with warp_sums
+  if (lane == 31) warp_sums[warp] = x;
+  __syncthreads();
+  if (warp == 0) {
+    int s = warp_sums[lane];
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, s, d);
+      if (lane >= d) s += y;
+    }
+    warp_sums[lane] = s;
+  }
+  __syncthreads();
+  total = warp_sums[31];
+  return x - v + (warp ? warp_sums[warp - 1] : 0);
+}
+
+// The lowest `want` free pages, ascending, into list; returns how many there are (<= want).
+__device__ int lowest_free(const int32_t* refs, int64_t P, int want, int32_t* list, int* warp_sums) {
+  int found = 0;
+  for (int64_t p0 = 0; p0 < P && found < want; p0 += NT) {
+    const int64_t p = p0 + threadIdx.x;
+    const int f = p < P && refs[p] == 0;
+    int total;
+    const int at = found + block_scan(f, warp_sums, total);
+    if (f && at < want) list[at] = int32_t(p);
+    found += total;
+  }
+  __syncthreads();
+  return min(found, want);
+}
+
+__device__ __forceinline__ void report(int* err) { atomicExch(err, MZB_ERR_PAGES); }
+
+// ---------------------------------------------------------------- append
+
+struct AppendArgs {
+  const uint8_t *k, *v;
+  uint8_t *kp, *vp;
+  const int32_t *table, *starts, *cu;
+  int64_t T, P, sk_t, sk_h, sv_t, sv_h, kp_p, kp_h, kp_t, vp_p, vp_h, vp_t;  // byte strides
+  int B, H, chunks, W, page, tok;                                          // chunks: 16-byte pieces of a row
+  int* err;
+};
+
+constexpr int AP_TOK = 8;
+
+__global__ void __launch_bounds__(256) append_kernel(AppendArgs a) {
+  __shared__ int64_t kdst[AP_TOK], vdst[AP_TOK];
+  const int64_t t0 = (int64_t)blockIdx.x * a.tok;
+  const int nt = int(min((int64_t)a.tok, a.T - t0));
+  if ((int)threadIdx.x < nt) {
+    const int64_t t = t0 + threadIdx.x;
+    int b = int(t);
+    int64_t i = 0;
+    bool ok = true;
+    if (a.cu) {
+      int lo = 0, hi = a.B;  // the last sequence that starts at or before t
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a.cu[mid] <= t) lo = mid; else hi = mid;
+      }
+      b = lo;
+      i = t - a.cu[lo];
+      ok = i >= 0 && t < a.cu[lo + 1];
+    }
+    int64_t d = -1, e = -1;
+    if (ok) {
+      const int64_t pos = (int64_t)a.starts[b] + i, j = pos / a.page;
+      if (pos >= 0 && j < a.W) {
+        const int64_t p = a.table[(int64_t)b * a.W + j];
+        if (p >= 0 && p < a.P) {
+          d = p * a.kp_p + (pos % a.page) * a.kp_t;
+          e = p * a.vp_p + (pos % a.page) * a.vp_t;
+        }
+      }
+      if (d < 0) report(a.err);
+    }
+    kdst[threadIdx.x] = d;
+    vdst[threadIdx.x] = e;
+  }
+  __syncthreads();
+  const int per = a.H * a.chunks;
+  for (int x = threadIdx.x; x < nt * per; x += 256) {
+    const int t = x / per, y = x % per, h = y / a.chunks, c = y % a.chunks;
+    if (kdst[t] < 0) continue;
+    const uint4 kv = *reinterpret_cast<const uint4*>(a.k + (t0 + t) * a.sk_t + h * a.sk_h + c * 16);
+    const uint4 vv = *reinterpret_cast<const uint4*>(a.v + (t0 + t) * a.sv_t + h * a.sv_h + c * 16);
+    *reinterpret_cast<uint4*>(a.kp + kdst[t] + h * a.kp_h + c * 16) = kv;
+    *reinterpret_cast<uint4*>(a.vp + vdst[t] + h * a.vp_h + c * 16) = vv;
+  }
+}
+
+// ---------------------------------------------------------------- reserve
+
+// One block: needs per sequence, their prefix sum, the lowest free pages, the table entries.
+__global__ void __launch_bounds__(NT) reserve_kernel(int32_t* table, int32_t* lens, int32_t* refs,
+                                                     const int32_t* n_new, int32_t* starts, int32_t* list, int B,
+                                                     int W, int64_t P, int page, int* err) {
+  __shared__ int ws[32];
+  int base = 0;
+  // pass 0 counts what is wanted, pass 1 gives it out
+  int have = 0;
+  for (int pass = 0; pass < 2; ++pass) {
+    int run = 0;
+    for (int b0 = 0; b0 < B; b0 += NT) {
+      const int b = b0 + threadIdx.x;
+      int need = 0, j0 = 0, j1 = 0;
+      int64_t len = 0, to = 0;
+      bool ok = false;
+      if (b < B) {
+        len = lens[b];
+        to = len + n_new[b];
+        ok = len >= 0 && n_new[b] >= 0 && to <= (int64_t)W * page;
+        if (ok) {
+          j0 = int((len + page - 1) / page);
+          j1 = int((to + page - 1) / page);
+          for (int j = j0; j < j1; ++j) need += table[(int64_t)b * W + j] < 0;
+        }
+      }
+      int total;
+      const int at = run + block_scan(need, ws, total);
+      run += total;
+      if (pass == 1 && b < B) {
+        starts[b] = int32_t(len);
+        if (ok && (need == 0 || at + need <= have)) {
+          int r = at;
+          for (int j = j0; j < j1; ++j)
+            if (table[(int64_t)b * W + j] < 0) {
+              const int32_t p = list[r++];
+              table[(int64_t)b * W + j] = p;
+              refs[p] = 1;
+            }
+          lens[b] = int32_t(to);
+        } else {
+          report(err);
+        }
+      }
+      __syncthreads();
+    }
+    if (pass == 0) {
+      base = run;
+      have = lowest_free(refs, P, int(min((int64_t)base, P)), list, ws);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- free
+
+// Exchanging the table entry for -1 makes a sequence named twice harmless.
+__global__ void __launch_bounds__(256) free_kernel(int32_t* table, int32_t* lens, int32_t* refs, const int32_t* seqs,
+                                                   int64_t n, int64_t S, int W, int64_t P, int* err) {
+  const int64_t i = blockIdx.y + (int64_t)gridDim.y * blockIdx.z;
+  if (i >= n) return;
+  const int64_t s = seqs[i];
+  if (s < 0 || s >= S) {
+    if (threadIdx.x == 0 && blockIdx.x == 0) report(err);
+    return;
+  }
+  const int j = blockIdx.x * 256 + threadIdx.x;
+  if (j == 0) lens[s] = 0;
+  if (j >= W) return;
+  const int p = atomicExch(&table[s * W + j], -1);
+  if (p >= 0 && p < P) atomicSub(&refs[p], 1);
+}
+
+// ---------------------------------------------------------------- fork
+
+// One block.  ws: pairs_src [n], pairs_dst [n], list [n], mark [S].
+__global__ void __launch_bounds__(NT) fork_kernel(int32_t* table, int32_t* lens, int32_t* refs, const int32_t* src,
+                                                  const int32_t* dst, int n, int32_t* ws, int64_t S, int W,
+                                                  int64_t P, int page, int* err) {
+  __shared__ int wsum[32];
+  int32_t *ps = ws, *pd = ws + n, *list = ws + 2 * (int64_t)n, *mark = ws + 3 * (int64_t)n;
+  auto in = [&](int64_t s) { return s >= 0 && s < S; };
+  // a pair is taken if both names are in the table, dst is named once and is no one's src
+  for (int i = threadIdx.x; i < n; i += NT) {
+    if (in(src[i])) mark[src[i]] = 0;
+    if (in(dst[i])) mark[dst[i]] = 0;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += NT) {
+    if (in(src[i])) atomicOr(&mark[src[i]], 1 << 30);
+    if (in(dst[i])) atomicAdd(&mark[dst[i]], 1);
+  }
+  __syncthreads();
+  auto taken = [&](int i) {
+    const int64_t s = src[i], d = dst[i];
+    return in(s) && in(d) && mark[d] == 1 && lens[s] >= 0 && lens[s] <= (int64_t)W * page;
+  };
+  const int64_t cells = (int64_t)n * W;
+  for (int64_t x = threadIdx.x; x < cells; x += NT) {  // release what the copies held
+    const int i = int(x / W);
+    if (!taken(i)) continue;
+    const int p = atomicExch(&table[(int64_t)dst[i] * W + x % W], -1);
+    if (p >= 0 && p < P) atomicSub(&refs[p], 1);
+  }
+  __syncthreads();
+  for (int64_t x = threadIdx.x; x < cells; x += NT) {  // share the full pages
+    const int i = int(x / W), j = int(x % W);
+    if (!taken(i) || j >= lens[src[i]] / page) continue;
+    const int p = table[(int64_t)src[i] * W + j];
+    if (p >= 0 && p < P) {
+      table[(int64_t)dst[i] * W + j] = p;
+      atomicAdd(&refs[p], 1);
+    } else {
+      report(err);
+    }
+  }
+  __syncthreads();
+  int want = 0;
+  for (int i0 = 0; i0 < n; i0 += NT) {  // ranks of the copies that need a page of their own
+    const int i = i0 + threadIdx.x;
+    int need = 0;
+    if (i < n) {
+      ps[i] = pd[i] = -1;
+      if (!taken(i)) {
+        report(err);
+      } else if (lens[src[i]] % page) {
+        const int p = table[(int64_t)src[i] * W + lens[src[i]] / page];
+        if (p >= 0 && p < P) {
+          need = 1;
+          ps[i] = p;
+        } else {
+          report(err);
+        }
+      }
+    }
+    int total;
+    const int at = want + block_scan(need, wsum, total);
+    if (i < n && need) pd[i] = at;
+    want += total;
+  }
+  __syncthreads();
+  const int have = lowest_free(refs, P, want, list, wsum);
+  for (int i = threadIdx.x; i < n; i += NT) {
+    if (!taken(i)) continue;
+    const int64_t d = dst[i], len = lens[src[i]];
+    int32_t got = int32_t(len);
+    if (len % page) {
+      const int32_t p = pd[i] >= 0 && pd[i] < have ? list[pd[i]] : -1;
+      if (p >= 0) {
+        table[d * W + len / page] = p;
+        refs[p] = 1;
+      } else {  // no page for the last tokens: the copy ends at its last full page
+        if (pd[i] >= 0) report(err);
+        got = int32_t(len / page * page);
+        ps[i] = -1;
+      }
+      pd[i] = p;
+    }
+    lens[d] = got;
+  }
+}
+
+// ---------------------------------------------------------------- compact
+
+// One block.  The i-th live page at an index >= n moves to the i-th hole below n (n = number
+// of live pages), so the pages that move and the holes are disjoint and the copies need no
+// order.  to [P]: where a page is afterwards (-1: free); pairs [2 * m]: (from, to) lists,
+// m = count[0].
+__global__ void __launch_bounds__(NT) compact_plan_kernel(const int32_t* refs, int32_t* new_refs, int32_t* to,
+                                                          int32_t* from_list, int32_t* hole_list, int32_t* count,
+                                                          int64_t P) {
+  __shared__ int ws[32];
+  int n = 0, total;
+  for (int64_t p0 = 0; p0 < P; p0 += NT) {
+    const int64_t p = p0 + threadIdx.x;
+    block_scan(p < P && refs[p] > 0, ws, total);
+    n += total;
+  }
+  int holes = 0, moved = 0;
+  for (int64_t p0 = 0; p0 < P; p0 += NT) {
+    const int64_t p = p0 + threadIdx.x;
+    const int r = p < P ? refs[p] : 0;
+    const int hole = p < n && r <= 0, move = p >= n && r > 0;
+    const int at = block_scan(p0 < n ? hole : 0, ws, total);
+    if (hole) hole_list[holes + at] = int32_t(p);
+    holes += total;
+    const int am = block_scan(move, ws, total);
+    if (move) from_list[moved + am] = int32_t(p);
+    moved += total;
+    if (p < P) {
+      to[p] = r > 0 ? int32_t(p) : -1;
+      new_refs[p] = p < n ? r : 0;
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < moved; i += NT) {
+    const int f = from_list[i], h = hole_list[i];
+    to[f] = h;
+    new_refs[h] = refs[f];
+  }
+  if (threadIdx.x == 0) count[0] = moved;
+}
+
+__global__ void __launch_bounds__(256) remap_kernel(const int32_t* table, int32_t* new_table, const int32_t* to,
+                                                    int64_t n, int64_t P, int* err) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int p = table[i];
+    int q = -1;
+    if (p >= 0) {
+      q = p < P ? to[p] : -1;
+      if (q < 0) report(err);  // a table names a free page or none of the pool's
+    }
+    new_table[i] = q;
+  }
+}
+
+// ---------------------------------------------------------------- copying pages
+
+constexpr int MAX_POOLS = 64;
+constexpr int CHUNK = 16384;  // bytes of a page that one block step copies: 256 threads x 4 x 16
+
+struct CopyArgs {
+  uint8_t* pool[MAX_POOLS];
+  int64_t stride[MAX_POOLS];  // bytes from page to page
+  int64_t bytes[MAX_POOLS];   // bytes of a page
+  const int32_t *src, *dst;   // src or dst -1: no copy
+  const int32_t* count;       // device count of pairs (null: n)
+  int64_t n, P;
+  int n_pools, chunks;  // chunks of the largest page
+  int* err;
+};
+
+__global__ void __launch_bounds__(256) copy_kernel(const __grid_constant__ CopyArgs a) {
+  const int64_t n = a.count ? min((int64_t)*a.count, a.n) : a.n;
+  const int64_t per = (int64_t)a.n_pools * a.chunks;
+  for (int64_t w = blockIdx.x; w < n * per; w += gridDim.x) {
+    const int64_t i = w / per;
+    const int pool = int(w % per) / a.chunks, c = int(w % per) % a.chunks;
+    const int64_t s = a.src[i], d = a.dst[i];
+    if (s < 0 && d < 0) continue;
+    if (s < 0 || d < 0 || s >= a.P || d >= a.P) {
+      if (threadIdx.x == 0) report(a.err);
+      continue;
+    }
+    const int64_t off = (int64_t)c * CHUNK, left = a.bytes[pool] - off;
+    const uint4* from = reinterpret_cast<const uint4*>(a.pool[pool] + s * a.stride[pool] + off);
+    uint4* to = reinterpret_cast<uint4*>(a.pool[pool] + d * a.stride[pool] + off);
+    uint4 v[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if ((int64_t)(threadIdx.x + 256 * q) * 16 < left) v[q] = from[threadIdx.x + 256 * q];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if ((int64_t)(threadIdx.x + 256 * q) * 16 < left) to[threadIdx.x + 256 * q] = v[q];
+  }
+}
+
+}  // namespace pages
+}  // namespace mzb
+
+using namespace mzb;
+
+#define MZB_POOL_SIZES(what, P, W, page)                                                                            \
+  MZB_REQUIRE((P) >= 1 && (P) < (int64_t(1) << 31) && (W) >= 1 && (page) >= 1 &&                                    \
+                  (int64_t)(W) * (page) < (int64_t(1) << 31),                                                       \
+              MZB_ERR_SHAPE, what ": bad sizes pages=%lld table width=%d page=%d", (long long)(P), int(W), int(page)); \
+  MZB_REQUIRE(err != nullptr, MZB_ERR_SHAPE, what ": needs an error word")
+
+extern "C" int mzb_kv_append(const void* k, const void* v, void* k_pages, void* v_pages, const int32_t* page_table,
+                             const int32_t* starts, const int32_t* cu, int64_t T, int B, int Hkv, int row_bytes,
+                             int page, int64_t P, int W, const int64_t* strides, int* err, void* stream) {
+  MZB_POOL_SIZES("kv_append", P, W, page);
+  MZB_REQUIRE(T >= 0 && B >= 1 && Hkv >= 1 && (cu != nullptr || T == B), MZB_ERR_SHAPE,
+              "kv_append: bad sizes T=%lld B=%d Hkv=%d", (long long)T, B, Hkv);
+  MZB_REQUIRE(row_bytes >= 16 && row_bytes % 16 == 0, MZB_ERR_ALIGN, "kv_append: rows of %d bytes (a multiple of 16)",
+              row_bytes);
+  for (const void* p : {k, v, (const void*)k_pages, (const void*)v_pages})
+    MZB_REQUIRE(reinterpret_cast<uintptr_t>(p) % 16 == 0, MZB_ERR_ALIGN, "kv_append: pointers must be 16-byte aligned");
+  for (int i = 0; i < 10; ++i)
+    MZB_REQUIRE(strides[i] % 16 == 0, MZB_ERR_ALIGN, "kv_append: strides must be multiples of 16 bytes");
+  if (T == 0) return MZB_OK;
+  const int tok = T <= 4 * num_sms() ? 1 : T <= 16 * num_sms() ? 4 : pages::AP_TOK;
+  pages::AppendArgs a{static_cast<const uint8_t*>(k), static_cast<const uint8_t*>(v), static_cast<uint8_t*>(k_pages),
+                      static_cast<uint8_t*>(v_pages), page_table, starts, cu, T, P, strides[0], strides[1],
+                      strides[2], strides[3], strides[4], strides[5], strides[6], strides[7], strides[8], strides[9],
+                      B, Hkv, row_bytes / 16, W, page, tok, err};
+  pages::append_kernel<<<unsigned((T + tok - 1) / tok), 256, 0, static_cast<cudaStream_t>(stream)>>>(a);
+  return launch_status("kv_append");
+}
+
+extern "C" int mzb_kv_reserve(int32_t* page_table, int32_t* seq_lens, int32_t* refs, const int32_t* n_new,
+                              int32_t* starts, int32_t* ws, int B, int W, int64_t P, int page, int* err,
+                              void* stream) {
+  MZB_POOL_SIZES("kv_reserve", P, W, page);
+  MZB_REQUIRE(B >= 0, MZB_ERR_SHAPE, "kv_reserve: bad B=%d", B);
+  if (B == 0) return MZB_OK;
+  pages::reserve_kernel<<<1, pages::NT, 0, static_cast<cudaStream_t>(stream)>>>(page_table, seq_lens, refs, n_new,
+                                                                                starts, ws, B, W, P, page, err);
+  return launch_status("kv_reserve");
+}
+
+extern "C" int mzb_kv_free(int32_t* page_table, int32_t* seq_lens, int32_t* refs, const int32_t* seqs, int64_t n,
+                           int64_t S, int W, int64_t P, int* err, void* stream) {
+  MZB_POOL_SIZES("kv_free", P, W, 1);
+  MZB_REQUIRE(n >= 0 && n < (int64_t(1) << 31) && S >= 1, MZB_ERR_SHAPE, "kv_free: bad sizes n=%lld S=%lld",
+              (long long)n, (long long)S);
+  if (n == 0) return MZB_OK;
+  const unsigned ny = unsigned(n < 65535 ? n : 65535), nz = unsigned((n + ny - 1) / ny);
+  pages::free_kernel<<<dim3(unsigned((W + 255) / 256), ny, nz), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+      page_table, seq_lens, refs, seqs, n, S, W, P, err);
+  return launch_status("kv_free");
+}
+
+extern "C" int mzb_kv_fork(int32_t* page_table, int32_t* seq_lens, int32_t* refs, const int32_t* src,
+                           const int32_t* dst, int n, int32_t* ws, int64_t S, int W, int64_t P, int page, int* err,
+                           void* stream) {
+  MZB_POOL_SIZES("kv_fork", P, W, page);
+  MZB_REQUIRE(n >= 0 && S >= 1 && S < (int64_t(1) << 31), MZB_ERR_SHAPE, "kv_fork: bad sizes n=%d S=%lld", n, (long long)S);
+  if (n == 0) return MZB_OK;
+  pages::fork_kernel<<<1, pages::NT, 0, static_cast<cudaStream_t>(stream)>>>(page_table, seq_lens, refs, src, dst, n,
+                                                                             ws, S, W, P, page, err);
+  return launch_status("kv_fork");
+}
+
+extern "C" int mzb_kv_compact(const int32_t* page_table, const int32_t* refs, int32_t* new_table, int32_t* new_refs,
+                              int32_t* ws, int64_t entries, int64_t P, int* err, void* stream) {
+  MZB_POOL_SIZES("kv_compact", P, 1, 1);
+  MZB_REQUIRE(entries >= 0, MZB_ERR_SHAPE, "kv_compact: bad table size %lld", (long long)entries);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  int32_t *from = ws, *hole = ws + P, *to = ws + 2 * P, *count = ws + 3 * P;
+  pages::compact_plan_kernel<<<1, pages::NT, 0, st>>>(refs, new_refs, to, from, hole, count, P);
+  if (int r = launch_status("kv_compact")) return r;
+  if (entries == 0) return MZB_OK;
+  const int64_t blocks = (entries + 255) / 256;
+  pages::remap_kernel<<<unsigned(blocks < 4 * num_sms() ? blocks : 4 * num_sms()), 256, 0, st>>>(
+      page_table, new_table, to, entries, P, err);
+  return launch_status("kv_compact(remap)");
+}
+
+extern "C" int mzb_kv_copy_pages(void* const* pools, const int64_t* page_bytes, const int64_t* page_strides,
+                                 int n_pools, const int32_t* src, const int32_t* dst, const int32_t* count, int64_t n,
+                                 int64_t P, int* err, void* stream) {
+  MZB_POOL_SIZES("kv_copy_pages", P, 1, 1);
+  MZB_REQUIRE(n >= 0 && n_pools >= 0, MZB_ERR_SHAPE, "kv_copy_pages: bad sizes n=%lld pools=%d", (long long)n, n_pools);
+  for (int i = 0; i < n_pools; ++i)
+    MZB_REQUIRE(reinterpret_cast<uintptr_t>(pools[i]) % 16 == 0 && page_bytes[i] >= 16 && page_bytes[i] % 16 == 0 &&
+                    page_strides[i] % 16 == 0,
+                MZB_ERR_ALIGN, "kv_copy_pages: pool %d: pages must be 16-byte aligned and multiples of 16 bytes", i);
+  if (n == 0) return MZB_OK;
+  for (int p0 = 0; p0 < n_pools; p0 += pages::MAX_POOLS) {
+    pages::CopyArgs a{};
+    a.n_pools = n_pools - p0 < pages::MAX_POOLS ? n_pools - p0 : pages::MAX_POOLS;
+    int64_t most = 0;
+    for (int i = 0; i < a.n_pools; ++i) {
+      a.pool[i] = static_cast<uint8_t*>(pools[p0 + i]);
+      a.stride[i] = page_strides[p0 + i];
+      a.bytes[i] = page_bytes[p0 + i];
+      most = most > a.bytes[i] ? most : a.bytes[i];
+    }
+    a.src = src; a.dst = dst; a.count = count; a.n = n; a.P = P; a.err = err;
+    a.chunks = int((most + pages::CHUNK - 1) / pages::CHUNK);
+    const int64_t work = n * a.n_pools * a.chunks, cap = 8 * num_sms();
+    pages::copy_kernel<<<unsigned(work < cap ? work : cap), 256, 0, static_cast<cudaStream_t>(stream)>>>(a);
+    if (int r = launch_status("kv_copy_pages")) return r;
+  }
+  return MZB_OK;
+}

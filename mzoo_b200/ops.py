@@ -73,6 +73,8 @@ def _err(dev, check: bool) -> torch.Tensor:
 def _raise_code(code: int, what: str) -> None:
     if code == _lib.MZB_ERR_BOUND:
         raise _lib.MzbError(f"{what}: error bound left too many top-k candidates")
+    if code == _lib.MZB_ERR_PAGES:
+        raise _lib.MzbError(f"{what}: a position past its page table, a page or sequence id out of range, or no free page")
     if code:
         raise _lib.MzbError(f"{what}: device error code {code} (a bounded device wait gave up)")
 
@@ -440,3 +442,152 @@ def kv_unpack(codes: torch.Tensor, scales: torch.Tensor, D: int, fmt: int) -> to
 @kv_unpack.register_fake
 def _(codes, scales, D, fmt):
     return codes.new_empty((codes.shape[0], D), dtype=torch.bfloat16)
+
+
+# ----------------------------------------------------------------------------- dense attention, pages
+#
+# Serving-step ops: defined through ``torch.library.Library`` (a schema and one Python kernel)
+# rather than ``custom_op``, whose per-call bookkeeping costs several times the launch of the
+# smallest decode step.
+
+_LIB = torch.library.Library("mzb", "FRAGMENT")
+
+
+def _define(schema: str, fake):
+    """Register the decorated function as the CUDA kernel of ``mzb::<schema>``."""
+    name = schema[:schema.index("(")]
+
+    def wrap(fn):
+        _LIB.define(schema)
+        _LIB.impl(name, fn, "CUDA")
+        torch.library.register_fake(f"mzb::{name}", fake, lib=_LIB)
+        return getattr(torch.ops.mzb, name).default
+    return wrap
+
+
+def _attn_out(q, *rest):
+    return torch.empty(q.shape, dtype=q.dtype, device=q.device), q.new_empty(q.shape[:2], dtype=torch.float32)
+
+
+@_define("gqa_prefill(Tensor q, Tensor k, Tensor v, Tensor cu_q, Tensor cu_k, bool causal, float scale, bool check)"
+         " -> (Tensor, Tensor)", _attn_out)
+def gqa_prefill(q, k, v, cu_q, cu_k, causal, scale, check):
+    """(o like q, lse fp32 [Tq, Hq]) of ``mzb_gqa_prefill`` (q / k / v with a dense last dimension)."""
+    dev = q.device
+    o, lse = _attn_out(q)
+    err = _err(dev, check)
+    call("mzb_gqa_prefill", q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), o.data_ptr(),
+         lse.data_ptr(), q.shape[0], k.shape[0], cu_q.shape[0] - 1, q.shape[1], k.shape[1], q.shape[2],
+         _lib.DTYPE_CODE[q.dtype], q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+         int(causal), scale, err.data_ptr(), stream_ptr(dev))
+    if check:
+        _raise_on(err, "gqa prefill")
+    return o, lse
+
+
+@_define("gqa_decode(Tensor q, Tensor k_pages, Tensor v_pages, Tensor page_table, Tensor seq_lens, float scale,"
+         " bool check) -> (Tensor, Tensor)", _attn_out)
+def gqa_decode(q, k_pages, v_pages, page_table, seq_lens, scale, check):
+    """(o like q, lse fp32 [B, Hq]) of ``mzb_gqa_decode``."""
+    dev = q.device
+    o, lse = _attn_out(q)
+    err = _err(dev, check)
+    (B, Hq, D), (P, Hkv, page, _), W = q.shape, k_pages.shape, page_table.shape[1]
+    ws = torch.empty(_lib.lib().mzb_gqa_decode_ws(B, Hq, Hkv, D, W, page), dtype=torch.float32, device=dev)
+    call("mzb_gqa_decode", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(),
+         seq_lens.data_ptr(), o.data_ptr(), lse.data_ptr(), ws.data_ptr(), B, Hq, Hkv, D, _lib.DTYPE_CODE[q.dtype],
+         page, P, W, q.stride(0), q.stride(1), *k_pages.stride()[:3], *v_pages.stride()[:3], scale, err.data_ptr(),
+         stream_ptr(dev))
+    if check:
+        _raise_on(err, "gqa decode")
+    return o, lse
+
+
+@_define("kv_append(Tensor k, Tensor v, Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor page_table, Tensor starts,"
+         " Tensor? cu, bool check) -> ()", lambda *a: None)
+def kv_append(k, v, k_pages, v_pages, page_table, starts, cu, check):
+    """``mzb_kv_append``: rows of k / v [T, Hkv, D] into k_pages / v_pages [P, Hkv, page, D]."""
+    dev, size = k.device, k.element_size()
+    err = _err(dev, check)
+    strides = (_lib.ctypes.c_int64 * 10)(*(size * x for t, n in ((k, 2), (v, 2)) for x in t.stride()[:n]),
+                                         *(size * p.stride(i) for p in (k_pages, v_pages) for i in (0, 1, 2)))
+    call("mzb_kv_append", k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(),
+         starts.data_ptr(), ptr(cu), k.shape[0], starts.shape[0], k.shape[1], k.shape[2] * size, k_pages.shape[2],
+         k_pages.shape[0], page_table.shape[1], strides, err.data_ptr(), stream_ptr(dev))
+    if check:
+        _raise_on(err, "kv append")
+
+
+@_define("kv_reserve(Tensor(a!) page_table, Tensor(b!) seq_lens, Tensor(c!) refs, Tensor n_new, int page, bool check)"
+         " -> Tensor", lambda page_table, seq_lens, *rest: torch.empty_like(seq_lens))
+def kv_reserve(page_table, seq_lens, refs, n_new, page, check):
+    """``mzb_kv_reserve``; returns the lengths before it."""
+    dev = page_table.device
+    err, starts, ws = _err(dev, check), torch.empty_like(seq_lens), torch.empty_like(refs)
+    call("mzb_kv_reserve", page_table.data_ptr(), seq_lens.data_ptr(), refs.data_ptr(), n_new.data_ptr(),
+         starts.data_ptr(), ws.data_ptr(), page_table.shape[0], page_table.shape[1], refs.shape[0], page,
+         err.data_ptr(), stream_ptr(dev))
+    if check:
+        _raise_on(err, "kv reserve")
+    return starts
+
+
+@_define("kv_free(Tensor(a!) page_table, Tensor(b!) seq_lens, Tensor(c!) refs, Tensor seqs, bool check) -> ()",
+         lambda *a: None)
+def kv_free(page_table, seq_lens, refs, seqs, check):
+    """``mzb_kv_free``."""
+    dev = page_table.device
+    err = _err(dev, check)
+    call("mzb_kv_free", page_table.data_ptr(), seq_lens.data_ptr(), refs.data_ptr(), seqs.data_ptr(), seqs.shape[0],
+         page_table.shape[0], page_table.shape[1], refs.shape[0], err.data_ptr(), stream_ptr(dev))
+    if check:
+        _raise_on(err, "kv free")
+
+
+def _copy(pools, src, dst, count, n, err, dev):
+    """One ``mzb_kv_copy_pages`` call; src / dst / count are device addresses."""
+    arr, m = _lib.ctypes.c_int64 * len(pools), len(pools)
+    call("mzb_kv_copy_pages", arr(*(p.data_ptr() for p in pools)),
+         arr(*(p.numel() // p.shape[0] * p.element_size() for p in pools)),
+         arr(*(p.stride(0) * p.element_size() for p in pools)), m, src, dst, count, n, pools[0].shape[0],
+         err.data_ptr(), stream_ptr(dev))
+
+
+@_define("kv_copy_pages(Tensor(a!)[] pools, Tensor src, Tensor dst, bool check) -> ()", lambda *a: None)
+def kv_copy_pages(pools, src, dst, check):
+    """``mzb_kv_copy_pages``: page src[i] to page dst[i] of every pool."""
+    dev = src.device
+    err = _err(dev, check)
+    _copy(pools, src.data_ptr(), dst.data_ptr(), None, src.shape[0], err, dev)
+    if check:
+        _raise_on(err, "kv copy pages")
+
+
+@_define("kv_fork(Tensor(a!)[] pools, Tensor(b!) page_table, Tensor(c!) seq_lens, Tensor(d!) refs, Tensor src,"
+         " Tensor dst, int page, bool check) -> ()", lambda *a: None)
+def kv_fork(pools, page_table, seq_lens, refs, src, dst, page, check):
+    """``mzb_kv_fork`` and the copies of the partly filled pages."""
+    dev, n, (S, W) = page_table.device, src.shape[0], page_table.shape
+    err, ws = _err(dev, check), torch.empty(3 * n + S, dtype=torch.int32, device=dev)
+    call("mzb_kv_fork", page_table.data_ptr(), seq_lens.data_ptr(), refs.data_ptr(), src.data_ptr(), dst.data_ptr(), n,
+         ws.data_ptr(), S, W, refs.shape[0], page, err.data_ptr(), stream_ptr(dev))
+    if pools:
+        _copy(pools, ws.data_ptr(), ws.data_ptr() + 4 * n, None, n, err, dev)
+    if check:
+        _raise_on(err, "kv fork")
+
+
+@_define("kv_compact(Tensor(a!)[] pools, Tensor page_table, Tensor refs, bool check) -> (Tensor, Tensor)",
+         lambda pools, page_table, refs, check: (torch.empty_like(page_table), torch.empty_like(refs)))
+def kv_compact(pools, page_table, refs, check):
+    """``mzb_kv_compact`` and the moves; returns the new (page_table, refs)."""
+    dev, P = page_table.device, refs.shape[0]
+    err, ws = _err(dev, check), torch.empty(3 * P + 1, dtype=torch.int32, device=dev)
+    table, new_refs = torch.empty_like(page_table), torch.empty_like(refs)
+    call("mzb_kv_compact", page_table.data_ptr(), refs.data_ptr(), table.data_ptr(), new_refs.data_ptr(), ws.data_ptr(),
+         page_table.numel(), P, err.data_ptr(), stream_ptr(dev))
+    if pools:
+        _copy(pools, ws.data_ptr(), ws.data_ptr() + 4 * P, ws.data_ptr() + 12 * P, P // 2, err, dev)
+    if check:
+        _raise_on(err, "kv compact")
+    return table, new_refs
