@@ -6,76 +6,705 @@
 //   causal);  o_i = sum_j e^(x_ij - lse_i) v_j,  lse_i = log sum_j e^x_ij.
 //   A row that sees no key: o = 0, lse = -inf.
 //
-// One warp per (token, head) row with an online softmax, D / 32 channels per lane.
-#include "common.cuh"
+// One pass over the keys with the running maximum and sum of a softmax (one thread per row).
+// A work item is one K / V head and up to two 128-row query tiles; the rows of a tile are
+// (token, head of the group) pairs, so all query heads of a group share each K / V tile and
+// the keys of a tile's last token bound its key range.  One block per SM, 384 threads:
+//   warps 0-3, 4-7  softmax, output and lse of query tile 0 and 1 (thread = row = TMEM lane)
+//   warp 8          TMA: query tiles, K and V tiles into one ring of slots
+//   warp 9          TMEM and the MMA-issuing thread
+//   warp 10         scheduler: next work items (the grid holds one block per item; a running
+//                   block cancels blocks that have not started and takes their items), the
+//                   longest key ranges first
+//   warp 11         repairs V tiles that reach past what some row sees: a NaN or infinity there
+//                   would reach that row as 0 * v.  Such values are taken out of the tile; the
+//                   rows that do see them add them in the epilogue.
+// The two query tiles take turns on the tensor cores: QK_0(j+1) is issued behind PV_0(j), so
+// one tile's products run while the other's exponentials do.  S and P of a tile share 128 TMEM
+// columns (P overwrites S), O takes D; a row's O is rescaled only when its maximum has grown
+// by more than 2^8 (fp32 sums and weights of at most 2^8 lose nothing by waiting).
+#include "tc.cuh"
 
 namespace mzb {
 namespace gqa {
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
+constexpr int BN = 128;  // keys per tile
+
+template <int D>
+struct PCfg {
+  static constexpr int DB = (D + 63) / 64;  // 64-channel column blocks (D = 96: the last half is zero fill)
+  static constexpr int Q_BYTES = DB * 128 * 128;
+  static constexpr int SLOT = DB * BN * 128;
+  static constexpr int NS = DB == 1 ? 8 : 5;  // ring slots (K and V tiles alternate)
+  static constexpr int TILES = 2 * Q_BYTES + NS * SLOT;
+  static constexpr int SMEM = TILES + 1024;
+  static constexpr int S_COL = 0, O_COL = 256;  // tile t: + 128 t
+  static_assert(SMEM <= 232448, "shared memory budget");
+};
 
 struct PrefillArgs {
-  const void *q, *k, *v;
+  const void* v;
   const int32_t *cu_q, *cu_k;
   void* o;
   float* lse;
-  int64_t Tq, Tk, sq_t, sq_h, sk_t, sk_h, sv_t, sv_h;
-  int B, Hq, Hkv, causal;
-  float scale;
+  int64_t Tq, Tk, sv_t, sv_h;
+  int B, Hq, Hkv, g, ntok, causal, neg;  // g = Hq / Hkv, ntok = 128 / g tokens per tile
+  float sl;                              // |scale| log2 e
+  int* err;
 };
 
+// One work item, in shared memory.
+struct Item {
+  int tok0, tok_end;  // first packed token, end of the sequence
+  int i0, shift;      // tok0's place in its sequence; keys seen by place i: min(nk, i + shift) (not causal: nk)
+  int k0, nk, hk;     // first packed key, keys, K / V head
+  int n0, n1;         // key tiles of the query tiles
+  int jfix;           // V tiles from here on reach past what some row sees
+  int done;
+};
+
+enum PBar { P_QF = 0, P_QE = 2, P_SF = 4, P_PF = 6, P_OF = 8, P_OE = 10, P_ITF = 12, P_ITE = 14, P_CLC = 16, P_KF = 17,
+            P_KE = P_KF + 8, P_VOK = P_KE + 8, P_NBAR = P_VOK + 8 };
+constexpr int ITEM_READERS = 8 + 3;  // softmax warps, TMA, MMA, repair
+
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// Maxima that a NaN passes through.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float max2(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+// 2^x of a pair for x in [-126, 126] on the FMA pipe: x = n + f with f in [-1/2, 1/2] (adding
+// 1.5 2^23 rounds to nearest), 2^f by the degree-4 polynomial of least maximal relative error
+// (2.6e-6, found by Remez exchange), n added to the exponent field.
+__device__ __forceinline__ float2 poly_exp2(uint64_t x2) {
+  const float2 xc = unpack_f32x2(x2);
+  const uint64_t x = pack_f32x2(fmaxf(xc.x, -126.0f), fmaxf(xc.y, -126.0f));
+  const uint64_t t = add_f32x2(x, pack_f32x2(12582912.0f, 12582912.0f));
+  const uint64_t r = add_f32x2(t, pack_f32x2(-12582912.0f, -12582912.0f));
+  const uint64_t f = ffma_f32x2(r, pack_f32x2(-1.0f, -1.0f), x);
+  uint64_t p = ffma_f32x2(f, pack_f32x2(9.570101911e-03f, 9.570101911e-03f),
+                          pack_f32x2(5.591786032e-02f, 5.591786032e-02f));
+  p = ffma_f32x2(p, f, pack_f32x2(2.402474483e-01f, 2.402474483e-01f));
+  p = ffma_f32x2(p, f, pack_f32x2(6.931218147e-01f, 6.931218147e-01f));
+  p = ffma_f32x2(p, f, pack_f32x2(9.999992614e-01f, 9.999992614e-01f));
+  const float2 tn = unpack_f32x2(t), pf = unpack_f32x2(p);
+  return make_float2(__uint_as_float(__float_as_uint(pf.x) + (__float_as_uint(tn.x) << 23)),
+                     __uint_as_float(__float_as_uint(pf.y) + (__float_as_uint(tn.y) << 23)));
+}
+
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (DT == MZB_BF16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+
+// Bits set where a 16-bit half of w is NaN or infinite (exponent all ones).
+template <int DT>
+__device__ __forceinline__ uint32_t nonfinite2(uint32_t w) {
+  constexpr uint32_t E = DT == MZB_BF16 ? 0x7f80u : 0x7c00u;
+  return ((w & E) == E ? 0xffffu : 0u) | ((w & (E << 16)) == (E << 16) ? 0xffff0000u : 0u);
+}
+
+// ---------------------------------------------------------------- work items
+
+// Query tile pairs of sequence b.
+__device__ __forceinline__ int pairs_of(const PrefillArgs& a, int b) {
+  if (b >= a.B) return 0;
+  const int n = a.cu_q[b + 1] - a.cu_q[b], span = 2 * a.ntok;
+  return n > 0 ? (n + span - 1) / span : 0;
+}
+
+__device__ __forceinline__ int warp_sum(int v) {
+#pragma unroll
+  for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  return v;
+}
+__device__ __forceinline__ int warp_scan(int v, int lane) {  // inclusive
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, v, d);
+    if (lane >= d) v += y;
+  }
+  return v;
+}
+
+// Item number -> (sequence, pair within it), by the scheduler warp.  Up to LPT sequences: by
+// descending pair index over all sequences (longest causal key ranges first), each lane
+// keeping the pair counts of the sequences lane, lane + 32, ...; more: sequence after
+// sequence, the last pair first, from a cursor (a block's item numbers only grow).
+struct Finder {
+  static constexpr int R = 8, LPT = 32 * R;
+  int n[R], top, cur_b, cur_at;
+
+  __device__ void init(const PrefillArgs& a, int lane) {
+    top = 0;
+    cur_b = cur_at = 0;
+    if (a.B > LPT) return;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      n[i] = pairs_of(a, lane + 32 * i);
+      top = max(top, n[i]);
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+  }
+  // pairs with index >= t
+  __device__ int above(int t) {
+    int s = 0;
+#pragma unroll
+    for (int i = 0; i < R; ++i) s += max(0, n[i] - t);
+    return warp_sum(s);
+  }
+  __device__ bool find(const PrefillArgs& a, int64_t r, int lane, int& b, int& pair) {
+    if (a.B > LPT) {
+      while (cur_b < a.B) {
+        const int c = pairs_of(a, cur_b + lane), inc = warp_scan(c, lane);
+        const unsigned hit = __ballot_sync(0xffffffffu, r < cur_at + inc);
+        if (hit) {
+          const int l = __ffs(hit) - 1;
+          b = cur_b + l;
+          pair = __shfl_sync(0xffffffffu, cur_at + inc, l) - 1 - int(r);
+          return true;
+        }
+        cur_at += __shfl_sync(0xffffffffu, inc, 31);
+        cur_b += 32;
+      }
+      return false;
+    }
+    if (r >= above(0)) return false;
+    int lo = 0, hi = top;  // above(lo) > r >= above(hi)
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (above(mid) > r) lo = mid; else hi = mid;
+    }
+    int rank = int(r) - above(hi);
+    pair = lo;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const unsigned m = __ballot_sync(0xffffffffu, n[i] > lo);
+      const int c = __popc(m);
+      if (rank >= 0 && rank < c) b = 32 * i + __fns(m, 0, rank + 1);
+      rank -= c;
+    }
+    return true;
+  }
+};
+
+__device__ __forceinline__ void fill_item(const PrefillArgs& a, int b, int pair, int hk, Item* m) {
+  const int q0 = a.cu_q[b], nq = a.cu_q[b + 1] - q0;
+  const int k0 = max(0, min(a.cu_k[b], int(a.Tk))), nk = max(0, min(a.cu_k[b + 1], int(a.Tk)) - k0);
+  const int i0 = pair * 2 * a.ntok;
+  m->tok0 = q0 + i0;
+  m->tok_end = q0 + nq;
+  m->i0 = i0;
+  m->shift = a.causal ? nk - nq + 1 : 0x3fffffff;
+  m->k0 = k0;
+  m->nk = nk;
+  m->hk = hk;
+  auto sees = [&](int i) { return a.causal ? max(0, min(nk, i + nk - nq + 1)) : nk; };
+  int n[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int first = i0 + t * a.ntok, last = min(first + a.ntok, nq) - 1;
+    n[t] = last >= first ? (sees(last) + BN - 1) / BN : 0;
+  }
+  m->n0 = n[0];
+  m->n1 = n[1];
+  m->jfix = sees(i0) / BN;  // the first token sees the fewest keys
+  m->done = 0;
+}
+
+// ---------------------------------------------------------------- kernel
+
 template <int DT, int D>
-__global__ void __launch_bounds__(256) prefill_kernel(PrefillArgs a) {
-  using E = Elem<DT>;
-  using T = typename E::T;
-  constexpr int C = D / 32;
-  const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (row >= a.Tq * a.Hq) return;
-  const int64_t t = row / a.Hq;
-  const int h = int(row % a.Hq), hk = h / (a.Hq / a.Hkv);
-  int lo = 0, hi = a.B;  // the last sequence that starts at or before t
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.cu_q[mid] <= t) lo = mid; else hi = mid;
+__global__ void __launch_bounds__(384, 1)
+    prefill_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+                   const __grid_constant__ CUtensorMap tv, const __grid_constant__ PrefillArgs a) {
+  using C = PCfg<D>;
+  using T = typename Elem<DT>::T;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint8_t* qs = smem;
+  uint8_t* ring = smem + 2 * C::Q_BYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::TILES);
+  Item* items = reinterpret_cast<Item*>(smem + C::TILES + 8 * P_NBAR + 16);  // [2]
+  uint4* clc = reinterpret_cast<uint4*>(smem + C::TILES + 512);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::TILES + 544);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::TILES + 548);
+  volatile int* bad_v = reinterpret_cast<volatile int*>(smem + C::TILES + 552);  // [4] by item number
+  static_assert(8 * P_NBAR + 16 + 2 * sizeof(Item) <= 512, "misc layout");
+  if (smem_u32(smem) & 1023) {
+    if (threadIdx.x == 0) atomicExch(a.err, MZB_ERR_ALIGN);
+    return;
   }
-  const int64_t k0 = max((int64_t)0, min((int64_t)a.cu_k[lo], a.Tk)), k1 = max(k0, min((int64_t)a.cu_k[lo + 1], a.Tk));
-  const int64_t nk = k1 - k0, nq = a.cu_q[lo + 1] - a.cu_q[lo];
-  int64_t n = a.causal ? min(nk, t - a.cu_q[lo] + nk - nq + 1) : nk;
-  if (t < a.cu_q[lo] || t >= a.cu_q[lo + 1]) n = 0;
-  float qv[C], acc[C];
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    qv[c] = E::load(static_cast<const T*>(a.q)[t * a.sq_t + h * a.sq_h + lane + 32 * c]);
-    acc[c] = 0.0f;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < P_NBAR; ++i) {
+      uint32_t c = 1;
+      if (i == P_PF || i == P_PF + 1 || i == P_OE || i == P_OE + 1) c = 4;
+      if (i == P_ITE || i == P_ITE + 1) c = ITEM_READERS;
+      if (i >= P_KE && i < P_KE + 8) c = 2;  // the last product that reads the slot; the repair warp
+      tc::mbar_init(&bars[i], c);
+    }
+    *abort_flag = 0;
+    tc::fence_barrier_init();
   }
-  float m = -INFINITY, l = 0.0f;
-  for (int64_t j = 0; j < n; ++j) {
-    const T* kr = static_cast<const T*>(a.k) + (k0 + j) * a.sk_t + hk * a.sk_h;
-    const T* vr = static_cast<const T*>(a.v) + (k0 + j) * a.sv_t + hk * a.sv_h;
-    float s = 0.0f;
-#pragma unroll
-    for (int c = 0; c < C; ++c) s += qv[c] * E::load(kr[lane + 32 * c]);
-#pragma unroll
-    for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-    s *= a.scale * LOG2E;
-    const float mn = fmaxf(m, s), ms = mn == -INFINITY ? 0.0f : mn;
-    const float al = exp2f(m - ms), p = exp2f(s - ms);
-    l = l * al + p;
-#pragma unroll
-    for (int c = 0; c < C; ++c) acc[c] = acc[c] * al + p * E::load(vr[lane + 32 * c]);
-    m = mn;
+  if (warp == 9) tc::tmem_alloc(tmem_slot, 512);
+  if (warp == 8 && lane == 0) {
+    tc::prefetch_tmap(&tq);
+    tc::prefetch_tmap(&tk);
+    tc::prefetch_tmap(&tv);
   }
-  const float inv = n > 0 ? 1.0f / l : 0.0f;
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+
+  // a wait that the whole warp agrees on; false: it (or another role) gave up
+  auto wait_all = [&](int bar, uint32_t parity, int code) -> bool {
+    const bool got = !*abort_flag && tc::mbar_wait(&bars[bar], parity, a.err, code);
+    if (__all_sync(0xffffffffu, got)) return true;
+    *abort_flag = 1;
+    return false;
+  };
+  // next item: every reader copies it and lets the slot go (the whole warp calls)
+  int itn = 0;
+  auto next_item = [&](Item& m) -> bool {
+    const int s = itn & 1;
+    if (!wait_all(P_ITF + s, (itn >> 1) & 1, 401)) return false;
+    m = items[s];
+    __syncwarp();
+    if (lane == 0) tc::mbar_arrive(&bars[P_ITE + s]);
+    ++itn;
+    return !m.done;
+  };
+  Item m;
+
+  // registers: 384 x 168 at launch = 256 x 208 (softmax) + 128 x 88
+  if (warp < 8) {
+    // ---------------------------------------------------------------- softmax, output
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    const int t = warp >> 2, sw = warp & 3, r = sw * 32 + lane;
+    const uint32_t scol = tc::taddr(tmem, sw * 32, C::S_COL + 128 * t), ocol = tc::taddr(tmem, sw * 32, C::O_COL + 128 * t);
+    const int rtok = r / a.g, rhead = r % a.g;
+    uint32_t ns = 0, no = 0;
+    while (next_item(m)) {
+      const int par = (itn - 1) & 3;
+      const int tok = m.tok0 + t * a.ntok + rtok, i = m.i0 + t * a.ntok + rtok;
+      const bool row_ok = rtok < a.ntok && tok < m.tok_end;
+      const int lim = row_ok ? max(0, min(m.nk, i + m.shift)) : 0x3fffffff;  // keys that this row sees
+      const int n = t ? m.n1 : m.n0;
+      float ms = 0.0f, mx = -INFINITY, lsum = 0.0f;  // running maximum (log2 domain) and sum
+      bool ok = true;
+      for (int j = 0; j < n; ++j, ++ns) {
+        if (!wait_all(P_SF + t, ns & 1, 409)) { ok = false; break; }
+        tc::fence_after_sync();
+        uint32_t sv[4][32];
 #pragma unroll
-  for (int c = 0; c < C; ++c) static_cast<T*>(a.o)[row * D + lane + 32 * c] = E::store(acc[c] * inv);
-  if (lane == 0) a.lse[row] = n > 0 ? (m + log2f(l)) * LN2 : -INFINITY;
+        for (int q = 0; q < 4; ++q) tc::tmem_ld32(scol + 32 * q, sv[q]);
+        tc::tmem_wait_ld();
+#pragma unroll
+        for (int q = 0; q < 4; ++q) tc::reg_after_wait(sv[q]);
+        const int vis = lim - j * BN;  // columns below this are seen
+        const bool whole = __all_sync(0xffffffffu, vis >= BN);
+        if (!whole) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (32 * q + e >= vis) sv[q][e] = 0xff800000u;
+        }
+        float m4[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          m4[q] = max3(__uint_as_float(sv[q][0]), __uint_as_float(sv[q][1]), __uint_as_float(sv[q][2]));
+#pragma unroll
+          for (int e = 3; e < 31; e += 2) m4[q] = max3(m4[q], __uint_as_float(sv[q][e]), __uint_as_float(sv[q][e + 1]));
+          m4[q] = max2(m4[q], __uint_as_float(sv[q][31]));
+        }
+        // a NaN or +infinite score makes the row NaN: through the maximum, since the polynomial
+        // exponential does not carry one
+        float mt = max2(max2(m4[0], m4[1]), max2(m4[2], m4[3])) * a.sl;
+        mt = mt < INFINITY ? mt : NAN;
+        const bool need = !(mt <= mx + 8.0f);
+        if (__any_sync(0xffffffffu, need)) {
+          const float mn = need ? mt : mx;
+          const float alpha = need ? fast_exp2(mx - mn) : 1.0f;
+          mx = mn;
+          lsum *= alpha;
+          ms = mx == -INFINITY ? 0.0f : mx;
+          if (j > 0) {  // S_FULL was committed behind the previous PV: O is complete
+#pragma unroll
+            for (int c0 = 0; c0 < D; c0 += 32) {
+              uint32_t ov[32];
+              tc::tmem_ld32(ocol + c0, ov);
+              tc::tmem_wait_ld();
+              tc::reg_after_wait(ov);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * alpha);
+              tc::tmem_st32(ocol + c0, ov);
+            }
+          }
+        }
+        const uint64_t sl2 = pack_f32x2(a.sl, a.sl), nm2 = pack_f32x2(-ms, -ms);
+        uint64_t acc[4] = {0, 0, 0, 0};
+        if (whole) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const uint64_t x = ffma_f32x2(pack_f32x2(__uint_as_float(sv[q][2 * e]), __uint_as_float(sv[q][2 * e + 1])), sl2, nm2);
+              float2 p;
+              if (e % 4 == 3) {
+                p = poly_exp2(x);
+              } else {
+                const float2 xf = unpack_f32x2(x);
+                p = make_float2(fast_exp2(xf.x), fast_exp2(xf.y));
+              }
+              acc[e & 3] = add_f32x2(acc[e & 3], pack_f32x2(p.x, p.y));
+              pk[e] = pack2<DT>(p.x, p.y);
+            }
+            tc::tmem_st16(scol + 16 * q, pk);
+          }
+        } else {  // masked scores are -inf: exactly 0 by the hardware exponential
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float2 xf = unpack_f32x2(
+                  ffma_f32x2(pack_f32x2(__uint_as_float(sv[q][2 * e]), __uint_as_float(sv[q][2 * e + 1])), sl2, nm2));
+              const float2 p = make_float2(fast_exp2(xf.x), fast_exp2(xf.y));
+              acc[e & 3] = add_f32x2(acc[e & 3], pack_f32x2(p.x, p.y));
+              pk[e] = pack2<DT>(p.x, p.y);
+            }
+            tc::tmem_st16(scol + 16 * q, pk);
+          }
+        }
+        const float2 s0 = unpack_f32x2(add_f32x2(add_f32x2(acc[0], acc[1]), add_f32x2(acc[2], acc[3])));
+        lsum += s0.x + s0.y;
+        tc::tmem_wait_st();
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&bars[P_PF + t]);
+      }
+      if (!ok) break;
+      const int64_t row = (int64_t)tok * a.Hq + m.hk * a.g + rhead;
+      uint4* orow = reinterpret_cast<uint4*>(static_cast<T*>(a.o) + row * D);
+      if (n == 0) {  // no row of this tile sees a key
+        if (row_ok) {
+#pragma unroll
+          for (int c = 0; c < D / 8; ++c) orow[c] = make_uint4(0, 0, 0, 0);
+          a.lse[row] = -INFINITY;
+        }
+        continue;
+      }
+      if (!wait_all(P_OF + t, no & 1, 410)) break;
+      ++no;
+      tc::fence_after_sync();
+      const bool bad = bad_v[par] != 0;
+      const float inv = lim > 0 ? 1.0f / lsum : 0.0f;
+#pragma unroll
+      for (int c0 = 0; c0 < D; c0 += 32) {
+        uint32_t ov[32];
+        tc::tmem_ld32(ocol + c0, ov);
+        tc::tmem_wait_ld();
+        tc::reg_after_wait(ov);
+        if (row_ok) {
+          float f[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) f[e] = lim > 0 ? __uint_as_float(ov[e]) * inv : 0.0f;
+          if (bad) {  // values taken out of the repaired tiles, for the rows that see them
+            for (int k = m.jfix * BN; k < lim; ++k) {
+              const T* vr = static_cast<const T*>(a.v) + (int64_t)(m.k0 + k) * a.sv_t + m.hk * a.sv_h + c0;
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                const float x = Elem<DT>::load(vr[e]);
+                if (!isfinite(x)) f[e] += x;
+              }
+            }
+          }
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            orow[c0 / 8 + c] = make_uint4(pack2<DT>(f[8 * c], f[8 * c + 1]), pack2<DT>(f[8 * c + 2], f[8 * c + 3]),
+                                          pack2<DT>(f[8 * c + 4], f[8 * c + 5]), pack2<DT>(f[8 * c + 6], f[8 * c + 7]));
+        }
+      }
+      if (row_ok) a.lse[row] = lim > 0 ? (mx + log2f(lsum)) * LN2 : -INFINITY;
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&bars[P_OE + t]);
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == 8) {
+      // ---------------------------------------------------------------- TMA
+      uint32_t g = 0, nq[2] = {0, 0};
+      const uint32_t qbytes = uint32_t(C::DB) * 128 * a.g * a.ntok;
+      while (next_item(m)) {
+        if (lane == 0) {
+        const int n = max(m.n0, m.n1);
+        bool ok = true;
+        auto load_q = [&](int t) {
+          if ((t ? m.n1 : m.n0) == 0) return;
+          if (!tc::mbar_wait(&bars[P_QE + t], (nq[t] & 1) ^ 1, a.err, 402)) { ok = false; return; }
+          ++nq[t];
+          tc::mbar_expect_tx(&bars[P_QF + t], qbytes);
+#pragma unroll
+          for (int cb = 0; cb < C::DB; ++cb)
+            tc::tma_load_3d(qs + t * C::Q_BYTES + cb * 128 * 128, &tq, &bars[P_QF + t], cb * 64, m.hk * a.g,
+                            m.tok0 + t * a.ntok);
+        };
+        auto load_kv = [&](const CUtensorMap* map, int j) {
+          const uint32_t s = g % C::NS;
+          if (!tc::mbar_wait(&bars[P_KE + s], ((g / C::NS) & 1) ^ 1, a.err, 403)) { ok = false; return; }
+          tc::mbar_expect_tx(&bars[P_KF + s], C::SLOT);
+#pragma unroll
+          for (int cb = 0; cb < C::DB; ++cb)
+            tc::tma_load_3d(ring + s * C::SLOT + cb * BN * 128, map, &bars[P_KF + s], cb * 64, m.hk, m.k0 + j * BN);
+          ++g;
+        };
+        load_q(0);
+        for (int j = 0; j < n && ok; ++j) {
+          load_kv(&tk, j);
+          if (j == 0 && ok) load_q(1);
+          if (ok) load_kv(&tv, j);
+        }
+        if (!ok) *abort_flag = 1;
+        }
+        __syncwarp();
+      }
+    } else if (warp == 9) {
+      // ---------------------------------------------------------------- MMA issue
+      const uint32_t fmt = DT == MZB_BF16 ? 1 : 0;
+      // a negative scale: the scores of -q (negate-A bit), so that larger is always more
+      const uint32_t idesc_qk = tc::make_idesc(128, BN, fmt, fmt) | (a.neg ? 1u << 13 : 0u);
+      const uint32_t idesc_pv = tc::make_idesc(128, D, fmt, fmt, false, true);
+      const uint32_t q_base = smem_u32(qs), r_base = smem_u32(ring);
+      uint32_t g = 0, nq[2] = {0, 0}, np[2] = {0, 0}, vok = 0;
+      while (next_item(m)) {
+        if (lane == 0) {
+        const int nt[2] = {m.n0, m.n1}, n = max(m.n0, m.n1);
+        bool ok = true;
+        auto full = [&](uint32_t gg) {
+          if (!tc::mbar_wait(&bars[P_KF + gg % C::NS], (gg / C::NS) & 1, a.err, 404)) ok = false;
+        };
+        auto qk = [&](int t, int j, uint32_t gk) {  // S_t = Q_t K_j^T
+          const uint64_t qd = tc::make_sdesc<128>(q_base + t * C::Q_BYTES, 16, 1024);
+          const uint64_t kd = tc::make_sdesc<128>(r_base + (gk % C::NS) * C::SLOT, 16, 1024);
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const int cb = kk >> 2, off = (kk & 3) * 32;
+            tc::mma_ss<0>(tmem + C::S_COL + 128 * t, tc::sdesc_add(qd, cb * 128 * 128 + off),
+                          tc::sdesc_add(kd, cb * BN * 128 + off), idesc_qk, kk > 0);
+          }
+          tc::mma_commit(&bars[P_SF + t]);
+          if (j == nt[t] - 1) tc::mma_commit(&bars[P_QE + t]);
+        };
+        // slots of this item: K_j at g + 2 j, V_j at g + 2 j + 1
+        if (n > 0) {
+          full(g);
+          for (int t = 0; t < 2 && ok; ++t)
+            if (nt[t] > 0) {
+              if (!tc::mbar_wait(&bars[P_QF + t], nq[t]++ & 1, a.err, 405)) { ok = false; break; }
+              tc::fence_after_sync();
+              qk(t, 0, g);
+            }
+          if (ok) tc::mma_commit(&bars[P_KE + g % C::NS]);
+        }
+        for (int j = 0; j < n && ok; ++j) {
+          const uint32_t gv = g + 2 * j + 1, gk = gv + 1, sv = gv % C::NS;
+          bool have_v = false, have_k = false;
+          for (int t = 0; t < 2 && ok; ++t) {
+            if (j >= nt[t]) continue;
+            if (!have_v) {
+              full(gv);
+              if (ok && j >= m.jfix) {
+                if (!tc::mbar_wait(&bars[P_VOK + sv], (vok >> sv) & 1, a.err, 406)) ok = false;
+                vok ^= 1u << sv;
+              }
+              have_v = true;
+            }
+            if (ok && j == 0 && !tc::mbar_wait(&bars[P_OE + t], ((nq[t] - 1) & 1) ^ 1, a.err, 407)) ok = false;
+            if (!ok || !tc::mbar_wait(&bars[P_PF + t], np[t]++ & 1, a.err, 408)) { ok = false; break; }
+            tc::fence_after_sync();
+            const uint64_t vd = tc::make_sdesc<128>(r_base + sv * C::SLOT, BN * 128, 1024);
+#pragma unroll
+            for (int kk = 0; kk < BN / 16; ++kk)
+              tc::mma_ts(tmem + C::O_COL + 128 * t, tmem + C::S_COL + 128 * t + 8 * kk, tc::sdesc_add(vd, kk * 16 * 128),
+                         idesc_pv, (j > 0 || kk > 0) ? 1u : 0u);
+            if (j == nt[t] - 1) tc::mma_commit(&bars[P_OF + t]);
+            if (j + 1 < nt[t]) {
+              if (!have_k) {
+                full(gk);
+                if (!ok) break;
+                tc::fence_after_sync();
+                have_k = true;
+              }
+              qk(t, j + 1, gk);
+            }
+          }
+          if (ok) {
+            tc::mma_commit(&bars[P_KE + sv]);
+            if (j + 1 < n) tc::mma_commit(&bars[P_KE + gk % C::NS]);
+          }
+        }
+        g += 2 * n;
+        if (!ok) *abort_flag = 1;
+        }
+        __syncwarp();
+      }
+    } else if (warp == 10) {
+      // ---------------------------------------------------------------- scheduler
+      Finder f;
+      f.init(a, lane);
+      int64_t idx = blockIdx.x;
+      int k = 0;
+      uint32_t tries = 0;
+      bool more = true;
+      while (more) {
+        int b = 0, pair = 0;
+        const bool real = f.find(a, idx / a.Hkv, lane, b, pair);
+        if (lane == 0) {  // ask for the next one before waiting for a free place
+          tc::mbar_expect_tx(&bars[P_CLC], 16);
+          asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                           smem_u32(clc)),
+                       "r"(smem_u32(&bars[P_CLC]))
+                       : "memory");
+        }
+        if (real) {
+          const int s = k & 1;
+          if (!wait_all(P_ITE + s, ((k >> 1) & 1) ^ 1, 411)) break;
+          if (lane == 0) {
+            fill_item(a, b, pair, int(idx % a.Hkv), &items[s]);
+            tc::mbar_arrive(&bars[P_ITF + s]);
+          }
+          ++k;
+        }
+        if (!wait_all(P_CLC, tries & 1, 412)) break;
+        ++tries;
+        uint32_t got, x;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t.reg .b128 h;\n\t.reg .b32 y, z, w;\n\t"
+            "ld.shared.b128 h, [%2];\n\t"
+            "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t"
+            "mov.u32 %1, 0;\n\t"
+            "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, y, z, w}, h;\n\t}"
+            : "=r"(got), "=r"(x)
+            : "r"(smem_u32(clc))
+            : "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the next answer is written behind this read
+        __syncwarp();
+        more = got != 0;
+        idx = x;
+      }
+      const int s = k & 1;
+      if (wait_all(P_ITE + s, ((k >> 1) & 1) ^ 1, 413) && lane == 0) {
+        items[s].done = 1;
+        tc::mbar_arrive(&bars[P_ITF + s]);
+      }
+    } else {
+      // ---------------------------------------------------------------- V repair
+      uint32_t g = 0;
+      while (next_item(m)) {
+        const int n = max(m.n0, m.n1), par = (itn - 1) & 3;
+        int found = 0;
+        if (lane == 0) bad_v[par] = 0;
+        __syncwarp();
+        // every fill of the ring passes here, so that this warp is neither ahead of the barriers'
+        // phases nor lapped by them
+        for (int f = 0; f < 2 * n; ++f, ++g) {
+          const uint32_t s = g % C::NS;
+          if (!wait_all(P_KF + s, (g / C::NS) & 1, 414)) break;
+          if (!(f & 1) || (f >> 1) < m.jfix) {
+            if (lane == 0) tc::mbar_arrive(&bars[P_KE + s]);
+            continue;
+          }
+          uint8_t* tile = ring + s * C::SLOT;
+          for (int x0 = 0; x0 < C::SLOT / 16; x0 += 32 * 8) {
+            uint4 w[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = *reinterpret_cast<const uint4*>(tile + (x0 + 32 * e + lane) * 16);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const uint4 z = make_uint4(nonfinite2<DT>(w[e].x), nonfinite2<DT>(w[e].y), nonfinite2<DT>(w[e].z),
+                                         nonfinite2<DT>(w[e].w));
+              if (z.x | z.y | z.z | z.w) {
+                *reinterpret_cast<uint4*>(tile + (x0 + 32 * e + lane) * 16) =
+                    make_uint4(w[e].x & ~z.x, w[e].y & ~z.y, w[e].z & ~z.z, w[e].w & ~z.w);
+                found = 1;
+              }
+            }
+          }
+          found = __any_sync(0xffffffffu, found);
+          if (found && lane == 0) bad_v[par] = 1;
+          tc::fence_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tc::mbar_arrive(&bars[P_VOK + s]);
+            tc::mbar_arrive(&bars[P_KE + s]);
+          }
+        }
+      }
+    }
+  }
+
+  tc::fence_before_sync();
+  __syncthreads();
+  if (warp == 9) {
+    tc::fence_after_sync();
+    tc::tmem_free(tmem, 512);
+  }
 }
 
 template <int DT, int D>
-int launch(const PrefillArgs& a, cudaStream_t st) {
-  prefill_kernel<DT, D><<<unsigned((a.Tq * a.Hq + 7) / 8), 256, 0, st>>>(a);
+int launch(const void* q, const void* k, PrefillArgs a, int64_t sq_t, int64_t sq_h, int64_t sk_t, int64_t sk_h,
+           cudaStream_t st) {
+  using C = PCfg<D>;
+  CUtensorMap m[3];
+  const void* base[3] = {q, k, a.v};
+  const int64_t str[3][2] = {{sq_h, sq_t}, {sk_h, sk_t}, {a.sv_h, a.sv_t}};
+  const int64_t heads[3] = {a.Hq, a.Hkv, a.Hkv}, toks[3] = {a.Tq, a.Tk, a.Tk};
+  for (int i = 0; i < 3; ++i) {
+    if (i > 0 && a.Tk == 0) {  // no keys at all: nothing is loaded through these
+      m[i] = m[0];
+      continue;
+    }
+    const uint64_t dims[3] = {uint64_t(D), uint64_t(heads[i]), uint64_t(toks[i])};
+    // the stride of a dimension of size 1 is never used: any legal one
+    const uint64_t s[2] = {heads[i] > 1 ? uint64_t(str[i][0]) * 2 : uint64_t(D) * 2,
+                           toks[i] > 1 ? uint64_t(str[i][1]) * 2 : uint64_t(D) * 2};
+    const uint32_t box[3] = {64, i ? 1u : uint32_t(a.g), i ? uint32_t(BN) : uint32_t(a.ntok)};
+    if (int r = encode_tmap(&m[i], DT == MZB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                            base[i], dims, s, box, CU_TENSOR_MAP_SWIZZLE_128B))
+      return r;
+  }
+  auto kern = prefill_kernel<DT, D>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
+    return launch_status("gqa_prefill(smem attr)");
+  // at least as many pairs of query tiles as any packing of Tq tokens into B sequences has
+  const int64_t pairs = a.Tq / (2 * a.ntok) + (a.B < a.Tq ? a.B : a.Tq);
+  MZB_REQUIRE(pairs * a.Hkv < (int64_t(1) << 31), MZB_ERR_SHAPE, "gqa_prefill: too large");
+  kern<<<unsigned(pairs * a.Hkv), 384, C::SMEM, st>>>(m[0], m[1], m[2], a);
   return launch_status("gqa_prefill");
 }
 
@@ -88,7 +717,7 @@ extern "C" int mzb_gqa_prefill(const void* q, const void* k, const void* v, cons
                                void* o, float* lse, int64_t Tq, int64_t Tk, int B, int Hq, int Hkv, int D, int dtype,
                                int64_t sq_t, int64_t sq_h, int64_t sk_t, int64_t sk_h, int64_t sv_t, int64_t sv_h,
                                int causal, float softmax_scale, int* err, void* stream) {
-  MZB_REQUIRE(Tq >= 0 && Tk >= 0 && B >= 1 && Tq < (int64_t(1) << 31) && Tk < (int64_t(1) << 31), MZB_ERR_SHAPE,
+  MZB_REQUIRE(Tq >= 0 && Tk >= 0 && B >= 1 && Tq < (int64_t(1) << 30) && Tk < (int64_t(1) << 30), MZB_ERR_SHAPE,
               "gqa_prefill: bad sizes Tq=%lld Tk=%lld B=%d", (long long)Tq, (long long)Tk, B);
   MZB_REQUIRE(Hkv >= 1 && Hq >= 1 && Hq % Hkv == 0 && Hq / Hkv <= 128, MZB_ERR_SHAPE,
               "gqa_prefill: query heads must be a multiple (at most 128) of the K/V heads, got %d and %d", Hq, Hkv);
@@ -96,12 +725,17 @@ extern "C" int mzb_gqa_prefill(const void* q, const void* k, const void* v, cons
   MZB_REQUIRE(dtype == MZB_BF16 || dtype == MZB_F16, MZB_ERR_UNSUPPORTED, "gqa_prefill: unsupported dtype %d", dtype);
   MZB_REQUIRE(err != nullptr, MZB_ERR_SHAPE, "gqa_prefill: needs an error word");
   if (Tq == 0) return MZB_OK;
-  gqa::PrefillArgs a{q, k, v, cu_q, cu_k, o, lse, Tq, Tk, sq_t, sq_h, sk_t, sk_h, sv_t, sv_h, B, Hq, Hkv, causal,
-                     softmax_scale};
+  gqa::PrefillArgs a{};
+  a.v = v; a.cu_q = cu_q; a.cu_k = cu_k; a.o = o; a.lse = lse;
+  a.Tq = Tq; a.Tk = Tk; a.sv_t = sv_t; a.sv_h = sv_h;
+  a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.g = Hq / Hkv; a.ntok = 128 / a.g; a.causal = causal;
+  a.neg = softmax_scale < 0;
+  a.sl = (softmax_scale < 0 ? -softmax_scale : softmax_scale) * gqa::LOG2E;
+  if (a.sl < 1e-37f) a.sl = 1e-37f;  // scale 0: all weights still 1, and a masked -inf stays -inf
+  a.err = err;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == MZB_BF16)
-    return D == 64 ? gqa::launch<MZB_BF16, 64>(a, st) : D == 96 ? gqa::launch<MZB_BF16, 96>(a, st)
-                                                                : gqa::launch<MZB_BF16, 128>(a, st);
-  return D == 64 ? gqa::launch<MZB_F16, 64>(a, st) : D == 96 ? gqa::launch<MZB_F16, 96>(a, st)
-                                                             : gqa::launch<MZB_F16, 128>(a, st);
+#define MZB_GO(DT, DD) gqa::launch<DT, DD>(q, k, a, sq_t, sq_h, sk_t, sk_h, st)
+  if (dtype == MZB_BF16) return D == 64 ? MZB_GO(MZB_BF16, 64) : D == 96 ? MZB_GO(MZB_BF16, 96) : MZB_GO(MZB_BF16, 128);
+  return D == 64 ? MZB_GO(MZB_F16, 64) : D == 96 ? MZB_GO(MZB_F16, 96) : MZB_GO(MZB_F16, 128);
+#undef MZB_GO
 }
