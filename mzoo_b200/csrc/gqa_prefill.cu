@@ -39,7 +39,7 @@ struct PCfg {
   static constexpr int SLOT = DB * BN * 128;
   static constexpr int NS = DB == 1 ? 8 : 5;  // ring slots (K and V tiles alternate)
   static constexpr int TILES = 2 * Q_BYTES + NS * SLOT;
-  static constexpr int SMEM = TILES + 1024;
+  static constexpr int SMEM = TILES + 1024 + 2048;
   static constexpr int S_COL = 0, O_COL = 256;  // tile t: + 128 t
   static_assert(SMEM <= 232448, "shared memory budget");
 };
@@ -65,9 +65,9 @@ struct Item {
   int done;
 };
 
-enum PBar { P_QF = 0, P_QE = 2, P_SF = 4, P_PF = 6, P_OF = 8, P_OE = 10, P_ITF = 12, P_ITE = 14, P_CLC = 16, P_KF = 17,
-            P_KE = P_KF + 8, P_VOK = P_KE + 8, P_NBAR = P_VOK + 8 };
-constexpr int ITEM_READERS = 8 + 3;  // softmax warps, TMA, MMA, repair
+enum PBar { P_QF = 0, P_QE = 2, P_SF = 4, P_PF = 6, P_OF = 10, P_OE = 12, P_ITF = 14, P_ITE = 16, P_CLC = 18, P_ASK = 19,
+            P_KF = 20, P_KE = P_KF + 8, P_VOK = P_KE + 8, P_NBAR = P_VOK + 8 };
+constexpr int ITEM_READERS = 16 + 3;  // softmax warps, TMA, MMA, repair
 
 __device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
   uint64_t d;
@@ -114,6 +114,13 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     const __half2 v = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&v);
   }
+}
+
+// 32 bytes of one row, one whole sector per thread (rows are 32-byte aligned: D / 2 elements are).
+__device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+               "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
 }
 
 // Bits set where a 16-bit half of w is NaN or infinite (exponent all ones).
@@ -235,7 +242,7 @@ __device__ __forceinline__ void fill_item(const PrefillArgs& a, int b, int pair,
 // ---------------------------------------------------------------- kernel
 
 template <int DT, int D>
-__global__ void __launch_bounds__(384, 1)
+__global__ void __launch_bounds__(640, 1)
     prefill_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                    const __grid_constant__ CUtensorMap tv, const __grid_constant__ PrefillArgs a) {
   using C = PCfg<D>;
@@ -246,6 +253,7 @@ __global__ void __launch_bounds__(384, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::TILES);
   Item* items = reinterpret_cast<Item*>(smem + C::TILES + 8 * P_NBAR + 16);  // [2]
   uint4* clc = reinterpret_cast<uint4*>(smem + C::TILES + 512);
+  float* exch = reinterpret_cast<float*>(smem + C::TILES + 1024);  // [2 tiles][2 halves][128]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::TILES + 544);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::TILES + 548);
   volatile int* bad_v = reinterpret_cast<volatile int*>(smem + C::TILES + 552);  // [4] by item number
@@ -258,7 +266,8 @@ __global__ void __launch_bounds__(384, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < P_NBAR; ++i) {
       uint32_t c = 1;
-      if (i == P_PF || i == P_PF + 1 || i == P_OE || i == P_OE + 1) c = 4;
+      if (i >= P_PF && i < P_PF + 4) c = 4;
+      if (i == P_OE || i == P_OE + 1) c = 8;
       if (i == P_ITE || i == P_ITE + 1) c = ITEM_READERS;
       if (i >= P_KE && i < P_KE + 8) c = 2;  // the last product that reads the slot; the repair warp
       tc::mbar_init(&bars[i], c);
@@ -266,8 +275,8 @@ __global__ void __launch_bounds__(384, 1)
     *abort_flag = 0;
     tc::fence_barrier_init();
   }
-  if (warp == 9) tc::tmem_alloc(tmem_slot, 512);
-  if (warp == 8 && lane == 0) {
+  if (warp == 17) tc::tmem_alloc(tmem_slot, 512);
+  if (warp == 16 && lane == 0) {
     tc::prefetch_tmap(&tq);
     tc::prefetch_tmap(&tk);
     tc::prefetch_tmap(&tv);
@@ -297,13 +306,17 @@ __global__ void __launch_bounds__(384, 1)
   };
   Item m;
 
-  // registers: 384 x 168 at launch = 256 x 208 (softmax) + 128 x 88
-  if (warp < 8) {
+  // registers: 640 x 96 at launch = 512 x 104 (softmax) + 128 x 64
+  if (warp < 16) {
     // ---------------------------------------------------------------- softmax, output
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    const int t = warp >> 2, sw = warp & 3, r = sw * 32 + lane;
-    const uint32_t scol = tc::taddr(tmem, sw * 32, C::S_COL + 128 * t), ocol = tc::taddr(tmem, sw * 32, C::O_COL + 128 * t);
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    const int t = warp >> 3, half = (warp >> 2) & 1, sw = warp & 3, r = sw * 32 + lane;
+    // this thread's 64 columns of its row's scores, its weights' place, its half of O's columns
+    const uint32_t scol = tc::taddr(tmem, sw * 32, C::S_COL + 128 * t + 64 * half);
+    const uint32_t ocol = tc::taddr(tmem, sw * 32, C::O_COL + 128 * t + D / 2 * half);
     const int rtok = r / a.g, rhead = r % a.g;
+    float* xch = exch + t * 256 + r;  // [half][128] of this tile: row maxima, at the end row sums
+    const int pair_bar = 1 + t * 4 + sw;
     uint32_t ns = 0, no = 0;
     while (next_item(m)) {
       const int par = (itn - 1) & 3;
@@ -311,22 +324,22 @@ __global__ void __launch_bounds__(384, 1)
       const bool row_ok = rtok < a.ntok && tok < m.tok_end;
       const int lim = row_ok ? max(0, min(m.nk, i + m.shift)) : 0x3fffffff;  // keys that this row sees
       const int n = t ? m.n1 : m.n0;
-      float ms = 0.0f, mx = -INFINITY, lsum = 0.0f;  // running maximum (log2 domain) and sum
+      float ms = 0.0f, mx = -INFINITY, lsum = 0.0f;  // running maximum (log2 domain), this half's sum
       bool ok = true;
       for (int j = 0; j < n; ++j, ++ns) {
         if (!wait_all(P_SF + t, ns & 1, 409)) { ok = false; break; }
         tc::fence_after_sync();
-        uint32_t sv[4][32];
+        uint32_t sv[2][32];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) tc::tmem_ld32(scol + 32 * q, sv[q]);
+        for (int q = 0; q < 2; ++q) tc::tmem_ld32(scol + 32 * q, sv[q]);
         tc::tmem_wait_ld();
 #pragma unroll
-        for (int q = 0; q < 4; ++q) tc::reg_after_wait(sv[q]);
-        const int vis = lim - j * BN;  // columns below this are seen
-        const bool whole = __all_sync(0xffffffffu, vis >= BN);
+        for (int q = 0; q < 2; ++q) tc::reg_after_wait(sv[q]);
+        const int vis = lim - j * BN - 64 * half;  // columns below this are seen
+        const bool whole = __all_sync(0xffffffffu, vis >= 64);
         if (!whole) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
+          for (int q = 0; q < 2; ++q)
 #pragma unroll
             for (int e = 0; e < 32; ++e)
               if (32 * q + e >= vis) sv[q][e] = 0xff800000u;
@@ -334,14 +347,19 @@ __global__ void __launch_bounds__(384, 1)
         float m4[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          m4[q] = max3(__uint_as_float(sv[q][0]), __uint_as_float(sv[q][1]), __uint_as_float(sv[q][2]));
+          const uint32_t* x = &sv[q >> 1][16 * (q & 1)];
+          m4[q] = max3(__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]));
 #pragma unroll
-          for (int e = 3; e < 31; e += 2) m4[q] = max3(m4[q], __uint_as_float(sv[q][e]), __uint_as_float(sv[q][e + 1]));
-          m4[q] = max2(m4[q], __uint_as_float(sv[q][31]));
+          for (int e = 3; e < 15; e += 2) m4[q] = max3(m4[q], __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+          m4[q] = max2(m4[q], __uint_as_float(x[15]));
         }
+        float mt = max2(max2(m4[0], m4[1]), max2(m4[2], m4[3]));
+        // the other half's maximum (it has read the last tile's: S_FULL follows both halves' P_FULL)
+        xch[128 * half] = mt;
+        tc::bar_sync(pair_bar, 64);
         // a NaN or +infinite score makes the row NaN: through the maximum, since the polynomial
         // exponential does not carry one
-        float mt = max2(max2(m4[0], m4[1]), max2(m4[2], m4[3])) * a.sl;
+        mt = max2(mt, xch[128 * (half ^ 1)]) * a.sl;
         mt = mt < INFINITY ? mt : NAN;
         const bool need = !(mt <= mx + 8.0f);
         if (__any_sync(0xffffffffu, need)) {
@@ -352,22 +370,22 @@ __global__ void __launch_bounds__(384, 1)
           ms = mx == -INFINITY ? 0.0f : mx;
           if (j > 0) {  // S_FULL was committed behind the previous PV: O is complete
 #pragma unroll
-            for (int c0 = 0; c0 < D; c0 += 32) {
-              uint32_t ov[32];
-              tc::tmem_ld32(ocol + c0, ov);
+            for (int c0 = 0; c0 < D / 2; c0 += 16) {
+              uint32_t ov[16];
+              tc::tmem_ld16(ocol + c0, ov);
               tc::tmem_wait_ld();
               tc::reg_after_wait(ov);
 #pragma unroll
-              for (int e = 0; e < 32; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * alpha);
-              tc::tmem_st32(ocol + c0, ov);
+              for (int e = 0; e < 16; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * alpha);
+              tc::tmem_st16(ocol + c0, ov);
             }
           }
         }
         const uint64_t sl2 = pack_f32x2(a.sl, a.sl), nm2 = pack_f32x2(-ms, -ms);
-        uint64_t acc[4] = {0, 0, 0, 0};
+        uint64_t acc[2] = {0, 0};
         if (whole) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
+          for (int q = 0; q < 2; ++q) {
             uint32_t pk[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
@@ -379,88 +397,93 @@ __global__ void __launch_bounds__(384, 1)
                 const float2 xf = unpack_f32x2(x);
                 p = make_float2(fast_exp2(xf.x), fast_exp2(xf.y));
               }
-              acc[e & 3] = add_f32x2(acc[e & 3], pack_f32x2(p.x, p.y));
+              acc[e & 1] = add_f32x2(acc[e & 1], pack_f32x2(p.x, p.y));
               pk[e] = pack2<DT>(p.x, p.y);
             }
             tc::tmem_st16(scol + 16 * q, pk);
           }
         } else {  // masked scores are -inf: exactly 0 by the hardware exponential
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
+          for (int q = 0; q < 2; ++q) {
             uint32_t pk[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
               const float2 xf = unpack_f32x2(
                   ffma_f32x2(pack_f32x2(__uint_as_float(sv[q][2 * e]), __uint_as_float(sv[q][2 * e + 1])), sl2, nm2));
               const float2 p = make_float2(fast_exp2(xf.x), fast_exp2(xf.y));
-              acc[e & 3] = add_f32x2(acc[e & 3], pack_f32x2(p.x, p.y));
+              acc[e & 1] = add_f32x2(acc[e & 1], pack_f32x2(p.x, p.y));
               pk[e] = pack2<DT>(p.x, p.y);
             }
             tc::tmem_st16(scol + 16 * q, pk);
           }
         }
-        const float2 s0 = unpack_f32x2(add_f32x2(add_f32x2(acc[0], acc[1]), add_f32x2(acc[2], acc[3])));
+        const float2 s0 = unpack_f32x2(add_f32x2(acc[0], acc[1]));
         lsum += s0.x + s0.y;
         tc::tmem_wait_st();
         tc::fence_before_sync();
         __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&bars[P_PF + t]);
+        if (lane == 0) tc::mbar_arrive(&bars[P_PF + 2 * t + half]);
       }
       if (!ok) break;
       const int64_t row = (int64_t)tok * a.Hq + m.hk * a.g + rhead;
-      uint4* orow = reinterpret_cast<uint4*>(static_cast<T*>(a.o) + row * D);
+      T* orow = static_cast<T*>(a.o) + row * D + D / 2 * half;
       if (n == 0) {  // no row of this tile sees a key
         if (row_ok) {
+          const uint32_t zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-          for (int c = 0; c < D / 8; ++c) orow[c] = make_uint4(0, 0, 0, 0);
-          a.lse[row] = -INFINITY;
+          for (int c0 = 0; c0 < D / 2; c0 += 16) store32(orow + c0, zero);
+          if (half == 0) a.lse[row] = -INFINITY;
         }
         continue;
       }
       if (!wait_all(P_OF + t, no & 1, 410)) break;
       ++no;
+      xch[128 * half] = lsum;  // the row's sum is both halves'
+      tc::bar_sync(pair_bar, 64);
+      lsum = __fadd_rn(xch[0], xch[128]);
+      tc::bar_sync(pair_bar, 64);
       tc::fence_after_sync();
       const bool bad = bad_v[par] != 0;
       const float inv = lim > 0 ? 1.0f / lsum : 0.0f;
 #pragma unroll
-      for (int c0 = 0; c0 < D; c0 += 32) {
-        uint32_t ov[32];
-        tc::tmem_ld32(ocol + c0, ov);
+      for (int c0 = 0; c0 < D / 2; c0 += 16) {
+        uint32_t ov[16];
+        tc::tmem_ld16(ocol + c0, ov);
         tc::tmem_wait_ld();
         tc::reg_after_wait(ov);
         if (row_ok) {
-          float f[32];
+          float f[16];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) f[e] = lim > 0 ? __uint_as_float(ov[e]) * inv : 0.0f;
+          for (int e = 0; e < 16; ++e) f[e] = lim > 0 ? __uint_as_float(ov[e]) * inv : 0.0f;
           if (bad) {  // values taken out of the repaired tiles, for the rows that see them
             for (int k = m.jfix * BN; k < lim; ++k) {
-              const T* vr = static_cast<const T*>(a.v) + (int64_t)(m.k0 + k) * a.sv_t + m.hk * a.sv_h + c0;
+              const T* vr = static_cast<const T*>(a.v) + (int64_t)(m.k0 + k) * a.sv_t + m.hk * a.sv_h + D / 2 * half + c0;
 #pragma unroll
-              for (int e = 0; e < 32; ++e) {
+              for (int e = 0; e < 16; ++e) {
                 const float x = Elem<DT>::load(vr[e]);
                 if (!isfinite(x)) f[e] += x;
               }
             }
           }
+          uint32_t w[8];
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-            orow[c0 / 8 + c] = make_uint4(pack2<DT>(f[8 * c], f[8 * c + 1]), pack2<DT>(f[8 * c + 2], f[8 * c + 3]),
-                                          pack2<DT>(f[8 * c + 4], f[8 * c + 5]), pack2<DT>(f[8 * c + 6], f[8 * c + 7]));
+          for (int e = 0; e < 8; ++e) w[e] = pack2<DT>(f[2 * e], f[2 * e + 1]);
+          store32(orow + c0, w);
         }
       }
-      if (row_ok) a.lse[row] = lim > 0 ? (mx + log2f(lsum)) * LN2 : -INFINITY;
+      if (row_ok && half == 0) a.lse[row] = lim > 0 ? (mx + log2f(lsum)) * LN2 : -INFINITY;
       tc::fence_before_sync();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&bars[P_OE + t]);
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    if (warp == 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (warp == 16) {
       // ---------------------------------------------------------------- TMA
       uint32_t g = 0, nq[2] = {0, 0};
       const uint32_t qbytes = uint32_t(C::DB) * 128 * a.g * a.ntok;
       while (next_item(m)) {
-        if (lane == 0) {
+        if (tc::elect_one()) {
         const int n = max(m.n0, m.n1);
         bool ok = true;
         auto load_q = [&](int t) {
@@ -482,17 +505,20 @@ __global__ void __launch_bounds__(384, 1)
             tc::tma_load_3d(ring + s * C::SLOT + cb * BN * 128, map, &bars[P_KF + s], cb * 64, m.hk, m.k0 + j * BN);
           ++g;
         };
+        const int ask = max(0, n - 3);  // the next item is bound late, or the last blocks' shares are uneven
         load_q(0);
         for (int j = 0; j < n && ok; ++j) {
           load_kv(&tk, j);
           if (j == 0 && ok) load_q(1);
           if (ok) load_kv(&tv, j);
+          if (j == ask) tc::mbar_arrive(&bars[P_ASK]);
         }
+        if (n == 0) tc::mbar_arrive(&bars[P_ASK]);
         if (!ok) *abort_flag = 1;
         }
         __syncwarp();
       }
-    } else if (warp == 9) {
+    } else if (warp == 17) {
       // ---------------------------------------------------------------- MMA issue
       const uint32_t fmt = DT == MZB_BF16 ? 1 : 0;
       // a negative scale: the scores of -q (negate-A bit), so that larger is always more
@@ -501,7 +527,7 @@ __global__ void __launch_bounds__(384, 1)
       const uint32_t q_base = smem_u32(qs), r_base = smem_u32(ring);
       uint32_t g = 0, nq[2] = {0, 0}, np[2] = {0, 0}, vok = 0;
       while (next_item(m)) {
-        if (lane == 0) {
+        if (tc::elect_one()) {
         const int nt[2] = {m.n0, m.n1}, n = max(m.n0, m.n1);
         bool ok = true;
         auto full = [&](uint32_t gg) {
@@ -522,19 +548,21 @@ __global__ void __launch_bounds__(384, 1)
         // slots of this item: K_j at g + 2 j, V_j at g + 2 j + 1
         if (n > 0) {
           full(g);
-          for (int t = 0; t < 2 && ok; ++t)
-            if (nt[t] > 0) {
-              if (!tc::mbar_wait(&bars[P_QF + t], nq[t]++ & 1, a.err, 405)) { ok = false; break; }
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            if (ok && nt[t] > 0) {
+              if (!tc::mbar_wait(&bars[P_QF + t], nq[t]++ & 1, a.err, 405)) ok = false;
               tc::fence_after_sync();
-              qk(t, 0, g);
+              if (ok) qk(t, 0, g);
             }
           if (ok) tc::mma_commit(&bars[P_KE + g % C::NS]);
         }
         for (int j = 0; j < n && ok; ++j) {
           const uint32_t gv = g + 2 * j + 1, gk = gv + 1, sv = gv % C::NS;
           bool have_v = false, have_k = false;
-          for (int t = 0; t < 2 && ok; ++t) {
-            if (j >= nt[t]) continue;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (!ok || j >= nt[t]) continue;
             if (!have_v) {
               full(gv);
               if (ok && j >= m.jfix) {
@@ -544,22 +572,27 @@ __global__ void __launch_bounds__(384, 1)
               have_v = true;
             }
             if (ok && j == 0 && !tc::mbar_wait(&bars[P_OE + t], ((nq[t] - 1) & 1) ^ 1, a.err, 407)) ok = false;
-            if (!ok || !tc::mbar_wait(&bars[P_PF + t], np[t]++ & 1, a.err, 408)) { ok = false; break; }
-            tc::fence_after_sync();
             const uint64_t vd = tc::make_sdesc<128>(r_base + sv * C::SLOT, BN * 128, 1024);
 #pragma unroll
-            for (int kk = 0; kk < BN / 16; ++kk)
-              tc::mma_ts(tmem + C::O_COL + 128 * t, tmem + C::S_COL + 128 * t + 8 * kk, tc::sdesc_add(vd, kk * 16 * 128),
-                         idesc_pv, (j > 0 || kk > 0) ? 1u : 0u);
+            for (int h = 0; h < 2; ++h) {  // the weights of 64 keys each
+              if (ok && !tc::mbar_wait(&bars[P_PF + 2 * t + h], np[t] & 1, a.err, 408)) ok = false;
+              if (!ok) continue;
+              tc::fence_after_sync();
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk)
+                tc::mma_ts(tmem + C::O_COL + 128 * t, tmem + C::S_COL + 128 * t + 64 * h + 8 * kk,
+                           tc::sdesc_add(vd, (4 * h + kk) * 16 * 128), idesc_pv, (j > 0 || h > 0 || kk > 0) ? 1u : 0u);
+            }
+            if (!ok) continue;
+            ++np[t];
             if (j == nt[t] - 1) tc::mma_commit(&bars[P_OF + t]);
             if (j + 1 < nt[t]) {
               if (!have_k) {
                 full(gk);
-                if (!ok) break;
                 tc::fence_after_sync();
                 have_k = true;
               }
-              qk(t, j + 1, gk);
+              if (ok) qk(t, j + 1, gk);
             }
           }
           if (ok) {
@@ -572,7 +605,7 @@ __global__ void __launch_bounds__(384, 1)
         }
         __syncwarp();
       }
-    } else if (warp == 10) {
+    } else if (warp == 18) {
       // ---------------------------------------------------------------- scheduler
       Finder f;
       f.init(a, lane);
@@ -583,13 +616,6 @@ __global__ void __launch_bounds__(384, 1)
       while (more) {
         int b = 0, pair = 0;
         const bool real = f.find(a, idx / a.Hkv, lane, b, pair);
-        if (lane == 0) {  // ask for the next one before waiting for a free place
-          tc::mbar_expect_tx(&bars[P_CLC], 16);
-          asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
-                           smem_u32(clc)),
-                       "r"(smem_u32(&bars[P_CLC]))
-                       : "memory");
-        }
         if (real) {
           const int s = k & 1;
           if (!wait_all(P_ITE + s, ((k >> 1) & 1) ^ 1, 411)) break;
@@ -597,7 +623,15 @@ __global__ void __launch_bounds__(384, 1)
             fill_item(a, b, pair, int(idx % a.Hkv), &items[s]);
             tc::mbar_arrive(&bars[P_ITF + s]);
           }
+          if (!wait_all(P_ASK, k & 1, 415)) break;
           ++k;
+        }
+        if (lane == 0) {
+          tc::mbar_expect_tx(&bars[P_CLC], 16);
+          asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                           smem_u32(clc)),
+                       "r"(smem_u32(&bars[P_CLC]))
+                       : "memory");
         }
         if (!wait_all(P_CLC, tries & 1, 412)) break;
         ++tries;
@@ -670,7 +704,7 @@ __global__ void __launch_bounds__(384, 1)
 
   tc::fence_before_sync();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == 17) {
     tc::fence_after_sync();
     tc::tmem_free(tmem, 512);
   }
@@ -704,7 +738,7 @@ int launch(const void* q, const void* k, PrefillArgs a, int64_t sq_t, int64_t sq
   // at least as many pairs of query tiles as any packing of Tq tokens into B sequences has
   const int64_t pairs = a.Tq / (2 * a.ntok) + (a.B < a.Tq ? a.B : a.Tq);
   MZB_REQUIRE(pairs * a.Hkv < (int64_t(1) << 31), MZB_ERR_SHAPE, "gqa_prefill: too large");
-  kern<<<unsigned(pairs * a.Hkv), 384, C::SMEM, st>>>(m[0], m[1], m[2], a);
+  kern<<<unsigned(pairs * a.Hkv), 640, C::SMEM, st>>>(m[0], m[1], m[2], a);
   return launch_status("gqa_prefill");
 }
 
@@ -724,6 +758,7 @@ extern "C" int mzb_gqa_prefill(const void* q, const void* k, const void* v, cons
   MZB_REQUIRE(D == 64 || D == 96 || D == 128, MZB_ERR_UNSUPPORTED, "gqa_prefill: unsupported head dim %d", D);
   MZB_REQUIRE(dtype == MZB_BF16 || dtype == MZB_F16, MZB_ERR_UNSUPPORTED, "gqa_prefill: unsupported dtype %d", dtype);
   MZB_REQUIRE(err != nullptr, MZB_ERR_SHAPE, "gqa_prefill: needs an error word");
+  MZB_REQUIRE(reinterpret_cast<uintptr_t>(o) % 32 == 0, MZB_ERR_ALIGN, "gqa_prefill: o must be 32-byte aligned");
   if (Tq == 0) return MZB_OK;
   gqa::PrefillArgs a{};
   a.v = v; a.cu_q = cu_q; a.cu_k = cu_k; a.o = o; a.lse = lse;

@@ -99,6 +99,16 @@ __device__ __forceinline__ void fence_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
+// One lane of a converged warp, named by elect.sync: inside `if (elect_one())` the compiler
+// knows that a single thread runs, so the uniform operands of tcgen05.mma (descriptors, TMEM
+// addresses) are moved without a loop over possibly different lanes, which costs ~100 cycles
+// per instruction behind a plain `lane == 0`.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
 // ---------------------------------------------------------------- tcgen05: TMEM
 
 // Allocate `ncols` TMEM columns (power of two >= 32); warp-collective.  The base address
