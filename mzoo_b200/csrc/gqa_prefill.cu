@@ -39,7 +39,7 @@ struct PCfg {
   static constexpr int SLOT = DB * BN * 128;
   static constexpr int NS = DB == 1 ? 8 : 5;  // ring slots (K and V tiles alternate)
   static constexpr int TILES = 2 * Q_BYTES + NS * SLOT;
-  static constexpr int SMEM = TILES + 1024 + 2048;
+  static constexpr int SMEM = TILES + 1024;
   static constexpr int S_COL = 0, O_COL = 256;  // tile t: + 128 t
   static_assert(SMEM <= 232448, "shared memory budget");
 };
@@ -67,7 +67,7 @@ struct Item {
 
 enum PBar { P_QF = 0, P_QE = 2, P_SF = 4, P_PF = 6, P_OF = 10, P_OE = 12, P_ITF = 14, P_ITE = 16, P_CLC = 18, P_ASK = 19,
             P_KF = 20, P_KE = P_KF + 8, P_VOK = P_KE + 8, P_NBAR = P_VOK + 8 };
-constexpr int ITEM_READERS = 16 + 3;  // softmax warps, TMA, MMA, repair
+constexpr int ITEM_READERS = 8 + 3;  // softmax warps, TMA, MMA, repair
 
 __device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
   uint64_t d;
@@ -242,7 +242,7 @@ __device__ __forceinline__ void fill_item(const PrefillArgs& a, int b, int pair,
 // ---------------------------------------------------------------- kernel
 
 template <int DT, int D>
-__global__ void __launch_bounds__(640, 1)
+__global__ void __launch_bounds__(384, 1)
     prefill_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                    const __grid_constant__ CUtensorMap tv, const __grid_constant__ PrefillArgs a) {
   using C = PCfg<D>;
@@ -253,7 +253,6 @@ __global__ void __launch_bounds__(640, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::TILES);
   Item* items = reinterpret_cast<Item*>(smem + C::TILES + 8 * P_NBAR + 16);  // [2]
   uint4* clc = reinterpret_cast<uint4*>(smem + C::TILES + 512);
-  float* exch = reinterpret_cast<float*>(smem + C::TILES + 1024);  // [2 tiles][2 halves][128]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::TILES + 544);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::TILES + 548);
   volatile int* bad_v = reinterpret_cast<volatile int*>(smem + C::TILES + 552);  // [4] by item number
@@ -267,7 +266,7 @@ __global__ void __launch_bounds__(640, 1)
     for (int i = 0; i < P_NBAR; ++i) {
       uint32_t c = 1;
       if (i >= P_PF && i < P_PF + 4) c = 4;
-      if (i == P_OE || i == P_OE + 1) c = 8;
+      if (i == P_OE || i == P_OE + 1) c = 4;
       if (i == P_ITE || i == P_ITE + 1) c = ITEM_READERS;
       if (i >= P_KE && i < P_KE + 8) c = 2;  // the last product that reads the slot; the repair warp
       tc::mbar_init(&bars[i], c);
@@ -275,8 +274,8 @@ __global__ void __launch_bounds__(640, 1)
     *abort_flag = 0;
     tc::fence_barrier_init();
   }
-  if (warp == 17) tc::tmem_alloc(tmem_slot, 512);
-  if (warp == 16 && lane == 0) {
+  if (warp == 9) tc::tmem_alloc(tmem_slot, 512);
+  if (warp == 8 && lane == 0) {
     tc::prefetch_tmap(&tq);
     tc::prefetch_tmap(&tk);
     tc::prefetch_tmap(&tv);
@@ -306,17 +305,13 @@ __global__ void __launch_bounds__(640, 1)
   };
   Item m;
 
-  // registers: 640 x 96 at launch = 512 x 104 (softmax) + 128 x 64
-  if (warp < 16) {
+  // registers: 384 x 168 at launch = 256 x 208 (softmax) + 128 x 88
+  if (warp < 8) {
     // ---------------------------------------------------------------- softmax, output
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
-    const int t = warp >> 3, half = (warp >> 2) & 1, sw = warp & 3, r = sw * 32 + lane;
-    // this thread's 64 columns of its row's scores, its weights' place, its half of O's columns
-    const uint32_t scol = tc::taddr(tmem, sw * 32, C::S_COL + 128 * t + 64 * half);
-    const uint32_t ocol = tc::taddr(tmem, sw * 32, C::O_COL + 128 * t + D / 2 * half);
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    const int t = warp >> 2, sw = warp & 3, r = sw * 32 + lane;
+    const uint32_t scol = tc::taddr(tmem, sw * 32, C::S_COL + 128 * t), ocol = tc::taddr(tmem, sw * 32, C::O_COL + 128 * t);
     const int rtok = r / a.g, rhead = r % a.g;
-    float* xch = exch + t * 256 + r;  // [half][128] of this tile: row maxima, at the end row sums
-    const int pair_bar = 1 + t * 4 + sw;
     uint32_t ns = 0, no = 0;
     while (next_item(m)) {
       const int par = (itn - 1) & 3;
@@ -324,22 +319,22 @@ __global__ void __launch_bounds__(640, 1)
       const bool row_ok = rtok < a.ntok && tok < m.tok_end;
       const int lim = row_ok ? max(0, min(m.nk, i + m.shift)) : 0x3fffffff;  // keys that this row sees
       const int n = t ? m.n1 : m.n0;
-      float ms = 0.0f, mx = -INFINITY, lsum = 0.0f;  // running maximum (log2 domain), this half's sum
+      float ms = 0.0f, mx = -INFINITY, lsum = 0.0f;  // running maximum (log2 domain) and sum
       bool ok = true;
       for (int j = 0; j < n; ++j, ++ns) {
         if (!wait_all(P_SF + t, ns & 1, 409)) { ok = false; break; }
         tc::fence_after_sync();
-        uint32_t sv[2][32];
+        uint32_t sv[4][32];
 #pragma unroll
-        for (int q = 0; q < 2; ++q) tc::tmem_ld32(scol + 32 * q, sv[q]);
+        for (int q = 0; q < 4; ++q) tc::tmem_ld32(scol + 32 * q, sv[q]);
         tc::tmem_wait_ld();
 #pragma unroll
-        for (int q = 0; q < 2; ++q) tc::reg_after_wait(sv[q]);
-        const int vis = lim - j * BN - 64 * half;  // columns below this are seen
-        const bool whole = __all_sync(0xffffffffu, vis >= 64);
+        for (int q = 0; q < 4; ++q) tc::reg_after_wait(sv[q]);
+        const int vis = lim - j * BN;  // columns below this are seen
+        const bool whole = __all_sync(0xffffffffu, vis >= BN);
         if (!whole) {
 #pragma unroll
-          for (int q = 0; q < 2; ++q)
+          for (int q = 0; q < 4; ++q)
 #pragma unroll
             for (int e = 0; e < 32; ++e)
               if (32 * q + e >= vis) sv[q][e] = 0xff800000u;
@@ -347,19 +342,14 @@ __global__ void __launch_bounds__(640, 1)
         float m4[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const uint32_t* x = &sv[q >> 1][16 * (q & 1)];
-          m4[q] = max3(__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]));
+          m4[q] = max3(__uint_as_float(sv[q][0]), __uint_as_float(sv[q][1]), __uint_as_float(sv[q][2]));
 #pragma unroll
-          for (int e = 3; e < 15; e += 2) m4[q] = max3(m4[q], __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
-          m4[q] = max2(m4[q], __uint_as_float(x[15]));
+          for (int e = 3; e < 31; e += 2) m4[q] = max3(m4[q], __uint_as_float(sv[q][e]), __uint_as_float(sv[q][e + 1]));
+          m4[q] = max2(m4[q], __uint_as_float(sv[q][31]));
         }
-        float mt = max2(max2(m4[0], m4[1]), max2(m4[2], m4[3]));
-        // the other half's maximum (it has read the last tile's: S_FULL follows both halves' P_FULL)
-        xch[128 * half] = mt;
-        tc::bar_sync(pair_bar, 64);
         // a NaN or +infinite score makes the row NaN: through the maximum, since the polynomial
         // exponential does not carry one
-        mt = max2(mt, xch[128 * (half ^ 1)]) * a.sl;
+        float mt = max2(max2(m4[0], m4[1]), max2(m4[2], m4[3])) * a.sl;
         mt = mt < INFINITY ? mt : NAN;
         const bool need = !(mt <= mx + 8.0f);
         if (__any_sync(0xffffffffu, need)) {
@@ -370,7 +360,7 @@ __global__ void __launch_bounds__(640, 1)
           ms = mx == -INFINITY ? 0.0f : mx;
           if (j > 0) {  // S_FULL was committed behind the previous PV: O is complete
 #pragma unroll
-            for (int c0 = 0; c0 < D / 2; c0 += 16) {
+            for (int c0 = 0; c0 < D; c0 += 16) {
               uint32_t ov[16];
               tc::tmem_ld16(ocol + c0, ov);
               tc::tmem_wait_ld();
@@ -385,7 +375,7 @@ __global__ void __launch_bounds__(640, 1)
         uint64_t acc[2] = {0, 0};
         if (whole) {
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
+          for (int q = 0; q < 4; ++q) {
             uint32_t pk[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
@@ -400,11 +390,17 @@ __global__ void __launch_bounds__(640, 1)
               acc[e & 1] = add_f32x2(acc[e & 1], pack_f32x2(p.x, p.y));
               pk[e] = pack2<DT>(p.x, p.y);
             }
-            tc::tmem_st16(scol + 16 * q, pk);
+            tc::tmem_st16(scol + 64 * (q >> 1) + 16 * (q & 1), pk);
+            if (q & 1) {  // 64 keys' weights: their product can start
+              tc::tmem_wait_st();
+              tc::fence_before_sync();
+              __syncwarp();
+              if (lane == 0) tc::mbar_arrive(&bars[P_PF + 2 * t + (q >> 1)]);
+            }
           }
         } else {  // masked scores are -inf: exactly 0 by the hardware exponential
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
+          for (int q = 0; q < 4; ++q) {
             uint32_t pk[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
@@ -414,39 +410,37 @@ __global__ void __launch_bounds__(640, 1)
               acc[e & 1] = add_f32x2(acc[e & 1], pack_f32x2(p.x, p.y));
               pk[e] = pack2<DT>(p.x, p.y);
             }
-            tc::tmem_st16(scol + 16 * q, pk);
+            tc::tmem_st16(scol + 64 * (q >> 1) + 16 * (q & 1), pk);
+            if (q & 1) {  // 64 keys' weights: their product can start
+              tc::tmem_wait_st();
+              tc::fence_before_sync();
+              __syncwarp();
+              if (lane == 0) tc::mbar_arrive(&bars[P_PF + 2 * t + (q >> 1)]);
+            }
           }
         }
         const float2 s0 = unpack_f32x2(add_f32x2(acc[0], acc[1]));
         lsum += s0.x + s0.y;
-        tc::tmem_wait_st();
-        tc::fence_before_sync();
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&bars[P_PF + 2 * t + half]);
       }
       if (!ok) break;
       const int64_t row = (int64_t)tok * a.Hq + m.hk * a.g + rhead;
-      T* orow = static_cast<T*>(a.o) + row * D + D / 2 * half;
+      T* orow = static_cast<T*>(a.o) + row * D;
       if (n == 0) {  // no row of this tile sees a key
         if (row_ok) {
           const uint32_t zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-          for (int c0 = 0; c0 < D / 2; c0 += 16) store32(orow + c0, zero);
-          if (half == 0) a.lse[row] = -INFINITY;
+          for (int c0 = 0; c0 < D; c0 += 16) store32(orow + c0, zero);
+          a.lse[row] = -INFINITY;
         }
         continue;
       }
       if (!wait_all(P_OF + t, no & 1, 410)) break;
       ++no;
-      xch[128 * half] = lsum;  // the row's sum is both halves'
-      tc::bar_sync(pair_bar, 64);
-      lsum = __fadd_rn(xch[0], xch[128]);
-      tc::bar_sync(pair_bar, 64);
       tc::fence_after_sync();
       const bool bad = bad_v[par] != 0;
       const float inv = lim > 0 ? 1.0f / lsum : 0.0f;
 #pragma unroll
-      for (int c0 = 0; c0 < D / 2; c0 += 16) {
+      for (int c0 = 0; c0 < D; c0 += 16) {
         uint32_t ov[16];
         tc::tmem_ld16(ocol + c0, ov);
         tc::tmem_wait_ld();
@@ -457,7 +451,7 @@ __global__ void __launch_bounds__(640, 1)
           for (int e = 0; e < 16; ++e) f[e] = lim > 0 ? __uint_as_float(ov[e]) * inv : 0.0f;
           if (bad) {  // values taken out of the repaired tiles, for the rows that see them
             for (int k = m.jfix * BN; k < lim; ++k) {
-              const T* vr = static_cast<const T*>(a.v) + (int64_t)(m.k0 + k) * a.sv_t + m.hk * a.sv_h + D / 2 * half + c0;
+              const T* vr = static_cast<const T*>(a.v) + (int64_t)(m.k0 + k) * a.sv_t + m.hk * a.sv_h + c0;
 #pragma unroll
               for (int e = 0; e < 16; ++e) {
                 const float x = Elem<DT>::load(vr[e]);
@@ -471,14 +465,14 @@ __global__ void __launch_bounds__(640, 1)
           store32(orow + c0, w);
         }
       }
-      if (row_ok && half == 0) a.lse[row] = lim > 0 ? (mx + log2f(lsum)) * LN2 : -INFINITY;
+      if (row_ok) a.lse[row] = lim > 0 ? (mx + log2f(lsum)) * LN2 : -INFINITY;
       tc::fence_before_sync();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&bars[P_OE + t]);
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-    if (warp == 16) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == 8) {
       // ---------------------------------------------------------------- TMA
       uint32_t g = 0, nq[2] = {0, 0};
       const uint32_t qbytes = uint32_t(C::DB) * 128 * a.g * a.ntok;
@@ -518,7 +512,7 @@ __global__ void __launch_bounds__(640, 1)
         }
         __syncwarp();
       }
-    } else if (warp == 17) {
+    } else if (warp == 9) {
       // ---------------------------------------------------------------- MMA issue
       const uint32_t fmt = DT == MZB_BF16 ? 1 : 0;
       // a negative scale: the scores of -q (negate-A bit), so that larger is always more
@@ -605,7 +599,7 @@ __global__ void __launch_bounds__(640, 1)
         }
         __syncwarp();
       }
-    } else if (warp == 18) {
+    } else if (warp == 10) {
       // ---------------------------------------------------------------- scheduler
       Finder f;
       f.init(a, lane);
@@ -704,7 +698,7 @@ __global__ void __launch_bounds__(640, 1)
 
   tc::fence_before_sync();
   __syncthreads();
-  if (warp == 17) {
+  if (warp == 9) {
     tc::fence_after_sync();
     tc::tmem_free(tmem, 512);
   }
@@ -738,7 +732,7 @@ int launch(const void* q, const void* k, PrefillArgs a, int64_t sq_t, int64_t sq
   // at least as many pairs of query tiles as any packing of Tq tokens into B sequences has
   const int64_t pairs = a.Tq / (2 * a.ntok) + (a.B < a.Tq ? a.B : a.Tq);
   MZB_REQUIRE(pairs * a.Hkv < (int64_t(1) << 31), MZB_ERR_SHAPE, "gqa_prefill: too large");
-  kern<<<unsigned(pairs * a.Hkv), 640, C::SMEM, st>>>(m[0], m[1], m[2], a);
+  kern<<<unsigned(pairs * a.Hkv), 384, C::SMEM, st>>>(m[0], m[1], m[2], a);
   return launch_status("gqa_prefill");
 }
 
