@@ -37,8 +37,9 @@ struct PCfg {
   static constexpr int DB = (D + 63) / 64;  // 64-channel column blocks (D = 96: the last half is zero fill)
   static constexpr int Q_BYTES = DB * 128 * 128;
   static constexpr int SLOT = DB * BN * 128;
-  static constexpr int NS = DB == 1 ? 8 : 5;  // ring slots (K and V tiles alternate)
-  static constexpr int TILES = 2 * Q_BYTES + NS * SLOT;
+  static constexpr int NS = DB == 1 ? 8 : 4;  // ring slots (K and V tiles alternate)
+  static constexpr int STAGE = 2 * Q_BYTES + NS * SLOT;  // output staging: 4 KB for each softmax warp
+  static constexpr int TILES = STAGE + 8 * 4096;
   static constexpr int SMEM = TILES + 1024;
   static constexpr int S_COL = 0, O_COL = 256;  // tile t: + 128 t
   static_assert(SMEM <= 232448, "shared memory budget");
@@ -61,7 +62,7 @@ struct Item {
   int i0, shift;      // tok0's place in its sequence; keys seen by place i: min(nk, i + shift) (not causal: nk)
   int k0, nk, hk;     // first packed key, keys, K / V head
   int n0, n1;         // key tiles of the query tiles
-  int jfix;           // V tiles from here on reach past what some row sees
+  int lim0, jfix;     // keys that tok0 sees (the fewest); V tiles from jfix on reach past them
   int done;
 };
 
@@ -123,6 +124,13 @@ __device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
                : "memory");
 }
 
+// Bits 15 and 31: a half of w is NaN or infinite (the exponent's lowest bit carries into the
+// sign's place when all its bits are set).
+template <int DT>
+__device__ __forceinline__ uint32_t hot2(uint32_t w) {
+  constexpr uint32_t E = DT == MZB_BF16 ? 0x7f807f80u : 0x7c007c00u, L = DT == MZB_BF16 ? 0x00800080u : 0x04000400u;
+  return ((w & E) + L) & 0x80008000u;
+}
 // Bits set where a 16-bit half of w is NaN or infinite (exponent all ones).
 template <int DT>
 __device__ __forceinline__ uint32_t nonfinite2(uint32_t w) {
@@ -132,112 +140,86 @@ __device__ __forceinline__ uint32_t nonfinite2(uint32_t w) {
 
 // ---------------------------------------------------------------- work items
 
-// Query tile pairs of sequence b.
-__device__ __forceinline__ int pairs_of(const PrefillArgs& a, int b) {
-  if (b >= a.B) return 0;
-  const int n = a.cu_q[b + 1] - a.cu_q[b], span = 2 * a.ntok;
-  return n > 0 ? (n + span - 1) / span : 0;
-}
-
-__device__ __forceinline__ int warp_sum(int v) {
-#pragma unroll
-  for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-  return v;
-}
-__device__ __forceinline__ int warp_scan(int v, int lane) {  // inclusive
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, v, d);
-    if (lane >= d) v += y;
-  }
-  return v;
-}
-
-// Item number -> (sequence, pair within it), by the scheduler warp.  Up to LPT sequences: by
-// descending pair index over all sequences (longest causal key ranges first), each lane
-// keeping the pair counts of the sequences lane, lane + 32, ...; more: sequence after
-// sequence, the last pair first, from a cursor (a block's item numbers only grow).
+// Item number -> (sequence, pair within it), by the scheduler warp.  Up to 32 sequences (a lane
+// for each): by descending pair index over all sequences, so that the longest causal key ranges
+// come first and the last blocks' shares are even; more: sequence after sequence, the last pair
+// first, from a cursor (a block's item numbers only grow).
 struct Finder {
-  static constexpr int R = 8, LPT = 32 * R;
-  int n[R], top, cur_b, cur_at;
+  int n, q0, nq, k0, nk;  // this lane's sequence (of 32 from cur_b)
+  int top, total, cur_b, cur_at;
 
+  __device__ void load(const PrefillArgs& a, int lane) {
+    const int b = cur_b + lane;
+    n = 0;
+    if (b < a.B) {
+      const int q1 = a.cu_q[b + 1], ka = a.cu_k[b], kb = a.cu_k[b + 1];
+      q0 = a.cu_q[b];
+      nq = q1 - q0;
+      k0 = max(0, min(ka, int(a.Tk)));
+      nk = max(0, min(kb, int(a.Tk)) - k0);
+      n = nq > 0 ? (nq + 2 * a.ntok - 1) / (2 * a.ntok) : 0;
+    }
+    total = __reduce_add_sync(0xffffffffu, n);
+    top = __reduce_max_sync(0xffffffffu, n);
+  }
   __device__ void init(const PrefillArgs& a, int lane) {
-    top = 0;
     cur_b = cur_at = 0;
-    if (a.B > LPT) return;
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      n[i] = pairs_of(a, lane + 32 * i);
-      top = max(top, n[i]);
+    load(a, lane);
+  }
+  __device__ int above(int t) { return __reduce_add_sync(0xffffffffu, max(0, n - t)); }  // pairs with index >= t
+  // -> the lane of the sequence, or -1 behind the last item
+  __device__ int find(const PrefillArgs& a, int64_t idx, int lane, int& pair) {
+    while (idx >= cur_at + total) {
+      if (cur_b + 32 >= a.B) return -1;
+      cur_at += total;
+      cur_b += 32;
+      load(a, lane);
     }
+    const int r = int(idx) - cur_at;
+    if (a.B > 32) {
+      int inc = n;
 #pragma unroll
-    for (int d = 16; d; d >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
-  }
-  // pairs with index >= t
-  __device__ int above(int t) {
-    int s = 0;
-#pragma unroll
-    for (int i = 0; i < R; ++i) s += max(0, n[i] - t);
-    return warp_sum(s);
-  }
-  __device__ bool find(const PrefillArgs& a, int64_t r, int lane, int& b, int& pair) {
-    if (a.B > LPT) {
-      while (cur_b < a.B) {
-        const int c = pairs_of(a, cur_b + lane), inc = warp_scan(c, lane);
-        const unsigned hit = __ballot_sync(0xffffffffu, r < cur_at + inc);
-        if (hit) {
-          const int l = __ffs(hit) - 1;
-          b = cur_b + l;
-          pair = __shfl_sync(0xffffffffu, cur_at + inc, l) - 1 - int(r);
-          return true;
-        }
-        cur_at += __shfl_sync(0xffffffffu, inc, 31);
-        cur_b += 32;
+      for (int d = 1; d < 32; d <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, inc, d);
+        if (lane >= d) inc += y;
       }
-      return false;
+      const int l = __ffs(__ballot_sync(0xffffffffu, r < inc)) - 1;
+      pair = __shfl_sync(0xffffffffu, inc, l) - 1 - r;
+      return l;
     }
-    if (r >= above(0)) return false;
     int lo = 0, hi = top;  // above(lo) > r >= above(hi)
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (above(mid) > r) lo = mid; else hi = mid;
     }
-    int rank = int(r) - above(hi);
     pair = lo;
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const unsigned m = __ballot_sync(0xffffffffu, n[i] > lo);
-      const int c = __popc(m);
-      if (rank >= 0 && rank < c) b = 32 * i + __fns(m, 0, rank + 1);
-      rank -= c;
-    }
-    return true;
+    const int rank = r - above(hi);  // among the sequences that have this pair
+    const unsigned have = __ballot_sync(0xffffffffu, n > lo);
+    const bool mine = n > lo && __popc(have & ((1u << lane) - 1)) == rank;
+    return __ffs(__ballot_sync(0xffffffffu, mine)) - 1;
+  }
+  // by the sequence's lane
+  __device__ void fill(const PrefillArgs& a, int pair, int hk, Item* m) {
+    const int i0 = pair * 2 * a.ntok;
+    auto sees = [&](int i) { return a.causal ? max(0, min(nk, i + nk - nq + 1)) : nk; };
+    auto tiles = [&](int t) {
+      const int first = i0 + t * a.ntok, last = min(first + a.ntok, nq) - 1;
+      return last >= first ? (sees(last) + BN - 1) / BN : 0;
+    };
+    m->tok0 = q0 + i0;
+    m->tok_end = q0 + nq;
+    m->i0 = i0;
+    m->shift = a.causal ? nk - nq + 1 : 0x3fffffff;
+    m->k0 = k0;
+    m->nk = nk;
+    m->hk = hk;
+    m->n0 = tiles(0);
+    m->n1 = tiles(1);
+    m->lim0 = sees(i0);
+    m->jfix = m->lim0 / BN;
+    m->done = 0;
   }
 };
-
-__device__ __forceinline__ void fill_item(const PrefillArgs& a, int b, int pair, int hk, Item* m) {
-  const int q0 = a.cu_q[b], nq = a.cu_q[b + 1] - q0;
-  const int k0 = max(0, min(a.cu_k[b], int(a.Tk))), nk = max(0, min(a.cu_k[b + 1], int(a.Tk)) - k0);
-  const int i0 = pair * 2 * a.ntok;
-  m->tok0 = q0 + i0;
-  m->tok_end = q0 + nq;
-  m->i0 = i0;
-  m->shift = a.causal ? nk - nq + 1 : 0x3fffffff;
-  m->k0 = k0;
-  m->nk = nk;
-  m->hk = hk;
-  auto sees = [&](int i) { return a.causal ? max(0, min(nk, i + nk - nq + 1)) : nk; };
-  int n[2];
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const int first = i0 + t * a.ntok, last = min(first + a.ntok, nq) - 1;
-    n[t] = last >= first ? (sees(last) + BN - 1) / BN : 0;
-  }
-  m->n0 = n[0];
-  m->n1 = n[1];
-  m->jfix = sees(i0) / BN;  // the first token sees the fewest keys
-  m->done = 0;
-}
 
 // ---------------------------------------------------------------- kernel
 
@@ -322,7 +304,11 @@ __global__ void __launch_bounds__(384, 1)
       float ms = 0.0f, mx = -INFINITY, lsum = 0.0f;  // running maximum (log2 domain) and sum
       bool ok = true;
       for (int j = 0; j < n; ++j, ++ns) {
-        if (!wait_all(P_SF + t, ns & 1, 409)) { ok = false; break; }
+        if (!__all_sync(0xffffffffu, tc::mbar_wait(&bars[P_SF + t], ns & 1, a.err, 409))) {
+          *abort_flag = 1;
+          ok = false;
+          break;
+        }
         tc::fence_after_sync();
         uint32_t sv[4][32];
 #pragma unroll
@@ -334,10 +320,12 @@ __global__ void __launch_bounds__(384, 1)
         const bool whole = __all_sync(0xffffffffu, vis >= BN);
         if (!whole) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
+          for (int q = 0; q < 4; ++q) {
+            if (__all_sync(0xffffffffu, vis >= 32 * q + 32)) continue;
 #pragma unroll
             for (int e = 0; e < 32; ++e)
               if (32 * q + e >= vis) sv[q][e] = 0xff800000u;
+          }
         }
         float m4[4];
 #pragma unroll
@@ -381,7 +369,7 @@ __global__ void __launch_bounds__(384, 1)
             for (int e = 0; e < 16; ++e) {
               const uint64_t x = ffma_f32x2(pack_f32x2(__uint_as_float(sv[q][2 * e]), __uint_as_float(sv[q][2 * e + 1])), sl2, nm2);
               float2 p;
-              if (e % 4 == 3) {
+              if (e % 8 == 7) {  // one pair in eight on the FMA pipe: measured best of 0, 1/8, 1/4, 3/8, 1/2
                 p = poly_exp2(x);
               } else {
                 const float2 xf = unpack_f32x2(x);
@@ -439,31 +427,50 @@ __global__ void __launch_bounds__(384, 1)
       tc::fence_after_sync();
       const bool bad = bad_v[par] != 0;
       const float inv = lim > 0 ? 1.0f / lsum : 0.0f;
+      // through shared memory, so that a store covers whole 128-byte lines of a few rows (a thread
+      // storing its own row touches 32 lines an instruction: 4000 cycles an item instead of ~1000);
+      // 16-byte pieces of a row at its index mod 8, which keeps both directions free of conflicts
+      uint8_t* stage = smem + C::STAGE + warp * 4096;
+      const int64_t row_at = row_ok ? row : -1;
 #pragma unroll
-      for (int c0 = 0; c0 < D; c0 += 16) {
-        uint32_t ov[16];
-        tc::tmem_ld16(ocol + c0, ov);
-        tc::tmem_wait_ld();
-        tc::reg_after_wait(ov);
-        if (row_ok) {
-          float f[16];
+      for (int cb = 0; cb < C::DB; ++cb) {
+        constexpr int W0 = D < 64 ? D : 64;
+        const int W = cb == C::DB - 1 ? D - 64 * cb : W0;  // channels of this block (a constant)
+        const int CH = W / 8, RPI = 32 / CH;               // 16-byte pieces of a row, rows of a store
 #pragma unroll
-          for (int e = 0; e < 16; ++e) f[e] = lim > 0 ? __uint_as_float(ov[e]) * inv : 0.0f;
-          if (bad) {  // values taken out of the repaired tiles, for the rows that see them
+        for (int c0 = 0; c0 < W; c0 += 32) {
+          uint32_t ov[32];
+          tc::tmem_ld32(ocol + 64 * cb + c0, ov);
+          tc::tmem_wait_ld();
+          tc::reg_after_wait(ov);
+          float f[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) f[e] = lim > 0 ? __uint_as_float(ov[e]) * inv : 0.0f;
+          if (bad && row_ok) {  // values taken out of the repaired tiles, for the rows that see them
             for (int k = m.jfix * BN; k < lim; ++k) {
-              const T* vr = static_cast<const T*>(a.v) + (int64_t)(m.k0 + k) * a.sv_t + m.hk * a.sv_h + c0;
+              const T* vr = static_cast<const T*>(a.v) + (int64_t)(m.k0 + k) * a.sv_t + m.hk * a.sv_h + 64 * cb + c0;
 #pragma unroll
-              for (int e = 0; e < 16; ++e) {
+              for (int e = 0; e < 32; ++e) {
                 const float x = Elem<DT>::load(vr[e]);
                 if (!isfinite(x)) f[e] += x;
               }
             }
           }
-          uint32_t w[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) w[e] = pack2<DT>(f[2 * e], f[2 * e + 1]);
-          store32(orow + c0, w);
+          for (int c = 0; c < 4; ++c)
+            *reinterpret_cast<uint4*>(stage + lane * 128 + (((c0 / 8 + c) ^ (lane & 7)) * 16)) =
+                make_uint4(pack2<DT>(f[8 * c], f[8 * c + 1]), pack2<DT>(f[8 * c + 2], f[8 * c + 3]),
+                           pack2<DT>(f[8 * c + 4], f[8 * c + 5]), pack2<DT>(f[8 * c + 6], f[8 * c + 7]));
         }
+        __syncwarp();
+#pragma unroll
+        for (int i8 = 0; i8 < CH; ++i8) {
+          const int rr = i8 * RPI + lane / CH, c = lane % CH;
+          const int64_t at = __shfl_sync(0xffffffffu, row_at, rr);
+          const uint4 x = *reinterpret_cast<const uint4*>(stage + rr * 128 + ((c ^ (rr & 7)) * 16));
+          if (at >= 0) *reinterpret_cast<uint4*>(static_cast<T*>(a.o) + at * D + 64 * cb + 8 * c) = x;
+        }
+        __syncwarp();
       }
       if (row_ok) a.lse[row] = lim > 0 ? (mx + log2f(lsum)) * LN2 : -INFINITY;
       tc::fence_before_sync();
@@ -608,13 +615,13 @@ __global__ void __launch_bounds__(384, 1)
       uint32_t tries = 0;
       bool more = true;
       while (more) {
-        int b = 0, pair = 0;
-        const bool real = f.find(a, idx / a.Hkv, lane, b, pair);
-        if (real) {
+        int pair = 0;
+        const int who = f.find(a, idx / a.Hkv, lane, pair);
+        if (who >= 0) {
           const int s = k & 1;
           if (!wait_all(P_ITE + s, ((k >> 1) & 1) ^ 1, 411)) break;
-          if (lane == 0) {
-            fill_item(a, b, pair, int(idx % a.Hkv), &items[s]);
+          if (lane == who) {
+            f.fill(a, pair, int(idx % a.Hkv), &items[s]);
             tc::mbar_arrive(&bars[P_ITF + s]);
           }
           if (!wait_all(P_ASK, k & 1, 415)) break;
@@ -667,20 +674,26 @@ __global__ void __launch_bounds__(384, 1)
             if (lane == 0) tc::mbar_arrive(&bars[P_KE + s]);
             continue;
           }
-          uint8_t* tile = ring + s * C::SLOT;
-          for (int x0 = 0; x0 < C::SLOT / 16; x0 += 32 * 8) {
+          // rows from the first one that the first token does not see; behind the last key of the
+          // packed tensor the copy has filled in zeros
+          const int r0 = max(0, m.lim0 - (f >> 1) * BN), r1 = min(BN, int(a.Tk) - m.k0 - (f >> 1) * BN);
+          uint8_t* tile = ring + s * C::SLOT + (lane & 7) * 16;
+          for (int x0 = r0 * C::DB + (lane >> 3); x0 < r1 * C::DB; x0 += 4 * 8) {
             uint4 w[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = *reinterpret_cast<const uint4*>(tile + (x0 + 32 * e + lane) * 16);
+            uint32_t off[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              const uint4 z = make_uint4(nonfinite2<DT>(w[e].x), nonfinite2<DT>(w[e].y), nonfinite2<DT>(w[e].z),
-                                         nonfinite2<DT>(w[e].w));
-              if (z.x | z.y | z.z | z.w) {
-                *reinterpret_cast<uint4*>(tile + (x0 + 32 * e + lane) * 16) =
-                    make_uint4(w[e].x & ~z.x, w[e].y & ~z.y, w[e].z & ~z.z, w[e].w & ~z.w);
-                found = 1;
-              }
+              const int x = min(x0 + 4 * e, r1 * C::DB - 1);
+              off[e] = (x % C::DB) * (BN * 128) + (x / C::DB) * 128;
+              w[e] = *reinterpret_cast<const uint4*>(tile + off[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              if (!(hot2<DT>(w[e].x) | hot2<DT>(w[e].y) | hot2<DT>(w[e].z) | hot2<DT>(w[e].w))) continue;
+              *reinterpret_cast<uint4*>(tile + off[e]) =
+                  make_uint4(w[e].x & ~nonfinite2<DT>(w[e].x), w[e].y & ~nonfinite2<DT>(w[e].y),
+                             w[e].z & ~nonfinite2<DT>(w[e].z), w[e].w & ~nonfinite2<DT>(w[e].w));
+              found = 1;
             }
           }
           found = __any_sync(0xffffffffu, found);
