@@ -87,12 +87,18 @@ __device__ __forceinline__ float max2(float a, float b) {
   return d;
 }
 
-// 2^x of a pair for x in [-126, 126] on the FMA pipe: x = n + f with f in [-1/2, 1/2] (adding
-// 1.5 2^23 rounds to nearest), 2^f by the degree-4 polynomial of least maximal relative error
-// (2.6e-6, found by Remez exchange), n added to the exponent field.
+__device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+// 2^x of a pair on the FMA pipe, 0 for x <= -127 (a masked -inf): x = n + f with f in
+// [-1/2, 1/2] (adding 1.5 2^23 rounds to nearest), 2^f by the degree-4 polynomial of least
+// maximal relative error (2.6e-6, found by Remez exchange), times 2^n built in the exponent field.
 __device__ __forceinline__ float2 poly_exp2(uint64_t x2) {
   const float2 xc = unpack_f32x2(x2);
-  const uint64_t x = pack_f32x2(fmaxf(xc.x, -126.0f), fmaxf(xc.y, -126.0f));
+  const uint64_t x = pack_f32x2(fmaxf(xc.x, -127.0f), fmaxf(xc.y, -127.0f));
   const uint64_t t = add_f32x2(x, pack_f32x2(12582912.0f, 12582912.0f));
   const uint64_t r = add_f32x2(t, pack_f32x2(-12582912.0f, -12582912.0f));
   const uint64_t f = ffma_f32x2(r, pack_f32x2(-1.0f, -1.0f), x);
@@ -101,9 +107,9 @@ __device__ __forceinline__ float2 poly_exp2(uint64_t x2) {
   p = ffma_f32x2(p, f, pack_f32x2(2.402474483e-01f, 2.402474483e-01f));
   p = ffma_f32x2(p, f, pack_f32x2(6.931218147e-01f, 6.931218147e-01f));
   p = ffma_f32x2(p, f, pack_f32x2(9.999992614e-01f, 9.999992614e-01f));
-  const float2 tn = unpack_f32x2(t), pf = unpack_f32x2(p);
-  return make_float2(__uint_as_float(__float_as_uint(pf.x) + (__float_as_uint(tn.x) << 23)),
-                     __uint_as_float(__float_as_uint(pf.y) + (__float_as_uint(tn.y) << 23)));
+  const float2 tn = unpack_f32x2(t);
+  return unpack_f32x2(mul_f32x2(p, pack_f32x2(__uint_as_float((__float_as_uint(tn.x) << 23) + 0x3f800000u),
+                                              __uint_as_float((__float_as_uint(tn.y) << 23) + 0x3f800000u))));
 }
 
 template <int DT>
@@ -115,13 +121,6 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     const __half2 v = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&v);
   }
-}
-
-// 32 bytes of one row, one whole sector per thread (rows are 32-byte aligned: D / 2 elements are).
-__device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
-  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
-               "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-               : "memory");
 }
 
 // Bits 15 and 31: a half of w is NaN or infinite (the exponent's lowest bit carries into the
@@ -310,23 +309,30 @@ __global__ void __launch_bounds__(384, 1)
           break;
         }
         tc::fence_after_sync();
+        const int vis = lim - j * BN;  // columns below this are seen
+        if (!__all_sync(0xffffffffu, vis >= BN)) {
+          // masked scores to -inf where they lie (a rolled loop: tiles like this are few, and long
+          // unrolled code that runs once an item is fetched anew each time)
+#pragma unroll 1
+          for (int c0 = 0; c0 < BN; c0 += 32) {
+            if (__all_sync(0xffffffffu, vis >= c0 + 32)) continue;
+            uint32_t x[32];
+            tc::tmem_ld32(scol + c0, x);
+            tc::tmem_wait_ld();
+            tc::reg_after_wait(x);
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (e >= vis - c0) x[e] = 0xff800000u;
+            tc::tmem_st32(scol + c0, x);
+          }
+          tc::tmem_wait_st();
+        }
         uint32_t sv[4][32];
 #pragma unroll
         for (int q = 0; q < 4; ++q) tc::tmem_ld32(scol + 32 * q, sv[q]);
         tc::tmem_wait_ld();
 #pragma unroll
         for (int q = 0; q < 4; ++q) tc::reg_after_wait(sv[q]);
-        const int vis = lim - j * BN;  // columns below this are seen
-        const bool whole = __all_sync(0xffffffffu, vis >= BN);
-        if (!whole) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            if (__all_sync(0xffffffffu, vis >= 32 * q + 32)) continue;
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (32 * q + e >= vis) sv[q][e] = 0xff800000u;
-          }
-        }
         float m4[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -347,64 +353,42 @@ __global__ void __launch_bounds__(384, 1)
           lsum *= alpha;
           ms = mx == -INFINITY ? 0.0f : mx;
           if (j > 0) {  // S_FULL was committed behind the previous PV: O is complete
-#pragma unroll
-            for (int c0 = 0; c0 < D; c0 += 16) {
-              uint32_t ov[16];
-              tc::tmem_ld16(ocol + c0, ov);
+#pragma unroll 1
+            for (int c0 = 0; c0 < D; c0 += 32) {
+              uint32_t ov[32];
+              tc::tmem_ld32(ocol + c0, ov);
               tc::tmem_wait_ld();
               tc::reg_after_wait(ov);
 #pragma unroll
-              for (int e = 0; e < 16; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * alpha);
-              tc::tmem_st16(ocol + c0, ov);
+              for (int e = 0; e < 32; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * alpha);
+              tc::tmem_st32(ocol + c0, ov);
             }
           }
         }
         const uint64_t sl2 = pack_f32x2(a.sl, a.sl), nm2 = pack_f32x2(-ms, -ms);
         uint64_t acc[2] = {0, 0};
-        if (whole) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint32_t pk[16];
+        for (int q = 0; q < 4; ++q) {
+          uint32_t pk[16];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const uint64_t x = ffma_f32x2(pack_f32x2(__uint_as_float(sv[q][2 * e]), __uint_as_float(sv[q][2 * e + 1])), sl2, nm2);
-              float2 p;
-              if (e % 8 == 7) {  // one pair in eight on the FMA pipe: measured best of 0, 1/8, 1/4, 3/8, 1/2
-                p = poly_exp2(x);
-              } else {
-                const float2 xf = unpack_f32x2(x);
-                p = make_float2(fast_exp2(xf.x), fast_exp2(xf.y));
-              }
-              acc[e & 1] = add_f32x2(acc[e & 1], pack_f32x2(p.x, p.y));
-              pk[e] = pack2<DT>(p.x, p.y);
+          for (int e = 0; e < 16; ++e) {
+            const uint64_t x = ffma_f32x2(pack_f32x2(__uint_as_float(sv[q][2 * e]), __uint_as_float(sv[q][2 * e + 1])), sl2, nm2);
+            float2 p;
+            if (e % 8 == 7) {  // one pair in eight on the FMA pipe: measured best of 0, 1/8, 1/4, 3/8, 1/2
+              p = poly_exp2(x);
+            } else {
+              const float2 xf = unpack_f32x2(x);
+              p = make_float2(fast_exp2(xf.x), fast_exp2(xf.y));
             }
-            tc::tmem_st16(scol + 64 * (q >> 1) + 16 * (q & 1), pk);
-            if (q & 1) {  // 64 keys' weights: their product can start
-              tc::tmem_wait_st();
-              tc::fence_before_sync();
-              __syncwarp();
-              if (lane == 0) tc::mbar_arrive(&bars[P_PF + 2 * t + (q >> 1)]);
-            }
+            acc[e & 1] = add_f32x2(acc[e & 1], pack_f32x2(p.x, p.y));
+            pk[e] = pack2<DT>(p.x, p.y);
           }
-        } else {  // masked scores are -inf: exactly 0 by the hardware exponential
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const float2 xf = unpack_f32x2(
-                  ffma_f32x2(pack_f32x2(__uint_as_float(sv[q][2 * e]), __uint_as_float(sv[q][2 * e + 1])), sl2, nm2));
-              const float2 p = make_float2(fast_exp2(xf.x), fast_exp2(xf.y));
-              acc[e & 1] = add_f32x2(acc[e & 1], pack_f32x2(p.x, p.y));
-              pk[e] = pack2<DT>(p.x, p.y);
-            }
-            tc::tmem_st16(scol + 64 * (q >> 1) + 16 * (q & 1), pk);
-            if (q & 1) {  // 64 keys' weights: their product can start
-              tc::tmem_wait_st();
-              tc::fence_before_sync();
-              __syncwarp();
-              if (lane == 0) tc::mbar_arrive(&bars[P_PF + 2 * t + (q >> 1)]);
-            }
+          tc::tmem_st16(scol + 64 * (q >> 1) + 16 * (q & 1), pk);
+          if (q & 1) {  // 64 keys' weights: their product can start
+            tc::tmem_wait_st();
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&bars[P_PF + 2 * t + (q >> 1)]);
           }
         }
         const float2 s0 = unpack_f32x2(add_f32x2(acc[0], acc[1]));
@@ -412,12 +396,11 @@ __global__ void __launch_bounds__(384, 1)
       }
       if (!ok) break;
       const int64_t row = (int64_t)tok * a.Hq + m.hk * a.g + rhead;
-      T* orow = static_cast<T*>(a.o) + row * D;
       if (n == 0) {  // no row of this tile sees a key
         if (row_ok) {
-          const uint32_t zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll
-          for (int c0 = 0; c0 < D; c0 += 16) store32(orow + c0, zero);
+          uint4* mine = reinterpret_cast<uint4*>(static_cast<T*>(a.o) + row * D);
+#pragma unroll 1
+          for (int c = 0; c < D / 8; ++c) mine[c] = make_uint4(0, 0, 0, 0);
           a.lse[row] = -INFINITY;
         }
         continue;
@@ -427,50 +410,50 @@ __global__ void __launch_bounds__(384, 1)
       tc::fence_after_sync();
       const bool bad = bad_v[par] != 0;
       const float inv = lim > 0 ? 1.0f / lsum : 0.0f;
-      // through shared memory, so that a store covers whole 128-byte lines of a few rows (a thread
-      // storing its own row touches 32 lines an instruction: 4000 cycles an item instead of ~1000);
-      // 16-byte pieces of a row at its index mod 8, which keeps both directions free of conflicts
+      // through shared memory, 32 channels at a time, so that a store covers 64 bytes of each of eight
+      // rows (a thread storing its own row touches 32 lines an instruction: ~4000 cycles an item);
+      // the 16-byte pieces of a row at its place mod 8 keep both directions free of conflicts
       uint8_t* stage = smem + C::STAGE + warp * 4096;
-      const int64_t row_at = row_ok ? row : -1;
+      T* orow[4];  // this lane's rows of the four stores of a block: 8 i + lane / 4
 #pragma unroll
-      for (int cb = 0; cb < C::DB; ++cb) {
-        constexpr int W0 = D < 64 ? D : 64;
-        const int W = cb == C::DB - 1 ? D - 64 * cb : W0;  // channels of this block (a constant)
-        const int CH = W / 8, RPI = 32 / CH;               // 16-byte pieces of a row, rows of a store
+      for (int i4 = 0; i4 < 4; ++i4) {
+        const int64_t at = __shfl_sync(0xffffffffu, row_ok ? row : -1, 8 * i4 + (lane >> 2));
+        orow[i4] = at < 0 ? nullptr : static_cast<T*>(a.o) + at * D + 8 * (lane & 3);
+      }
+#pragma unroll 1
+      for (int c0 = 0; c0 < D; c0 += 32) {
+        uint32_t ov[32];
+        tc::tmem_ld32(ocol + c0, ov);
+        tc::tmem_wait_ld();
+        tc::reg_after_wait(ov);
 #pragma unroll
-        for (int c0 = 0; c0 < W; c0 += 32) {
-          uint32_t ov[32];
-          tc::tmem_ld32(ocol + 64 * cb + c0, ov);
-          tc::tmem_wait_ld();
-          tc::reg_after_wait(ov);
-          float f[32];
+        for (int e = 0; e < 32; ++e) ov[e] = lim > 0 ? __float_as_uint(__uint_as_float(ov[e]) * inv) : 0u;
 #pragma unroll
-          for (int e = 0; e < 32; ++e) f[e] = lim > 0 ? __uint_as_float(ov[e]) * inv : 0.0f;
-          if (bad && row_ok) {  // values taken out of the repaired tiles, for the rows that see them
-            for (int k = m.jfix * BN; k < lim; ++k) {
-              const T* vr = static_cast<const T*>(a.v) + (int64_t)(m.k0 + k) * a.sv_t + m.hk * a.sv_h + 64 * cb + c0;
+        for (int c = 0; c < 4; ++c) {
+          const uint32_t* x = &ov[8 * c];
+          auto f2 = [&](int e) { return pack2<DT>(__uint_as_float(x[e]), __uint_as_float(x[e + 1])); };
+          *reinterpret_cast<uint4*>(stage + lane * 64 + ((c ^ ((lane >> 1) & 3)) * 16)) = make_uint4(f2(0), f2(2), f2(4), f2(6));
+        }
+        __syncwarp();
 #pragma unroll
-              for (int e = 0; e < 32; ++e) {
-                const float x = Elem<DT>::load(vr[e]);
-                if (!isfinite(x)) f[e] += x;
-              }
-            }
+        for (int i4 = 0; i4 < 4; ++i4) {
+          const int rr = 8 * i4 + (lane >> 2);
+          const uint4 x = *reinterpret_cast<const uint4*>(stage + rr * 64 + (((lane & 3) ^ ((rr >> 1) & 3)) * 16));
+          if (orow[i4]) *reinterpret_cast<uint4*>(orow[i4] + c0) = x;
+        }
+        __syncwarp();
+      }
+      if (bad && row_ok) {  // values taken out of the repaired tiles, for the rows that see them
+        T* mine = static_cast<T*>(a.o) + row * D;
+#pragma unroll 1
+        for (int k = m.jfix * BN; k < lim; ++k) {
+          const T* vr = static_cast<const T*>(a.v) + (int64_t)(m.k0 + k) * a.sv_t + m.hk * a.sv_h;
+#pragma unroll 1
+          for (int e = 0; e < D; ++e) {
+            const float x = Elem<DT>::load(vr[e]);
+            if (!isfinite(x)) mine[e] = Elem<DT>::store(Elem<DT>::load(mine[e]) + x);
           }
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-            *reinterpret_cast<uint4*>(stage + lane * 128 + (((c0 / 8 + c) ^ (lane & 7)) * 16)) =
-                make_uint4(pack2<DT>(f[8 * c], f[8 * c + 1]), pack2<DT>(f[8 * c + 2], f[8 * c + 3]),
-                           pack2<DT>(f[8 * c + 4], f[8 * c + 5]), pack2<DT>(f[8 * c + 6], f[8 * c + 7]));
         }
-        __syncwarp();
-#pragma unroll
-        for (int i8 = 0; i8 < CH; ++i8) {
-          const int rr = i8 * RPI + lane / CH, c = lane % CH;
-          const int64_t at = __shfl_sync(0xffffffffu, row_at, rr);
-          const uint4 x = *reinterpret_cast<const uint4*>(stage + rr * 128 + ((c ^ (rr & 7)) * 16));
-          if (at >= 0) *reinterpret_cast<uint4*>(static_cast<T*>(a.o) + at * D + 64 * cb + 8 * c) = x;
-        }
-        __syncwarp();
       }
       if (row_ok) a.lse[row] = lim > 0 ? (mx + log2f(lsum)) * LN2 : -INFINITY;
       tc::fence_before_sync();
@@ -765,7 +748,7 @@ extern "C" int mzb_gqa_prefill(const void* q, const void* k, const void* v, cons
   MZB_REQUIRE(D == 64 || D == 96 || D == 128, MZB_ERR_UNSUPPORTED, "gqa_prefill: unsupported head dim %d", D);
   MZB_REQUIRE(dtype == MZB_BF16 || dtype == MZB_F16, MZB_ERR_UNSUPPORTED, "gqa_prefill: unsupported dtype %d", dtype);
   MZB_REQUIRE(err != nullptr, MZB_ERR_SHAPE, "gqa_prefill: needs an error word");
-  MZB_REQUIRE(reinterpret_cast<uintptr_t>(o) % 32 == 0, MZB_ERR_ALIGN, "gqa_prefill: o must be 32-byte aligned");
+  MZB_REQUIRE(reinterpret_cast<uintptr_t>(o) % 16 == 0, MZB_ERR_ALIGN, "gqa_prefill: o must be 16-byte aligned");
   if (Tq == 0) return MZB_OK;
   gqa::PrefillArgs a{};
   a.v = v; a.cu_q = cu_q; a.cu_k = cu_k; a.o = o; a.lse = lse;
