@@ -123,12 +123,17 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   }
 }
 
-// Bits 15 and 31: a half of w is NaN or infinite (the exponent's lowest bit carries into the
-// sign's place when all its bits are set).
+// Larger magnitude of the halves of m and w; a NaN passes through.
 template <int DT>
-__device__ __forceinline__ uint32_t hot2(uint32_t w) {
-  constexpr uint32_t E = DT == MZB_BF16 ? 0x7f807f80u : 0x7c007c00u, L = DT == MZB_BF16 ? 0x00800080u : 0x04000400u;
-  return ((w & E) + L) & 0x80008000u;
+__device__ __forceinline__ uint32_t maxabs2(uint32_t m, uint32_t w) {
+  if constexpr (DT == MZB_BF16) {
+    const __nv_bfloat162 r = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&m),
+                                         __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w)));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  } else {
+    const __half2 r = __hmax2_nan(*reinterpret_cast<const __half2*>(&m), __habs2(*reinterpret_cast<const __half2*>(&w)));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
 }
 // Bits set where a 16-bit half of w is NaN or infinite (exponent all ones).
 template <int DT>
@@ -409,7 +414,7 @@ __global__ void __launch_bounds__(384, 1)
       ++no;
       tc::fence_after_sync();
       const bool bad = bad_v[par] != 0;
-      const float inv = lim > 0 ? 1.0f / lsum : 0.0f;
+      const float inv = lim > 0 ? 1.0f / lsum : 0.0f;  // a row without keys in a tile with some: O is 0
       // through shared memory, 32 channels at a time, so that a store covers 64 bytes of each of eight
       // rows (a thread storing its own row touches 32 lines an instruction: ~4000 cycles an item);
       // the 16-byte pieces of a row at its place mod 8 keep both directions free of conflicts
@@ -420,27 +425,43 @@ __global__ void __launch_bounds__(384, 1)
         const int64_t at = __shfl_sync(0xffffffffu, row_ok ? row : -1, 8 * i4 + (lane >> 2));
         orow[i4] = at < 0 ? nullptr : static_cast<T*>(a.o) + at * D + 8 * (lane & 3);
       }
+      uint8_t* st_at = stage + lane * 64;
+      const uint8_t* ld_at = stage + (lane >> 2) * 64 + (((lane & 3) ^ ((lane >> 3) & 3)) * 16);
+      const uint64_t inv2 = pack_f32x2(inv, inv);
+      constexpr int CB = D % 64 ? 1 : 2;  // blocks of 32 channels in flight
 #pragma unroll 1
-      for (int c0 = 0; c0 < D; c0 += 32) {
-        uint32_t ov[32];
-        tc::tmem_ld32(ocol + c0, ov);
+      for (int c0 = 0; c0 < D; c0 += 32 * CB) {
+        uint32_t ov[CB][32];
+#pragma unroll
+        for (int b = 0; b < CB; ++b) tc::tmem_ld32(ocol + c0 + 32 * b, ov[b]);
         tc::tmem_wait_ld();
-        tc::reg_after_wait(ov);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) ov[e] = lim > 0 ? __float_as_uint(__uint_as_float(ov[e]) * inv) : 0u;
+        for (int b = 0; b < CB; ++b) {
+          tc::reg_after_wait(ov[b]);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const uint32_t* x = &ov[8 * c];
-          auto f2 = [&](int e) { return pack2<DT>(__uint_as_float(x[e]), __uint_as_float(x[e + 1])); };
-          *reinterpret_cast<uint4*>(stage + lane * 64 + ((c ^ ((lane >> 1) & 3)) * 16)) = make_uint4(f2(0), f2(2), f2(4), f2(6));
+          for (int c = 0; c < 4; ++c) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 x = unpack_f32x2(mul_f32x2(
+                  pack_f32x2(__uint_as_float(ov[b][8 * c + 2 * e]), __uint_as_float(ov[b][8 * c + 2 * e + 1])), inv2));
+              w[e] = pack2<DT>(x.x, x.y);
+            }
+            *reinterpret_cast<uint4*>(st_at + 2048 * b + ((c ^ ((lane >> 1) & 3)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
         }
         __syncwarp();
+        uint4 x[CB][4];
 #pragma unroll
-        for (int i4 = 0; i4 < 4; ++i4) {
-          const int rr = 8 * i4 + (lane >> 2);
-          const uint4 x = *reinterpret_cast<const uint4*>(stage + rr * 64 + (((lane & 3) ^ ((rr >> 1) & 3)) * 16));
-          if (orow[i4]) *reinterpret_cast<uint4*>(orow[i4] + c0) = x;
-        }
+        for (int b = 0; b < CB; ++b)
+#pragma unroll
+          for (int i4 = 0; i4 < 4; ++i4) x[b][i4] = *reinterpret_cast<const uint4*>(ld_at + 2048 * b + 512 * i4);
+#pragma unroll
+        for (int i4 = 0; i4 < 4; ++i4)
+          if (orow[i4]) {
+#pragma unroll
+            for (int b = 0; b < CB; ++b) *reinterpret_cast<uint4*>(orow[i4] + c0 + 32 * b) = x[b][i4];
+          }
         __syncwarp();
       }
       if (bad && row_ok) {  // values taken out of the repaired tiles, for the rows that see them
@@ -661,25 +682,29 @@ __global__ void __launch_bounds__(384, 1)
           // packed tensor the copy has filled in zeros
           const int r0 = max(0, m.lim0 - (f >> 1) * BN), r1 = min(BN, int(a.Tk) - m.k0 - (f >> 1) * BN);
           uint8_t* tile = ring + s * C::SLOT + (lane & 7) * 16;
-          for (int x0 = r0 * C::DB + (lane >> 3); x0 < r1 * C::DB; x0 += 4 * 8) {
+          const int x1 = r1 * C::DB;  // 128-byte row pieces, four a step
+          uint32_t top = 0;           // largest magnitudes of this lane's halves; NaN passes
+#pragma unroll 1
+          for (int x0 = r0 * C::DB + (lane >> 3); x0 < x1; x0 += 4 * 8) {
             uint4 w[8];
-            uint32_t off[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              const int x = min(x0 + 4 * e, r1 * C::DB - 1);
-              off[e] = (x % C::DB) * (BN * 128) + (x / C::DB) * 128;
-              w[e] = *reinterpret_cast<const uint4*>(tile + off[e]);
+              const int x = min(x0 + 4 * e, x1 - 1);
+              w[e] = *reinterpret_cast<const uint4*>(tile + (x % C::DB) * (BN * 128) + (x / C::DB) * 128);
             }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              if (!(hot2<DT>(w[e].x) | hot2<DT>(w[e].y) | hot2<DT>(w[e].z) | hot2<DT>(w[e].w))) continue;
-              *reinterpret_cast<uint4*>(tile + off[e]) =
-                  make_uint4(w[e].x & ~nonfinite2<DT>(w[e].x), w[e].y & ~nonfinite2<DT>(w[e].y),
-                             w[e].z & ~nonfinite2<DT>(w[e].z), w[e].w & ~nonfinite2<DT>(w[e].w));
-              found = 1;
+            for (int e = 0; e < 8; ++e) top = maxabs2<DT>(maxabs2<DT>(maxabs2<DT>(maxabs2<DT>(top, w[e].x), w[e].y), w[e].z), w[e].w);
+          }
+          if (__any_sync(0xffffffffu, nonfinite2<DT>(top) != 0)) {
+            found = 1;
+#pragma unroll 1
+            for (int x = r0 * C::DB + (lane >> 3); x < x1; x += 4) {
+              uint4* at = reinterpret_cast<uint4*>(tile + (x % C::DB) * (BN * 128) + (x / C::DB) * 128);
+              const uint4 w = *at;
+              *at = make_uint4(w.x & ~nonfinite2<DT>(w.x), w.y & ~nonfinite2<DT>(w.y), w.z & ~nonfinite2<DT>(w.z),
+                               w.w & ~nonfinite2<DT>(w.w));
             }
           }
-          found = __any_sync(0xffffffffu, found);
           if (found && lane == 0) bad_v[par] = 1;
           tc::fence_async_smem();
           __syncwarp();
