@@ -4,93 +4,553 @@
 //   key t < len[b] of sequence b is slot t % page of page table[b, t / page];
 //   o = softmax(scale q K^T) V; a sequence of length 0: o = 0, lse = -inf.
 //
-// One block of 8 warps per (sequence, head): the warps share the keys and are joined.
-#include "common.cuh"
+// The live part of the cache is read once and everything else is small, so the kernel is
+// built to keep HBM busy.  The keys of every (sequence, K / V head) are cut into tiles of 64,
+// the tiles of all of them form one list, and each of one block per SM takes an equal run of
+// it, whatever the lengths: a warp walks the page tables and feeds a ring of shared-memory
+// stages (K and V of one tile each, ~200 KB in flight per SM) by TMA, eight warps do the
+// products.  The query heads of a group are the 16 rows of mma.sync tiles (the tensor work is
+// ~20 % of the time that the bytes take, so larger tensor instructions would gain nothing): a
+// group of up to 16 heads is split over the keys by 4 x 2 warps, a larger one over head tiles.
+// A (sequence, head) that lies in several blocks' runs leaves its (maximum, sum, output) parts in
+// a workspace; a second kernel, started early and waiting, joins them in a fixed order.
+#include "tc.cuh"
 
 namespace mzb {
-namespace gqa {
+namespace gqad {
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
+constexpr int TK = 64;         // keys per tile
+constexpr int MIN_TILES = 4;   // a block's run is at least this long
+constexpr int MAX_BLOCKS = 160;
+constexpr int MAX_STAGES = 12;
 
 struct DecodeArgs {
-  const void *q, *k, *v;
+  const void* q;
   const int32_t *table, *lens;
   void* o;
   float* lse;
-  int64_t P, sq_b, sq_h, sk_p, sk_h, sk_t, sv_p, sv_h, sv_t;
-  int B, Hq, Hkv, W, page;
-  float scale;
+  float* ws;
+  int64_t P, sq_b, sq_h;
+  int B, Hq, Hkv, g, W, page, stages, blocks;  // blocks 0: one block per (sequence, head), no parts
+  float sl;                                    // scale * log2 e
+  int* err;
 };
 
-template <int DT, int D>
-__global__ void __launch_bounds__(256) decode_kernel(DecodeArgs a) {
-  using E = Elem<DT>;
-  using T = typename E::T;
-  constexpr int C = D / 32;
-  __shared__ float sm[8], sl[8], so[8][D];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int b = blockIdx.x / a.Hq, h = blockIdx.x % a.Hq, hk = h / (a.Hq / a.Hkv);
-  const int64_t n = max((int64_t)0, min((int64_t)a.lens[b], (int64_t)a.W * a.page));
-  float qv[C], acc[C];
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    qv[c] = E::load(static_cast<const T*>(a.q)[b * a.sq_b + h * a.sq_h + lane + 32 * c]);
-    acc[c] = 0.0f;
+// ws: int2 [B * Hkv] (first, last block of a (sequence, head); -1: empty), then for each of
+// 2 * MAX_BLOCKS parts: float2 [g] (maximum, sum), float [g][D].
+__device__ __forceinline__ int2* ws_span(const DecodeArgs& a) { return reinterpret_cast<int2*>(a.ws); }
+__device__ __forceinline__ float* ws_part(const DecodeArgs& a, int part, int D) {
+  const int64_t head = ((int64_t)a.B * a.Hkv * 2 + 3) & ~int64_t(3);
+  return a.ws + head + (int64_t)part * a.g * (D + 2);
+}
+
+// What the loading warp tells the computing ones about a stage.
+struct Meta {
+  int b, hk, keys, flags;  // keys of the tile that exist; FIRST / LAST tile of the block's segment
+  int part;                // -1: the segment is the whole (sequence, head), else its part number
+};
+constexpr int FIRST = 1, LAST = 2, END = 4;
+
+template <int D>
+struct DCfg {
+  static constexpr int DB = (D + 63) / 64;
+  static constexpr int K_BYTES = DB * TK * 128;
+  static constexpr int STAGE = 2 * K_BYTES;
+};
+
+template <int DT>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (DT == MZB_BF16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <bool TRANS>
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  if constexpr (TRANS)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+  else
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (DT == MZB_BF16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
   }
-  float m = -INFINITY, l = 0.0f;
-  for (int64_t j = warp; j < n; j += 8) {
-    const int64_t p = min(max((int64_t)a.table[(int64_t)b * a.W + j / a.page], (int64_t)0), a.P - 1), r = j % a.page;
-    const T* kr = static_cast<const T*>(a.k) + p * a.sk_p + hk * a.sk_h + r * a.sk_t;
-    const T* vr = static_cast<const T*>(a.v) + p * a.sv_p + hk * a.sv_h + r * a.sv_t;
-    float s = 0.0f;
-#pragma unroll
-    for (int c = 0; c < C; ++c) s += qv[c] * E::load(kr[lane + 32 * c]);
-#pragma unroll
-    for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-    s *= a.scale * LOG2E;
-    const float mn = fmaxf(m, s), ms = mn == -INFINITY ? 0.0f : mn;
-    const float al = exp2f(m - ms), pr = exp2f(s - ms);
-    l = l * al + pr;
-#pragma unroll
-    for (int c = 0; c < C; ++c) acc[c] = acc[c] * al + pr * E::load(vr[lane + 32 * c]);
-    m = mn;
+}
+template <int DT>
+__device__ __forceinline__ float2 unpack2(uint32_t v) {
+  if constexpr (DT == MZB_BF16) return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
+  else return __half22float2(*reinterpret_cast<const __half2*>(&v));
+}
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+
+__device__ __forceinline__ int len_of(const DecodeArgs& a, int b) { return max(0, min(a.lens[b], a.W * a.page)); }
+
+// MT: head tiles of 16.  Warps: MT 1: tiles alternate between two groups of four warps, each warp 16 keys;
+// MT > 1: warp = head tile x key part, each part TK / (8 / MT) keys of every tile.
+template <int DT, int D, int MT>
+__global__ void __launch_bounds__(288, 1)
+    decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                  const __grid_constant__ DecodeArgs a) {
+  using C = DCfg<D>;
+  using T = typename Elem<DT>::T;
+  constexpr int KP = MT == 1 ? 4 : 8 / MT;  // warps that share a tile's keys
+  constexpr int STEPS = TK / KP / 16;       // 16-key steps of a warp per tile
+  constexpr int PARTS = 8 / MT;             // partial results of a head tile to merge
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ uint64_t full[MAX_STAGES], empty[MAX_STAGES];
+  __shared__ Meta meta[MAX_STAGES];
+  __shared__ float sm_m[8][16], sm_l[8][16];
+  __shared__ int abort_s;
+  volatile int* abort_flag = &abort_s;
+  float* merge = reinterpret_cast<float*>(smem + a.stages * C::STAGE);  // [8 warps][min(g, 16)][D]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (smem_u32(smem) & 1023) {
+    if (threadIdx.x == 0) atomicExch(a.err, MZB_ERR_ALIGN);
+    return;
   }
-  if (lane == 0) { sm[warp] = m; sl[warp] = l; }
-#pragma unroll
-  for (int c = 0; c < C; ++c) so[warp][lane + 32 * c] = acc[c];
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < a.stages; ++i) {
+      tc::mbar_init(&full[i], 1);
+      tc::mbar_init(&empty[i], 8);  // every warp lets every stage go, so none is lapped by the ring
+    }
+    abort_s = 0;
+    tc::fence_barrier_init();
+  }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   __syncthreads();
-  if (warp) return;
-  float mt = -INFINITY, lt = 0.0f;
-  for (int w = 0; w < 8; ++w) mt = fmaxf(mt, sm[w]);
-  const float ms = mt == -INFINITY ? 0.0f : mt;
+
+  if (warp == 8) {
+    // ---------------------------------------------------------------- loads
+    if (lane == 0) {
+      tc::prefetch_tmap(&tk);
+      tc::prefetch_tmap(&tv);
+    }
+    // this block's run of tiles: first (sequence, head, tile) and how many
+    int b = 0, hk = 0, t0 = 0;
+    int64_t left = 0;
+    if (a.blocks == 0) {
+      b = blockIdx.x / a.Hkv;
+      hk = blockIdx.x % a.Hkv;
+      left = (len_of(a, b) + TK - 1) / TK;
+    } else {
+      int64_t total = 0;
+      for (int b0 = 0; b0 < a.B; b0 += 32) {
+        int64_t n = b0 + lane < a.B ? (len_of(a, b0 + lane) + TK - 1) / TK : 0;
 #pragma unroll
-  for (int c = 0; c < C; ++c) acc[c] = 0.0f;
-  for (int w = 0; w < 8; ++w) {
-    const float al = exp2f(sm[w] - ms);
-    lt += sl[w] * al;
+        for (int d = 16; d; d >>= 1) n += __shfl_xor_sync(0xffffffffu, n, d);
+        total += n;
+      }
+      total *= a.Hkv;
+      const int64_t per = max((int64_t)MIN_TILES, (total + a.blocks - 1) / a.blocks), lo = per * blockIdx.x;
+      left = min(per, total - lo);
+      if (left > 0) {
+        int64_t at = 0;
+        for (int b0 = 0;; b0 += 32) {
+          const int64_t n = b0 + lane < a.B ? (int64_t)((len_of(a, b0 + lane) + TK - 1) / TK) * a.Hkv : 0;
+          int64_t inc = n;
 #pragma unroll
-    for (int c = 0; c < C; ++c) acc[c] += so[w][lane + 32 * c] * al;
+          for (int d = 1; d < 32; d <<= 1) {
+            const int64_t y = __shfl_up_sync(0xffffffffu, inc, d);
+            if (lane >= d) inc += y;
+          }
+          const unsigned hit = __ballot_sync(0xffffffffu, lo < at + inc);
+          if (hit) {
+            const int l = __ffs(hit) - 1;
+            b = b0 + l;
+            const int64_t in = lo - at - __shfl_sync(0xffffffffu, inc - n, l);
+            const int64_t tiles = __shfl_sync(0xffffffffu, n, l) / a.Hkv;
+            hk = int(in / tiles);
+            t0 = int(in % tiles);
+            break;
+          }
+          at += __shfl_sync(0xffffffffu, inc, 31);
+        }
+      }
+    }
+    const int rows = min(a.page, TK);            // rows of a TMA box
+    const int per_tile = TK / rows;              // boxes of a tile (per K / V and column block)
+    uint32_t g = 0;
+    bool ok = true;
+    while (left > 0 && ok) {
+      const int len = len_of(a, b), tiles = (len + TK - 1) / TK;
+      const int n = int(min((int64_t)(tiles - t0), left));  // this block's segment: tiles t0 .. t0 + n
+      const bool begins = t0 == 0, ends = t0 + n == tiles;
+      const int part = begins && ends ? -1 : begins ? 2 * (int)blockIdx.x + 1 : 2 * (int)blockIdx.x;
+      if (lane == 0 && a.blocks) {
+        int2* span = &ws_span(a)[(int64_t)b * a.Hkv + hk];
+        if (begins) span->x = blockIdx.x;
+        if (ends) span->y = blockIdx.x;
+      }
+      // page ids of 32 boxes at a time, one per lane, the next ones in flight meanwhile
+      const int32_t* row = a.table + (int64_t)b * a.W;
+      const int box0 = t0 * per_tile, boxes = (len + rows - 1) / rows;  // boxes with live keys
+      auto ids = [&](int x) {  // box x of the sequence
+        int p = 0;
+        if (x < boxes) p = row[(int64_t)x * rows / a.page];
+        return max(0, min(p, int(a.P - 1)));
+      };
+      int cur = ids(box0 + lane), nxt = ids(box0 + 32 + lane), base = box0;
+      for (int i = 0; i < n; ++i, ++g) {
+        const int t = t0 + i, keys = min(TK, len - t * TK), live = (keys + rows - 1) / rows;
+        const uint32_t s = g % a.stages;
+        if ((t * per_tile) - base >= 32) {
+          base += 32;
+          cur = nxt;
+          nxt = ids(base + 32 + lane);
+        }
+        const bool got = !*abort_flag && tc::mbar_wait(&empty[s], ((g / a.stages) & 1) ^ 1, a.err, 421);
+        if (!__all_sync(0xffffffffu, got)) { ok = false; break; }
+        if (lane == 0) {
+          meta[s] = Meta{b, hk, keys, (i == 0 ? FIRST : 0) | (i == n - 1 ? LAST : 0), part};
+          tc::mbar_expect_tx(&full[s], uint32_t(live) * rows * 128 * C::DB * 2);
+        }
+        __syncwarp();
+        // copy x of the tile: box x / (2 DB), K or V, column block
+        {
+          const int x = lane, box = x / (2 * C::DB), kv = (x / C::DB) & 1, cb = x % C::DB;
+          static_assert((TK / 16) * 2 * C::DB <= 32, "a lane for each copy");
+          const int pid = __shfl_sync(0xffffffffu, cur, min((t * per_tile + box) - base, 31));
+          if (box < live)
+            tma_load_4d(smem + s * C::STAGE + kv * C::K_BYTES + cb * TK * 128 + box * rows * 128, kv ? &tv : &tk, &full[s],
+                        cb * 64, (t * TK + box * rows) % a.page, hk, pid);
+        }
+        __syncwarp();
+      }
+      left -= n;
+      t0 = 0;
+      if (++hk == a.Hkv) {
+        hk = 0;
+        ++b;
+        while (left > 0 && len_of(a, b) == 0) ++b;
+      }
+    }
+    // the end, as a stage without data
+    const uint32_t s = g % a.stages;
+    const bool got = ok && !*abort_flag && tc::mbar_wait(&empty[s], ((g / a.stages) & 1) ^ 1, a.err, 422);
+    if (__all_sync(0xffffffffu, got)) {
+      if (lane == 0) {
+        meta[s].flags = END;
+        tc::mbar_arrive(&full[s]);
+      }
+    } else {
+      *abort_flag = 1;
+    }
+  } else {
+    // ---------------------------------------------------------------- products
+    // sequences without keys
+    if (a.blocks) {
+      for (int b = blockIdx.x; b < a.B; b += gridDim.x)
+        if (a.lens[b] <= 0 || a.W == 0) {
+          for (int x = threadIdx.x; x < a.Hq * D / 8; x += 256)
+            reinterpret_cast<uint4*>(static_cast<T*>(a.o) + (int64_t)b * a.Hq * D)[x] = make_uint4(0, 0, 0, 0);
+          for (int x = threadIdx.x; x < a.Hq; x += 256) a.lse[(int64_t)b * a.Hq + x] = -INFINITY;
+          for (int x = threadIdx.x; x < a.Hkv; x += 256) ws_span(a)[(int64_t)b * a.Hkv + x] = make_int2(-1, -1);
+        }
+    } else if (len_of(a, blockIdx.x / a.Hkv) == 0) {
+      const int64_t row = (int64_t)(blockIdx.x / a.Hkv) * a.Hq + blockIdx.x % a.Hkv * a.g;
+      for (int x = threadIdx.x; x < a.g * D / 8; x += 256)
+        reinterpret_cast<uint4*>(static_cast<T*>(a.o) + row * D)[x] = make_uint4(0, 0, 0, 0);
+      for (int x = threadIdx.x; x < a.g; x += 256) a.lse[row + x] = -INFINITY;
+    }
+    const int mt = MT == 1 ? 0 : warp % MT, kp = MT == 1 ? (warp & 3) : warp / MT, grp = MT == 1 ? warp >> 2 : 0;
+    const int r0 = lane >> 2, c0 = (lane & 3) * 2;
+    uint32_t qf[D / 16][4];
+    float o[D / 8][4], m[2], l[2];
+    auto clear = [&]() {
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][e] = 0.0f;
+      m[0] = m[1] = -INFINITY;
+      l[0] = l[1] = 0.0f;
+    };
+    clear();
+    // ldmatrix rows of this lane: K: matrices (keys 0-7, 8-15) x (channels 0-7, 8-15) as (b0, b1) of two key
+    // blocks; V transposed: (keys 0-7, 8-15) x (channels 0-7, 8-15) as (b0, b1) of two channel blocks
+    const int krow = (lane & 7) + ((lane >> 4) << 3), kch = (lane >> 3) & 1;
+    const int vrow = lane & 15, vch = lane >> 4;
+    for (uint32_t g = 0;; ++g) {
+      const uint32_t s = g % a.stages;
+      const bool got = !*abort_flag && tc::mbar_wait(&full[s], (g / a.stages) & 1, a.err, 423);
+      if (!__all_sync(0xffffffffu, got)) {
+        *abort_flag = 1;
+        break;
+      }
+      const Meta w = meta[s];
+      if (w.flags & END) break;
+      if (w.flags & FIRST) {  // this group's query rows
+        const T* q = static_cast<const T*>(a.q) + (int64_t)w.b * a.sq_b;
+        auto ld = [&](int row, int ch) {
+          const int h = mt * 16 + row;
+          return h < a.g ? *reinterpret_cast<const uint32_t*>(q + (int64_t)(w.hk * a.g + h) * a.sq_h + ch) : 0u;
+        };
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          qf[kk][0] = ld(r0, 16 * kk + c0);
+          qf[kk][1] = ld(r0 + 8, 16 * kk + c0);
+          qf[kk][2] = ld(r0, 16 * kk + c0 + 8);
+          qf[kk][3] = ld(r0 + 8, 16 * kk + c0 + 8);
+        }
+      }
+      if (MT > 1 || (g & 1) == grp) {
+        const uint32_t kt = smem_u32(smem + s * C::STAGE), vt = kt + C::K_BYTES;
+#pragma unroll 1
+        for (int st = 0; st < STEPS; ++st) {
+          const int key0 = (kp * STEPS + st) * 16;
+          if (key0 >= w.keys) break;
+          float sc[2][4] = {};
+          const int kr = key0 + krow;
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            uint32_t bk[4];
+            const int ch = 2 * kk + kch;  // 16-byte piece
+            ldsm4<false>(bk, kt + (ch >> 3) * (TK * 128) + kr * 128 + (((ch & 7) ^ (kr & 7)) * 16));
+            mma16816<DT>(sc[0], qf[kk], bk[0], bk[1]);
+            mma16816<DT>(sc[1], qf[kk], bk[2], bk[3]);
+          }
+          const int vis = w.keys - key0;  // keys of these 16 that exist
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              sc[n][e] *= a.sl;
+              if (8 * n + c0 + (e & 1) >= vis) sc[n][e] = -INFINITY;
+            }
+          float mt2[2];
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            float x = fmaxf(fmaxf(sc[0][2 * r], sc[0][2 * r + 1]), fmaxf(sc[1][2 * r], sc[1][2 * r + 1]));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+            mt2[r] = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+          }
+          // O and the sums are rescaled only when a maximum has grown by more than 2^8
+          if (__any_sync(0xffffffffu, mt2[0] > m[0] + 8.0f || mt2[1] > m[1] + 8.0f)) {
+            float al[2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const float mn = fmaxf(m[r], mt2[r]);
+              al[r] = mn == -INFINITY ? 1.0f : fast_exp2(m[r] - mn);
+              m[r] = mn;
+              l[r] *= al[r];
+            }
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[i][e] *= al[e >> 1];
+          }
+          const float ms[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
+          float p[2][4];
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              p[n][e] = fast_exp2(sc[n][e] - ms[e >> 1]);
+              l[e >> 1] += p[n][e];
+            }
+          // the weights as a sum of two numbers of the type (16 bits and more): the products have room
+          uint32_t ph[4], pl[4];
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const uint32_t h2 = pack2<DT>(p[n][2 * r], p[n][2 * r + 1]);
+              const float2 f = unpack2<DT>(h2);
+              ph[2 * n + r] = h2;
+              pl[2 * n + r] = pack2<DT>(p[n][2 * r] - f.x, p[n][2 * r + 1] - f.y);
+            }
+          const bool tail = vis < 16;
+          const uint32_t k01 = tail ? (c0 < vis ? 0xffffu : 0u) | (c0 + 1 < vis ? 0xffff0000u : 0u) : ~0u;
+          const uint32_t k89 = tail ? (c0 + 8 < vis ? 0xffffu : 0u) | (c0 + 9 < vis ? 0xffff0000u : 0u) : ~0u;
+          const int vr = key0 + vrow;
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
+            uint32_t bv[4];
+            const int ch = 2 * i + vch;
+            ldsm4<true>(bv, vt + (ch >> 3) * (TK * 128) + vr * 128 + (((ch & 7) ^ (vr & 7)) * 16));
+            if (tail) {  // what lies behind the sequence's end must not meet its zero weights
+              bv[0] &= k01;
+              bv[1] &= k89;
+              bv[2] &= k01;
+              bv[3] &= k89;
+            }
+            mma16816<DT>(o[2 * i], ph, bv[0], bv[1]);
+            mma16816<DT>(o[2 * i + 1], ph, bv[2], bv[3]);
+            mma16816<DT>(o[2 * i], pl, bv[0], bv[1]);
+            mma16816<DT>(o[2 * i + 1], pl, bv[2], bv[3]);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&empty[s]);
+      if (w.flags & LAST) {
+        // ------------------------------------------------------------ merge the warps' results
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+          l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+        }
+        const int gr = min(a.g, 16);
+        if ((lane & 3) == 0) {
+          sm_m[warp][r0] = m[0];
+          sm_m[warp][r0 + 8] = m[1];
+          sm_l[warp][r0] = l[0];
+          sm_l[warp][r0 + 8] = l[1];
+        }
+        float* mine = merge + warp * gr * D;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          if (r0 < gr) *reinterpret_cast<float2*>(mine + r0 * D + 8 * i + c0) = make_float2(o[i][0], o[i][1]);
+          if (r0 + 8 < gr) *reinterpret_cast<float2*>(mine + (r0 + 8) * D + 8 * i + c0) = make_float2(o[i][2], o[i][3]);
+        }
+        tc::bar_sync(1, 256);
+        for (int x = threadIdx.x; x < a.g * (D / 2); x += 256) {
+          const int h = x / (D / 2), d = (x % (D / 2)) * 2, tile = h >> 4, r = h & 15;
+          float mx = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < PARTS; ++i) mx = fmaxf(mx, sm_m[MT == 1 ? i : i * MT + tile][r]);
+          const float ms = mx == -INFINITY ? 0.0f : mx;
+          float ls = 0.0f;
+          float2 acc = make_float2(0.0f, 0.0f);
+#pragma unroll
+          for (int i = 0; i < PARTS; ++i) {
+            const int wp = MT == 1 ? i : i * MT + tile;
+            const float al = fast_exp2(sm_m[wp][r] - ms);
+            const float2 v = *reinterpret_cast<const float2*>(merge + (wp * gr + r) * D + d);
+            ls += sm_l[wp][r] * al;
+            acc.x += v.x * al;
+            acc.y += v.y * al;
+          }
+          if (w.part < 0) {
+            const int64_t row = (int64_t)w.b * a.Hq + w.hk * a.g + h;
+            const float inv = 1.0f / ls;
+            *reinterpret_cast<uint32_t*>(static_cast<T*>(a.o) + row * D + d) = pack2<DT>(acc.x * inv, acc.y * inv);
+            if (d == 0) a.lse[row] = (mx + log2f(ls)) * LN2;
+          } else {
+            float* to = ws_part(a, w.part, D);
+            *reinterpret_cast<float2*>(to + 2 * a.g + h * D + d) = acc;
+            if (d == 0) *reinterpret_cast<float2*>(to + 2 * h) = make_float2(mx, ls);
+          }
+        }
+        tc::bar_sync(1, 256);
+        clear();
+      }
+    }
   }
-  const float inv = n > 0 ? 1.0f / lt : 0.0f;
-  const int64_t row = (int64_t)b * a.Hq + h;
-#pragma unroll
-  for (int c = 0; c < C; ++c) static_cast<T*>(a.o)[row * D + lane + 32 * c] = E::store(acc[c] * inv);
-  if (lane == 0) a.lse[row] = n > 0 ? (mt + log2f(lt)) * LN2 : -INFINITY;
 }
 
+// One warp per (sequence, query head) that lies in several blocks' runs.
 template <int DT, int D>
-int launch(const DecodeArgs& a, cudaStream_t st) {
-  decode_kernel<DT, D><<<unsigned(a.B) * a.Hq, 256, 0, st>>>(a);
-  return launch_status("gqa_decode");
+__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ DecodeArgs a) {
+  using T = typename Elem<DT>::T;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (row >= (int64_t)a.B * a.Hq) return;
+  const int64_t b = row / a.Hq;
+  const int hq = int(row % a.Hq), hk = hq / a.g, h = hq % a.g;
+  const int2 span = ws_span(a)[b * a.Hkv + hk];
+  if (span.x == span.y) return;
+  auto part = [&](int c) { return ws_part(a, c == span.x ? 2 * c + 1 : 2 * c, D); };
+  float mx = -INFINITY;
+  for (int c = span.x + lane; c <= span.y; c += 32) mx = fmaxf(mx, part(c)[2 * h]);
+#pragma unroll
+  for (int d = 16; d; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+  const float ms = mx == -INFINITY ? 0.0f : mx;
+  float ls = 0.0f, acc[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) acc[i] = 0.0f;
+#pragma unroll 4
+  for (int c = span.x; c <= span.y; ++c) {
+    const float* p = part(c);
+    const float2 ml = *reinterpret_cast<const float2*>(p + 2 * h);
+    const float al = fast_exp2(ml.x - ms);
+    ls += ml.y * al;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) acc[i] += p[2 * a.g + h * D + lane + 32 * i] * al;
+  }
+  const float inv = 1.0f / ls;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) static_cast<T*>(a.o)[row * D + lane + 32 * i] = Elem<DT>::store(acc[i] * inv);
+  if (lane == 0) a.lse[row] = (mx + log2f(ls)) * LN2;
 }
 
-}  // namespace gqa
+int block_count() { return num_sms() < MAX_BLOCKS ? num_sms() : MAX_BLOCKS; }
+
+// Tables of at most MIN_TILES tiles: one block per (sequence, head), nothing to join.
+bool short_table(int W, int page) { return (int64_t)W * page <= MIN_TILES * TK; }
+
+template <int DT, int D, int MT>
+int launch(const void* k, const void* v, DecodeArgs a, const int64_t* sk, const int64_t* sv, cudaStream_t st) {
+  using C = DCfg<D>;
+  CUtensorMap m[2];
+  for (int i = 0; i < 2; ++i) {
+    const int64_t* s = i ? sv : sk;  // page, head, token
+    const uint64_t dims[4] = {uint64_t(D), uint64_t(a.page), uint64_t(a.Hkv), uint64_t(a.P)};
+    // the stride of a dimension of size 1 is never used: any legal one
+    const uint64_t str[3] = {uint64_t(s[2]) * 2, a.Hkv > 1 ? uint64_t(s[1]) * 2 : uint64_t(D) * 2,
+                             a.P > 1 ? uint64_t(s[0]) * 2 : uint64_t(D) * 2};
+    const uint32_t box[4] = {64, uint32_t(a.page < TK ? a.page : TK), 1, 1};
+    if (int r = encode_tmap(&m[i], DT == MZB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                            i ? v : k, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B))
+      return r;
+  }
+  const int merge = 8 * (a.g < 16 ? a.g : 16) * D * 4;
+  const int budget = 227 * 1024 - 4096 - merge;
+  a.stages = budget / C::STAGE < MAX_STAGES ? budget / C::STAGE : MAX_STAGES;
+  a.blocks = short_table(a.W, a.page) ? 0 : block_count();
+  auto kern = decode_kernel<DT, D, MT>;
+  const int smem = a.stages * C::STAGE + merge;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return launch_status("gqa_decode(smem attr)");
+  kern<<<a.blocks ? a.blocks : a.B * a.Hkv, 288, smem, st>>>(m[0], m[1], a);
+  if (int r = launch_status("gqa_decode")) return r;
+  if (!a.blocks) return MZB_OK;
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(unsigned(((int64_t)a.B * a.Hq + 3) / 4));
+  cfg.blockDim = dim3(128);
+  cfg.stream = st;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, join_kernel<DT, D>, a);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    set_error("gqa_decode(join): launch failed: %s", cudaGetErrorString(e));
+    return MZB_ERR_LAUNCH;
+  }
+  return MZB_OK;
+}
+
+}  // namespace gqad
 }  // namespace mzb
 
 using namespace mzb;
 
-extern "C" int64_t mzb_gqa_decode_ws(int B, int Hq, int Hkv, int D, int W, int page) { return 0; }
+extern "C" int64_t mzb_gqa_decode_ws(int B, int Hq, int Hkv, int D, int W, int page) {
+  if (B <= 0 || Hkv <= 0 || Hq <= 0 || gqad::short_table(W, page)) return 0;
+  return (((int64_t)B * Hkv * 2 + 3) & ~int64_t(3)) + 2 * (int64_t)gqad::block_count() * (Hq / Hkv) * (D + 2);
+}
 
 extern "C" int mzb_gqa_decode(const void* q, const void* k_pages, const void* v_pages, const int32_t* page_table,
                               const int32_t* seq_lens, void* o, float* lse, float* ws, int B, int Hq, int Hkv, int D,
@@ -99,20 +559,30 @@ extern "C" int mzb_gqa_decode(const void* q, const void* k_pages, const void* v_
                               float softmax_scale, int* err, void* stream) {
   MZB_REQUIRE(B >= 0 && P >= 1 && P < (int64_t(1) << 31) && W >= 0 && (int64_t)W * page < (int64_t(1) << 31),
               MZB_ERR_SHAPE, "gqa_decode: bad sizes B=%d pages=%lld table width=%d page=%d", B, (long long)P, W, page);
-  MZB_REQUIRE(Hkv >= 1 && Hq >= 1 && Hq % Hkv == 0 && Hq / Hkv <= 128, MZB_ERR_SHAPE,
+  MZB_REQUIRE(Hkv >= 1 && Hq >= 1 && Hq % Hkv == 0 && Hq / Hkv <= 128 && (int64_t)B * Hq < (int64_t(1) << 31), MZB_ERR_SHAPE,
               "gqa_decode: query heads must be a multiple (at most 128) of the K/V heads, got %d and %d", Hq, Hkv);
   MZB_REQUIRE(D == 64 || D == 96 || D == 128, MZB_ERR_UNSUPPORTED, "gqa_decode: unsupported head dim %d", D);
   MZB_REQUIRE(page == 16 || page == 32 || page == 64 || page == 128, MZB_ERR_UNSUPPORTED,
               "gqa_decode: unsupported page size %d (16, 32, 64 or 128 tokens)", page);
   MZB_REQUIRE(dtype == MZB_BF16 || dtype == MZB_F16, MZB_ERR_UNSUPPORTED, "gqa_decode: unsupported dtype %d", dtype);
   MZB_REQUIRE(err != nullptr, MZB_ERR_SHAPE, "gqa_decode: needs an error word");
+  MZB_REQUIRE(reinterpret_cast<uintptr_t>(q) % 4 == 0 && reinterpret_cast<uintptr_t>(o) % 16 == 0 && sq_b % 2 == 0 && sq_h % 2 == 0,
+              MZB_ERR_ALIGN, "gqa_decode: q rows must be 4-byte and o 16-byte aligned");
   if (B == 0) return MZB_OK;
-  gqa::DecodeArgs a{q, k_pages, v_pages, page_table, seq_lens, o, lse, P, sq_b, sq_h, sk_p, sk_h, sk_t, sv_p, sv_h,
-                    sv_t, B, Hq, Hkv, W, page, softmax_scale};
+  gqad::DecodeArgs a{};
+  a.q = q; a.table = page_table; a.lens = seq_lens; a.o = o; a.lse = lse; a.ws = ws;
+  a.P = P; a.sq_b = sq_b; a.sq_h = sq_h;
+  a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.g = Hq / Hkv; a.W = W; a.page = page;
+  a.sl = softmax_scale * gqad::LOG2E;
+  a.err = err;
+  const int64_t sk[3] = {sk_p, sk_h, sk_t}, sv[3] = {sv_p, sv_h, sv_t};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == MZB_BF16)
-    return D == 64 ? gqa::launch<MZB_BF16, 64>(a, st) : D == 96 ? gqa::launch<MZB_BF16, 96>(a, st)
-                                                                : gqa::launch<MZB_BF16, 128>(a, st);
-  return D == 64 ? gqa::launch<MZB_F16, 64>(a, st) : D == 96 ? gqa::launch<MZB_F16, 96>(a, st)
-                                                             : gqa::launch<MZB_F16, 128>(a, st);
+#define MZB_GO(DT, DD)                                                                              \
+  (a.g <= 16 ? gqad::launch<DT, DD, 1>(k_pages, v_pages, a, sk, sv, st)                             \
+   : a.g <= 32 ? gqad::launch<DT, DD, 2>(k_pages, v_pages, a, sk, sv, st)                           \
+   : a.g <= 64 ? gqad::launch<DT, DD, 4>(k_pages, v_pages, a, sk, sv, st)                           \
+               : gqad::launch<DT, DD, 8>(k_pages, v_pages, a, sk, sv, st))
+  if (dtype == MZB_BF16) return D == 64 ? MZB_GO(MZB_BF16, 64) : D == 96 ? MZB_GO(MZB_BF16, 96) : MZB_GO(MZB_BF16, 128);
+  return D == 64 ? MZB_GO(MZB_F16, 64) : D == 96 ? MZB_GO(MZB_F16, 96) : MZB_GO(MZB_F16, 128);
+#undef MZB_GO
 }
