@@ -298,7 +298,7 @@ MZB_API int mzb_gqa_decode(const void* q, const void* k_pages, const void* v_pag
  * int32 [S], refs int32 [P] (tables that name the page; 0 = free).  What cannot be done is left
  * out and sets *err = MZB_ERR_PAGES; new pages are the lowest free ids.
  * mzb_kv_append  -- row i of sequence b (rows cu[b] .. cu[b+1]; cu NULL: row b) of k, v goes to
- *   position starts[b] + i.  strides: 10 byte strides: k token, head; v token, head; k_pages page,
+ *   position starts[b] + i.  strides: 10 element strides: k token, head; v token, head; k_pages page,
  *   head, token; v_pages page, head, token.  Rows of row_bytes (a multiple of 16) bytes.
  * mzb_kv_reserve -- sequence b grows by n_new[b] tokens (all or none): pages are taken in
  *   (sequence, position) order, seq_lens is raised, starts[b] is the old length.  ws: P ints.
@@ -316,7 +316,8 @@ MZB_API int mzb_gqa_decode(const void* q, const void* k_pages, const void* v_pag
  */
 MZB_API int mzb_kv_append(const void* k, const void* v, void* k_pages, void* v_pages, const int32_t* page_table,
                           const int32_t* starts, const int32_t* cu, int64_t T, int B, int Hkv, int row_bytes,
-                          int page, int64_t P, int W, const int64_t* strides, int* err, void* stream);
+                          int page, int64_t P, int W, int elem_bytes, const int64_t* strides, int* err,
+                          void* stream);
 MZB_API int mzb_kv_reserve(int32_t* page_table, int32_t* seq_lens, int32_t* refs, const int32_t* n_new,
                            int32_t* starts, int32_t* ws, int B, int W, int64_t P, int page, int* err, void* stream);
 MZB_API int mzb_kv_free(int32_t* page_table, int32_t* seq_lens, int32_t* refs, const int32_t* seqs, int64_t n,

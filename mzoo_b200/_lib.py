@@ -66,7 +66,7 @@ SIGNATURES = {
     "mzb_gqa_decode_ws": [_I32, _I32, _I32, _I32, _I32, _I32],
     "mzb_gqa_decode": [_P, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _I64, _I32, _I64, _I64,
                        _I64, _I64, _I64, _I64, _I64, _I64, _F32, _P, _P],
-    "mzb_kv_append": [_P, _P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _I64, _I32, _P, _P, _P],
+    "mzb_kv_append": [_P, _P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _I64, _I32, _I32, _P, _P, _P],
     "mzb_kv_reserve": [_P, _P, _P, _P, _P, _P, _I32, _I32, _I64, _I32, _P, _P],
     "mzb_kv_free": [_P, _P, _P, _P, _I64, _I64, _I32, _I64, _P, _P],
     "mzb_kv_fork": [_P, _P, _P, _P, _P, _I32, _P, _I64, _I32, _I64, _I32, _P, _P],
@@ -100,6 +100,11 @@ def lib() -> ctypes.CDLL:
 
 def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def raw_stream(device: torch.device) -> int:
+    """``stream_ptr`` without building a Stream object (2 us a call, a fifth of a small decode step)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def check(status: int, what: str) -> None:

@@ -388,7 +388,8 @@ using namespace mzb;
 
 extern "C" int mzb_kv_append(const void* k, const void* v, void* k_pages, void* v_pages, const int32_t* page_table,
                              const int32_t* starts, const int32_t* cu, int64_t T, int B, int Hkv, int row_bytes,
-                             int page, int64_t P, int W, const int64_t* strides, int* err, void* stream) {
+                             int page, int64_t P, int W, int elem_bytes, const int64_t* strides, int* err,
+                          void* stream) {
   MZB_POOL_SIZES("kv_append", P, W, page);
   MZB_REQUIRE(T >= 0 && B >= 1 && Hkv >= 1 && (cu != nullptr || T == B), MZB_ERR_SHAPE,
               "kv_append: bad sizes T=%lld B=%d Hkv=%d", (long long)T, B, Hkv);
@@ -396,13 +397,20 @@ extern "C" int mzb_kv_append(const void* k, const void* v, void* k_pages, void* 
               row_bytes);
   for (const void* p : {k, v, (const void*)k_pages, (const void*)v_pages})
     MZB_REQUIRE(reinterpret_cast<uintptr_t>(p) % 16 == 0, MZB_ERR_ALIGN, "kv_append: pointers must be 16-byte aligned");
-  for (int i = 0; i < 10; ++i)
-    MZB_REQUIRE(strides[i] % 16 == 0, MZB_ERR_ALIGN, "kv_append: strides must be multiples of 16 bytes");
+  MZB_REQUIRE(elem_bytes >= 1 && elem_bytes <= 16, MZB_ERR_UNSUPPORTED, "kv_append: elements of %d bytes", elem_bytes);
+  int64_t sb[10];
+  for (int i = 0; i < 10; ++i) {
+    sb[i] = strides[i] * elem_bytes;
+    // the stride of a single head, slot or page is never used
+    const bool one = (i == 1 || i == 3 || i == 5 || i == 8) ? Hkv == 1 : (i == 4 || i == 7) ? P == 1 : (i == 6 || i == 9) ? page == 1 : T == 1;
+    if (one) sb[i] = 0;
+    MZB_REQUIRE(sb[i] % 16 == 0, MZB_ERR_ALIGN, "kv_append: strides must be multiples of 16 bytes");
+  }
   if (T == 0) return MZB_OK;
   const int tok = T <= 4 * num_sms() ? 1 : T <= 16 * num_sms() ? 4 : pages::AP_TOK;
   pages::AppendArgs a{static_cast<const uint8_t*>(k), static_cast<const uint8_t*>(v), static_cast<uint8_t*>(k_pages),
-                      static_cast<uint8_t*>(v_pages), page_table, starts, cu, T, P, strides[0], strides[1],
-                      strides[2], strides[3], strides[4], strides[5], strides[6], strides[7], strides[8], strides[9],
+                      static_cast<uint8_t*>(v_pages), page_table, starts, cu, T, P, sb[0], sb[1],
+                      sb[2], sb[3], sb[4], sb[5], sb[6], sb[7], sb[8], sb[9],
                       B, Hkv, row_bytes / 16, W, page, tok, err};
   pages::append_kernel<<<unsigned((T + tok - 1) / tok), 256, 0, static_cast<cudaStream_t>(stream)>>>(a);
   return launch_status("kv_append");

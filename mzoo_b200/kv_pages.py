@@ -21,13 +21,15 @@ from ._lib import require_cuda
 
 
 def _state(**tensors):
-    require_cuda(*tensors.values())
-    dev = next(iter(tensors.values())).device
+    first = -1
     for name, t in tensors.items():
-        assert t.dtype == torch.int32 and t.is_contiguous() and t.device == dev, \
-            f"{name} must be a contiguous int32 tensor on {dev}, got {t.dtype} on {t.device}"
-        want = 2 if name == "page_table" else 1
-        assert t.dim() == want, f"{name} must have {want} dimension(s), got {tuple(t.shape)}"
+        i = t.get_device()
+        if first < 0:
+            first = i
+            require_cuda(t)
+        assert i == first and t.dtype == torch.int32 and t.is_contiguous(), \
+            f"{name} must be a contiguous int32 tensor on cuda:{first}, got {t.dtype} on {t.device}"
+        assert t.dim() == (2 if name == "page_table" else 1), f"{name} has {t.dim()} dimensions: {tuple(t.shape)}"
 
 
 def _table(page_table, seq_lens, refs):
@@ -39,14 +41,28 @@ def _table(page_table, seq_lens, refs):
 def _pools(pools, pages, dev):
     pools = list(pools)
     for p in pools:
-        require_cuda(p)
-        assert p.device == dev and p.dim() >= 2 and p.shape[0] == pages, \
-            f"each pool must be [{pages}, ...] on {dev}, got {tuple(p.shape)} on {p.device}"
-        assert p[0].is_contiguous() and p.stride(0) >= p[0].numel(), "a pool's pages must be dense and apart"
-        n = p.element_size()
-        assert p[0].numel() * n % 16 == 0 and p.stride(0) * n % 16 == 0 and p.storage_offset() * n % 16 == 0 and p[0].numel(), \
+        shape, stride = p.shape, p.stride()
+        assert p.device == dev and len(shape) >= 2 and shape[0] == pages, \
+            f"each pool must be [{pages}, ...] on {dev}, got {tuple(shape)} on {p.device}"
+        n, size = p.numel() // max(1, shape[0]), p.element_size()
+        assert (p.is_contiguous() or p[0].is_contiguous()) and (stride[0] >= n or pages == 1), \
+            "a pool's pages must be dense and apart"
+        assert n and n * size % 16 == 0 and (stride[0] * size % 16 == 0 or pages == 1) and p.storage_offset() * size % 16 == 0, \
             "a pool's pages must be 16-byte aligned and a multiple of 16 bytes"
     return pools
+
+
+def _rows_ok(t, size, apart=False):
+    """Dense rows on 16-byte boundaries (``apart``: no two of them the same memory)."""
+    if t.storage_offset() * size & 15:
+        return False
+    *outer, last = t.stride()
+    if last != 1:
+        return False
+    for x in outer:
+        if x * size & 15 or (apart and not x):
+            return not any([n > 1 and (x * size & 15 or (apart and not x)) for n, x in zip(t.shape, outer)])
+    return True
 
 
 def append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -54,31 +70,27 @@ def append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     """Write k / v ``[T, Hkv, D]`` into k_pages / v_pages ``[P, Hkv, page, D]`` (any strides over dense
     rows): row i of sequence b, rows ``cu[b] .. cu[b+1]`` (``cu`` None: row b, one token each), goes
     to position ``starts[b] + i``."""
-    require_cuda(k, v, k_pages, v_pages)
-    _state(page_table=page_table, starts=starts, **({} if cu is None else {"cu": cu}))
-    dt, dev = k.dtype, k.device
-    for t in (v, k_pages, v_pages):
-        assert t.dtype == dt and t.device == dev, f"k, v and the pools must be {dt} on {dev}, got {t.dtype} on {t.device}"
-    assert page_table.device == dev, f"page_table must be on {dev}, got {page_table.device}"
-    assert k.dim() == 3 and k.shape == v.shape, f"k and v must be [tokens, heads, D], got {tuple(k.shape)}, {tuple(v.shape)}"
-    assert k_pages.dim() == 4 and k_pages.shape == v_pages.shape and k_pages.shape[1] == k.shape[1] \
-        and k_pages.shape[3] == k.shape[2] and k_pages.numel(), \
-        f"the pools must be [pages, {k.shape[1]}, page, {k.shape[2]}], got {tuple(k_pages.shape)}, {tuple(v_pages.shape)}"
-    B, size = starts.shape[0], k.element_size()
-    assert B >= 1 and page_table.shape[0] == B and page_table.shape[1] >= 1, \
-        f"page_table must have one row for each of the {B} sequences, got {tuple(page_table.shape)}"
-    assert (cu is None and k.shape[0] == B) or (cu is not None and cu.shape[0] == B + 1), \
-        f"rows of {B} sequences: cu must be [{B + 1}], or None with one row each (got {k.shape[0]} rows)"
-    assert k.shape[2] * size % 16 == 0, f"rows must be a multiple of 16 bytes, got {k.shape[2]} x {dt}"
-
-    def ok(t):
-        return t.stride(-1) == 1 and t.storage_offset() * size % 16 == 0 and all(
-            n <= 1 or s * size % 16 == 0 for n, s in zip(t.shape[:-1], t.stride()[:-1]))
-    for t in (k_pages, v_pages):
-        assert ok(t) and all(n <= 1 or s > 0 for n, s in zip(t.shape, t.stride())), \
-            "the pools need dense, 16-byte aligned rows"
-    ops.kv_append(k if ok(k) else k.contiguous(), v if ok(v) else v.contiguous(), k_pages, v_pages, page_table, starts,
-                  cu, check)
+    if cu is None:
+        _state(page_table=page_table, starts=starts)
+    else:
+        _state(page_table=page_table, starts=starts, cu=cu)
+    dt, ks, ps = k.dtype, k.shape, k_pages.shape
+    i = page_table.get_device()
+    for t in (k, v, k_pages, v_pages):
+        assert t.dtype == dt and t.get_device() == i, \
+            f"k, v and the pools must be {dt} on cuda:{i}, got {t.dtype} on {t.device}"
+    assert len(ks) == 3 and ks == v.shape, f"k and v must be [tokens, heads, D], got {tuple(ks)}, {tuple(v.shape)}"
+    assert len(ps) == 4 and ps == v_pages.shape and ps[1] == ks[1] and ps[3] == ks[2] and ps[0] and ps[2], \
+        f"the pools must be [pages, {ks[1]}, page, {ks[2]}], got {tuple(ps)}, {tuple(v_pages.shape)}"
+    B, size, (rows, width) = len(starts), k.element_size(), page_table.shape
+    assert B >= 1 and rows == B and width >= 1, \
+        f"page_table must have one row for each of the {B} sequences, got {rows} x {width}"
+    assert ks[0] == B if cu is None else len(cu) == B + 1, \
+        f"rows of {B} sequences: cu must be [{B + 1}], or None with one row each (got {ks[0]} rows)"
+    assert ks[2] * size % 16 == 0 and ks[1] >= 1, f"rows must be a multiple of 16 bytes, got {ks[2]} x {dt}"
+    assert _rows_ok(k_pages, size, True) and _rows_ok(v_pages, size, True), "the pools need dense, 16-byte aligned rows"
+    ops.kv_append(k if _rows_ok(k, size) else k.contiguous(), v if _rows_ok(v, size) else v.contiguous(), k_pages, v_pages,
+                  page_table, starts, cu, check)
 
 
 def reserve(page_table: torch.Tensor, seq_lens: torch.Tensor, refs: torch.Tensor, n_new: torch.Tensor, *, page_size: int,

@@ -6,6 +6,9 @@ torch (the library never allocates), passes raw pointers and the current stream 
 implementation so it traces under ``torch.compile`` / ``FakeTensor`` without running.
 """
 
+import ctypes
+import functools
+
 import torch
 
 from . import _lib
@@ -451,6 +454,15 @@ def _(codes, scales, D, fmt):
 # smallest decode step.
 
 _LIB = torch.library.Library("mzb", "FRAGMENT")
+_I64x10 = ctypes.c_int64 * 10
+
+
+def _call_on(dev, name, *args):
+    """``call`` with the tensors' device current."""
+    if torch._C._cuda_getDevice() == dev.index:
+        return call(name, *args)
+    with torch.cuda.device(dev):
+        return call(name, *args)
 
 
 def _define(schema: str, fake):
@@ -466,7 +478,8 @@ def _define(schema: str, fake):
 
 
 def _attn_out(q, *rest):
-    return torch.empty(q.shape, dtype=q.dtype, device=q.device), q.new_empty(q.shape[:2], dtype=torch.float32)
+    return (torch.empty_like(q, memory_format=torch.contiguous_format),
+            torch.empty(q.shape[0], q.shape[1], dtype=torch.float32, device=q.device))
 
 
 @_define("gqa_prefill(Tensor q, Tensor k, Tensor v, Tensor cu_q, Tensor cu_k, bool causal, float scale, bool check)"
@@ -474,15 +487,22 @@ def _attn_out(q, *rest):
 def gqa_prefill(q, k, v, cu_q, cu_k, causal, scale, check):
     """(o like q, lse fp32 [Tq, Hq]) of ``mzb_gqa_prefill`` (q / k / v with a dense last dimension)."""
     dev = q.device
-    o, lse = _attn_out(q)
+    Tq, Hq, D = q.shape
+    o = torch.empty_like(q, memory_format=torch.contiguous_format)
+    lse = torch.empty(Tq, Hq, dtype=torch.float32, device=dev)
     err = _err(dev, check)
-    call("mzb_gqa_prefill", q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), o.data_ptr(),
-         lse.data_ptr(), q.shape[0], k.shape[0], cu_q.shape[0] - 1, q.shape[1], k.shape[1], q.shape[2],
-         _lib.DTYPE_CODE[q.dtype], q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-         int(causal), scale, err.data_ptr(), stream_ptr(dev))
+    (sq_t, sq_h, _), (sk_t, sk_h, _), (sv_t, sv_h, _), (Tk, Hkv, _) = q.stride(), k.stride(), v.stride(), k.shape
+    _call_on(dev, "mzb_gqa_prefill", q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), o.data_ptr(),
+         lse.data_ptr(), Tq, Tk, len(cu_q) - 1, Hq, Hkv, D, _lib.DTYPE_CODE[q.dtype], sq_t, sq_h, sk_t, sk_h, sv_t,
+         sv_h, causal, scale, err.data_ptr(), _lib.raw_stream(dev))
     if check:
         _raise_on(err, "gqa prefill")
     return o, lse
+
+
+@functools.lru_cache(maxsize=256)
+def _gqa_decode_ws(B: int, Hq: int, Hkv: int, D: int, W: int, page: int, device_index: int) -> int:
+    return _lib.lib().mzb_gqa_decode_ws(B, Hq, Hkv, D, W, page)
 
 
 @_define("gqa_decode(Tensor q, Tensor k_pages, Tensor v_pages, Tensor page_table, Tensor seq_lens, float scale,"
@@ -490,14 +510,17 @@ def gqa_prefill(q, k, v, cu_q, cu_k, causal, scale, check):
 def gqa_decode(q, k_pages, v_pages, page_table, seq_lens, scale, check):
     """(o like q, lse fp32 [B, Hq]) of ``mzb_gqa_decode``."""
     dev = q.device
-    o, lse = _attn_out(q)
-    err = _err(dev, check)
     (B, Hq, D), (P, Hkv, page, _), W = q.shape, k_pages.shape, page_table.shape[1]
-    ws = torch.empty(_lib.lib().mzb_gqa_decode_ws(B, Hq, Hkv, D, W, page), dtype=torch.float32, device=dev)
-    call("mzb_gqa_decode", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(),
-         seq_lens.data_ptr(), o.data_ptr(), lse.data_ptr(), ws.data_ptr(), B, Hq, Hkv, D, _lib.DTYPE_CODE[q.dtype],
-         page, P, W, q.stride(0), q.stride(1), *k_pages.stride()[:3], *v_pages.stride()[:3], scale, err.data_ptr(),
-         stream_ptr(dev))
+    o = torch.empty_like(q, memory_format=torch.contiguous_format)
+    lse = torch.empty(B, Hq, dtype=torch.float32, device=dev)
+    n = _gqa_decode_ws(B, Hq, Hkv, D, W, page, dev.index)
+    ws = torch.empty(n, dtype=torch.float32, device=dev) if n else None
+    err = _err(dev, check)
+    (sq_b, sq_h, _), (sk_p, sk_h, sk_t, _), (sv_p, sv_h, sv_t, _) = q.stride(), k_pages.stride(), v_pages.stride()
+    _call_on(dev, "mzb_gqa_decode", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(),
+         seq_lens.data_ptr(), o.data_ptr(), lse.data_ptr(), ws.data_ptr() if n else None, B, Hq, Hkv, D,
+         _lib.DTYPE_CODE[q.dtype], page, P, W, sq_b, sq_h, sk_p, sk_h, sk_t, sv_p, sv_h, sv_t, scale, err.data_ptr(),
+         _lib.raw_stream(dev))
     if check:
         _raise_on(err, "gqa decode")
     return o, lse
@@ -507,13 +530,13 @@ def gqa_decode(q, k_pages, v_pages, page_table, seq_lens, scale, check):
          " Tensor? cu, bool check) -> ()", lambda *a: None)
 def kv_append(k, v, k_pages, v_pages, page_table, starts, cu, check):
     """``mzb_kv_append``: rows of k / v [T, Hkv, D] into k_pages / v_pages [P, Hkv, page, D]."""
-    dev, size = k.device, k.element_size()
+    dev, size, (T, H, D), (P, _, page, _) = k.device, k.element_size(), k.shape, k_pages.shape
     err = _err(dev, check)
-    strides = (_lib.ctypes.c_int64 * 10)(*(size * x for t, n in ((k, 2), (v, 2)) for x in t.stride()[:n]),
-                                         *(size * p.stride(i) for p in (k_pages, v_pages) for i in (0, 1, 2)))
-    call("mzb_kv_append", k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(),
-         starts.data_ptr(), ptr(cu), k.shape[0], starts.shape[0], k.shape[1], k.shape[2] * size, k_pages.shape[2],
-         k_pages.shape[0], page_table.shape[1], strides, err.data_ptr(), stream_ptr(dev))
+    _call_on(dev, "mzb_kv_append", k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(),
+         starts.data_ptr(), None if cu is None else cu.data_ptr(), T, len(starts), H, D * size, page, P,
+         page_table.shape[1], size,
+         _I64x10(*k.stride()[:2], *v.stride()[:2], *k_pages.stride()[:3], *v_pages.stride()[:3]), err.data_ptr(),
+         _lib.raw_stream(dev))
     if check:
         _raise_on(err, "kv append")
 
@@ -524,9 +547,9 @@ def kv_reserve(page_table, seq_lens, refs, n_new, page, check):
     """``mzb_kv_reserve``; returns the lengths before it."""
     dev = page_table.device
     err, starts, ws = _err(dev, check), torch.empty_like(seq_lens), torch.empty_like(refs)
-    call("mzb_kv_reserve", page_table.data_ptr(), seq_lens.data_ptr(), refs.data_ptr(), n_new.data_ptr(),
+    _call_on(dev, "mzb_kv_reserve", page_table.data_ptr(), seq_lens.data_ptr(), refs.data_ptr(), n_new.data_ptr(),
          starts.data_ptr(), ws.data_ptr(), page_table.shape[0], page_table.shape[1], refs.shape[0], page,
-         err.data_ptr(), stream_ptr(dev))
+         err.data_ptr(), _lib.raw_stream(dev))
     if check:
         _raise_on(err, "kv reserve")
     return starts
@@ -538,19 +561,19 @@ def kv_free(page_table, seq_lens, refs, seqs, check):
     """``mzb_kv_free``."""
     dev = page_table.device
     err = _err(dev, check)
-    call("mzb_kv_free", page_table.data_ptr(), seq_lens.data_ptr(), refs.data_ptr(), seqs.data_ptr(), seqs.shape[0],
-         page_table.shape[0], page_table.shape[1], refs.shape[0], err.data_ptr(), stream_ptr(dev))
+    _call_on(dev, "mzb_kv_free", page_table.data_ptr(), seq_lens.data_ptr(), refs.data_ptr(), seqs.data_ptr(), seqs.shape[0],
+         page_table.shape[0], page_table.shape[1], refs.shape[0], err.data_ptr(), _lib.raw_stream(dev))
     if check:
         _raise_on(err, "kv free")
 
 
 def _copy(pools, src, dst, count, n, err, dev):
     """One ``mzb_kv_copy_pages`` call; src / dst / count are device addresses."""
-    arr, m = _lib.ctypes.c_int64 * len(pools), len(pools)
-    call("mzb_kv_copy_pages", arr(*(p.data_ptr() for p in pools)),
+    arr, m = ctypes.c_int64 * len(pools), len(pools)
+    _call_on(dev, "mzb_kv_copy_pages", arr(*(p.data_ptr() for p in pools)),
          arr(*(p.numel() // p.shape[0] * p.element_size() for p in pools)),
          arr(*(p.stride(0) * p.element_size() for p in pools)), m, src, dst, count, n, pools[0].shape[0],
-         err.data_ptr(), stream_ptr(dev))
+         err.data_ptr(), _lib.raw_stream(dev))
 
 
 @_define("kv_copy_pages(Tensor(a!)[] pools, Tensor src, Tensor dst, bool check) -> ()", lambda *a: None)
@@ -569,8 +592,8 @@ def kv_fork(pools, page_table, seq_lens, refs, src, dst, page, check):
     """``mzb_kv_fork`` and the copies of the partly filled pages."""
     dev, n, (S, W) = page_table.device, src.shape[0], page_table.shape
     err, ws = _err(dev, check), torch.empty(3 * n + S, dtype=torch.int32, device=dev)
-    call("mzb_kv_fork", page_table.data_ptr(), seq_lens.data_ptr(), refs.data_ptr(), src.data_ptr(), dst.data_ptr(), n,
-         ws.data_ptr(), S, W, refs.shape[0], page, err.data_ptr(), stream_ptr(dev))
+    _call_on(dev, "mzb_kv_fork", page_table.data_ptr(), seq_lens.data_ptr(), refs.data_ptr(), src.data_ptr(), dst.data_ptr(), n,
+         ws.data_ptr(), S, W, refs.shape[0], page, err.data_ptr(), _lib.raw_stream(dev))
     if pools:
         _copy(pools, ws.data_ptr(), ws.data_ptr() + 4 * n, None, n, err, dev)
     if check:
@@ -584,8 +607,8 @@ def kv_compact(pools, page_table, refs, check):
     dev, P = page_table.device, refs.shape[0]
     err, ws = _err(dev, check), torch.empty(3 * P + 1, dtype=torch.int32, device=dev)
     table, new_refs = torch.empty_like(page_table), torch.empty_like(refs)
-    call("mzb_kv_compact", page_table.data_ptr(), refs.data_ptr(), table.data_ptr(), new_refs.data_ptr(), ws.data_ptr(),
-         page_table.numel(), P, err.data_ptr(), stream_ptr(dev))
+    _call_on(dev, "mzb_kv_compact", page_table.data_ptr(), refs.data_ptr(), table.data_ptr(), new_refs.data_ptr(), ws.data_ptr(),
+         page_table.numel(), P, err.data_ptr(), _lib.raw_stream(dev))
     if pools:
         _copy(pools, ws.data_ptr(), ws.data_ptr() + 4 * P, ws.data_ptr() + 12 * P, P // 2, err, dev)
     if check:
