@@ -304,15 +304,14 @@ MZB_API int mzb_gqa_decode(const void* q, const void* k_pages, const void* v_pag
  *   (sequence, position) order, seq_lens is raised, starts[b] is the old length.  ws: P ints.
  * mzb_kv_free    -- the sequences seqs[0..n): refs - 1 for their pages, entries -1, length 0.
  * mzb_kv_fork    -- dst[i] becomes a copy of src[i]: what dst held is released, full pages are
- *   shared (refs + 1), a partly filled last page gets a page of its own.  dst distinct and
- *   disjoint from src (other pairs are left out, as an error).  ws: 3 n + S ints; its first 2 n
- *   are then the pages to copy: sources [n], destinations [n] (-1: none).
+ *   shared (refs + 1), a partly filled last page is copied to a page of its own in every pool.
+ *   dst distinct and disjoint from src (other pairs are left out, as an error).  ws: 3 n + S ints.
  * mzb_kv_compact -- n = pages with refs > 0; the i-th of them at an id >= n moves to the i-th
- *   free id below n.  new_table, new_refs: the state after it.  ws: 3 P + 1 ints: sources [P],
- *   destinations [P], the map [P], the number of moves.
- * mzb_kv_copy_pages -- page src[i] to page dst[i] (both -1: none) in n_pools pools of P pages
- *   (page_bytes, page_strides: host arrays; multiples of 16 bytes); count (device, may be
- *   NULL): the number of pairs, at most n.  No destination may be a source or named twice.
+ *   free id below n, in every pool.  new_table, new_refs: the state after it.  ws: 3 P + 1 ints.
+ * mzb_kv_copy_pages -- page src[i] to page dst[i] (both -1: none) in every pool.  No destination
+ *   may be a source or named twice.
+ * pools: a host array of (address, bytes of a page, bytes from page to page) for each of n_pools
+ *   pools of P pages; all multiples of 16.
  */
 MZB_API int mzb_kv_append(const void* k, const void* v, void* k_pages, void* v_pages, const int32_t* page_table,
                           const int32_t* starts, const int32_t* cu, int64_t T, int B, int Hkv, int row_bytes,
@@ -323,12 +322,13 @@ MZB_API int mzb_kv_reserve(int32_t* page_table, int32_t* seq_lens, int32_t* refs
 MZB_API int mzb_kv_free(int32_t* page_table, int32_t* seq_lens, int32_t* refs, const int32_t* seqs, int64_t n,
                         int64_t S, int W, int64_t P, int* err, void* stream);
 MZB_API int mzb_kv_fork(int32_t* page_table, int32_t* seq_lens, int32_t* refs, const int32_t* src, const int32_t* dst,
-                        int n, int32_t* ws, int64_t S, int W, int64_t P, int page, int* err, void* stream);
+                        int n, int32_t* ws, int64_t S, int W, int64_t P, int page, const int64_t* pools, int n_pools,
+                        int* err, void* stream);
 MZB_API int mzb_kv_compact(const int32_t* page_table, const int32_t* refs, int32_t* new_table, int32_t* new_refs,
-                           int32_t* ws, int64_t entries, int64_t P, int* err, void* stream);
-MZB_API int mzb_kv_copy_pages(void* const* pools, const int64_t* page_bytes, const int64_t* page_strides, int n_pools,
-                              const int32_t* src, const int32_t* dst, const int32_t* count, int64_t n, int64_t P,
-                              int* err, void* stream);
+                           int32_t* ws, int64_t entries, int64_t P, const int64_t* pools, int n_pools, int* err,
+                           void* stream);
+MZB_API int mzb_kv_copy_pages(const int64_t* pools, int n_pools, const int32_t* src, const int32_t* dst, int64_t n,
+                              int64_t P, int* err, void* stream);
 
 /* Self-test of the bounded device waits (no counterpart in the reference: it checks this
  * library's own failure path).  One thread waits on an mbarrier nothing arrives on; after

@@ -69,9 +69,9 @@ SIGNATURES = {
     "mzb_kv_append": [_P, _P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _I64, _I32, _I32, _P, _P, _P],
     "mzb_kv_reserve": [_P, _P, _P, _P, _P, _P, _I32, _I32, _I64, _I32, _P, _P],
     "mzb_kv_free": [_P, _P, _P, _P, _I64, _I64, _I32, _I64, _P, _P],
-    "mzb_kv_fork": [_P, _P, _P, _P, _P, _I32, _P, _I64, _I32, _I64, _I32, _P, _P],
-    "mzb_kv_compact": [_P, _P, _P, _P, _P, _I64, _I64, _P, _P],
-    "mzb_kv_copy_pages": [_P, _P, _P, _I32, _P, _P, _P, _I64, _I64, _P, _P],
+    "mzb_kv_fork": [_P, _P, _P, _P, _P, _I32, _P, _I64, _I32, _I64, _I32, _P, _I32, _P, _P],
+    "mzb_kv_compact": [_P, _P, _P, _P, _P, _I64, _I64, _P, _I32, _P, _P],
+    "mzb_kv_copy_pages": [_P, _I32, _P, _P, _I64, _I64, _P, _P],
 }
 _RESTYPE = {"mzb_last_error": ctypes.c_char_p, "mzb_gqa_decode_ws": _I64}
 

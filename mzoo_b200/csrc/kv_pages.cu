@@ -7,7 +7,7 @@
 // the order of the sequences that ask, so equal inputs give equal tables.  What cannot be
 // done (a position past the table, a page id outside the pool, no free page) is left out and
 // recorded as MZB_ERR_PAGES in the error word.
-#include "common.cuh"
+#include "tc.cuh"
 
 namespace mzb {
 namespace pages {
@@ -42,15 +42,38 @@ __device__ __forceinline__ int block_scan(int v, int* warp_sums, int& total) {
   return x - v + (warp ? warp_sums[warp - 1] : 0);
 }
 
+constexpr int PT = 8;  // consecutive elements of a thread in the scans
+
+__device__ __forceinline__ void load_refs(const int32_t* refs, int64_t p0, int64_t P, int32_t none, int32_t (&r)[PT]) {
+  if (p0 + PT <= P && (reinterpret_cast<uintptr_t>(refs) & 15) == 0) {
+#pragma unroll
+    for (int e = 0; e < PT; e += 4) {
+      const int4 x = __ldcg(reinterpret_cast<const int4*>(refs + p0 + e));
+      r[e] = x.x;
+      r[e + 1] = x.y;
+      r[e + 2] = x.z;
+      r[e + 3] = x.w;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < PT; ++e) r[e] = p0 + e < P ? __ldcg(refs + p0 + e) : none;
+  }
+}
+
 // The lowest `want` free pages, ascending, into list; returns how many there are (<= want).
 __device__ int lowest_free(const int32_t* refs, int64_t P, int want, int32_t* list, int* warp_sums) {
   int found = 0;
-  for (int64_t p0 = 0; p0 < P && found < want; p0 += NT) {
-    const int64_t p = p0 + threadIdx.x;
-    const int f = p < P && refs[p] == 0;
-    int total;
-    const int at = found + block_scan(f, warp_sums, total);
-    if (f && at < want) list[at] = int32_t(p);
+  for (int64_t c0 = 0; c0 < P && found < want; c0 += NT * PT) {
+    const int64_t p0 = c0 + threadIdx.x * PT;
+    int32_t r[PT];
+    load_refs(refs, p0, P, 1, r);
+    int f = 0, total;
+#pragma unroll
+    for (int e = 0; e < PT; ++e) f += r[e] == 0;
+    int at = found + block_scan(f, warp_sums, total);
+#pragma unroll
+    for (int e = 0; e < PT; ++e)
+      if (r[e] == 0 && at < want) list[at++] = int32_t(p0 + e);
     found += total;
   }
   __syncthreads();
@@ -70,51 +93,79 @@ struct AppendArgs {
   int* err;
 };
 
-constexpr int AP_TOK = 8;
+constexpr int AP_TOK = 8, AP_IN_FLIGHT = 4;  // tokens of a block, K and V pieces of a thread
 
-__global__ void __launch_bounds__(256) append_kernel(AppendArgs a) {
+// A copy: bound by HBM.  The rows are requested before their places are known, so that the
+// search for the sequence and the table's look-up (three dependent loads) pass while they are
+// on their way.
+__global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ AppendArgs a) {
   __shared__ int64_t kdst[AP_TOK], vdst[AP_TOK];
   const int64_t t0 = (int64_t)blockIdx.x * a.tok;
-  const int nt = int(min((int64_t)a.tok, a.T - t0));
-  if ((int)threadIdx.x < nt) {
-    const int64_t t = t0 + threadIdx.x;
+  const int nt = int(min((int64_t)a.tok, a.T - t0)), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int per = a.H * a.chunks, n = nt * per;
+  uint4 kv[AP_IN_FLIGHT], vv[AP_IN_FLIGHT];
+  auto request = [&](int x0) {
+#pragma unroll
+    for (int i = 0; i < AP_IN_FLIGHT; ++i) {
+      const int x = x0 + 256 * i;
+      if (x < n) {
+        const int t = x / per, y = x % per, h = y / a.chunks, c = y % a.chunks;
+        kv[i] = __ldcs(reinterpret_cast<const uint4*>(a.k + (t0 + t) * a.sk_t + h * a.sk_h + c * 16));
+        vv[i] = __ldcs(reinterpret_cast<const uint4*>(a.v + (t0 + t) * a.sv_t + h * a.sv_h + c * 16));
+      }
+    }
+  };
+  request(threadIdx.x);
+  if (warp < nt) {  // a warp for each token
+    const int64_t t = t0 + warp;
     int b = int(t);
     int64_t i = 0;
     bool ok = true;
     if (a.cu) {
-      int lo = 0, hi = a.B;  // the last sequence that starts at or before t
+      int lo = 0, hi = a.B;  // the last sequence that starts at or before t, 32 probes at a time
       while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (a.cu[mid] <= t) lo = mid; else hi = mid;
+        const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+        const unsigned m = __ballot_sync(0xffffffffu, at < hi && a.cu[at < hi ? at : lo] <= t);
+        const int last = m ? 31 - __clz(m) : 0;
+        lo = lo + last * step;
+        hi = min(hi, lo + step);
       }
       b = lo;
-      i = t - a.cu[lo];
-      ok = i >= 0 && t < a.cu[lo + 1];
+      const int q0 = a.cu[b], q1 = a.cu[b + 1];
+      i = t - q0;
+      ok = i >= 0 && t < q1;
     }
-    int64_t d = -1, e = -1;
-    if (ok) {
-      const int64_t pos = (int64_t)a.starts[b] + i, j = pos / a.page;
-      if (pos >= 0 && j < a.W) {
-        const int64_t p = a.table[(int64_t)b * a.W + j];
-        if (p >= 0 && p < a.P) {
-          d = p * a.kp_p + (pos % a.page) * a.kp_t;
-          e = p * a.vp_p + (pos % a.page) * a.vp_t;
+    if (lane == 0) {
+      int64_t d = -1, e = -1;
+      if (ok) {
+        const int64_t pos = (int64_t)a.starts[b] + i, j = pos / a.page;
+        if (pos >= 0 && j < a.W) {
+          const int64_t p = a.table[(int64_t)b * a.W + j];
+          if (p >= 0 && p < a.P) {
+            d = p * a.kp_p + (pos % a.page) * a.kp_t;
+            e = p * a.vp_p + (pos % a.page) * a.vp_t;
+          }
         }
+        if (d < 0) report(a.err);
       }
-      if (d < 0) report(a.err);
+      kdst[warp] = d;
+      vdst[warp] = e;
     }
-    kdst[threadIdx.x] = d;
-    vdst[threadIdx.x] = e;
   }
   __syncthreads();
-  const int per = a.H * a.chunks;
-  for (int x = threadIdx.x; x < nt * per; x += 256) {
-    const int t = x / per, y = x % per, h = y / a.chunks, c = y % a.chunks;
-    if (kdst[t] < 0) continue;
-    const uint4 kv = *reinterpret_cast<const uint4*>(a.k + (t0 + t) * a.sk_t + h * a.sk_h + c * 16);
-    const uint4 vv = *reinterpret_cast<const uint4*>(a.v + (t0 + t) * a.sv_t + h * a.sv_h + c * 16);
-    *reinterpret_cast<uint4*>(a.kp + kdst[t] + h * a.kp_h + c * 16) = kv;
-    *reinterpret_cast<uint4*>(a.vp + vdst[t] + h * a.vp_h + c * 16) = vv;
+  for (int x0 = threadIdx.x; x0 < n; x0 += 256 * AP_IN_FLIGHT) {
+    if (x0 >= 256 * AP_IN_FLIGHT) request(x0);
+#pragma unroll
+    for (int i = 0; i < AP_IN_FLIGHT; ++i) {
+      const int x = x0 + 256 * i;
+      if (x < n) {
+        const int t = x / per, y = x % per, h = y / a.chunks, c = y % a.chunks;
+        if (kdst[t] >= 0) {
+          *reinterpret_cast<uint4*>(a.kp + kdst[t] + h * a.kp_h + c * 16) = kv[i];
+          *reinterpret_cast<uint4*>(a.vp + vdst[t] + h * a.vp_h + c * 16) = vv[i];
+        }
+      }
+    }
   }
 }
 
@@ -193,58 +244,78 @@ __global__ void __launch_bounds__(256) free_kernel(int32_t* table, int32_t* lens
 
 // ---------------------------------------------------------------- fork
 
-// One block.  ws: pairs_src [n], pairs_dst [n], list [n], mark [S].
-__global__ void __launch_bounds__(NT) fork_kernel(int32_t* table, int32_t* lens, int32_t* refs, const int32_t* src,
-                                                  const int32_t* dst, int n, int32_t* ws, int64_t S, int W,
-                                                  int64_t P, int page, int* err) {
+// One cluster of FORK_CTAS blocks, which share the table's cells and meet at cluster barriers
+// (a release / acquire of global memory too).  ws: pairs_src [n], pairs_dst [n], list [n], mark [S].
+constexpr int FORK_CTAS = 8;
+
+__global__ void __cluster_dims__(FORK_CTAS, 1, 1) __launch_bounds__(NT)
+    fork_kernel(int32_t* table, int32_t* lens, int32_t* refs, const int32_t* src, const int32_t* dst, int n, int32_t* ws,
+                int64_t S, int W, int64_t P, int page, int* err) {
   __shared__ int wsum[32];
   int32_t *ps = ws, *pd = ws + n, *list = ws + 2 * (int64_t)n, *mark = ws + 3 * (int64_t)n;
+  const int tid = blockIdx.x * NT + threadIdx.x;
+  constexpr int ALL = FORK_CTAS * NT;
   auto in = [&](int64_t s) { return s >= 0 && s < S; };
   // a pair is taken if both names are in the table, dst is named once and is no one's src
-  for (int i = threadIdx.x; i < n; i += NT) {
-    if (in(src[i])) mark[src[i]] = 0;
-    if (in(dst[i])) mark[dst[i]] = 0;
+  for (int i = tid; i < n; i += ALL) {
+    const int s = src[i], d = dst[i];
+    if (in(s)) mark[s] = 0;
+    if (in(d)) mark[d] = 0;
   }
-  __syncthreads();
-  for (int i = threadIdx.x; i < n; i += NT) {
-    if (in(src[i])) atomicOr(&mark[src[i]], 1 << 30);
-    if (in(dst[i])) atomicAdd(&mark[dst[i]], 1);
+  tc::cluster_sync();
+  for (int i = tid; i < n; i += ALL) {
+    const int s = src[i], d = dst[i];
+    if (in(s)) atomicOr(&mark[s], 1 << 30);
+    if (in(d)) atomicAdd(&mark[d], 1);
   }
-  __syncthreads();
-  auto taken = [&](int i) {
+  tc::cluster_sync();
+  // full pages of pair i, -1: not taken
+  auto full_of = [&](int i) {
     const int64_t s = src[i], d = dst[i];
-    return in(s) && in(d) && mark[d] == 1 && lens[s] >= 0 && lens[s] <= (int64_t)W * page;
+    if (!in(s) || !in(d)) return -1;
+    const int len = lens[s], m = __ldcg(&mark[d]);
+    return m == 1 && len >= 0 && len <= (int64_t)W * page ? len / page : -1;
   };
-  const int64_t cells = (int64_t)n * W;
-  for (int64_t x = threadIdx.x; x < cells; x += NT) {  // release what the copies held
-    const int i = int(x / W);
-    if (!taken(i)) continue;
-    const int p = atomicExch(&table[(int64_t)dst[i] * W + x % W], -1);
-    if (p >= 0 && p < P) atomicSub(&refs[p], 1);
-  }
-  __syncthreads();
-  for (int64_t x = threadIdx.x; x < cells; x += NT) {  // share the full pages
-    const int i = int(x / W), j = int(x % W);
-    if (!taken(i) || j >= lens[src[i]] / page) continue;
-    const int p = table[(int64_t)src[i] * W + j];
-    if (p >= 0 && p < P) {
-      table[(int64_t)dst[i] * W + j] = p;
-      atomicAdd(&refs[p], 1);
-    } else {
-      report(err);
+  // a warp for each pair: what dst held is released, src's full pages are shared.  The counts of a page
+  // only add up, and no source row is written, so the order does not matter.
+  for (int i = tid >> 5; i < n; i += ALL / 32) {
+    const int full = full_of(i);
+    if (full < 0) continue;
+    int32_t* to = table + (int64_t)dst[i] * W;
+    const int32_t* from = table + (int64_t)src[i] * W;
+    for (int j0 = threadIdx.x & 31; j0 < W; j0 += 32 * 8) {
+      int was[8], now[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int j = j0 + 32 * e;
+        was[e] = j < W ? to[j] : -1;
+        now[e] = j < full ? from[j] : -1;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int j = j0 + 32 * e;
+        if (j >= W) continue;
+        const bool share = now[e] >= 0 && now[e] < P;
+        if (j < full && !share) report(err);
+        if (was[e] != -1 || share) to[j] = share ? now[e] : -1;
+        if (was[e] >= 0 && was[e] < P) atomicSub(&refs[was[e]], 1);
+        if (share) atomicAdd(&refs[now[e]], 1);
+      }
     }
   }
-  __syncthreads();
+  tc::cluster_sync();
+  if (blockIdx.x) return;
   int want = 0;
   for (int i0 = 0; i0 < n; i0 += NT) {  // ranks of the copies that need a page of their own
     const int i = i0 + threadIdx.x;
     int need = 0;
     if (i < n) {
       ps[i] = pd[i] = -1;
-      if (!taken(i)) {
+      const int full = full_of(i);
+      if (full < 0) {
         report(err);
       } else if (lens[src[i]] % page) {
-        const int p = table[(int64_t)src[i] * W + lens[src[i]] / page];
+        const int p = table[(int64_t)src[i] * W + full];
         if (p >= 0 && p < P) {
           need = 1;
           ps[i] = p;
@@ -261,17 +332,19 @@ __global__ void __launch_bounds__(NT) fork_kernel(int32_t* table, int32_t* lens,
   __syncthreads();
   const int have = lowest_free(refs, P, want, list, wsum);
   for (int i = threadIdx.x; i < n; i += NT) {
-    if (!taken(i)) continue;
-    const int64_t d = dst[i], len = lens[src[i]];
-    int32_t got = int32_t(len);
+    const int full = full_of(i);
+    if (full < 0) continue;
+    const int64_t d = dst[i];
+    const int len = lens[src[i]];
+    int32_t got = len;
     if (len % page) {
       const int32_t p = pd[i] >= 0 && pd[i] < have ? list[pd[i]] : -1;
       if (p >= 0) {
-        table[d * W + len / page] = p;
+        table[d * W + full] = p;
         refs[p] = 1;
       } else {  // no page for the last tokens: the copy ends at its last full page
         if (pd[i] >= 0) report(err);
-        got = int32_t(len / page * page);
+        got = full * page;
         ps[i] = -1;
       }
       pd[i] = p;
@@ -284,32 +357,43 @@ __global__ void __launch_bounds__(NT) fork_kernel(int32_t* table, int32_t* lens,
 
 // One block.  The i-th live page at an index >= n moves to the i-th hole below n (n = number
 // of live pages), so the pages that move and the holes are disjoint and the copies need no
-// order.  to [P]: where a page is afterwards (-1: free); pairs [2 * m]: (from, to) lists,
-// m = count[0].
+// order.  to [P]: where a page is afterwards (-1: free); (from, hole) lists of m = count[0] moves.
 __global__ void __launch_bounds__(NT) compact_plan_kernel(const int32_t* refs, int32_t* new_refs, int32_t* to,
                                                           int32_t* from_list, int32_t* hole_list, int32_t* count,
                                                           int64_t P) {
   __shared__ int ws[32];
-  int n = 0, total;
-  for (int64_t p0 = 0; p0 < P; p0 += NT) {
-    const int64_t p = p0 + threadIdx.x;
-    block_scan(p < P && refs[p] > 0, ws, total);
-    n += total;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  int n, mine = 0;
+  for (int64_t p0 = threadIdx.x * PT; p0 < P; p0 += NT * PT) {
+    int32_t r[PT];
+    load_refs(refs, p0, P, 0, r);
+#pragma unroll
+    for (int e = 0; e < PT; ++e) mine += r[e] > 0;
   }
+  block_scan(mine, ws, n);
   int holes = 0, moved = 0;
-  for (int64_t p0 = 0; p0 < P; p0 += NT) {
-    const int64_t p = p0 + threadIdx.x;
-    const int r = p < P ? refs[p] : 0;
-    const int hole = p < n && r <= 0, move = p >= n && r > 0;
-    const int at = block_scan(p0 < n ? hole : 0, ws, total);
-    if (hole) hole_list[holes + at] = int32_t(p);
-    holes += total;
-    const int am = block_scan(move, ws, total);
-    if (move) from_list[moved + am] = int32_t(p);
-    moved += total;
-    if (p < P) {
-      to[p] = r > 0 ? int32_t(p) : -1;
-      new_refs[p] = p < n ? r : 0;
+  for (int64_t c0 = 0; c0 < P; c0 += NT * PT) {
+    const int64_t p0 = c0 + threadIdx.x * PT;
+    int32_t r[PT];
+    load_refs(refs, p0, P, 0, r);
+    int hm = 0, total;  // holes in the low half, moves in the high half: at most NT * PT each
+#pragma unroll
+    for (int e = 0; e < PT; ++e) hm += p0 + e < n ? (r[e] <= 0) : (r[e] > 0) << 16;
+    const int at = block_scan(hm, ws, total);
+    int ah = holes + (at & 0xffff), am = moved + (at >> 16);
+    holes += total & 0xffff;
+    moved += total >> 16;
+#pragma unroll
+    for (int e = 0; e < PT; ++e) {
+      const int64_t p = p0 + e;
+      if (p >= P) continue;
+      if (p < n) {
+        if (r[e] <= 0) hole_list[ah++] = int32_t(p);
+      } else if (r[e] > 0) {
+        from_list[am++] = int32_t(p);
+      }
+      to[p] = r[e] > 0 ? int32_t(p) : -1;
+      new_refs[p] = p < n && r[e] > 0 ? r[e] : 0;
     }
   }
   __syncthreads();
@@ -321,23 +405,11 @@ __global__ void __launch_bounds__(NT) compact_plan_kernel(const int32_t* refs, i
   if (threadIdx.x == 0) count[0] = moved;
 }
 
-__global__ void __launch_bounds__(256) remap_kernel(const int32_t* table, int32_t* new_table, const int32_t* to,
-                                                    int64_t n, int64_t P, int* err) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    const int p = table[i];
-    int q = -1;
-    if (p >= 0) {
-      q = p < P ? to[p] : -1;
-      if (q < 0) report(err);  // a table names a free page or none of the pool's
-    }
-    new_table[i] = q;
-  }
-}
-
 // ---------------------------------------------------------------- copying pages
 
 constexpr int MAX_POOLS = 64;
 constexpr int CHUNK = 16384;  // bytes of a page that one block step copies: 256 threads x 4 x 16
+constexpr int COPY_BLOCKS = 8;  // blocks of an SM
 
 struct CopyArgs {
   uint8_t* pool[MAX_POOLS];
@@ -348,9 +420,23 @@ struct CopyArgs {
   int64_t n, P;
   int n_pools, chunks;  // chunks of the largest page
   int* err;
+  // a page table to rewrite with a map of the pages (null: none)
+  const int32_t *table, *to;
+  int32_t* new_table;
+  int64_t entries;
 };
 
 __global__ void __launch_bounds__(256) copy_kernel(const __grid_constant__ CopyArgs a) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // behind the kernel that made the lists
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.entries; i += (int64_t)gridDim.x * 256) {
+    const int p = a.table[i];
+    int q = -1;
+    if (p >= 0) {
+      q = p < a.P ? a.to[p] : -1;
+      if (q < 0) report(a.err);  // a table names a free page or none of the pool's
+    }
+    a.new_table[i] = q;
+  }
   const int64_t n = a.count ? min((int64_t)*a.count, a.n) : a.n;
   const int64_t per = (int64_t)a.n_pools * a.chunks;
   for (int64_t w = blockIdx.x; w < n * per; w += gridDim.x) {
@@ -365,14 +451,59 @@ __global__ void __launch_bounds__(256) copy_kernel(const __grid_constant__ CopyA
     const int64_t off = (int64_t)c * CHUNK, left = a.bytes[pool] - off;
     const uint4* from = reinterpret_cast<const uint4*>(a.pool[pool] + s * a.stride[pool] + off);
     uint4* to = reinterpret_cast<uint4*>(a.pool[pool] + d * a.stride[pool] + off);
-    uint4 v[4];
+    uint4 v[CHUNK / 4096];
+    if (left >= CHUNK) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      if ((int64_t)(threadIdx.x + 256 * q) * 16 < left) v[q] = from[threadIdx.x + 256 * q];
+      for (int q = 0; q < CHUNK / 4096; ++q) v[q] = __ldcs(from + threadIdx.x + 256 * q);
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      if ((int64_t)(threadIdx.x + 256 * q) * 16 < left) to[threadIdx.x + 256 * q] = v[q];
+      for (int q = 0; q < CHUNK / 4096; ++q) __stcs(to + threadIdx.x + 256 * q, v[q]);
+    } else {
+#pragma unroll
+      for (int q = 0; q < CHUNK / 4096; ++q)
+        if ((int64_t)(threadIdx.x + 256 * q) * 16 < left) v[q] = from[threadIdx.x + 256 * q];
+#pragma unroll
+      for (int q = 0; q < CHUNK / 4096; ++q)
+        if ((int64_t)(threadIdx.x + 256 * q) * 16 < left) to[threadIdx.x + 256 * q] = v[q];
+    }
   }
+}
+
+// One launch for up to MAX_POOLS pools, allowed to start while the kernel before it runs.
+int copy_pages(const int64_t* pools, int n_pools, CopyArgs a, const char* what, cudaStream_t st) {
+  for (int i = 0; i < n_pools; ++i)
+    MZB_REQUIRE(pools[3 * i] % 16 == 0 && pools[3 * i + 1] >= 16 && pools[3 * i + 1] % 16 == 0 && pools[3 * i + 2] % 16 == 0,
+                MZB_ERR_ALIGN, "%s: pool %d: pages must be 16-byte aligned and multiples of 16 bytes", what, i);
+  for (int p0 = 0; p0 < n_pools || (p0 == 0 && a.entries); p0 += MAX_POOLS) {
+    a.n_pools = n_pools - p0 < MAX_POOLS ? n_pools - p0 : MAX_POOLS;
+    int64_t most = 16;
+    for (int i = 0; i < a.n_pools; ++i) {
+      const int64_t* x = pools + 3 * (p0 + i);
+      a.pool[i] = reinterpret_cast<uint8_t*>(x[0]);
+      a.bytes[i] = x[1];
+      a.stride[i] = x[2];
+      most = most > a.bytes[i] ? most : a.bytes[i];
+    }
+    a.chunks = int((most + CHUNK - 1) / CHUNK);
+    const int64_t work = a.n * a.n_pools * a.chunks, rows = (a.entries + 255) / 256, cap = COPY_BLOCKS * num_sms();
+    const int64_t want = work > rows ? work : rows;
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(unsigned(want < 1 ? 1 : want < cap ? want : cap));
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, copy_kernel, a);
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      set_error("%s: launch failed: %s", what, cudaGetErrorString(e));
+      return MZB_ERR_LAUNCH;
+    }
+    a.entries = 0;
+  }
+  return MZB_OK;
 }
 
 }  // namespace pages
@@ -440,56 +571,41 @@ extern "C" int mzb_kv_free(int32_t* page_table, int32_t* seq_lens, int32_t* refs
 }
 
 extern "C" int mzb_kv_fork(int32_t* page_table, int32_t* seq_lens, int32_t* refs, const int32_t* src,
-                           const int32_t* dst, int n, int32_t* ws, int64_t S, int W, int64_t P, int page, int* err,
-                           void* stream) {
+                           const int32_t* dst, int n, int32_t* ws, int64_t S, int W, int64_t P, int page,
+                           const int64_t* pools, int n_pools, int* err, void* stream) {
   MZB_POOL_SIZES("kv_fork", P, W, page);
-  MZB_REQUIRE(n >= 0 && S >= 1 && S < (int64_t(1) << 31), MZB_ERR_SHAPE, "kv_fork: bad sizes n=%d S=%lld", n, (long long)S);
+  MZB_REQUIRE(n >= 0 && S >= 1 && S < (int64_t(1) << 31) && n_pools >= 0, MZB_ERR_SHAPE, "kv_fork: bad sizes n=%d S=%lld", n,
+              (long long)S);
   if (n == 0) return MZB_OK;
-  pages::fork_kernel<<<1, pages::NT, 0, static_cast<cudaStream_t>(stream)>>>(page_table, seq_lens, refs, src, dst, n,
-                                                                             ws, S, W, P, page, err);
-  return launch_status("kv_fork");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  pages::fork_kernel<<<pages::FORK_CTAS, pages::NT, 0, st>>>(page_table, seq_lens, refs, src, dst, n, ws, S, W, P, page, err);
+  if (int r = launch_status("kv_fork")) return r;
+  pages::CopyArgs a{};
+  a.src = ws; a.dst = ws + n; a.n = n; a.P = P; a.err = err;
+  return pages::copy_pages(pools, n_pools, a, "kv_fork(copy)", st);
 }
 
 extern "C" int mzb_kv_compact(const int32_t* page_table, const int32_t* refs, int32_t* new_table, int32_t* new_refs,
-                              int32_t* ws, int64_t entries, int64_t P, int* err, void* stream) {
+                              int32_t* ws, int64_t entries, int64_t P, const int64_t* pools, int n_pools, int* err,
+                              void* stream) {
   MZB_POOL_SIZES("kv_compact", P, 1, 1);
-  MZB_REQUIRE(entries >= 0, MZB_ERR_SHAPE, "kv_compact: bad table size %lld", (long long)entries);
+  MZB_REQUIRE(entries >= 0 && n_pools >= 0, MZB_ERR_SHAPE, "kv_compact: bad table size %lld", (long long)entries);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int32_t *from = ws, *hole = ws + P, *to = ws + 2 * P, *count = ws + 3 * P;
   pages::compact_plan_kernel<<<1, pages::NT, 0, st>>>(refs, new_refs, to, from, hole, count, P);
   if (int r = launch_status("kv_compact")) return r;
-  if (entries == 0) return MZB_OK;
-  const int64_t blocks = (entries + 255) / 256;
-  pages::remap_kernel<<<unsigned(blocks < 4 * num_sms() ? blocks : 4 * num_sms()), 256, 0, st>>>(
-      page_table, new_table, to, entries, P, err);
-  return launch_status("kv_compact(remap)");
+  pages::CopyArgs a{};
+  a.src = from; a.dst = hole; a.count = count; a.n = P / 2; a.P = P; a.err = err;
+  a.table = page_table; a.to = to; a.new_table = new_table; a.entries = entries;
+  return pages::copy_pages(pools, n_pools, a, "kv_compact(copy)", st);
 }
 
-extern "C" int mzb_kv_copy_pages(void* const* pools, const int64_t* page_bytes, const int64_t* page_strides,
-                                 int n_pools, const int32_t* src, const int32_t* dst, const int32_t* count, int64_t n,
+extern "C" int mzb_kv_copy_pages(const int64_t* pools, int n_pools, const int32_t* src, const int32_t* dst, int64_t n,
                                  int64_t P, int* err, void* stream) {
   MZB_POOL_SIZES("kv_copy_pages", P, 1, 1);
   MZB_REQUIRE(n >= 0 && n_pools >= 0, MZB_ERR_SHAPE, "kv_copy_pages: bad sizes n=%lld pools=%d", (long long)n, n_pools);
-  for (int i = 0; i < n_pools; ++i)
-    MZB_REQUIRE(reinterpret_cast<uintptr_t>(pools[i]) % 16 == 0 && page_bytes[i] >= 16 && page_bytes[i] % 16 == 0 &&
-                    page_strides[i] % 16 == 0,
-                MZB_ERR_ALIGN, "kv_copy_pages: pool %d: pages must be 16-byte aligned and multiples of 16 bytes", i);
   if (n == 0) return MZB_OK;
-  for (int p0 = 0; p0 < n_pools; p0 += pages::MAX_POOLS) {
-    pages::CopyArgs a{};
-    a.n_pools = n_pools - p0 < pages::MAX_POOLS ? n_pools - p0 : pages::MAX_POOLS;
-    int64_t most = 0;
-    for (int i = 0; i < a.n_pools; ++i) {
-      a.pool[i] = static_cast<uint8_t*>(pools[p0 + i]);
-      a.stride[i] = page_strides[p0 + i];
-      a.bytes[i] = page_bytes[p0 + i];
-      most = most > a.bytes[i] ? most : a.bytes[i];
-    }
-    a.src = src; a.dst = dst; a.count = count; a.n = n; a.P = P; a.err = err;
-    a.chunks = int((most + pages::CHUNK - 1) / pages::CHUNK);
-    const int64_t work = n * a.n_pools * a.chunks, cap = 8 * num_sms();
-    pages::copy_kernel<<<unsigned(work < cap ? work : cap), 256, 0, static_cast<cudaStream_t>(stream)>>>(a);
-    if (int r = launch_status("kv_copy_pages")) return r;
-  }
-  return MZB_OK;
+  pages::CopyArgs a{};
+  a.src = src; a.dst = dst; a.n = n; a.P = P; a.err = err;
+  return pages::copy_pages(pools, n_pools, a, "kv_copy_pages", static_cast<cudaStream_t>(stream));
 }

@@ -40,14 +40,15 @@ def _table(page_table, seq_lens, refs):
 
 def _pools(pools, pages, dev):
     pools = list(pools)
+    i = dev.index
     for p in pools:
-        shape, stride = p.shape, p.stride()
-        assert p.device == dev and len(shape) >= 2 and shape[0] == pages, \
+        shape, step = p.shape, p.stride(0)
+        assert p.get_device() == i and len(shape) >= 2 and shape[0] == pages, \
             f"each pool must be [{pages}, ...] on {dev}, got {tuple(shape)} on {p.device}"
-        n, size = p.numel() // max(1, shape[0]), p.element_size()
-        assert (p.is_contiguous() or p[0].is_contiguous()) and (stride[0] >= n or pages == 1), \
+        n, size = p.numel() // pages, p.element_size()
+        assert (p.is_contiguous() or p[0].is_contiguous()) and (step >= n or pages == 1), \
             "a pool's pages must be dense and apart"
-        assert n and n * size % 16 == 0 and (stride[0] * size % 16 == 0 or pages == 1) and p.storage_offset() * size % 16 == 0, \
+        assert n and not (n * size & 15 or (step * size & 15 and pages > 1) or p.storage_offset() * size & 15), \
             "a pool's pages must be 16-byte aligned and a multiple of 16 bytes"
     return pools
 
@@ -143,4 +144,5 @@ def copy_pages(pools, src: torch.Tensor, dst: torch.Tensor, *, check: bool = Fal
     pools = list(pools)
     assert pools, "copy_pages needs at least one pool"
     assert src.shape == dst.shape, f"src and dst must have one length, got {src.shape[0]} and {dst.shape[0]}"
+    assert pools[0].dim() and pools[0].shape[0], "the pools must not be empty"
     ops.kv_copy_pages(_pools(pools, pools[0].shape[0], src.device), src, dst, check)

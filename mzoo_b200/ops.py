@@ -567,13 +567,13 @@ def kv_free(page_table, seq_lens, refs, seqs, check):
         _raise_on(err, "kv free")
 
 
-def _copy(pools, src, dst, count, n, err, dev):
-    """One ``mzb_kv_copy_pages`` call; src / dst / count are device addresses."""
-    arr, m = ctypes.c_int64 * len(pools), len(pools)
-    _call_on(dev, "mzb_kv_copy_pages", arr(*(p.data_ptr() for p in pools)),
-         arr(*(p.numel() // p.shape[0] * p.element_size() for p in pools)),
-         arr(*(p.stride(0) * p.element_size() for p in pools)), m, src, dst, count, n, pools[0].shape[0],
-         err.data_ptr(), _lib.raw_stream(dev))
+def _pool_array(pools):
+    """(address, bytes of a page, bytes from page to page) of each pool, as the C ABI takes them."""
+    flat = []
+    for p in pools:
+        n, size = p.shape[0], p.element_size()
+        flat += (p.data_ptr(), p.numel() // n * size, p.stride(0) * size)
+    return (ctypes.c_int64 * len(flat))(*flat)
 
 
 @_define("kv_copy_pages(Tensor(a!)[] pools, Tensor src, Tensor dst, bool check) -> ()", lambda *a: None)
@@ -581,7 +581,8 @@ def kv_copy_pages(pools, src, dst, check):
     """``mzb_kv_copy_pages``: page src[i] to page dst[i] of every pool."""
     dev = src.device
     err = _err(dev, check)
-    _copy(pools, src.data_ptr(), dst.data_ptr(), None, src.shape[0], err, dev)
+    _call_on(dev, "mzb_kv_copy_pages", _pool_array(pools), len(pools), src.data_ptr(), dst.data_ptr(), len(src),
+             len(pools[0]), err.data_ptr(), _lib.raw_stream(dev))
     if check:
         _raise_on(err, "kv copy pages")
 
@@ -589,13 +590,12 @@ def kv_copy_pages(pools, src, dst, check):
 @_define("kv_fork(Tensor(a!)[] pools, Tensor(b!) page_table, Tensor(c!) seq_lens, Tensor(d!) refs, Tensor src,"
          " Tensor dst, int page, bool check) -> ()", lambda *a: None)
 def kv_fork(pools, page_table, seq_lens, refs, src, dst, page, check):
-    """``mzb_kv_fork`` and the copies of the partly filled pages."""
-    dev, n, (S, W) = page_table.device, src.shape[0], page_table.shape
+    """``mzb_kv_fork``."""
+    dev, n, (S, W) = page_table.device, len(src), page_table.shape
     err, ws = _err(dev, check), torch.empty(3 * n + S, dtype=torch.int32, device=dev)
-    _call_on(dev, "mzb_kv_fork", page_table.data_ptr(), seq_lens.data_ptr(), refs.data_ptr(), src.data_ptr(), dst.data_ptr(), n,
-         ws.data_ptr(), S, W, refs.shape[0], page, err.data_ptr(), _lib.raw_stream(dev))
-    if pools:
-        _copy(pools, ws.data_ptr(), ws.data_ptr() + 4 * n, None, n, err, dev)
+    _call_on(dev, "mzb_kv_fork", page_table.data_ptr(), seq_lens.data_ptr(), refs.data_ptr(), src.data_ptr(),
+             dst.data_ptr(), n, ws.data_ptr(), S, W, len(refs), page, _pool_array(pools), len(pools), err.data_ptr(),
+             _lib.raw_stream(dev))
     if check:
         _raise_on(err, "kv fork")
 
@@ -603,14 +603,12 @@ def kv_fork(pools, page_table, seq_lens, refs, src, dst, page, check):
 @_define("kv_compact(Tensor(a!)[] pools, Tensor page_table, Tensor refs, bool check) -> (Tensor, Tensor)",
          lambda pools, page_table, refs, check: (torch.empty_like(page_table), torch.empty_like(refs)))
 def kv_compact(pools, page_table, refs, check):
-    """``mzb_kv_compact`` and the moves; returns the new (page_table, refs)."""
-    dev, P = page_table.device, refs.shape[0]
+    """``mzb_kv_compact``; returns the new (page_table, refs)."""
+    dev, P = page_table.device, len(refs)
     err, ws = _err(dev, check), torch.empty(3 * P + 1, dtype=torch.int32, device=dev)
     table, new_refs = torch.empty_like(page_table), torch.empty_like(refs)
-    _call_on(dev, "mzb_kv_compact", page_table.data_ptr(), refs.data_ptr(), table.data_ptr(), new_refs.data_ptr(), ws.data_ptr(),
-         page_table.numel(), P, err.data_ptr(), _lib.raw_stream(dev))
-    if pools:
-        _copy(pools, ws.data_ptr(), ws.data_ptr() + 4 * P, ws.data_ptr() + 12 * P, P // 2, err, dev)
+    _call_on(dev, "mzb_kv_compact", page_table.data_ptr(), refs.data_ptr(), table.data_ptr(), new_refs.data_ptr(),
+             ws.data_ptr(), page_table.numel(), P, _pool_array(pools), len(pools), err.data_ptr(), _lib.raw_stream(dev))
     if check:
         _raise_on(err, "kv compact")
     return table, new_refs
