@@ -364,7 +364,11 @@ __global__ void __launch_bounds__(NT) compact_plan_kernel(const int32_t* refs, i
   __shared__ int ws[32];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   int n, mine = 0;
-  for (int64_t p0 = threadIdx.x * PT; p0 < P; p0 += NT * PT) {
+  int32_t first[PT];  // the first chunk stays in registers
+  load_refs(refs, threadIdx.x * PT, P, 0, first);
+#pragma unroll
+  for (int e = 0; e < PT; ++e) mine += first[e] > 0;
+  for (int64_t p0 = (NT + threadIdx.x) * PT; p0 < P; p0 += NT * PT) {
     int32_t r[PT];
     load_refs(refs, p0, P, 0, r);
 #pragma unroll
@@ -374,8 +378,13 @@ __global__ void __launch_bounds__(NT) compact_plan_kernel(const int32_t* refs, i
   int holes = 0, moved = 0;
   for (int64_t c0 = 0; c0 < P; c0 += NT * PT) {
     const int64_t p0 = c0 + threadIdx.x * PT;
-    int32_t r[PT];
-    load_refs(refs, p0, P, 0, r);
+    int32_t r[PT], goes[PT], left[PT];
+    if (c0 == 0) {
+#pragma unroll
+      for (int e = 0; e < PT; ++e) r[e] = first[e];
+    } else {
+      load_refs(refs, p0, P, 0, r);
+    }
     int hm = 0, total;  // holes in the low half, moves in the high half: at most NT * PT each
 #pragma unroll
     for (int e = 0; e < PT; ++e) hm += p0 + e < n ? (r[e] <= 0) : (r[e] > 0) << 16;
@@ -386,14 +395,25 @@ __global__ void __launch_bounds__(NT) compact_plan_kernel(const int32_t* refs, i
 #pragma unroll
     for (int e = 0; e < PT; ++e) {
       const int64_t p = p0 + e;
-      if (p >= P) continue;
       if (p < n) {
         if (r[e] <= 0) hole_list[ah++] = int32_t(p);
       } else if (r[e] > 0) {
         from_list[am++] = int32_t(p);
       }
-      to[p] = r[e] > 0 ? int32_t(p) : -1;
-      new_refs[p] = p < n && r[e] > 0 ? r[e] : 0;
+      goes[e] = r[e] > 0 ? int32_t(p) : -1;
+      left[e] = p < n && r[e] > 0 ? r[e] : 0;
+    }
+    if (p0 + PT <= P && ((reinterpret_cast<uintptr_t>(to) | reinterpret_cast<uintptr_t>(new_refs)) & 15) == 0) {
+#pragma unroll
+      for (int e = 0; e < PT; e += 4) {
+        *reinterpret_cast<int4*>(to + p0 + e) = make_int4(goes[e], goes[e + 1], goes[e + 2], goes[e + 3]);
+        *reinterpret_cast<int4*>(new_refs + p0 + e) = make_int4(left[e], left[e + 1], left[e + 2], left[e + 3]);
+      }
+    } else {
+      for (int e = 0; e < PT && p0 + e < P; ++e) {
+        to[p0 + e] = goes[e];
+        new_refs[p0 + e] = left[e];
+      }
     }
   }
   __syncthreads();
@@ -409,7 +429,7 @@ __global__ void __launch_bounds__(NT) compact_plan_kernel(const int32_t* refs, i
 
 constexpr int MAX_POOLS = 64;
 constexpr int CHUNK = 16384;  // bytes of a page that one block step copies: 256 threads x 4 x 16
-constexpr int COPY_BLOCKS = 8;  // blocks of an SM
+constexpr int COPY_BLOCKS = 32;  // blocks per SM at most: 8 resident ones that stay take 5 % longer, more empty ones cost too
 
 struct CopyArgs {
   uint8_t* pool[MAX_POOLS];
@@ -454,9 +474,9 @@ __global__ void __launch_bounds__(256) copy_kernel(const __grid_constant__ CopyA
     uint4 v[CHUNK / 4096];
     if (left >= CHUNK) {
 #pragma unroll
-      for (int q = 0; q < CHUNK / 4096; ++q) v[q] = __ldcs(from + threadIdx.x + 256 * q);
+      for (int q = 0; q < CHUNK / 4096; ++q) v[q] = from[threadIdx.x + 256 * q];
 #pragma unroll
-      for (int q = 0; q < CHUNK / 4096; ++q) __stcs(to + threadIdx.x + 256 * q, v[q]);
+      for (int q = 0; q < CHUNK / 4096; ++q) to[threadIdx.x + 256 * q] = v[q];
     } else {
 #pragma unroll
       for (int q = 0; q < CHUNK / 4096; ++q)
