@@ -41,7 +41,13 @@ struct PCfg {
   static constexpr int STAGE = 2 * Q_BYTES + NS * SLOT;  // output staging: 4 KB for each softmax warp
   static constexpr int TILES = STAGE + 8 * 4096;
   static constexpr int SMEM = TILES + 1024;
-  static constexpr int S_COL = 0, O_COL = 256;  // tile t: + 128 t
+  // TMEM columns.  D = 64 has room for P beside S: S is free for the next QK^T as soon as the softmax
+  // has read it, so the products leave the softmax's chain (SEP).  Else P takes S's place, 64 keys
+  // in the front of each half of it, and QK_t(j+1) follows PV_t(j).
+  static constexpr bool SEP = D == 64;
+  static constexpr int S_COL = 0;                           // + 128 t
+  static constexpr int P_COL = SEP ? 256 : 0, P_TILE = SEP ? 64 : 128, P_HALF = SEP ? 32 : 64;
+  static constexpr int O_COL = SEP ? 384 : 256, O_TILE = SEP ? 64 : 128;
   static_assert(SMEM <= 232448, "shared memory budget");
 };
 
@@ -67,7 +73,7 @@ struct Item {
 };
 
 enum PBar { P_QF = 0, P_QE = 2, P_SF = 4, P_PF = 6, P_OF = 10, P_OE = 12, P_ITF = 14, P_ITE = 16, P_CLC = 18, P_ASK = 19,
-            P_KF = 20, P_KE = P_KF + 8, P_VOK = P_KE + 8, P_NBAR = P_VOK + 8 };
+            P_KF = 20, P_KE = P_KF + 8, P_VOK = P_KE + 8, P_SE = P_VOK + 8, P_PE = P_SE + 2, P_NBAR = P_PE + 2 };
 constexpr int ITEM_READERS = 8 + 3;  // softmax warps, TMA, MMA, repair
 
 __device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
@@ -251,7 +257,7 @@ __global__ void __launch_bounds__(384, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < P_NBAR; ++i) {
       uint32_t c = 1;
-      if (i >= P_PF && i < P_PF + 4) c = 4;
+      if ((i >= P_PF && i < P_PF + 4) || i == P_SE || i == P_SE + 1) c = 4;
       if (i == P_OE || i == P_OE + 1) c = 4;
       if (i == P_ITE || i == P_ITE + 1) c = ITEM_READERS;
       if (i >= P_KE && i < P_KE + 8) c = 2;  // the last product that reads the slot; the repair warp
@@ -296,7 +302,8 @@ __global__ void __launch_bounds__(384, 1)
     // ---------------------------------------------------------------- softmax, output
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const int t = warp >> 2, sw = warp & 3, r = sw * 32 + lane;
-    const uint32_t scol = tc::taddr(tmem, sw * 32, C::S_COL + 128 * t), ocol = tc::taddr(tmem, sw * 32, C::O_COL + 128 * t);
+    const uint32_t scol = tc::taddr(tmem, sw * 32, C::S_COL + 128 * t), ocol = tc::taddr(tmem, sw * 32, C::O_COL + C::O_TILE * t);
+    const uint32_t pcol = tc::taddr(tmem, sw * 32, C::P_COL + C::P_TILE * t);
     const int rtok = r / a.g, rhead = r % a.g;
     uint32_t ns = 0, no = 0;
     while (next_item(m)) {
@@ -338,6 +345,11 @@ __global__ void __launch_bounds__(384, 1)
         tc::tmem_wait_ld();
 #pragma unroll
         for (int q = 0; q < 4; ++q) tc::reg_after_wait(sv[q]);
+        if constexpr (C::SEP) {  // the next scores may come
+          tc::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(&bars[P_SE + t]);
+        }
         float m4[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -351,13 +363,22 @@ __global__ void __launch_bounds__(384, 1)
         float mt = max2(max2(m4[0], m4[1]), max2(m4[2], m4[3])) * a.sl;
         mt = mt < INFINITY ? mt : NAN;
         const bool need = !(mt <= mx + 8.0f);
+        bool behind = C::SEP && j > 0;  // the previous PV may still read P and add to O
+        auto after_pv = [&]() {
+          if (!behind) return true;
+          behind = false;
+          const bool got = wait_all(P_PE + t, (ns - 1) & 1, 416);
+          tc::fence_after_sync();
+          return got;
+        };
         if (__any_sync(0xffffffffu, need)) {
+          if (!after_pv()) { ok = false; break; }
           const float mn = need ? mt : mx;
           const float alpha = need ? fast_exp2(mx - mn) : 1.0f;
           mx = mn;
           lsum *= alpha;
           ms = mx == -INFINITY ? 0.0f : mx;
-          if (j > 0) {  // S_FULL was committed behind the previous PV: O is complete
+          if (j > 0) {  // (not SEP: S_FULL was committed behind the previous PV, so O is complete)
 #pragma unroll 1
             for (int c0 = 0; c0 < D; c0 += 32) {
               uint32_t ov[32];
@@ -388,7 +409,8 @@ __global__ void __launch_bounds__(384, 1)
             acc[e & 1] = add_f32x2(acc[e & 1], pack_f32x2(p.x, p.y));
             pk[e] = pack2<DT>(p.x, p.y);
           }
-          tc::tmem_st16(scol + 64 * (q >> 1) + 16 * (q & 1), pk);
+          if (q == 0 && !after_pv()) { ok = false; break; }
+          tc::tmem_st16(pcol + C::P_HALF * (q >> 1) + 16 * (q & 1), pk);
           if (q & 1) {  // 64 keys' weights: their product can start
             tc::tmem_wait_st();
             tc::fence_before_sync();
@@ -396,6 +418,7 @@ __global__ void __launch_bounds__(384, 1)
             if (lane == 0) tc::mbar_arrive(&bars[P_PF + 2 * t + (q >> 1)]);
           }
         }
+        if (!ok) break;
         const float2 s0 = unpack_f32x2(add_f32x2(acc[0], acc[1]));
         lsum += s0.x + s0.y;
       }
@@ -530,7 +553,8 @@ __global__ void __launch_bounds__(384, 1)
       const uint32_t idesc_qk = tc::make_idesc(128, BN, fmt, fmt) | (a.neg ? 1u << 13 : 0u);
       const uint32_t idesc_pv = tc::make_idesc(128, D, fmt, fmt, false, true);
       const uint32_t q_base = smem_u32(qs), r_base = smem_u32(ring);
-      uint32_t g = 0, nq[2] = {0, 0}, np[2] = {0, 0}, vok = 0;
+      uint32_t g = 0, nq[2] = {0, 0}, np[2] = {0, 0}, se[2] = {0, 0}, vok = 0;
+      bool k_seen[2];
       while (next_item(m)) {
         if (tc::elect_one()) {
         const int nt[2] = {m.n0, m.n1}, n = max(m.n0, m.n1);
@@ -550,6 +574,35 @@ __global__ void __launch_bounds__(384, 1)
           tc::mma_commit(&bars[P_SF + t]);
           if (j == nt[t] - 1) tc::mma_commit(&bars[P_QE + t]);
         };
+        auto pv = [&](int t, int j, uint32_t gv) {  // O_t += P_t V_j, 64 keys as their weights come
+          if (ok && j == 0 && !tc::mbar_wait(&bars[P_OE + t], ((nq[t] - 1) & 1) ^ 1, a.err, 407)) ok = false;
+          const uint64_t vd = tc::make_sdesc<128>(r_base + (gv % C::NS) * C::SLOT, BN * 128, 1024);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (ok && !tc::mbar_wait(&bars[P_PF + 2 * t + h], np[t] & 1, a.err, 408)) ok = false;
+            if (!ok) continue;
+            tc::fence_after_sync();
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              tc::mma_ts(tmem + C::O_COL + C::O_TILE * t, tmem + C::P_COL + C::P_TILE * t + C::P_HALF * h + 8 * kk,
+                         tc::sdesc_add(vd, (4 * h + kk) * 16 * 128), idesc_pv, (j > 0 || h > 0 || kk > 0) ? 1u : 0u);
+          }
+          if (!ok) return;
+          ++np[t];
+          if constexpr (C::SEP) tc::mma_commit(&bars[P_PE + t]);
+          if (j == nt[t] - 1) tc::mma_commit(&bars[P_OF + t]);
+        };
+        int v_seen = -1;
+        auto full_v = [&](int j, uint32_t gv) {  // V_j is there, and repaired where it has to be
+          if (v_seen == j) return;
+          v_seen = j;
+          full(gv);
+          const uint32_t sv = gv % C::NS;
+          if (ok && j >= m.jfix) {
+            if (!tc::mbar_wait(&bars[P_VOK + sv], (vok >> sv) & 1, a.err, 406)) ok = false;
+            vok ^= 1u << sv;
+          }
+        };
         // slots of this item: K_j at g + 2 j, V_j at g + 2 j + 1
         if (n > 0) {
           full(g);
@@ -562,47 +615,61 @@ __global__ void __launch_bounds__(384, 1)
             }
           if (ok) tc::mma_commit(&bars[P_KE + g % C::NS]);
         }
-        for (int j = 0; j < n && ok; ++j) {
-          const uint32_t gv = g + 2 * j + 1, gk = gv + 1, sv = gv % C::NS;
-          bool have_v = false, have_k = false;
-#pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            if (!ok || j >= nt[t]) continue;
-            if (!have_v) {
-              full(gv);
-              if (ok && j >= m.jfix) {
-                if (!tc::mbar_wait(&bars[P_VOK + sv], (vok >> sv) & 1, a.err, 406)) ok = false;
-                vok ^= 1u << sv;
-              }
-              have_v = true;
+        if constexpr (C::SEP) {
+          // in the order of events when tile 1 is half a step behind: QK_0(j+1), PV_1(j-1), QK_1(j+1), PV_0(j)
+          auto next_qk = [&](int t, int j) {  // QK_t(j+1), once the softmax has read S_t(j)
+            if (!ok || j + 1 >= nt[t]) return;
+            if (!tc::mbar_wait(&bars[P_SE + t], se[t]++ & 1, a.err, 417)) ok = false;
+            if (!k_seen[j & 1]) {
+              full(g + 2 * j + 2);
+              k_seen[j & 1] = true;
             }
-            if (ok && j == 0 && !tc::mbar_wait(&bars[P_OE + t], ((nq[t] - 1) & 1) ^ 1, a.err, 407)) ok = false;
-            const uint64_t vd = tc::make_sdesc<128>(r_base + sv * C::SLOT, BN * 128, 1024);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {  // the weights of 64 keys each
-              if (ok && !tc::mbar_wait(&bars[P_PF + 2 * t + h], np[t] & 1, a.err, 408)) ok = false;
-              if (!ok) continue;
-              tc::fence_after_sync();
-#pragma unroll
-              for (int kk = 0; kk < 4; ++kk)
-                tc::mma_ts(tmem + C::O_COL + 128 * t, tmem + C::S_COL + 128 * t + 64 * h + 8 * kk,
-                           tc::sdesc_add(vd, (4 * h + kk) * 16 * 128), idesc_pv, (j > 0 || h > 0 || kk > 0) ? 1u : 0u);
-            }
-            if (!ok) continue;
-            ++np[t];
-            if (j == nt[t] - 1) tc::mma_commit(&bars[P_OF + t]);
-            if (j + 1 < nt[t]) {
-              if (!have_k) {
-                full(gk);
-                tc::fence_after_sync();
-                have_k = true;
+            tc::fence_after_sync();
+            if (ok) qk(t, j + 1, g + 2 * j + 2);
+          };
+          for (int j = 0; j <= n && ok; ++j) {
+            k_seen[j & 1] = false;
+            next_qk(0, j);
+            if (j > 0) {
+              if (ok && j - 1 < nt[1]) {
+                full_v(j - 1, g + 2 * j - 1);
+                pv(1, j - 1, g + 2 * j - 1);
               }
-              if (ok) qk(t, j + 1, gk);
+              if (ok) tc::mma_commit(&bars[P_KE + (g + 2 * j - 1) % C::NS]);
+            }
+            next_qk(1, j);
+            if (ok && j + 1 < n) tc::mma_commit(&bars[P_KE + (g + 2 * j + 2) % C::NS]);
+            if (ok && j < nt[0]) {
+              full_v(j, g + 2 * j + 1);
+              pv(0, j, g + 2 * j + 1);
             }
           }
-          if (ok) {
-            tc::mma_commit(&bars[P_KE + sv]);
-            if (j + 1 < n) tc::mma_commit(&bars[P_KE + gk % C::NS]);
+          // the softmax's last read of a tile's S is behind its last QK^T; its arrival is still to be counted
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            if (nt[t] > 0) ++se[t];
+        } else {
+          for (int j = 0; j < n && ok; ++j) {
+            const uint32_t gv = g + 2 * j + 1, gk = gv + 1;
+            bool have_k = false;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              if (!ok || j >= nt[t]) continue;
+              full_v(j, gv);
+              pv(t, j, gv);
+              if (ok && j + 1 < nt[t]) {
+                if (!have_k) {
+                  full(gk);
+                  tc::fence_after_sync();
+                  have_k = true;
+                }
+                if (ok) qk(t, j + 1, gk);
+              }
+            }
+            if (ok) {
+              tc::mma_commit(&bars[P_KE + gv % C::NS]);
+              if (j + 1 < n) tc::mma_commit(&bars[P_KE + gk % C::NS]);
+            }
           }
         }
         g += 2 * n;
