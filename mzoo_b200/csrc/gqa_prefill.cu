@@ -151,12 +151,12 @@ __device__ __forceinline__ uint32_t nonfinite2(uint32_t w) {
 // ---------------------------------------------------------------- work items
 
 // Item number -> (sequence, pair within it), by the scheduler warp.  Up to 32 sequences (a lane
-// for each): by descending pair index over all sequences, so that the longest causal key ranges
-// come first and the last blocks' shares are even; more: sequence after sequence, the last pair
-// first, from a cursor (a block's item numbers only grow).
+// for each): by descending end of the pair's key range, so that the longest items come first and
+// the last blocks' shares are even; more: sequence after sequence, the last pair first, from a
+// cursor (a block's item numbers only grow).
 struct Finder {
   int n, q0, nq, k0, nk;  // this lane's sequence (of 32 from cur_b)
-  int top, total, cur_b, cur_at;
+  int low, top, total, cur_b, cur_at;
 
   __device__ void load(const PrefillArgs& a, int lane) {
     const int b = cur_b + lane;
@@ -170,13 +170,20 @@ struct Finder {
       n = nq > 0 ? (nq + 2 * a.ntok - 1) / (2 * a.ntok) : 0;
     }
     total = __reduce_add_sync(0xffffffffu, n);
-    top = __reduce_max_sync(0xffffffffu, n);
+    low = __reduce_min_sync(0xffffffffu, n ? end_of(a, 0) : 0x7fffffff);
+    top = __reduce_max_sync(0xffffffffu, n ? end_of(a, n - 1) : -0x7fffffff);
   }
+  // a pair's key range ends here (or at the sequence's end)
+  __device__ int end_of(const PrefillArgs& a, int pair) { return nk - nq + (pair + 1) * 2 * a.ntok; }
   __device__ void init(const PrefillArgs& a, int lane) {
     cur_b = cur_at = 0;
     load(a, lane);
   }
-  __device__ int above(int t) { return __reduce_add_sync(0xffffffffu, max(0, n - t)); }  // pairs with index >= t
+  // pairs that end at x or later
+  __device__ int above(const PrefillArgs& a, int x) {
+    const int before = max(0, x - end_of(a, 0) + 2 * a.ntok - 1) / (2 * a.ntok);
+    return __reduce_add_sync(0xffffffffu, n ? max(0, n - before) : 0);
+  }
   // -> the lane of the sequence, or -1 behind the last item
   __device__ int find(const PrefillArgs& a, int64_t idx, int lane, int& pair) {
     while (idx >= cur_at + total) {
@@ -197,16 +204,18 @@ struct Finder {
       pair = __shfl_sync(0xffffffffu, inc, l) - 1 - r;
       return l;
     }
-    int lo = 0, hi = top;  // above(lo) > r >= above(hi)
+    int lo = low, hi = top + 1;  // above(lo) > r >= above(hi)
     while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (above(mid) > r) lo = mid; else hi = mid;
+      const int mid = lo + (hi - lo) / 2;
+      if (above(a, mid) > r) lo = mid; else hi = mid;
     }
-    pair = lo;
-    const int rank = r - above(hi);  // among the sequences that have this pair
-    const unsigned have = __ballot_sync(0xffffffffu, n > lo);
-    const bool mine = n > lo && __popc(have & ((1u << lane) - 1)) == rank;
-    return __ffs(__ballot_sync(0xffffffffu, mine)) - 1;
+    // the sequences that have a pair with this end, at most one each
+    const int off = lo - end_of(a, 0), mine = off >= 0 && off % (2 * a.ntok) == 0 ? off / (2 * a.ntok) : n;
+    const unsigned have = __ballot_sync(0xffffffffu, mine < n);
+    const int rank = r - above(a, hi);
+    const int l = __ffs(__ballot_sync(0xffffffffu, mine < n && __popc(have & ((1u << lane) - 1)) == rank)) - 1;
+    pair = __shfl_sync(0xffffffffu, mine, max(l, 0));
+    return l;
   }
   // by the sequence's lane
   __device__ void fill(const PrefillArgs& a, int pair, int hk, Item* m) {
