@@ -275,16 +275,18 @@ MZB_API int mzb_kv_unpack_fp4(const uint8_t* codes, const uint8_t* scales, void*
  *   cu_k[b+1] of k / v (int32 [B+1], ascending from 0).  Row i of a sequence of nq tokens and
  *   nk keys sees the keys j <= i + nk - nq (causal) or all; head h reads K / V head
  *   h / (Hq / Hkv).  o [Tq, Hq, D] and lse fp32 [Tq, Hq] (natural log) dense; a row that sees
- *   no key has o = 0 and lse = -inf.  Hq / Hkv at most 128; D in {64, 96, 128}.
+ *   no key has o = 0 and lse = -inf.  Hq / Hkv at most 128; D in {64, 96, 128}.  ws:
+ *   mzb_gqa_prefill_ws(...) floats (0 unless few rows meet many keys), 16-byte aligned.
  * mzb_gqa_decode -- one token per sequence over a paged cache.  q [B, Hq, D]; k_pages /
  *   v_pages [P, Hkv, page, D] by their page, head and token strides in elements; key t of
  *   sequence b is slot t % page of page page_table[b, t / page], t < min(seq_lens[b], W * page).
  *   Entries past a sequence's length are never used (ids outside [0, P) are clamped).
  *   ws: mzb_gqa_decode_ws(...) floats.  page in {16, 32, 64, 128}.
  */
+MZB_API int64_t mzb_gqa_prefill_ws(int64_t Tq, int64_t Tk, int B, int Hq, int Hkv, int D);
 MZB_API int mzb_gqa_prefill(const void* q, const void* k, const void* v, const int32_t* cu_q, const int32_t* cu_k,
-                            void* o, float* lse, int64_t Tq, int64_t Tk, int B, int Hq, int Hkv, int D, int dtype,
-                            int64_t sq_t, int64_t sq_h, int64_t sk_t, int64_t sk_h, int64_t sv_t, int64_t sv_h,
+                            void* o, float* lse, float* ws, int64_t Tq, int64_t Tk, int B, int Hq, int Hkv, int D,
+                            int dtype, int64_t sq_t, int64_t sq_h, int64_t sk_t, int64_t sk_h, int64_t sv_t, int64_t sv_h,
                             int causal, float softmax_scale, int* err, void* stream);
 MZB_API int64_t mzb_gqa_decode_ws(int B, int Hq, int Hkv, int D, int W, int page);
 MZB_API int mzb_gqa_decode(const void* q, const void* k_pages, const void* v_pages, const int32_t* page_table,

@@ -61,7 +61,8 @@ SIGNATURES = {
     "mzb_kv_unpack_fp8": [_P, _P, _P, _I64, _I32, _P],
     "mzb_kv_pack_fp4": [_P, _P, _P, _I64, _I32, _P],
     "mzb_kv_unpack_fp4": [_P, _P, _P, _I64, _I32, _P],
-    "mzb_gqa_prefill": [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I32, _I32, _I32, _I32, _I32, _I64, _I64, _I64, _I64,
+    "mzb_gqa_prefill_ws": [_I64, _I64, _I32, _I32, _I32, _I32],
+    "mzb_gqa_prefill": [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I32, _I32, _I32, _I32, _I32, _I64, _I64, _I64, _I64,
                         _I64, _I64, _I32, _F32, _P, _P],
     "mzb_gqa_decode_ws": [_I32, _I32, _I32, _I32, _I32, _I32],
     "mzb_gqa_decode": [_P, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _I64, _I32, _I64, _I64,
@@ -73,7 +74,7 @@ SIGNATURES = {
     "mzb_kv_compact": [_P, _P, _P, _P, _P, _I64, _I64, _P, _I32, _P, _P],
     "mzb_kv_copy_pages": [_P, _I32, _P, _P, _I64, _I64, _P, _P],
 }
-_RESTYPE = {"mzb_last_error": ctypes.c_char_p, "mzb_gqa_decode_ws": _I64}
+_RESTYPE = {"mzb_last_error": ctypes.c_char_p, "mzb_gqa_decode_ws": _I64, "mzb_gqa_prefill_ws": _I64}
 
 _lib = None
 

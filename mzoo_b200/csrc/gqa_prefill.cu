@@ -23,6 +23,7 @@
 // one tile's products run while the other's exponentials do.  S and P of a tile share 128 TMEM
 // columns (P overwrites S), O takes D; a row's O is rescaled only when its maximum has grown
 // by more than 2^8 (fp32 sums and weights of at most 2^8 lose nothing by waiting).
+// Where few rows meet many keys, an item's key range is cut into parts that a second kernel joins.
 #include "tc.cuh"
 
 namespace mzb {
@@ -60,14 +61,20 @@ struct PrefillArgs {
   int B, Hq, Hkv, g, ntok, causal, neg;  // g = Hq / Hkv, ntok = 128 / g tokens per tile
   float sl;                              // |scale| log2 e
   int* err;
+  // a call with few work items cuts the longer key ranges into up to `splits` (1: none) parts
+  int splits;
+  int* parts;         // [Tq, Hq]: parts of a row; 1: written in place
+  float *plse, *po;   // [splits, Tq * Hq], [splits, Tq * Hq, D]
 };
+constexpr int MIN_PART = 6;  // key tiles of a part at least (a part costs a block's start and its share of the join)
 
-// One work item, in shared memory.
+// One work item, in shared memory.  Of a part, k0, nk and shift are those of its keys alone.
 struct Item {
   int tok0, tok_end;  // first packed token, end of the sequence
   int i0, shift;      // tok0's place in its sequence; keys seen by place i: min(nk, i + shift) (not causal: nk)
   int k0, nk, hk;     // first packed key, keys, K / V head
   int n0, n1;         // key tiles of the query tiles
+  int part, of;       // which part of how many
   int lim0, jfix;     // keys that tok0 sees (the fewest); V tiles from jfix on reach past them
   int done;
 };
@@ -185,14 +192,14 @@ struct Finder {
     return __reduce_add_sync(0xffffffffu, n ? max(0, n - before) : 0);
   }
   // -> the lane of the sequence, or -1 behind the last item
-  __device__ int find(const PrefillArgs& a, int64_t idx, int lane, int& pair) {
+  __device__ int find(const PrefillArgs& a, int idx, int lane, int& pair) {
     while (idx >= cur_at + total) {
       if (cur_b + 32 >= a.B) return -1;
       cur_at += total;
       cur_b += 32;
       load(a, lane);
     }
-    const int r = int(idx) - cur_at;
+    const int r = idx - cur_at;
     if (a.B > 32) {
       int inc = n;
 #pragma unroll
@@ -217,32 +224,44 @@ struct Finder {
     pair = __shfl_sync(0xffffffffu, mine, max(l, 0));
     return l;
   }
-  // by the sequence's lane
-  __device__ void fill(const PrefillArgs& a, int pair, int hk, Item* m) {
-    const int i0 = pair * 2 * a.ntok;
-    auto sees = [&](int i) { return a.causal ? max(0, min(nk, i + nk - nq + 1)) : nk; };
-    auto tiles = [&](int t) {
-      const int first = i0 + t * a.ntok, last = min(first + a.ntok, nq) - 1;
-      return last >= first ? (sees(last) + BN - 1) / BN : 0;
-    };
+  // by the sequence's lane: the item, or part `part` of it
+  __device__ void fill(const PrefillArgs& a, int pair, int hk, int part, int of, Item* m) {
+    const int i0 = pair * 2 * a.ntok, n = max(tiles(a, i0, 0), tiles(a, i0, 1));
+    // (an item without parts: plain numbers, no division)
+    const int j0 = of == 1 ? 0 : int((int64_t)n * part / of), j1 = of == 1 ? n : int((int64_t)n * (part + 1) / of);
     m->tok0 = q0 + i0;
     m->tok_end = q0 + nq;
     m->i0 = i0;
-    m->shift = a.causal ? nk - nq + 1 : 0x3fffffff;
-    m->k0 = k0;
-    m->nk = nk;
+    m->shift = a.causal ? nk - nq + 1 - j0 * BN : 0x3fffffff;
+    m->k0 = k0 + j0 * BN;
+    m->nk = min(nk, j1 * BN) - j0 * BN;
     m->hk = hk;
-    m->n0 = tiles(0);
-    m->n1 = tiles(1);
-    m->lim0 = sees(i0);
+    m->n0 = max(0, min(tiles(a, i0, 0), j1) - j0);
+    m->n1 = max(0, min(tiles(a, i0, 1), j1) - j0);
+    m->lim0 = max(0, min(m->nk, sees(a, i0) - j0 * BN));
     m->jfix = m->lim0 / BN;
+    m->part = part;
+    m->of = of;
     m->done = 0;
+  }
+  // keys that place i of this lane's sequence sees; key tiles of query tile t of the pair at i0
+  __device__ int sees(const PrefillArgs& a, int i) { return a.causal ? max(0, min(nk, i + nk - nq + 1)) : nk; }
+  __device__ int tiles(const PrefillArgs& a, int i0, int t) {
+    const int first = i0 + t * a.ntok, last = min(first + a.ntok, nq) - 1;
+    return last >= first ? (sees(a, last) + BN - 1) / BN : 0;
+  }
+  // parts of this lane's pair
+  __device__ int parts_of(const PrefillArgs& a, int pair) {
+    const int i0 = pair * 2 * a.ntok;
+    return max(1, min(a.splits, max(tiles(a, i0, 0), tiles(a, i0, 1)) / MIN_PART));
   }
 };
 
 // ---------------------------------------------------------------- kernel
 
-template <int DT, int D>
+// CUT: items may be parts of a key range (compiled apart: its registers and branches would cost the
+// calls without parts 2-4 %).
+template <int DT, int D, bool CUT>
 __global__ void __launch_bounds__(384, 1)
     prefill_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                    const __grid_constant__ CUtensorMap tv, const __grid_constant__ PrefillArgs a) {
@@ -285,6 +304,7 @@ __global__ void __launch_bounds__(384, 1)
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = *tmem_slot;
+  if constexpr (CUT) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // a wait that the whole warp agrees on; false: it (or another role) gave up
   auto wait_all = [&](int bar, uint32_t parity, int code) -> bool {
@@ -433,8 +453,14 @@ __global__ void __launch_bounds__(384, 1)
       }
       if (!ok) break;
       const int64_t row = (int64_t)tok * a.Hq + m.hk * a.g + rhead;
+      if (CUT && row_ok && m.part == 0) a.parts[row] = m.of;
+      const bool cut = CUT && m.of > 1;  // into the workspace, in 32 bits
+      float* prow = cut ? a.po + ((int64_t)m.part * a.Tq * a.Hq + row) * D : nullptr;
+      float* lse_at = cut ? a.plse + (int64_t)m.part * a.Tq * a.Hq + row : a.lse + row;
       if (n == 0) {  // no row of this tile sees a key
-        if (row_ok) {
+        if (row_ok && cut) {
+          *lse_at = -INFINITY;  // the part's output is not read
+        } else if (row_ok) {
           uint4* mine = reinterpret_cast<uint4*>(static_cast<T*>(a.o) + row * D);
 #pragma unroll 1
           for (int c = 0; c < D / 8; ++c) mine[c] = make_uint4(0, 0, 0, 0);
@@ -461,8 +487,24 @@ __global__ void __launch_bounds__(384, 1)
       const uint8_t* ld_at = stage + (lane >> 2) * 64 + (((lane & 3) ^ ((lane >> 3) & 3)) * 16);
       const uint64_t inv2 = pack_f32x2(inv, inv);
       constexpr int CB = D % 64 ? 1 : 2;  // blocks of 32 channels in flight
+      if (CUT && cut) {
 #pragma unroll 1
-      for (int c0 = 0; c0 < D; c0 += 32 * CB) {
+        for (int c0 = 0; c0 < D; c0 += 32) {
+          uint32_t ov[32];
+          tc::tmem_ld32(ocol + c0, ov);
+          tc::tmem_wait_ld();
+          tc::reg_after_wait(ov);
+          if (row_ok) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              *reinterpret_cast<float4*>(prow + c0 + e) =
+                  make_float4(__uint_as_float(ov[e]) * inv, __uint_as_float(ov[e + 1]) * inv,
+                              __uint_as_float(ov[e + 2]) * inv, __uint_as_float(ov[e + 3]) * inv);
+          }
+        }
+      }
+#pragma unroll 1
+      for (int c0 = cut ? D : 0; c0 < D; c0 += 32 * CB) {
         uint32_t ov[CB][32];
 #pragma unroll
         for (int b = 0; b < CB; ++b) tc::tmem_ld32(ocol + c0 + 32 * b, ov[b]);
@@ -504,11 +546,12 @@ __global__ void __launch_bounds__(384, 1)
 #pragma unroll 1
           for (int e = 0; e < D; ++e) {
             const float x = Elem<DT>::load(vr[e]);
-            if (!isfinite(x)) mine[e] = Elem<DT>::store(Elem<DT>::load(mine[e]) + x);
+            if (isfinite(x)) continue;
+            if (cut) prow[e] += x; else mine[e] = Elem<DT>::store(Elem<DT>::load(mine[e]) + x);
           }
         }
       }
-      if (row_ok) a.lse[row] = lim > 0 ? (mx + log2f(lsum)) * LN2 : -INFINITY;
+      if (row_ok) *lse_at = lim > 0 ? (mx + log2f(lsum)) * LN2 : -INFINITY;
       tc::fence_before_sync();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&bars[P_OE + t]);
@@ -690,18 +733,24 @@ __global__ void __launch_bounds__(384, 1)
       // ---------------------------------------------------------------- scheduler
       Finder f;
       f.init(a, lane);
-      int64_t idx = blockIdx.x;
+      uint32_t idx = blockIdx.x;
       int k = 0;
       uint32_t tries = 0;
       bool more = true;
       while (more) {
         int pair = 0;
-        const int who = f.find(a, idx / a.Hkv, lane, pair);
+        const uint32_t item = CUT ? idx / uint32_t(a.splits) : idx, part = CUT ? idx % uint32_t(a.splits) : 0;
+        int who = f.find(a, int(item / uint32_t(a.Hkv)), lane, pair);
+        int of = 1;
+        if (CUT && who >= 0) {
+          of = __shfl_sync(0xffffffffu, f.parts_of(a, pair), who);
+          if (int(part) >= of) who = -1;
+        }
         if (who >= 0) {
           const int s = k & 1;
           if (!wait_all(P_ITE + s, ((k >> 1) & 1) ^ 1, 411)) break;
           if (lane == who) {
-            f.fill(a, pair, int(idx % a.Hkv), &items[s]);
+            f.fill(a, pair, int(item % uint32_t(a.Hkv)), int(part), of, &items[s]);
             tc::mbar_arrive(&bars[P_ITF + s]);
           }
           if (!wait_all(P_ASK, k & 1, 415)) break;
@@ -801,6 +850,53 @@ __global__ void __launch_bounds__(384, 1)
   }
 }
 
+// A warp per row: the parts of a cut key range, in their order.
+template <int DT, int D>
+__global__ void __launch_bounds__(256) prefill_join_kernel(const __grid_constant__ PrefillArgs a) {
+  using T = typename Elem<DT>::T;
+  constexpr int C = D / 32;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int lane = threadIdx.x & 31;
+  const int64_t rows = a.Tq * a.Hq, row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const int n = a.parts[row];
+  if (n <= 1) return;
+  float top = -INFINITY;
+  bool nan = false;
+  for (int i = 0; i < n; ++i) {
+    const float x = a.plse[i * rows + row];
+    top = fmaxf(top, x);
+    nan |= x != x;
+  }
+  const float ref = top == -INFINITY ? 0.0f : top;
+  float sum = nan ? NAN : 0.0f, acc[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) acc[c] = 0.0f;
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) {
+    const float x = a.plse[i * rows + row];
+    if (x == -INFINITY) continue;  // a part without keys for this row has no output
+    const float w = exp2f((x - ref) * LOG2E);
+    sum += w;
+#pragma unroll
+    for (int c = 0; c < C; ++c) acc[c] += w * a.po[(i * rows + row) * D + lane + 32 * c];
+  }
+  const float inv = top == -INFINITY && !nan ? 0.0f : 1.0f / sum;
+#pragma unroll
+  for (int c = 0; c < C; ++c) static_cast<T*>(a.o)[row * D + lane + 32 * c] = Elem<DT>::store(acc[c] * inv);
+  if (lane == 0) a.lse[row] = sum == 0.0f ? -INFINITY : ref + logf(sum);
+}
+
+// Query tile pairs: at least as many as any packing of Tq tokens into B sequences has.
+int64_t pairs_bound(int64_t Tq, int B, int g) { return Tq / (2 * (128 / g)) + (B < Tq ? B : Tq); }
+
+// Parts of a key range: only where the items would leave more than half of the SMs without work.
+int split_count(int64_t Tq, int64_t Tk, int B, int Hq, int Hkv) {
+  const int64_t items = pairs_bound(Tq, B, Hq / Hkv) * Hkv, most = (Tk + BN - 1) / BN / MIN_PART;
+  const int64_t n = num_sms() / items;
+  return int(n < 2 || most < 2 ? 1 : n < most ? n : most);
+}
+
 template <int DT, int D>
 int launch(const void* q, const void* k, PrefillArgs a, int64_t sq_t, int64_t sq_h, int64_t sk_t, int64_t sk_h,
            cudaStream_t st) {
@@ -823,14 +919,30 @@ int launch(const void* q, const void* k, PrefillArgs a, int64_t sq_t, int64_t sq
                             base[i], dims, s, box, CU_TENSOR_MAP_SWIZZLE_128B))
       return r;
   }
-  auto kern = prefill_kernel<DT, D>;
+  auto kern = a.splits > 1 ? prefill_kernel<DT, D, true> : prefill_kernel<DT, D, false>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
     return launch_status("gqa_prefill(smem attr)");
-  // at least as many pairs of query tiles as any packing of Tq tokens into B sequences has
-  const int64_t pairs = a.Tq / (2 * a.ntok) + (a.B < a.Tq ? a.B : a.Tq);
-  MZB_REQUIRE(pairs * a.Hkv < (int64_t(1) << 31), MZB_ERR_SHAPE, "gqa_prefill: too large");
-  kern<<<unsigned(pairs * a.Hkv), 384, C::SMEM, st>>>(m[0], m[1], m[2], a);
-  return launch_status("gqa_prefill");
+  const int64_t blocks = pairs_bound(a.Tq, a.B, a.g) * a.Hkv * a.splits;
+  MZB_REQUIRE(blocks < (int64_t(1) << 31), MZB_ERR_SHAPE, "gqa_prefill: too large");
+  kern<<<unsigned(blocks), 384, C::SMEM, st>>>(m[0], m[1], m[2], a);
+  if (int r = launch_status("gqa_prefill")) return r;
+  if (a.splits == 1) return MZB_OK;
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(unsigned((a.Tq * a.Hq + 7) / 8));
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, prefill_join_kernel<DT, D>, a);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    set_error("gqa_prefill(join): launch failed: %s", cudaGetErrorString(e));
+    return MZB_ERR_LAUNCH;
+  }
+  return MZB_OK;
 }
 
 }  // namespace gqa
@@ -838,8 +950,14 @@ int launch(const void* q, const void* k, PrefillArgs a, int64_t sq_t, int64_t sq
 
 using namespace mzb;
 
+extern "C" int64_t mzb_gqa_prefill_ws(int64_t Tq, int64_t Tk, int B, int Hq, int Hkv, int D) {
+  if (Tq <= 0 || Tk <= 0 || B <= 0 || Hkv <= 0 || Hq < Hkv || Hq % Hkv || Hq / Hkv > 128) return 0;
+  const int n = gqa::split_count(Tq, Tk, B, Hq, Hkv);
+  return n == 1 ? 0 : ((Tq * Hq * (n + 1) + 3) & ~int64_t(3)) + n * Tq * Hq * D;
+}
+
 extern "C" int mzb_gqa_prefill(const void* q, const void* k, const void* v, const int32_t* cu_q, const int32_t* cu_k,
-                               void* o, float* lse, int64_t Tq, int64_t Tk, int B, int Hq, int Hkv, int D, int dtype,
+                               void* o, float* lse, float* ws, int64_t Tq, int64_t Tk, int B, int Hq, int Hkv, int D, int dtype,
                                int64_t sq_t, int64_t sq_h, int64_t sk_t, int64_t sk_h, int64_t sv_t, int64_t sv_h,
                                int causal, float softmax_scale, int* err, void* stream) {
   MZB_REQUIRE(Tq >= 0 && Tk >= 0 && B >= 1 && Tq < (int64_t(1) << 30) && Tk < (int64_t(1) << 30), MZB_ERR_SHAPE,
@@ -859,6 +977,11 @@ extern "C" int mzb_gqa_prefill(const void* q, const void* k, const void* v, cons
   a.sl = (softmax_scale < 0 ? -softmax_scale : softmax_scale) * gqa::LOG2E;
   if (a.sl < 1e-37f) a.sl = 1e-37f;  // scale 0: all weights still 1, and a masked -inf stays -inf
   a.err = err;
+  a.splits = gqa::split_count(Tq, Tk, B, Hq, Hkv);
+  MZB_REQUIRE(a.splits == 1 || ws != nullptr, MZB_ERR_SHAPE, "gqa_prefill: needs a workspace");
+  a.parts = reinterpret_cast<int*>(ws);
+  a.plse = ws + Tq * Hq;
+  a.po = ws + ((Tq * Hq * (a.splits + 1) + 3) & ~int64_t(3));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
 #define MZB_GO(DT, DD) gqa::launch<DT, DD>(q, k, a, sq_t, sq_h, sk_t, sk_h, st)
   if (dtype == MZB_BF16) return D == 64 ? MZB_GO(MZB_BF16, 64) : D == 96 ? MZB_GO(MZB_BF16, 96) : MZB_GO(MZB_BF16, 128);

@@ -490,14 +490,23 @@ def gqa_prefill(q, k, v, cu_q, cu_k, causal, scale, check):
     Tq, Hq, D = q.shape
     o = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty(Tq, Hq, dtype=torch.float32, device=dev)
+    Tk, Hkv, _ = k.shape
+    B = len(cu_q) - 1
+    n = _gqa_prefill_ws(Tq, Tk, B, Hq, Hkv, D, dev.index) if Tq * Hq <= 1 << 15 else 0  # more rows are never split
+    ws = torch.empty(n, dtype=torch.float32, device=dev) if n else None
     err = _err(dev, check)
-    (sq_t, sq_h, _), (sk_t, sk_h, _), (sv_t, sv_h, _), (Tk, Hkv, _) = q.stride(), k.stride(), v.stride(), k.shape
+    (sq_t, sq_h, _), (sk_t, sk_h, _), (sv_t, sv_h, _) = q.stride(), k.stride(), v.stride()
     _call_on(dev, "mzb_gqa_prefill", q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), o.data_ptr(),
-         lse.data_ptr(), Tq, Tk, len(cu_q) - 1, Hq, Hkv, D, _lib.DTYPE_CODE[q.dtype], sq_t, sq_h, sk_t, sk_h, sv_t,
+         lse.data_ptr(), ws.data_ptr() if n else None, Tq, Tk, B, Hq, Hkv, D, _lib.DTYPE_CODE[q.dtype], sq_t, sq_h, sk_t, sk_h, sv_t,
          sv_h, causal, scale, err.data_ptr(), _lib.raw_stream(dev))
     if check:
         _raise_on(err, "gqa prefill")
     return o, lse
+
+
+@functools.lru_cache(maxsize=256)
+def _gqa_prefill_ws(Tq: int, Tk: int, B: int, Hq: int, Hkv: int, D: int, device_index: int) -> int:
+    return _lib.lib().mzb_gqa_prefill_ws(Tq, Tk, B, Hq, Hkv, D)
 
 
 @functools.lru_cache(maxsize=256)

@@ -131,6 +131,28 @@ def test_prefill_long_rows(cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv,d", [(1, 1, 64), (12, 2, 96), (8, 8, 128), (40, 1, 128)])
+@pytest.mark.parametrize("new,keys", [([1], [1537]), ([2, 5, 1], [1600, 3, 4000]), ([9], [8 * 128]), ([33, 0, 7], [1800, 2000, 0]),
+                                      ([3000], [900]), ([20], [12 * 128 + 7])])
+def test_prefill_few_rows_many_keys(cuda, hq, hkv, d, new, keys):
+    """Key ranges cut into parts and joined, rows without keys among them."""
+    if sum(new) * hq > 4000:
+        hq = hkv
+    _prefill(cuda, torch.bfloat16, hq, hkv, d, new, keys)
+    _prefill(cuda, torch.float16, hq, hkv, d, new, keys, causal=False, scale=-0.2)
+
+
+@pytest.mark.gpu
+def test_prefill_parts_keep_nan_apart(cuda):
+    """In a cut key range, values that a row does not see stay out of it and those it sees arrive."""
+    def edit(q, k, v):
+        v[2990, :, 3] = math.inf   # token 2 of 12 new ones and later see it
+        v[2995] = math.nan
+        v[100, :, 7] = -math.inf   # in the first part, seen by all
+    _prefill(cuda, torch.bfloat16, 4, 2, 128, [12], [3000], edit=edit)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("scale", [0.0, 0.5, -0.3])
 def test_prefill_scale_and_fused_projection(cuda, scale):
     _prefill(cuda, torch.bfloat16, 6, 2, 128, [50, 131], [50, 131], scale=scale, fused=True)
@@ -394,7 +416,7 @@ def test_c_entry_refusals():
     from mzoo_b200 import _lib
     lib = _lib.lib()
     pre = lambda D=64, hq=4, hkv=2, dt=1, B=1: lib.mzb_gqa_prefill(  # noqa: E731
-        0, 0, 0, 0, 0, 0, 0, 8, 8, B, hq, hkv, D, dt, 256, 64, 128, 64, 128, 64, 1, 1.0, None, None)
+        0, 0, 0, 0, 0, 0, 0, 0, 8, 8, B, hq, hkv, D, dt, 256, 64, 128, 64, 128, 64, 1, 1.0, None, None)
     assert pre(D=80) == _lib.MZB_ERR_UNSUPPORTED and b"head dim" in lib.mzb_last_error()
     assert pre(hq=5) == _lib.MZB_ERR_SHAPE and pre(dt=0) == _lib.MZB_ERR_UNSUPPORTED and pre(B=0) == _lib.MZB_ERR_SHAPE
     assert pre() == _lib.MZB_ERR_SHAPE and b"error word" in lib.mzb_last_error()
