@@ -477,8 +477,18 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Decod
   const int hq = int(row % a.Hq), hk = hq / a.g, h = hq % a.g;
   const int2 span = ws_span(a)[b * a.Hkv + hk];
   if (span.x == span.y) return;
-  const int n = span.y - span.x + 1;
+  const int n = min(span.y - span.x + 1, MAX_BLOCKS);
   auto part = [&](int i) { return ws_part(a, i == 0 ? 2 * span.x + 1 : 2 * (span.x + i), D); };
+  // the first eight parts of each warp are on their way while the weights are found
+  constexpr int AHEAD = 8;
+  float2 va[AHEAD], vb[AHEAD];
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i)
+    if (lane < C4 && warp + 4 * i < n) {
+      const float* p = part(warp + 4 * i) + 2 * a.g + h * D + 4 * lane;
+      va[i] = *reinterpret_cast<const float2*>(p);
+      vb[i] = *reinterpret_cast<const float2*>(p + 2);
+    }
   // every warp for itself: the same numbers in the same order
   float2 ml[PER];
   float mx = -INFINITY, ls = 0.0f;
@@ -502,8 +512,17 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Decod
   __syncthreads();
   if (lane < C4) {
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-    for (int i = warp; i < n; i += 4) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+      if (warp + 4 * i < n) {
+        const float al = weight[warp + 4 * i];
+        acc.x += va[i].x * al;
+        acc.y += va[i].y * al;
+        acc.z += vb[i].x * al;
+        acc.w += vb[i].y * al;
+      }
+#pragma unroll 4
+    for (int i = warp + 4 * AHEAD; i < n; i += 4) {
       const float* p = part(i) + 2 * a.g + h * D + 4 * lane;
       const float2 x = *reinterpret_cast<const float2*>(p), y = *reinterpret_cast<const float2*>(p + 2);
       const float al = weight[i];

@@ -169,9 +169,10 @@ struct Finder {
     const int b = cur_b + lane;
     n = 0;
     if (b < a.B) {
-      const int q1 = a.cu_q[b + 1], ka = a.cu_k[b], kb = a.cu_k[b + 1];
-      q0 = a.cu_q[b];
-      nq = q1 - q0;
+      // (whatever the offsets hold, rows stay inside the tensors)
+      const int qa = a.cu_q[b], qb = a.cu_q[b + 1], ka = a.cu_k[b], kb = a.cu_k[b + 1];
+      q0 = max(0, min(qa, int(a.Tq)));
+      nq = max(0, min(qb, int(a.Tq)) - q0);
       k0 = max(0, min(ka, int(a.Tk)));
       nk = max(0, min(kb, int(a.Tk)) - k0);
       n = nq > 0 ? (nq + 2 * a.ntok - 1) / (2 * a.ntok) : 0;

@@ -115,7 +115,7 @@ def test_prefill_lengths(cuda, n):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("new,keys", [([3, 70], [200, 131]), ([128], [384]), ([1, 1, 1], [1, 129, 300]),
-                                      ([40, 5], [3, 0]), ([300], [20]), ([0, 9, 0], [50, 9, 0]), ([200], [129])])
+                                      ([40, 5], [3, 0]), ([5], [0]), ([300], [20]), ([0, 9, 0], [50, 9, 0]), ([200], [129])])
 @pytest.mark.parametrize("causal", [True, False])
 def test_prefill_other_key_lengths(cuda, new, keys, causal):
     """Chunks over earlier keys, and fewer keys than tokens: rows that see no key."""
@@ -128,6 +128,46 @@ def test_prefill_long_rows(cuda):
     """Many key tiles; a few rows of a long prompt."""
     _prefill(cuda, torch.bfloat16, 2, 1, 128, [3], [5000])
     _prefill(cuda, torch.float16, 2, 1, 64, [200], [2300])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seqs", [32, 33, 64, 301])
+def test_prefill_many_sequences(cuda, seqs):
+    g = torch.Generator().manual_seed(seqs)
+    new = torch.randint(0, 40, (seqs,), generator=g).tolist()
+    keys = [n + int(p) for n, p in zip(new, torch.randint(0, 30, (seqs,), generator=g))]
+    _prefill(cuda, torch.bfloat16, 4, 2, 64, new, new)
+    _prefill(cuda, torch.float16, 3, 1, 64, new, keys)
+
+
+@pytest.mark.gpu
+def test_prefill_no_tokens_and_wild_offsets(cuda):
+    """No tokens; offsets that leave the tensors touch nothing outside them."""
+    none = torch.zeros(0, 4, 64, dtype=torch.bfloat16, device=cuda)
+    o, lse = gqa_attn.prefill(none, none, none, torch.zeros(2, dtype=torch.int32, device=cuda), check=True)
+    assert o.shape == (0, 4, 64) and lse.shape == (0, 4)
+    big = torch.randn(3000, 4, 64, device=cuda).to(torch.bfloat16)
+    q = big[1000:1100]
+    wild = torch.tensor([-50, 60, 2 ** 30, 40, 5000], dtype=torch.int32, device=cuda)
+    gqa_attn.prefill(q, big[:200], big[:200], wild, wild, check=True)
+    want = gqa_attn.prefill(q[:60], big[:60], big[:60], _cu([60]).to(cuda))[0]
+    wild = torch.tensor([-9, 60, 100], dtype=torch.int32, device=cuda)
+    got = gqa_attn.prefill(q, big[:200], big[:200], wild, wild, check=True)[0]
+    assert torch.equal(got[:60], want)
+
+
+@pytest.mark.gpu
+def test_prefill_offsets_past_32_bits(cuda):
+    """Outputs behind 2^31 elements; thousands of sequences."""
+    T, hq, n = 270000, 64, 100
+    q = torch.empty(T, hq, 128, dtype=torch.bfloat16, device=cuda)
+    q.copy_(torch.randn(hq, 128, device=cuda, generator=torch.Generator(device=cuda).manual_seed(0)))
+    q[-n:] = torch.randn(n, hq, 128, device=cuda).to(torch.bfloat16)
+    k, v = (torch.randn(T, 1, 128, device=cuda).to(torch.bfloat16) for _ in range(2))
+    cu = torch.arange(0, T + 1, n, dtype=torch.int32, device=cuda)
+    o, lse = gqa_attn.prefill(q, k, v, cu, check=True)
+    want = gqa_attn.prefill(q[-n:].clone(), k[-n:], v[-n:], _cu([n]).to(cuda), check=True)
+    assert o.numel() > 2 ** 31 and torch.equal(o[-n:], want[0]) and torch.equal(lse[-n:], want[1])
 
 
 @pytest.mark.gpu
@@ -323,6 +363,56 @@ def test_decode_token_major_pool_and_wild_ids(cuda):
     wild = torch.where(table < 0, torch.tensor([2 ** 31 - 1, -2 ** 31, -7] * 3, dtype=torch.int32), table)
     got = gqa_attn.decode(q, both[:, 0].transpose(1, 2), both[:, 1].transpose(1, 2), wild.to(cuda), lens, check=True)
     assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.gpu
+def test_decode_offsets_past_32_bits_and_empty_batches(cuda):
+    g = torch.Generator().manual_seed(9)
+    P, hkv, page, d = 18000, 8, 128, 128
+    kp, vp = (torch.empty(P, hkv, page, d, dtype=torch.bfloat16, device=cuda) for _ in range(2))
+    assert kp.numel() > 2 ** 31
+    few = [_randn(g, torch.bfloat16, 3, hkv, page, d).to(cuda) for _ in range(2)]
+    for pool, x in zip((kp, vp), few):
+        pool[P - 3:] = x
+    q, lens = _randn(g, torch.bfloat16, 1, 16, d).to(cuda), torch.tensor([300], dtype=torch.int32, device=cuda)
+    table = torch.tensor([[P - 1, P - 3, P - 2]], dtype=torch.int32, device=cuda)
+    got = gqa_attn.decode(q, kp, vp, table, lens, check=True)
+    want = gqa_attn.decode(q, *few, table - (P - 3), lens, check=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    o, lse = gqa_attn.decode(q[:0], *few, table[:0], lens[:0], check=True)
+    assert o.shape == (0, 16, d) and lse.shape == (0, 16)
+    o, lse = gqa_attn.decode(q, *few, table[:, :0], lens, check=True)
+    assert not o.any() and bool((lse == -math.inf).all())
+
+
+@pytest.mark.gpu
+def test_decode_step_in_a_graph(cuda):
+    """A captured step (cache write and attention) follows the lengths and tables of its replay."""
+    from mzoo_b200 import kv_pages
+    g = torch.Generator().manual_seed(4)
+    B, hq, hkv, d, page, W = 5, 8, 2, 64, 16, 40
+    q, k, v = (_randn(g, torch.bfloat16, B, h, d).to(cuda) for h in (hq, hkv, hkv))
+    kp, vp = (_randn(g, torch.bfloat16, B * W, hkv, page, d).to(cuda) for _ in range(2))
+    table = torch.randperm(B * W, generator=g).view(B, W).to(torch.int32).to(cuda)
+    lens = torch.tensor([1, 17, 600, 0, 40], dtype=torch.int32, device=cuda)
+
+    def step():
+        kv_pages.append(k, v, kp, vp, table, lens)
+        return gqa_attn.decode(q, kp, vp, table, lens + 1)
+    side = torch.cuda.Stream(cuda)
+    side.wait_stream(torch.cuda.current_stream(cuda))
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream(cuda).wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for n in ([3, 90, 620, 5, 0], [0, 0, 639, 16, 15]):
+        lens.copy_(torch.tensor(n, dtype=torch.int32))
+        table.copy_(table.flip(0))
+        q.copy_(q.flip(0))
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, step()))
 
 
 @pytest.mark.gpu
