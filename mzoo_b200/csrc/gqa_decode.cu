@@ -144,19 +144,29 @@ __global__ void __launch_bounds__(288, 1)
       tc::prefetch_tmap(&tk);
       tc::prefetch_tmap(&tv);
     }
-    // this block's run of tiles: first (sequence, head, tile) and how many
-    int b = 0, hk = 0, t0 = 0;
+    // this block's run of tiles: first (sequence, head, tile) and how many.  A lane keeps the length of
+    // one sequence of the 32 from `base_b`: every look at a length is a shuffle, not another load.
+    int b = 0, hk = 0, t0 = 0, base_b = 0, my_len = 0;
     int64_t left = 0;
+    auto load_lens = [&](int from) {
+      base_b = from;
+      my_len = from + lane < a.B ? len_of(a, from + lane) : 0;
+    };
+    auto len_at = [&](int x) {  // (the whole warp; x only grows)
+      if (x >= base_b + 32) load_lens(x);
+      return __shfl_sync(0xffffffffu, my_len, x - base_b);
+    };
+    auto tiles_of = [](int len) { return (len + TK - 1) / TK; };
     if (a.blocks == 0) {
       b = blockIdx.x / a.Hkv;
       hk = blockIdx.x % a.Hkv;
-      left = (len_of(a, b) + TK - 1) / TK;
+      load_lens(b);
+      left = tiles_of(len_at(b));
     } else {
       int64_t total = 0;
       for (int b0 = 0; b0 < a.B; b0 += 32) {
-        int64_t n = b0 + lane < a.B ? (len_of(a, b0 + lane) + TK - 1) / TK : 0;
-#pragma unroll
-        for (int d = 16; d; d >>= 1) n += __shfl_xor_sync(0xffffffffu, n, d);
+        load_lens(b0);
+        const int64_t n = __reduce_add_sync(0xffffffffu, tiles_of(my_len));
         total += n;
       }
       total *= a.Hkv;
@@ -165,7 +175,8 @@ __global__ void __launch_bounds__(288, 1)
       if (left > 0) {
         int64_t at = 0;
         for (int b0 = 0;; b0 += 32) {
-          const int64_t n = b0 + lane < a.B ? (int64_t)((len_of(a, b0 + lane) + TK - 1) / TK) * a.Hkv : 0;
+          if (b0 != base_b) load_lens(b0);
+          const int64_t n = (int64_t)tiles_of(my_len) * a.Hkv;
           int64_t inc = n;
 #pragma unroll
           for (int d = 1; d < 32; d <<= 1) {
@@ -177,7 +188,7 @@ __global__ void __launch_bounds__(288, 1)
             const int l = __ffs(hit) - 1;
             b = b0 + l;
             const int64_t in = lo - at - __shfl_sync(0xffffffffu, inc - n, l);
-            const int64_t tiles = __shfl_sync(0xffffffffu, n, l) / a.Hkv;
+            const int tiles = __shfl_sync(0xffffffffu, tiles_of(my_len), l);
             hk = int(in / tiles);
             t0 = int(in % tiles);
             break;
@@ -190,8 +201,8 @@ __global__ void __launch_bounds__(288, 1)
     const int per_tile = TK / rows;              // boxes of a tile (per K / V and column block)
     uint32_t g = 0;
     bool ok = true;
-    while (left > 0 && ok) {
-      const int len = len_of(a, b), tiles = (len + TK - 1) / TK;
+    while (left > 0 && ok && b < a.B) {
+      const int len = len_at(b), tiles = tiles_of(len);
       const int n = int(min((int64_t)(tiles - t0), left));  // this block's segment: tiles t0 .. t0 + n
       const bool begins = t0 == 0, ends = t0 + n == tiles;
       const int part = begins && ends ? -1 : begins ? 2 * (int)blockIdx.x + 1 : 2 * (int)blockIdx.x;
@@ -246,7 +257,7 @@ __global__ void __launch_bounds__(288, 1)
       if (++hk == a.Hkv) {
         hk = 0;
         ++b;
-        while (left > 0 && len_of(a, b) == 0) ++b;
+        while (left > 0 && b < a.B && len_at(b) == 0) ++b;
       }
     }
     // the end, as a stage without data
