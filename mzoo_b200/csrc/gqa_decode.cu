@@ -33,7 +33,7 @@ struct DecodeArgs {
   float* lse;
   float* ws;
   int64_t P, sq_b, sq_h;
-  int B, Hq, Hkv, g, W, page, stages, blocks;  // blocks 0: one block per (sequence, head), no parts
+  int B, Hq, Hkv, g, W, page, page_log, stages, blocks;  // blocks 0: one block per (sequence, head), no parts
   float sl;                                    // scale * log2 e
   int* err;
 };
@@ -197,9 +197,11 @@ __global__ void __launch_bounds__(288, 1)
         }
       }
     }
-    const int rows = min(a.page, TK);            // rows of a TMA box
-    const int per_tile = TK / rows;              // boxes of a tile (per K / V and column block)
-    uint32_t g = 0;
+    // rows of a TMA box, boxes of a tile (per K / V and column block), as powers of two: a division by a
+    // number of the launch costs ~80 cycles, and five of them a tile made this loop the limit
+    const int rows_log = min(a.page_log, 6), rows = 1 << rows_log, tile_log = 6 - rows_log;
+    int s = 0;
+    uint32_t phase = 0;
     bool ok = true;
     while (left > 0 && ok && b < a.B) {
       const int len = len_at(b), tiles = tiles_of(len);
@@ -213,33 +215,32 @@ __global__ void __launch_bounds__(288, 1)
       }
       // page ids of 32 boxes at a time, one per lane, the next ones in flight meanwhile
       const int32_t* row = a.table + (int64_t)b * a.W;
-      const int box0 = t0 * per_tile, boxes = (len + rows - 1) / rows;  // boxes with live keys
+      const int box0 = t0 << tile_log, boxes = (len + rows - 1) >> rows_log;  // boxes with live keys
       auto ids = [&](int x) {  // box x of the sequence
         int p = 0;
-        if (x < boxes) p = row[(int64_t)x * rows / a.page];
+        if (x < boxes) p = row[x >> (a.page_log - rows_log)];
         return max(0, min(p, int(a.P - 1)));
       };
       int cur = ids(box0 + lane), nxt = ids(box0 + 32 + lane), base = box0;
-      for (int i = 0; i < n; ++i, ++g) {
-        const int t = t0 + i, keys = min(TK, len - t * TK), live = (keys + rows - 1) / rows;
-        const uint32_t s = g % a.stages;
-        if ((t * per_tile) - base >= 32) {
+      for (int i = 0; i < n; ++i) {
+        const int t = t0 + i, keys = min(TK, len - t * TK), live = (keys + rows - 1) >> rows_log;
+        if ((t << tile_log) - base >= 32) {
           base += 32;
           cur = nxt;
           nxt = ids(base + 32 + lane);
         }
-        const bool got = !*abort_flag && tc::mbar_wait(&empty[s], ((g / a.stages) & 1) ^ 1, a.err, 421);
+        const bool got = !*abort_flag && tc::mbar_wait(&empty[s], phase ^ 1, a.err, 421);
         if (!__all_sync(0xffffffffu, got)) { ok = false; break; }
         // page ids of the tile's boxes, then all copies by one elected lane (behind a condition that
         // differs by lane each copy's operands are made uniform in a loop: ~700 ns a tile)
         int pid[4];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) pid[x] = __shfl_sync(0xffffffffu, cur, min(t * per_tile + x - base, 31));
+        for (int x = 0; x < 4; ++x) pid[x] = __shfl_sync(0xffffffffu, cur, min((t << tile_log) + x - base, 31));
         if (tc::elect_one()) {
           meta[s] = Meta{b, hk, keys, (i == 0 ? FIRST : 0) | (i == n - 1 ? LAST : 0), part};
           tc::mbar_expect_tx(&full[s], uint32_t(live) * rows * 128 * C::DB * 2);
           uint8_t* to = smem + s * C::STAGE;
-          const int slot = (t * TK) % a.page;
+          const int slot = (t * TK) & (a.page - 1);
 #pragma unroll
           for (int x = 0; x < 4; ++x)
             if (x < live) {
@@ -251,6 +252,10 @@ __global__ void __launch_bounds__(288, 1)
             }
         }
         __syncwarp();
+        if (++s == a.stages) {
+          s = 0;
+          phase ^= 1;
+        }
       }
       left -= n;
       t0 = 0;
@@ -261,8 +266,7 @@ __global__ void __launch_bounds__(288, 1)
       }
     }
     // the end, as a stage without data
-    const uint32_t s = g % a.stages;
-    const bool got = ok && !*abort_flag && tc::mbar_wait(&empty[s], ((g / a.stages) & 1) ^ 1, a.err, 422);
+    const bool got = ok && !*abort_flag && tc::mbar_wait(&empty[s], phase ^ 1, a.err, 422);
     if (__all_sync(0xffffffffu, got)) {
       if (lane == 0) {
         meta[s].flags = END;
@@ -305,9 +309,14 @@ __global__ void __launch_bounds__(288, 1)
     // blocks; V transposed: (keys 0-7, 8-15) x (channels 0-7, 8-15) as (b0, b1) of two channel blocks
     const int krow = (lane & 7) + ((lane >> 4) << 3), kch = (lane >> 3) & 1;
     const int vrow = lane & 15, vch = lane >> 4;
+    int s = -1;
+    uint32_t phase = 0;
     for (uint32_t g = 0;; ++g) {
-      const uint32_t s = g % a.stages;
-      const bool got = !*abort_flag && tc::mbar_wait(&full[s], (g / a.stages) & 1, a.err, 423);
+      if (++s == a.stages) {
+        s = 0;
+        phase ^= 1;
+      }
+      const bool got = !*abort_flag && tc::mbar_wait(&full[s], phase, a.err, 423);
       if (!__all_sync(0xffffffffu, got)) {
         *abort_flag = 1;
         break;
@@ -641,6 +650,7 @@ extern "C" int mzb_gqa_decode(const void* q, const void* k_pages, const void* v_
   a.q = q; a.table = page_table; a.lens = seq_lens; a.o = o; a.lse = lse; a.ws = ws;
   a.P = P; a.sq_b = sq_b; a.sq_h = sq_h;
   a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.g = Hq / Hkv; a.W = W; a.page = page;
+  a.page_log = page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7;
   a.sl = softmax_scale * gqad::LOG2E;
   a.err = err;
   const int64_t sk[3] = {sk_p, sk_h, sk_t}, sv[3] = {sv_p, sv_h, sv_t};
