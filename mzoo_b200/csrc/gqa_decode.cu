@@ -5,13 +5,13 @@
 //   o = softmax(scale q K^T) V; a sequence of length 0: o = 0, lse = -inf.
 //
 // The live part of the cache is read once and everything else is small, so the kernel is
-// built to keep HBM busy.  The keys of every (sequence, K / V head) are cut into tiles of 64,
+// built to keep HBM busy.  The keys of every (sequence, K / V head) are cut into tiles of 128,
 // the tiles of all of them form one list, and each of one block per SM takes an equal run of
 // it, whatever the lengths: a warp walks the page tables and feeds a ring of shared-memory
 // stages (K and V of one tile each, ~200 KB in flight per SM) by TMA, eight warps do the
 // products.  The query heads of a group are the 16 rows of mma.sync tiles (the tensor work is
 // ~20 % of the time that the bytes take, so larger tensor instructions would gain nothing): a
-// group of up to 16 heads is split over the keys by 4 x 2 warps, a larger one over head tiles.
+// group of up to 16 heads is split over a tile's keys by eight warps, a larger one over head tiles too.
 // A (sequence, head) that lies in several blocks' runs leaves its (maximum, sum, output) parts in
 // a workspace; a second kernel, started early and waiting, joins them in a fixed order.
 #include "tc.cuh"
@@ -21,8 +21,8 @@ namespace gqad {
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
-constexpr int TK = 64;         // keys per tile
-constexpr int MIN_TILES = 4;   // a block's run is at least this long
+constexpr int TK = 128, TK_LOG = 7;  // keys per tile
+constexpr int MIN_TILES = 2;         // a block's run is at least this long
 constexpr int MAX_BLOCKS = 160;
 constexpr int MAX_STAGES = 12;
 
@@ -104,15 +104,14 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, u
 
 __device__ __forceinline__ int len_of(const DecodeArgs& a, int b) { return max(0, min(a.lens[b], a.W * a.page)); }
 
-// MT: head tiles of 16.  Warps: MT 1: tiles alternate between two groups of four warps, each warp 16 keys;
-// MT > 1: warp = head tile x key part, each part TK / (8 / MT) keys of every tile.
+// MT: head tiles of 16.  A warp has one of them and TK / (8 / MT) keys of every tile (MT 1: 16).
 template <int DT, int D, int MT>
 __global__ void __launch_bounds__(288, 1)
     decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                   const __grid_constant__ DecodeArgs a) {
   using C = DCfg<D>;
   using T = typename Elem<DT>::T;
-  constexpr int KP = MT == 1 ? 4 : 8 / MT;  // warps that share a tile's keys
+  constexpr int KP = 8 / MT;                // warps that share a tile's keys
   constexpr int STEPS = TK / KP / 16;       // 16-key steps of a warp per tile
   constexpr int PARTS = 8 / MT;             // partial results of a head tile to merge
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -121,7 +120,7 @@ __global__ void __launch_bounds__(288, 1)
   __shared__ float sm_m[8][16], sm_l[8][16];
   __shared__ int abort_s;
   volatile int* abort_flag = &abort_s;
-  float* merge = reinterpret_cast<float*>(smem + a.stages * C::STAGE);  // [8 warps][min(g, 16)][D]
+  float* merge = reinterpret_cast<float*>(smem + a.stages * C::STAGE);  // [8 warps][min(g, 16)][D / 2]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (smem_u32(smem) & 1023) {
     if (threadIdx.x == 0) atomicExch(a.err, MZB_ERR_ALIGN);
@@ -199,7 +198,7 @@ __global__ void __launch_bounds__(288, 1)
     }
     // rows of a TMA box, boxes of a tile (per K / V and column block), as powers of two: a division by a
     // number of the launch costs ~80 cycles, and five of them a tile made this loop the limit
-    const int rows_log = min(a.page_log, 6), rows = 1 << rows_log, tile_log = 6 - rows_log;
+    const int rows_log = min(a.page_log, TK_LOG), rows = 1 << rows_log, tile_log = TK_LOG - rows_log;
     int s = 0;
     uint32_t phase = 0;
     bool ok = true;
@@ -233,16 +232,16 @@ __global__ void __launch_bounds__(288, 1)
         if (!__all_sync(0xffffffffu, got)) { ok = false; break; }
         // page ids of the tile's boxes, then all copies by one elected lane (behind a condition that
         // differs by lane each copy's operands are made uniform in a loop: ~700 ns a tile)
-        int pid[4];
+        int pid[8];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) pid[x] = __shfl_sync(0xffffffffu, cur, min((t << tile_log) + x - base, 31));
+        for (int x = 0; x < 8; ++x) pid[x] = __shfl_sync(0xffffffffu, cur, min((t << tile_log) + x - base, 31));
         if (tc::elect_one()) {
           meta[s] = Meta{b, hk, keys, (i == 0 ? FIRST : 0) | (i == n - 1 ? LAST : 0), part};
           tc::mbar_expect_tx(&full[s], uint32_t(live) * rows * 128 * C::DB * 2);
           uint8_t* to = smem + s * C::STAGE;
           const int slot = (t * TK) & (a.page - 1);
 #pragma unroll
-          for (int x = 0; x < 4; ++x)
+          for (int x = 0; x < 8; ++x)
             if (x < live) {
 #pragma unroll
               for (int cb = 0; cb < C::DB; ++cb) {
@@ -292,7 +291,7 @@ __global__ void __launch_bounds__(288, 1)
         reinterpret_cast<uint4*>(static_cast<T*>(a.o) + row * D)[x] = make_uint4(0, 0, 0, 0);
       for (int x = threadIdx.x; x < a.g; x += 256) a.lse[row + x] = -INFINITY;
     }
-    const int mt = MT == 1 ? 0 : warp % MT, kp = MT == 1 ? (warp & 3) : warp / MT, grp = MT == 1 ? warp >> 2 : 0;
+    const int mt = warp % MT, kp = warp / MT;
     const int r0 = lane >> 2, c0 = (lane & 3) * 2;
     uint32_t qf[D / 16][4];
     float o[D / 8][4], m[2], l[2];
@@ -311,7 +310,7 @@ __global__ void __launch_bounds__(288, 1)
     const int vrow = lane & 15, vch = lane >> 4;
     int s = -1;
     uint32_t phase = 0;
-    for (uint32_t g = 0;; ++g) {
+    while (true) {
       if (++s == a.stages) {
         s = 0;
         phase ^= 1;
@@ -337,7 +336,7 @@ __global__ void __launch_bounds__(288, 1)
           qf[kk][3] = ld(r0 + 8, 16 * kk + c0 + 8);
         }
       }
-      if (MT > 1 || (g & 1) == grp) {
+      {
         const uint32_t kt = smem_u32(smem + s * C::STAGE), vt = kt + C::K_BYTES;
 #pragma unroll 1
         for (int st = 0; st < STEPS; ++st) {
@@ -441,42 +440,47 @@ __global__ void __launch_bounds__(288, 1)
           sm_l[warp][r0] = l[0];
           sm_l[warp][r0 + 8] = l[1];
         }
-        float* mine = merge + warp * gr * D;
+        // in two halves of the channels: the ring needs the shared memory more
+        float* mine = merge + warp * gr * (D / 2);
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          if (r0 < gr) *reinterpret_cast<float2*>(mine + r0 * D + 8 * i + c0) = make_float2(o[i][0], o[i][1]);
-          if (r0 + 8 < gr) *reinterpret_cast<float2*>(mine + (r0 + 8) * D + 8 * i + c0) = make_float2(o[i][2], o[i][3]);
-        }
-        tc::bar_sync(1, 256);
-        for (int x = threadIdx.x; x < a.g * (D / 2); x += 256) {
-          const int h = x / (D / 2), d = (x % (D / 2)) * 2, tile = h >> 4, r = h & 15;
-          float mx = -INFINITY;
+        for (int half = 0; half < 2; ++half) {
 #pragma unroll
-          for (int i = 0; i < PARTS; ++i) mx = fmaxf(mx, sm_m[MT == 1 ? i : i * MT + tile][r]);
-          const float ms = mx == -INFINITY ? 0.0f : mx;
-          float ls = 0.0f;
-          float2 acc = make_float2(0.0f, 0.0f);
-#pragma unroll
-          for (int i = 0; i < PARTS; ++i) {
-            const int wp = MT == 1 ? i : i * MT + tile;
-            const float al = fast_exp2(sm_m[wp][r] - ms);
-            const float2 v = *reinterpret_cast<const float2*>(merge + (wp * gr + r) * D + d);
-            ls += sm_l[wp][r] * al;
-            acc.x += v.x * al;
-            acc.y += v.y * al;
+          for (int i = 0; i < D / 16; ++i) {
+            const float(&x)[4] = o[half * (D / 16) + i];
+            if (r0 < gr) *reinterpret_cast<float2*>(mine + r0 * (D / 2) + 8 * i + c0) = make_float2(x[0], x[1]);
+            if (r0 + 8 < gr) *reinterpret_cast<float2*>(mine + (r0 + 8) * (D / 2) + 8 * i + c0) = make_float2(x[2], x[3]);
           }
-          if (w.part < 0) {
-            const int64_t row = (int64_t)w.b * a.Hq + w.hk * a.g + h;
-            const float inv = 1.0f / ls;
-            *reinterpret_cast<uint32_t*>(static_cast<T*>(a.o) + row * D + d) = pack2<DT>(acc.x * inv, acc.y * inv);
-            if (d == 0) a.lse[row] = (mx + log2f(ls)) * LN2;
-          } else {
-            float* to = ws_part(a, w.part, D);
-            *reinterpret_cast<float2*>(to + 2 * a.g + h * D + d) = acc;
-            if (d == 0) *reinterpret_cast<float2*>(to + 2 * h) = make_float2(mx, ls);
+          tc::bar_sync(1, 256);
+          for (int x = threadIdx.x; x < a.g * (D / 4); x += 256) {
+            const int h = x / (D / 4), dh = (x % (D / 4)) * 2, d = half * (D / 2) + dh, tile = h >> 4, r = h & 15;
+            float mx = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < PARTS; ++i) mx = fmaxf(mx, sm_m[i * MT + tile][r]);
+            const float ms = mx == -INFINITY ? 0.0f : mx;
+            float ls = 0.0f;
+            float2 acc = make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int i = 0; i < PARTS; ++i) {
+              const int wp = i * MT + tile;
+              const float al = fast_exp2(sm_m[wp][r] - ms);
+              const float2 v = *reinterpret_cast<const float2*>(merge + (wp * gr + r) * (D / 2) + dh);
+              ls += sm_l[wp][r] * al;
+              acc.x += v.x * al;
+              acc.y += v.y * al;
+            }
+            if (w.part < 0) {
+              const int64_t row = (int64_t)w.b * a.Hq + w.hk * a.g + h;
+              const float inv = 1.0f / ls;
+              *reinterpret_cast<uint32_t*>(static_cast<T*>(a.o) + row * D + d) = pack2<DT>(acc.x * inv, acc.y * inv);
+              if (d == 0) a.lse[row] = (mx + log2f(ls)) * LN2;
+            } else {
+              float* to = ws_part(a, w.part, D);
+              *reinterpret_cast<float2*>(to + 2 * a.g + h * D + d) = acc;
+              if (d == 0) *reinterpret_cast<float2*>(to + 2 * h) = make_float2(mx, ls);
+            }
           }
+          tc::bar_sync(1, 256);
         }
-        tc::bar_sync(1, 256);
         clear();
       }
     }
@@ -590,8 +594,8 @@ int launch(const void* k, const void* v, DecodeArgs a, const int64_t* sk, const 
                             i ? v : k, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B))
       return r;
   }
-  const int merge = 8 * (a.g < 16 ? a.g : 16) * D * 4;
-  const int budget = 227 * 1024 - 4096 - merge;
+  const int merge = 8 * (a.g < 16 ? a.g : 16) * (D / 2) * 4;
+  const int budget = 227 * 1024 - 2048 - merge;  // 2 KB: the static arrays
   a.stages = budget / C::STAGE < MAX_STAGES ? budget / C::STAGE : MAX_STAGES;
   a.blocks = short_table(a.W, a.page) ? 0 : block_count();
   auto kern = decode_kernel<DT, D, MT>;
