@@ -13,6 +13,7 @@ import torch
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libmzb200.so")
+TORCH_LIB_PATH = os.path.join(_HERE, "libmzb200_torch.so")  # the serving ops' torch kernels, over libmzb200.so
 
 MZB_OK = 0
 MZB_ERR_SHAPE = -1
@@ -99,13 +100,26 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+torch_ops_loaded = False
+
+
+def load_torch_ops() -> None:
+    """Register the C++ kernels of the serving ops with torch (once)."""
+    global torch_ops_loaded
+    if not torch_ops_loaded:
+        if not os.path.exists(TORCH_LIB_PATH):
+            raise ImportError(f"{TORCH_LIB_PATH} is missing: build it with `python -m mzoo_b200.build` "
+                              "(mzoo_b200 has no CPU or eager fallback)")
+        lib()  # libmzb200.so, which it is linked to
+        msg = ctypes.create_string_buffer(2000)
+        if ctypes.CDLL(TORCH_LIB_PATH).mzb_torch_register(msg, ctypes.c_size_t(len(msg))):
+            raise ImportError(f"{TORCH_LIB_PATH} does not fit this package (build it with `python -m mzoo_b200.build "
+                              f"--force`): {msg.value.decode(errors='replace').splitlines()[0]}")
+        torch_ops_loaded = True
+
+
 def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
-
-
-def raw_stream(device: torch.device) -> int:
-    """``stream_ptr`` without building a Stream object (2 us a call, a fifth of a small decode step)."""
-    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def check(status: int, what: str) -> None:

@@ -1,0 +1,179 @@
+// The serving-step ops of torch.library (`mzb::gqa_*`, `mzb::kv_*`) as C++ kernels over the C ABI:
+// allocation, current stream, one C call.  Through ctypes and the dispatcher's way back into
+// Python such a call takes ~16 us of the host, more than the smallest decode step takes on the
+// device; here ~6.  Schemas and fake implementations are declared in ops.py; argument checks
+// with their messages are the wrappers' (gqa_attn.py, kv_pages.py) and the C ABI's.
+#include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
+#include <ATen/ops/empty_like.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/library.h>
+
+#include "../../include/mzb200.h"
+
+namespace {
+
+using at::Tensor;
+
+// A non-zero status becomes a RuntimeError whose last word is the status; ops.py turns it into
+// the exception that the other ops raise.
+void ok(int status, const char* what) {
+  if (status != MZB_OK) TORCH_CHECK(false, what, ": ", mzb_last_error(), " [mzb status ", status, "]");
+}
+
+int code_of(const Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return MZB_F32;
+    case at::kBFloat16: return MZB_BF16;
+    case at::kHalf: return MZB_F16;
+    default: return -1;
+  }
+}
+
+struct Call {  // the tensor's device and that device's current stream
+  c10::cuda::CUDAGuard guard;
+  void* stream;
+  explicit Call(const Tensor& t) : guard(t.device()), stream(c10::cuda::getCurrentCUDAStream(t.device().index()).stream()) {}
+};
+
+template <class T = int32_t>
+T* ptr(const Tensor& t) {
+  return static_cast<T*>(t.data_ptr());
+}
+
+using Err = std::optional<Tensor>;  // (None only where nothing is launched: fake tensors, tracing)
+int* word(const Err& err) {
+  TORCH_CHECK(err.has_value(), "a launch needs its error word");
+  return static_cast<int*>(err->data_ptr());
+}
+
+Tensor floats(int64_t n, const Tensor& like) { return at::empty({n}, like.options().dtype(at::kFloat)); }
+Tensor ints(int64_t n, const Tensor& like) { return at::empty({n}, like.options().dtype(at::kInt)); }
+
+// (address, bytes of a page, bytes from page to page) of each pool
+std::vector<int64_t> pool_array(at::TensorList pools) {
+  std::vector<int64_t> x;
+  x.reserve(3 * pools.size());
+  for (const Tensor& p : pools) {
+    const int64_t size = p.element_size();
+    x.insert(x.end(), {reinterpret_cast<int64_t>(p.data_ptr()), p.numel() / std::max<int64_t>(1, p.size(0)) * size, p.stride(0) * size});
+  }
+  return x;
+}
+
+std::tuple<Tensor, Tensor> gqa_prefill(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu_q,
+                                       const Tensor& cu_k, const Err& err, bool causal, double scale) {
+  TORCH_CHECK(q.dim() == 3 && k.dim() == 3 && v.dim() == 3 && cu_q.numel() >= 2, "gqa_prefill: bad dimensions");
+  Call c(q);
+  const int64_t Tq = q.size(0), Tk = k.size(0), Hq = q.size(1), Hkv = k.size(1), D = q.size(2), B = cu_q.numel() - 1;
+  Tensor o = at::empty({Tq, Hq, D}, q.options()), lse = at::empty({Tq, Hq}, q.options().dtype(at::kFloat)), ws;
+  const int64_t n = mzb_gqa_prefill_ws(Tq, Tk, int(B), int(Hq), int(Hkv), int(D));
+  if (n) ws = floats(n, q);
+  ok(mzb_gqa_prefill(q.data_ptr(), k.data_ptr(), v.data_ptr(), ptr(cu_q), ptr(cu_k), o.data_ptr(), ptr<float>(lse),
+                     n ? ptr<float>(ws) : nullptr, Tq, Tk, int(B), int(Hq), int(Hkv), int(D), code_of(q), q.stride(0),
+                     q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), causal, float(scale), word(err),
+                     c.stream),
+     "mzb_gqa_prefill");
+  return {o, lse};
+}
+
+std::tuple<Tensor, Tensor> gqa_decode(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages,
+                                      const Tensor& page_table, const Tensor& seq_lens, const Err& err, double scale) {
+  TORCH_CHECK(q.dim() == 3 && k_pages.dim() == 4 && v_pages.dim() == 4 && page_table.dim() == 2, "gqa_decode: bad dimensions");
+  Call c(q);
+  const int64_t B = q.size(0), Hq = q.size(1), D = q.size(2), P = k_pages.size(0), Hkv = k_pages.size(1),
+                page = k_pages.size(2), W = page_table.size(1);
+  Tensor o = at::empty({B, Hq, D}, q.options()), lse = at::empty({B, Hq}, q.options().dtype(at::kFloat)), ws;
+  const int64_t n = mzb_gqa_decode_ws(int(B), int(Hq), int(Hkv), int(D), int(W), int(page));
+  if (n) ws = floats(n, q);
+  ok(mzb_gqa_decode(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), ptr(page_table), ptr(seq_lens), o.data_ptr(),
+                    ptr<float>(lse), n ? ptr<float>(ws) : nullptr, int(B), int(Hq), int(Hkv), int(D), code_of(q),
+                    int(page), P, int(W), q.stride(0), q.stride(1), k_pages.stride(0), k_pages.stride(1),
+                    k_pages.stride(2), v_pages.stride(0), v_pages.stride(1), v_pages.stride(2), float(scale), word(err),
+                    c.stream),
+     "mzb_gqa_decode");
+  return {o, lse};
+}
+
+void kv_append(const Tensor& k, const Tensor& v, Tensor k_pages, Tensor v_pages, const Tensor& page_table,
+               const Tensor& starts, const std::optional<Tensor>& cu, const Err& err) {
+  TORCH_CHECK(k.dim() == 3 && v.dim() == 3 && k_pages.dim() == 4 && v_pages.dim() == 4 && page_table.dim() == 2,
+              "kv_append: bad dimensions");
+  Call c(k);
+  const int size = int(k.element_size());
+  const int64_t strides[10] = {k.stride(0),       k.stride(1),       v.stride(0),       v.stride(1),       k_pages.stride(0),
+                               k_pages.stride(1), k_pages.stride(2), v_pages.stride(0), v_pages.stride(1), v_pages.stride(2)};
+  ok(mzb_kv_append(k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), ptr(page_table), ptr(starts),
+                   cu ? ptr(*cu) : nullptr, k.size(0), int(starts.numel()), int(k.size(1)), int(k.size(2)) * size,
+                   int(k_pages.size(2)), k_pages.size(0), int(page_table.size(1)), size, strides, word(err), c.stream),
+     "mzb_kv_append");
+}
+
+Tensor kv_reserve(Tensor page_table, Tensor seq_lens, Tensor refs, const Tensor& n_new, const Err& err, int64_t page) {
+  Call c(page_table);
+  Tensor starts = at::empty_like(seq_lens), ws = ints(refs.numel(), refs);
+  ok(mzb_kv_reserve(ptr(page_table), ptr(seq_lens), ptr(refs), ptr(n_new), ptr(starts), ptr(ws), int(page_table.size(0)),
+                    int(page_table.size(1)), refs.numel(), int(page), word(err), c.stream),
+     "mzb_kv_reserve");
+  return starts;
+}
+
+void kv_free(Tensor page_table, Tensor seq_lens, Tensor refs, const Tensor& seqs, const Err& err) {
+  Call c(page_table);
+  ok(mzb_kv_free(ptr(page_table), ptr(seq_lens), ptr(refs), ptr(seqs), seqs.numel(), page_table.size(0),
+                 int(page_table.size(1)), refs.numel(), word(err), c.stream),
+     "mzb_kv_free");
+}
+
+void kv_copy_pages(at::TensorList pools, const Tensor& src, const Tensor& dst, const Err& err) {
+  TORCH_CHECK(!pools.empty(), "kv_copy_pages: no pool");
+  Call c(src);
+  const std::vector<int64_t> x = pool_array(pools);
+  ok(mzb_kv_copy_pages(x.data(), int(pools.size()), ptr(src), ptr(dst), src.numel(), pools[0].size(0), word(err), c.stream),
+     "mzb_kv_copy_pages");
+}
+
+void kv_fork(at::TensorList pools, Tensor page_table, Tensor seq_lens, Tensor refs, const Tensor& src, const Tensor& dst,
+             const Err& err, int64_t page) {
+  Call c(page_table);
+  const int64_t n = src.numel(), S = page_table.size(0);
+  Tensor ws = ints(3 * n + S, refs);
+  const std::vector<int64_t> x = pool_array(pools);
+  ok(mzb_kv_fork(ptr(page_table), ptr(seq_lens), ptr(refs), ptr(src), ptr(dst), int(n), ptr(ws), S,
+                 int(page_table.size(1)), refs.numel(), int(page), x.data(), int(pools.size()), word(err), c.stream),
+     "mzb_kv_fork");
+}
+
+std::tuple<Tensor, Tensor> kv_compact(at::TensorList pools, const Tensor& page_table, const Tensor& refs, const Err& err) {
+  Call c(page_table);
+  const int64_t P = refs.numel();
+  Tensor ws = ints(3 * P + 1, refs), table = at::empty_like(page_table), new_refs = at::empty_like(refs);
+  const std::vector<int64_t> x = pool_array(pools);
+  ok(mzb_kv_compact(ptr(page_table), ptr(refs), ptr(table), ptr(new_refs), ptr(ws), page_table.numel(), P, x.data(),
+                    int(pools.size()), word(err), c.stream),
+     "mzb_kv_compact");
+  return {table, new_refs};
+}
+
+}  // namespace
+
+// Called once by the Python side (not a static initialiser, whose exception at a stale build's
+// other schema would end the process): 0, or -1 with the reason in msg.
+extern "C" __attribute__((visibility("default"))) int mzb_torch_register(char* msg, size_t size) {
+  try {
+    static torch::Library m(torch::Library::IMPL, "mzb", c10::DispatchKey::CUDA, __FILE__, __LINE__);
+    m.impl("gqa_prefill", &gqa_prefill);
+    m.impl("gqa_decode", &gqa_decode);
+    m.impl("kv_append", &kv_append);
+    m.impl("kv_reserve", &kv_reserve);
+    m.impl("kv_free", &kv_free);
+    m.impl("kv_copy_pages", &kv_copy_pages);
+    m.impl("kv_fork", &kv_fork);
+    m.impl("kv_compact", &kv_compact);
+    return 0;
+  } catch (const std::exception& e) {
+    snprintf(msg, size, "%s", e.what());
+    return -1;
+  }
+}

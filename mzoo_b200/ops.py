@@ -6,8 +6,7 @@ torch (the library never allocates), passes raw pointers and the current stream 
 implementation so it traces under ``torch.compile`` / ``FakeTensor`` without running.
 """
 
-import ctypes
-import functools
+import os
 
 import torch
 
@@ -449,32 +448,19 @@ def _(codes, scales, D, fmt):
 
 # ----------------------------------------------------------------------------- dense attention, pages
 #
-# Serving-step ops: defined through ``torch.library.Library`` (a schema and one Python kernel)
-# rather than ``custom_op``, whose per-call bookkeeping costs several times the launch of the
-# smallest decode step.
+# Serving-step ops: declared here with their fake implementations; their CUDA kernels are C++
+# (``csrc/torch_ops.cpp``, loaded at import or at the first call) over the same C ABI, since the
+# way through ctypes takes the host longer than the smallest decode step takes the device.
 
 _LIB = torch.library.Library("mzb", "FRAGMENT")
-_I64x10 = ctypes.c_int64 * 10
 
 
-def _call_on(dev, name, *args):
-    """``call`` with the tensors' device current."""
-    if torch._C._cuda_getDevice() == dev.index:
-        return call(name, *args)
-    with torch.cuda.device(dev):
-        return call(name, *args)
-
-
-def _define(schema: str, fake):
-    """Register the decorated function as the CUDA kernel of ``mzb::<schema>``."""
+def _declare(schema: str, fake):
+    """Declare ``mzb::<schema>`` -> the op's overload."""
     name = schema[:schema.index("(")]
-
-    def wrap(fn):
-        _LIB.define(schema)
-        _LIB.impl(name, fn, "CUDA")
-        torch.library.register_fake(f"mzb::{name}", fake, lib=_LIB)
-        return getattr(torch.ops.mzb, name).default
-    return wrap
+    _LIB.define(schema)
+    torch.library.register_fake(f"mzb::{name}", fake, lib=_LIB)
+    return getattr(torch.ops.mzb, name).default
 
 
 def _attn_out(q, *rest):
@@ -482,142 +468,137 @@ def _attn_out(q, *rest):
             torch.empty(q.shape[0], q.shape[1], dtype=torch.float32, device=q.device))
 
 
-@_define("gqa_prefill(Tensor q, Tensor k, Tensor v, Tensor cu_q, Tensor cu_k, bool causal, float scale, bool check)"
-         " -> (Tensor, Tensor)", _attn_out)
+_gqa_prefill = _declare("gqa_prefill(Tensor q, Tensor k, Tensor v, Tensor cu_q, Tensor cu_k, Tensor(a!)? err, bool causal,"
+                        " float scale) -> (Tensor, Tensor)", _attn_out)
+_gqa_decode = _declare("gqa_decode(Tensor q, Tensor k_pages, Tensor v_pages, Tensor page_table, Tensor seq_lens,"
+                       " Tensor(a!)? err, float scale) -> (Tensor, Tensor)", _attn_out)
+_kv_append = _declare("kv_append(Tensor k, Tensor v, Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor page_table, Tensor starts,"
+                      " Tensor? cu, Tensor(c!)? err) -> ()", lambda *a: None)
+_kv_reserve = _declare("kv_reserve(Tensor(a!) page_table, Tensor(b!) seq_lens, Tensor(c!) refs, Tensor n_new,"
+                       " Tensor(d!)? err, int page) -> Tensor", lambda page_table, seq_lens, *a: torch.empty_like(seq_lens))
+_kv_free = _declare("kv_free(Tensor(a!) page_table, Tensor(b!) seq_lens, Tensor(c!) refs, Tensor seqs,"
+                    " Tensor(d!)? err) -> ()", lambda *a: None)
+_kv_copy_pages = _declare("kv_copy_pages(Tensor(a!)[] pools, Tensor src, Tensor dst, Tensor(b!)? err) -> ()", lambda *a: None)
+_kv_fork = _declare("kv_fork(Tensor(a!)[] pools, Tensor(b!) page_table, Tensor(c!) seq_lens, Tensor(d!) refs, Tensor src,"
+                    " Tensor dst, Tensor(e!)? err, int page) -> ()", lambda *a: None)
+_kv_compact = _declare("kv_compact(Tensor(a!)[] pools, Tensor page_table, Tensor refs, Tensor(b!)? err) -> (Tensor, Tensor)",
+                       lambda pools, page_table, refs, err: (torch.empty_like(page_table), torch.empty_like(refs)))
+
+
+def _word(t, check: bool):
+    """The error word of a launch on t's device; none where t is not real (fake, traced)."""
+    if type(t) is not torch.Tensor:
+        return None
+    if not _lib.torch_ops_loaded:
+        _lib.load_torch_ops()
+    if check:
+        return _err(t.device, True)
+    w = _ERR_WORDS.get(t.get_device())
+    return _err(t.device, False) if w is None else w
+
+
+def _failed(e: RuntimeError):
+    """Raise the error of ``torch_ops.cpp`` as the exception that ``_lib.check`` raises."""
+    text, _, status = str(e).partition(" [mzb status ")
+    if not status:
+        raise e
+    code = int(status.split("]")[0])
+    if code in (_lib.MZB_ERR_SHAPE, _lib.MZB_ERR_UNSUPPORTED, _lib.MZB_ERR_ALIGN):
+        raise AssertionError(text) from None
+    raise _lib.MzbError(f"{text} (status {code})") from None
+
+
 def gqa_prefill(q, k, v, cu_q, cu_k, causal, scale, check):
     """(o like q, lse fp32 [Tq, Hq]) of ``mzb_gqa_prefill`` (q / k / v with a dense last dimension)."""
-    dev = q.device
-    Tq, Hq, D = q.shape
-    o = torch.empty_like(q, memory_format=torch.contiguous_format)
-    lse = torch.empty(Tq, Hq, dtype=torch.float32, device=dev)
-    Tk, Hkv, _ = k.shape
-    B = len(cu_q) - 1
-    n = _gqa_prefill_ws(Tq, Tk, B, Hq, Hkv, D, dev.index) if Tq * Hq <= 1 << 15 else 0  # more rows are never split
-    ws = torch.empty(n, dtype=torch.float32, device=dev) if n else None
-    err = _err(dev, check)
-    (sq_t, sq_h, _), (sk_t, sk_h, _), (sv_t, sv_h, _) = q.stride(), k.stride(), v.stride()
-    _call_on(dev, "mzb_gqa_prefill", q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), o.data_ptr(),
-         lse.data_ptr(), ws.data_ptr() if n else None, Tq, Tk, B, Hq, Hkv, D, _lib.DTYPE_CODE[q.dtype], sq_t, sq_h, sk_t, sk_h, sv_t,
-         sv_h, causal, scale, err.data_ptr(), _lib.raw_stream(dev))
+    err = _word(q, check)
+    try:
+        out = _gqa_prefill(q, k, v, cu_q, cu_k, err, causal, scale)
+    except RuntimeError as e:
+        _failed(e)
     if check:
         _raise_on(err, "gqa prefill")
-    return o, lse
+    return out
 
 
-@functools.lru_cache(maxsize=256)
-def _gqa_prefill_ws(Tq: int, Tk: int, B: int, Hq: int, Hkv: int, D: int, device_index: int) -> int:
-    return _lib.lib().mzb_gqa_prefill_ws(Tq, Tk, B, Hq, Hkv, D)
-
-
-@functools.lru_cache(maxsize=256)
-def _gqa_decode_ws(B: int, Hq: int, Hkv: int, D: int, W: int, page: int, device_index: int) -> int:
-    return _lib.lib().mzb_gqa_decode_ws(B, Hq, Hkv, D, W, page)
-
-
-@_define("gqa_decode(Tensor q, Tensor k_pages, Tensor v_pages, Tensor page_table, Tensor seq_lens, float scale,"
-         " bool check) -> (Tensor, Tensor)", _attn_out)
 def gqa_decode(q, k_pages, v_pages, page_table, seq_lens, scale, check):
     """(o like q, lse fp32 [B, Hq]) of ``mzb_gqa_decode``."""
-    dev = q.device
-    (B, Hq, D), (P, Hkv, page, _), W = q.shape, k_pages.shape, page_table.shape[1]
-    o = torch.empty_like(q, memory_format=torch.contiguous_format)
-    lse = torch.empty(B, Hq, dtype=torch.float32, device=dev)
-    n = _gqa_decode_ws(B, Hq, Hkv, D, W, page, dev.index)
-    ws = torch.empty(n, dtype=torch.float32, device=dev) if n else None
-    err = _err(dev, check)
-    (sq_b, sq_h, _), (sk_p, sk_h, sk_t, _), (sv_p, sv_h, sv_t, _) = q.stride(), k_pages.stride(), v_pages.stride()
-    _call_on(dev, "mzb_gqa_decode", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(),
-         seq_lens.data_ptr(), o.data_ptr(), lse.data_ptr(), ws.data_ptr() if n else None, B, Hq, Hkv, D,
-         _lib.DTYPE_CODE[q.dtype], page, P, W, sq_b, sq_h, sk_p, sk_h, sk_t, sv_p, sv_h, sv_t, scale, err.data_ptr(),
-         _lib.raw_stream(dev))
+    err = _word(q, check)
+    try:
+        out = _gqa_decode(q, k_pages, v_pages, page_table, seq_lens, err, scale)
+    except RuntimeError as e:
+        _failed(e)
     if check:
         _raise_on(err, "gqa decode")
-    return o, lse
+    return out
 
 
-@_define("kv_append(Tensor k, Tensor v, Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor page_table, Tensor starts,"
-         " Tensor? cu, bool check) -> ()", lambda *a: None)
 def kv_append(k, v, k_pages, v_pages, page_table, starts, cu, check):
     """``mzb_kv_append``: rows of k / v [T, Hkv, D] into k_pages / v_pages [P, Hkv, page, D]."""
-    dev, size, (T, H, D), (P, _, page, _) = k.device, k.element_size(), k.shape, k_pages.shape
-    err = _err(dev, check)
-    _call_on(dev, "mzb_kv_append", k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(),
-         starts.data_ptr(), None if cu is None else cu.data_ptr(), T, len(starts), H, D * size, page, P,
-         page_table.shape[1], size,
-         _I64x10(*k.stride()[:2], *v.stride()[:2], *k_pages.stride()[:3], *v_pages.stride()[:3]), err.data_ptr(),
-         _lib.raw_stream(dev))
+    err = _word(k, check)
+    try:
+        _kv_append(k, v, k_pages, v_pages, page_table, starts, cu, err)
+    except RuntimeError as e:
+        _failed(e)
     if check:
         _raise_on(err, "kv append")
 
 
-@_define("kv_reserve(Tensor(a!) page_table, Tensor(b!) seq_lens, Tensor(c!) refs, Tensor n_new, int page, bool check)"
-         " -> Tensor", lambda page_table, seq_lens, *rest: torch.empty_like(seq_lens))
 def kv_reserve(page_table, seq_lens, refs, n_new, page, check):
     """``mzb_kv_reserve``; returns the lengths before it."""
-    dev = page_table.device
-    err, starts, ws = _err(dev, check), torch.empty_like(seq_lens), torch.empty_like(refs)
-    _call_on(dev, "mzb_kv_reserve", page_table.data_ptr(), seq_lens.data_ptr(), refs.data_ptr(), n_new.data_ptr(),
-         starts.data_ptr(), ws.data_ptr(), page_table.shape[0], page_table.shape[1], refs.shape[0], page,
-         err.data_ptr(), _lib.raw_stream(dev))
+    err = _word(page_table, check)
+    try:
+        starts = _kv_reserve(page_table, seq_lens, refs, n_new, err, page)
+    except RuntimeError as e:
+        _failed(e)
     if check:
         _raise_on(err, "kv reserve")
     return starts
 
 
-@_define("kv_free(Tensor(a!) page_table, Tensor(b!) seq_lens, Tensor(c!) refs, Tensor seqs, bool check) -> ()",
-         lambda *a: None)
 def kv_free(page_table, seq_lens, refs, seqs, check):
     """``mzb_kv_free``."""
-    dev = page_table.device
-    err = _err(dev, check)
-    _call_on(dev, "mzb_kv_free", page_table.data_ptr(), seq_lens.data_ptr(), refs.data_ptr(), seqs.data_ptr(), seqs.shape[0],
-         page_table.shape[0], page_table.shape[1], refs.shape[0], err.data_ptr(), _lib.raw_stream(dev))
+    err = _word(page_table, check)
+    try:
+        _kv_free(page_table, seq_lens, refs, seqs, err)
+    except RuntimeError as e:
+        _failed(e)
     if check:
         _raise_on(err, "kv free")
 
 
-def _pool_array(pools):
-    """(address, bytes of a page, bytes from page to page) of each pool, as the C ABI takes them."""
-    flat = []
-    for p in pools:
-        n, size = p.shape[0], p.element_size()
-        flat += (p.data_ptr(), p.numel() // n * size, p.stride(0) * size)
-    return (ctypes.c_int64 * len(flat))(*flat)
-
-
-@_define("kv_copy_pages(Tensor(a!)[] pools, Tensor src, Tensor dst, bool check) -> ()", lambda *a: None)
 def kv_copy_pages(pools, src, dst, check):
     """``mzb_kv_copy_pages``: page src[i] to page dst[i] of every pool."""
-    dev = src.device
-    err = _err(dev, check)
-    _call_on(dev, "mzb_kv_copy_pages", _pool_array(pools), len(pools), src.data_ptr(), dst.data_ptr(), len(src),
-             len(pools[0]), err.data_ptr(), _lib.raw_stream(dev))
+    err = _word(src, check)
+    try:
+        _kv_copy_pages(pools, src, dst, err)
+    except RuntimeError as e:
+        _failed(e)
     if check:
         _raise_on(err, "kv copy pages")
 
 
-@_define("kv_fork(Tensor(a!)[] pools, Tensor(b!) page_table, Tensor(c!) seq_lens, Tensor(d!) refs, Tensor src,"
-         " Tensor dst, int page, bool check) -> ()", lambda *a: None)
 def kv_fork(pools, page_table, seq_lens, refs, src, dst, page, check):
     """``mzb_kv_fork``."""
-    dev, n, (S, W) = page_table.device, len(src), page_table.shape
-    err, ws = _err(dev, check), torch.empty(3 * n + S, dtype=torch.int32, device=dev)
-    _call_on(dev, "mzb_kv_fork", page_table.data_ptr(), seq_lens.data_ptr(), refs.data_ptr(), src.data_ptr(),
-             dst.data_ptr(), n, ws.data_ptr(), S, W, len(refs), page, _pool_array(pools), len(pools), err.data_ptr(),
-             _lib.raw_stream(dev))
+    err = _word(page_table, check)
+    try:
+        _kv_fork(pools, page_table, seq_lens, refs, src, dst, err, page)
+    except RuntimeError as e:
+        _failed(e)
     if check:
         _raise_on(err, "kv fork")
 
 
-@_define("kv_compact(Tensor(a!)[] pools, Tensor page_table, Tensor refs, bool check) -> (Tensor, Tensor)",
-         lambda pools, page_table, refs, check: (torch.empty_like(page_table), torch.empty_like(refs)))
 def kv_compact(pools, page_table, refs, check):
     """``mzb_kv_compact``; returns the new (page_table, refs)."""
-    dev, P = page_table.device, len(refs)
-    err, ws = _err(dev, check), torch.empty(3 * P + 1, dtype=torch.int32, device=dev)
-    table, new_refs = torch.empty_like(page_table), torch.empty_like(refs)
-    _call_on(dev, "mzb_kv_compact", page_table.data_ptr(), refs.data_ptr(), table.data_ptr(), new_refs.data_ptr(),
-             ws.data_ptr(), page_table.numel(), P, _pool_array(pools), len(pools), err.data_ptr(), _lib.raw_stream(dev))
+    err = _word(page_table, check)
+    try:
+        out = _kv_compact(pools, page_table, refs, err)
+    except RuntimeError as e:
+        _failed(e)
     if check:
         _raise_on(err, "kv compact")
-    return table, new_refs
+    return out
+
+
+if os.path.exists(_lib.TORCH_LIB_PATH):
+    _lib.load_torch_ops()

@@ -517,5 +517,30 @@ def test_c_entry_refusals():
 
 
 def test_ops_are_registered():
-    assert {"gqa_prefill", "gqa_decode", "kv_append", "kv_reserve", "kv_fork", "kv_free", "kv_compact",
-            "kv_copy_pages"} <= set(dir(torch.ops.mzb)) and ops.gqa_prefill is torch.ops.mzb.gqa_prefill.default
+    """Schemas and fake implementations at import, the C++ kernels once the libraries are built."""
+    from mzoo_b200 import _lib, build
+    names = {"gqa_prefill", "gqa_decode", "kv_append", "kv_reserve", "kv_fork", "kv_free", "kv_compact", "kv_copy_pages"}
+    assert names <= set(dir(torch.ops.mzb))
+    build.build()
+    _lib.load_torch_ops()
+    assert all(torch._C._dispatch_has_kernel_for_dispatch_key(f"mzb::{n}", "CUDA") for n in names)
+
+
+def test_errors_keep_their_kinds():
+    """A status of the C ABI that comes through the C++ ops is the exception the other ops raise."""
+    from mzoo_b200 import _lib
+    for status, kind in ((_lib.MZB_ERR_SHAPE, AssertionError), (_lib.MZB_ERR_ALIGN, AssertionError),
+                         (_lib.MZB_ERR_UNSUPPORTED, AssertionError), (_lib.MZB_ERR_LAUNCH, _lib.MzbError)):
+        with pytest.raises(kind, match="gqa: why"):
+            ops._failed(RuntimeError(f"gqa: why [mzb status {status}]"))
+    with pytest.raises(RuntimeError, match="another"):
+        ops._failed(RuntimeError("another"))
+
+
+@pytest.mark.gpu
+def test_library_refusals_are_assertions(cuda):
+    """What only the library can see: a misaligned base address of foreign storage."""
+    raw = torch.zeros(4 * 2 * 64 + 8, dtype=torch.bfloat16, device=cuda)
+    odd = torch.empty(0, dtype=torch.bfloat16, device=cuda).set_(raw.untyped_storage()[2:], 0, (4, 2, 64))
+    with pytest.raises(AssertionError, match="aligned"):
+        gqa_attn.prefill(odd, odd, odd, _cu([4]).to(cuda))
