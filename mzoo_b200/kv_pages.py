@@ -57,6 +57,8 @@ def _rows_ok(t, size, apart=False):
     """Dense rows on 16-byte boundaries (``apart``: no two of them the same memory)."""
     if t.storage_offset() * size & 15:
         return False
+    if t.is_contiguous():  # rows are multiples of 16 bytes
+        return True
     *outer, last = t.stride()
     if last != 1:
         return False
