@@ -64,7 +64,7 @@ def _int32(name, t, *shape):
     """An int32 tensor with as many dimensions as `shape` and its first size (None: any), dense."""
     got = t.shape
     assert t.dtype == torch.int32, f"{name} must be int32, got {t.dtype}"
-    assert len(got) == len(shape) and (shape[0] is None or got[0] == shape[0]), \
+    assert len(got) == len(shape) and shape[0] in (None, got[0]), \
         f"{name} has shape {tuple(got)}, not {shape}"
     return t if t.is_contiguous() else t.contiguous()
 
@@ -86,12 +86,13 @@ def prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tenso
         f"k and v must be [tokens, heads, {qs[-1]}], got {tuple(ks)} and {tuple(v.shape)}"
     _check_heads(qs, ks[1])
     cu_q = _int32("cu_q", cu_q, None)
-    assert len(cu_q) >= 2, "cu_q needs at least one sequence"
+    n = cu_q.shape[0]
+    assert n >= 2, "cu_q needs at least one sequence"
     if cu_k is None:
         assert ks[0] == qs[0], f"without cu_k, k must have q's {qs[0]} tokens, got {ks[0]}"
         cu_k = cu_q
     else:
-        cu_k = _int32("cu_k", cu_k, len(cu_q))
+        cu_k = _int32("cu_k", cu_k, n)
     return ops.gqa_prefill(q if _aligned(q) else q.contiguous(), k if _aligned(k) else k.contiguous(),
                            v if _aligned(v) else v.contiguous(), cu_q, cu_k, causal,
                            qs[2] ** -0.5 if softmax_scale is None else float(softmax_scale), check)

@@ -85,10 +85,10 @@ def append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     assert len(ks) == 3 and ks == v.shape, f"k and v must be [tokens, heads, D], got {tuple(ks)}, {tuple(v.shape)}"
     assert len(ps) == 4 and ps == v_pages.shape and ps[1] == ks[1] and ps[3] == ks[2] and ps[0] and ps[2], \
         f"the pools must be [pages, {ks[1]}, page, {ks[2]}], got {tuple(ps)}, {tuple(v_pages.shape)}"
-    B, size, (rows, width) = len(starts), k.element_size(), page_table.shape
+    B, size, (rows, width) = starts.shape[0], k.element_size(), page_table.shape
     assert B >= 1 and rows == B and width >= 1, \
         f"page_table must have one row for each of the {B} sequences, got {rows} x {width}"
-    assert ks[0] == B if cu is None else len(cu) == B + 1, \
+    assert ks[0] == B if cu is None else cu.shape[0] == B + 1, \
         f"rows of {B} sequences: cu must be [{B + 1}], or None with one row each (got {ks[0]} rows)"
     assert ks[2] * size % 16 == 0 and ks[1] >= 1, f"rows must be a multiple of 16 bytes, got {ks[2]} x {dt}"
     assert _rows_ok(k_pages, size, True) and _rows_ok(v_pages, size, True), "the pools need dense, 16-byte aligned rows"
