@@ -654,6 +654,7 @@ extern "C" int mzb_gqa_decode(const void* q, const void* k_pages, const void* v_
   MZB_REQUIRE(err != nullptr, MZB_ERR_SHAPE, "gqa_decode: needs an error word");
   MZB_REQUIRE(reinterpret_cast<uintptr_t>(q) % 4 == 0 && reinterpret_cast<uintptr_t>(o) % 16 == 0 && sq_b % 2 == 0 && sq_h % 2 == 0,
               MZB_ERR_ALIGN, "gqa_decode: q rows must be 4-byte and o 16-byte aligned");
+  MZB_REQUIRE(ws != nullptr || B == 0 || gqad::short_table(W, page), MZB_ERR_SHAPE, "gqa_decode: needs a workspace");
   if (B == 0) return MZB_OK;
   gqad::DecodeArgs a{};
   a.q = q; a.table = page_table; a.lens = seq_lens; a.o = o; a.lse = lse; a.ws = ws;

@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(384, 1)
   };
   Item m;
 
-  // registers: 384 x 168 at launch = 256 x 208 (softmax) + 128 x 88
+  // registers: 384 x 168 at launch (the host checks it) = 256 x 208 (softmax) + 128 x 88
   if (warp < 8) {
     // ---------------------------------------------------------------- softmax, output
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
@@ -934,6 +934,15 @@ int launch(const void* q, const void* k, PrefillArgs a, int64_t sq_t, int64_t sq
   auto kern = a.splits > 1 ? prefill_kernel<DT, D, true> : prefill_kernel<DT, D, false>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
     return launch_status("gqa_prefill(smem attr)");
+  // the softmax warps' larger share of the registers would be waited for without end if the kernel
+  // were built with fewer at launch
+  static const int regs = [] {
+    cudaFuncAttributes x, y;
+    return cudaFuncGetAttributes(&x, prefill_kernel<DT, D, true>) == cudaSuccess &&
+                   cudaFuncGetAttributes(&y, prefill_kernel<DT, D, false>) == cudaSuccess
+               ? (x.numRegs < y.numRegs ? x.numRegs : y.numRegs) : 0;
+  }();
+  MZB_REQUIRE(regs * 384 >= 256 * 208 + 128 * 88, MZB_ERR_LAUNCH, "gqa_prefill: built with %d registers a thread", regs);
   const int64_t blocks = pairs_bound(a.Tq, a.B, a.g) * a.Hkv * a.splits;
   MZB_REQUIRE(blocks < (int64_t(1) << 31), MZB_ERR_SHAPE, "gqa_prefill: too large");
   kern<<<unsigned(blocks), 384, C::SMEM, st>>>(m[0], m[1], m[2], a);
@@ -972,7 +981,7 @@ extern "C" int mzb_gqa_prefill(const void* q, const void* k, const void* v, cons
                                void* o, float* lse, float* ws, int64_t Tq, int64_t Tk, int B, int Hq, int Hkv, int D, int dtype,
                                int64_t sq_t, int64_t sq_h, int64_t sk_t, int64_t sk_h, int64_t sv_t, int64_t sv_h,
                                int causal, float softmax_scale, int* err, void* stream) {
-  MZB_REQUIRE(Tq >= 0 && Tk >= 0 && B >= 1 && Tq < (int64_t(1) << 30) && Tk < (int64_t(1) << 30), MZB_ERR_SHAPE,
+  MZB_REQUIRE(Tq >= 0 && Tk >= 0 && B >= 1 && Tq < (int64_t(1) << 29) && Tk < (int64_t(1) << 29), MZB_ERR_SHAPE,
               "gqa_prefill: bad sizes Tq=%lld Tk=%lld B=%d", (long long)Tq, (long long)Tk, B);
   MZB_REQUIRE(Hkv >= 1 && Hq >= 1 && Hq % Hkv == 0 && Hq / Hkv <= 128, MZB_ERR_SHAPE,
               "gqa_prefill: query heads must be a multiple (at most 128) of the K/V heads, got %d and %d", Hq, Hkv);
