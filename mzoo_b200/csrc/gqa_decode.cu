@@ -19,6 +19,8 @@
 // (6.8 TB/s; a copy's rate is 6.54); one of 131001 keys (0.54 GB) in 85 us + 6 us of join.  Small calls are
 // bound by latency: ~4 us from the start to the first tile (lengths, page ids, the copy: three
 // dependent trips to memory), 6 us in all for 77 keys.
+#include <type_traits>
+
 #include "tc.cuh"
 
 namespace mzb {
@@ -30,6 +32,9 @@ constexpr int TK = 128, TK_LOG = 7;  // keys per tile
 constexpr int MIN_TILES = 2;         // a block's run is at least this long
 constexpr int MAX_BLOCKS = 160;
 constexpr int MAX_STAGES = 12;
+constexpr int THREADS = 384;         // eight warps for the products, four for the loads (one of them works)
+constexpr int PRODUCT_REGS = 208, LOAD_REGS = 88;
+constexpr int MERGE_BYTES = 16384;   // the eight warps' results of a few rows at a time
 
 struct DecodeArgs {
   const void* q;
@@ -41,6 +46,7 @@ struct DecodeArgs {
   int B, Hq, Hkv, g, W, page, page_log, stages, blocks;  // blocks 0: one block per (sequence, head), no parts
   float sl;                                    // scale * log2 e
   int* err;
+  bool q16;  // query rows in 16-byte pieces
 };
 
 // ws: int2 [B * Hkv] (first, last block of a (sequence, head); -1: empty), then for each of
@@ -52,9 +58,10 @@ __device__ __forceinline__ float* ws_part(const DecodeArgs& a, int part, int D) 
 }
 
 // What the loading warp tells the computing ones about a stage.
-struct Meta {
-  int b, hk, keys, flags;  // keys of the tile that exist; FIRST / LAST tile of the block's segment
-  int part;                // -1: the segment is the whole (sequence, head), else its part number
+struct __align__(16) Meta {
+  int b, hk;
+  uint16_t keys, flags;  // keys of the tile that exist; FIRST / LAST tile of the block's segment
+  int part;              // -1: the segment is the whole (sequence, head), else its part number
 };
 constexpr int FIRST = 1, LAST = 2, END = 4;
 
@@ -63,6 +70,8 @@ struct DCfg {
   static constexpr int DB = (D + 63) / 64;
   static constexpr int K_BYTES = DB * TK * 128;
   static constexpr int STAGE = 2 * K_BYTES;
+  static constexpr int QROW = D * 2 + 16;        // bytes from query row to row: no two of eight on the same banks
+  static constexpr int ROWS = D == 64 ? 8 : 4;   // rows of a merging pass
 };
 
 template <int DT>
@@ -107,25 +116,46 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, u
       : "memory");
 }
 
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+// The barrier's phase waits for this thread's copies so far, too.
+__device__ __forceinline__ void copies_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// All lanes wait for a phase; nobody waits on once a wait of the block has run out of time.
+__device__ __forceinline__ bool wait_stage(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err, int code) {
+  bool got = tc::mbar_try_wait(bar, parity);
+  if (__all_sync(0xffffffffu, got)) return true;
+  if (!got) got = !*abort_flag && tc::mbar_wait(bar, parity, err, code);
+  return __all_sync(0xffffffffu, got);
+}
+
 __device__ __forceinline__ int len_of(const DecodeArgs& a, int b) { return max(0, min(a.lens[b], a.W * a.page)); }
 
-// MT: head tiles of 16.  A warp has one of them and TK / (8 / MT) keys of every tile (MT 1: 16).
+// MT: head tiles of 16.  A warp has one of them and, 32 at a time, its share of the tile's keys.  With one head
+// tile four warps share a key tile and the other four have the next one: a warp's chain of products and
+// exponentials (~1 us) is spread over two tiles' time.
 template <int DT, int D, int MT>
-__global__ void __launch_bounds__(288, 1)
+__global__ void __launch_bounds__(THREADS, 1)
     decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                   const __grid_constant__ DecodeArgs a) {
   using C = DCfg<D>;
   using T = typename Elem<DT>::T;
-  constexpr int KP = 8 / MT;                // warps that share a tile's keys
-  constexpr int STEPS = TK / KP / 16;       // 16-key steps of a warp per tile
-  constexpr int PARTS = 8 / MT;             // partial results of a head tile to merge
+  constexpr int GROUPS = MT == 1 ? 2 : 1;       // warps 0-3 and 4-7 take tiles in turn
+  constexpr int KP = 8 / MT / GROUPS;           // warps that share a tile's keys
+  constexpr int STEPS = TK / KP / 32;           // 32-key steps of a warp per tile
+  constexpr int PARTS = 8 / MT;                 // partial results of a head tile to merge
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ uint64_t full[MAX_STAGES], empty[MAX_STAGES];
   __shared__ Meta meta[MAX_STAGES];
   __shared__ float sm_m[8][16], sm_l[8][16];
   __shared__ int abort_s;
   volatile int* abort_flag = &abort_s;
-  float* merge = reinterpret_cast<float*>(smem + a.stages * C::STAGE);  // [8 warps][min(g, 16)][D / 2]
+  float* merge = reinterpret_cast<float*>(smem + a.stages * C::STAGE);  // [8 warps][ROWS][D]
+  uint8_t* q_rows = smem + a.stages * C::STAGE + MERGE_BYTES;           // MT 1: [stages][g] rows of QROW bytes
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (smem_u32(smem) & 1023) {
     if (threadIdx.x == 0) atomicExch(a.err, MZB_ERR_ALIGN);
@@ -142,8 +172,10 @@ __global__ void __launch_bounds__(288, 1)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   __syncthreads();
 
-  if (warp == 8) {
-    // ---------------------------------------------------------------- loads
+  if (warp >= 8) {
+    // ---------------------------------------------------------------- loads (one warp of four)
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(LOAD_REGS));
+    if (warp > 8) return;
     if (lane == 0) {
       tc::prefetch_tmap(&tk);
       tc::prefetch_tmap(&tv);
@@ -233,15 +265,28 @@ __global__ void __launch_bounds__(288, 1)
           cur = nxt;
           nxt = ids(base + 32 + lane);
         }
-        const bool got = !*abort_flag && tc::mbar_wait(&empty[s], phase ^ 1, a.err, 421);
-        if (!__all_sync(0xffffffffu, got)) { ok = false; break; }
+        ok = wait_stage(&empty[s], phase ^ 1, abort_flag, a.err, 421);
+        if (!ok) break;
+        if (MT == 1 && i == 0) {  // the segment's query rows come with its first tile
+          const T* q = static_cast<const T*>(a.q) + (int64_t)b * a.sq_b + (int64_t)hk * a.g * a.sq_h;
+          const uint32_t to = smem_u32(q_rows) + s * a.g * C::QROW;
+          auto rows_by = [&](auto piece) {
+            constexpr int BYTES = decltype(piece)::value, N = D * 2 / BYTES;
+            for (int x = lane; x < a.g * N; x += 32)
+              copy_async<BYTES>(to + x / N * C::QROW + x % N * BYTES, q + (int64_t)(x / N) * a.sq_h + x % N * (BYTES / 2));
+          };
+          if (a.q16) rows_by(std::integral_constant<int, 16>());
+          else rows_by(std::integral_constant<int, 4>());
+          copies_arrive(&full[s]);
+          __syncwarp();
+        }
         // page ids of the tile's boxes, then all copies by one elected lane (behind a condition that
         // differs by lane each copy's operands are made uniform in a loop: ~700 ns a tile)
         int pid[8];
 #pragma unroll
         for (int x = 0; x < 8; ++x) pid[x] = __shfl_sync(0xffffffffu, cur, min((t << tile_log) + x - base, 31));
         if (tc::elect_one()) {
-          meta[s] = Meta{b, hk, keys, (i == 0 ? FIRST : 0) | (i == n - 1 ? LAST : 0), part};
+          meta[s] = Meta{b, hk, uint16_t(keys), uint16_t((i == 0 ? FIRST : 0) | (i == n - 1 ? LAST : 0)), part};
           tc::mbar_expect_tx(&full[s], uint32_t(live) * rows * 128 * C::DB * 2);
           uint8_t* to = smem + s * C::STAGE;
           const int slot = (t * TK) & (a.page - 1);
@@ -270,8 +315,7 @@ __global__ void __launch_bounds__(288, 1)
       }
     }
     // the end, as a stage without data
-    const bool got = ok && !*abort_flag && tc::mbar_wait(&empty[s], phase ^ 1, a.err, 422);
-    if (__all_sync(0xffffffffu, got)) {
+    if (ok && wait_stage(&empty[s], phase ^ 1, abort_flag, a.err, 422)) {
       if (lane == 0) {
         meta[s].flags = END;
         tc::mbar_arrive(&full[s]);
@@ -281,6 +325,7 @@ __global__ void __launch_bounds__(288, 1)
     }
   } else {
     // ---------------------------------------------------------------- products
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PRODUCT_REGS));
     // sequences without keys
     if (a.blocks) {
       for (int b = blockIdx.x; b < a.B; b += gridDim.x)
@@ -296,7 +341,7 @@ __global__ void __launch_bounds__(288, 1)
         reinterpret_cast<uint4*>(static_cast<T*>(a.o) + row * D)[x] = make_uint4(0, 0, 0, 0);
       for (int x = threadIdx.x; x < a.g; x += 256) a.lse[row + x] = -INFINITY;
     }
-    const int mt = warp % MT, kp = warp / MT;
+    const int mt = warp % MT, kp = warp / MT % KP, turn = warp / (8 / GROUPS);
     const int r0 = lane >> 2, c0 = (lane & 3) * 2;
     uint32_t qf[D / 16][4];
     float o[D / 8][4], m[2], l[2];
@@ -313,64 +358,73 @@ __global__ void __launch_bounds__(288, 1)
     // blocks; V transposed: (keys 0-7, 8-15) x (channels 0-7, 8-15) as (b0, b1) of two channel blocks
     const int krow = (lane & 7) + ((lane >> 4) << 3), kch = (lane >> 3) & 1;
     const int vrow = lane & 15, vch = lane >> 4;
-    int s = -1;
+    int s = -1, nth = 1;
     uint32_t phase = 0;
     while (true) {
+      nth ^= 1;
       if (++s == a.stages) {
         s = 0;
         phase ^= 1;
       }
-      const bool got = !*abort_flag && tc::mbar_wait(&full[s], phase, a.err, 423);
-      if (!__all_sync(0xffffffffu, got)) {
+      if (!wait_stage(&full[s], phase, abort_flag, a.err, 423)) {
         *abort_flag = 1;
         break;
       }
       const Meta w = meta[s];
       if (w.flags & END) break;
       if (w.flags & FIRST) {  // this group's query rows
-        const T* q = static_cast<const T*>(a.q) + (int64_t)w.b * a.sq_b;
-        auto ld = [&](int row, int ch) {
-          const int h = mt * 16 + row;
-          return h < a.g ? *reinterpret_cast<const uint32_t*>(q + (int64_t)(w.hk * a.g + h) * a.sq_h + ch) : 0u;
-        };
+        if constexpr (MT == 1) {  // (rows behind the last repeat it: their results go nowhere)
+          const uint32_t from = smem_u32(q_rows) + (s * a.g + min(lane & 15, a.g - 1)) * C::QROW + (lane >> 4) * 16;
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          qf[kk][0] = ld(r0, 16 * kk + c0);
-          qf[kk][1] = ld(r0 + 8, 16 * kk + c0);
-          qf[kk][2] = ld(r0, 16 * kk + c0 + 8);
-          qf[kk][3] = ld(r0 + 8, 16 * kk + c0 + 8);
+          for (int kk = 0; kk < D / 16; ++kk) ldsm4<false>(qf[kk], from + kk * 32);
+        } else {
+          const T* q = static_cast<const T*>(a.q) + (int64_t)w.b * a.sq_b;
+          auto ld = [&](int row, int ch) {
+            const int h = mt * 16 + row;
+            return h < a.g ? *reinterpret_cast<const uint32_t*>(q + (int64_t)(w.hk * a.g + h) * a.sq_h + ch) : 0u;
+          };
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            qf[kk][0] = ld(r0, 16 * kk + c0);
+            qf[kk][1] = ld(r0 + 8, 16 * kk + c0);
+            qf[kk][2] = ld(r0, 16 * kk + c0 + 8);
+            qf[kk][3] = ld(r0 + 8, 16 * kk + c0 + 8);
+          }
         }
       }
-      {
+      if (GROUPS == 1 || nth == turn) {
         const uint32_t kt = smem_u32(smem + s * C::STAGE), vt = kt + C::K_BYTES;
 #pragma unroll 1
         for (int st = 0; st < STEPS; ++st) {
-          const int key0 = (kp * STEPS + st) * 16;
+          const int key0 = (kp * STEPS + st) * 32;
           if (key0 >= w.keys) break;
-          float sc[2][4] = {};
-          const int kr = key0 + krow;
+          float sc[4][4] = {};
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
-            uint32_t bk[4];
             const int ch = 2 * kk + kch;  // 16-byte piece
-            ldsm4<false>(bk, kt + (ch >> 3) * (TK * 128) + kr * 128 + (((ch & 7) ^ (kr & 7)) * 16));
-            mma16816<DT>(sc[0], qf[kk], bk[0], bk[1]);
-            mma16816<DT>(sc[1], qf[kk], bk[2], bk[3]);
-          }
-          const int vis = w.keys - key0;  // keys of these 16 that exist
 #pragma unroll
-          for (int n = 0; n < 2; ++n)
+            for (int x = 0; x < 2; ++x) {
+              uint32_t bk[4];
+              const int kr = key0 + 16 * x + krow;
+              ldsm4<false>(bk, kt + (ch >> 3) * (TK * 128) + kr * 128 + (((ch & 7) ^ (kr & 7)) * 16));
+              mma16816<DT>(sc[2 * x], qf[kk], bk[0], bk[1]);
+              mma16816<DT>(sc[2 * x + 1], qf[kk], bk[2], bk[3]);
+            }
+          }
+          const int vis = w.keys - key0;  // keys of these 32 that exist
+          float mt2[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+          for (int n = 0; n < 4; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               sc[n][e] *= a.sl;
               if (8 * n + c0 + (e & 1) >= vis) sc[n][e] = -INFINITY;
+              mt2[e >> 1] = fmaxf(mt2[e >> 1], sc[n][e]);
             }
-          float mt2[2];
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            float x = fmaxf(fmaxf(sc[0][2 * r], sc[0][2 * r + 1]), fmaxf(sc[1][2 * r], sc[1][2 * r + 1]));
-            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-            mt2[r] = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+            mt2[r] = fmaxf(mt2[r], __shfl_xor_sync(0xffffffffu, mt2[r], 1));
+            mt2[r] = fmaxf(mt2[r], __shfl_xor_sync(0xffffffffu, mt2[r], 2));
           }
           // O and the sums are rescaled only when a maximum has grown by more than 2^8
           if (__any_sync(0xffffffffu, mt2[0] > m[0] + 8.0f || mt2[1] > m[1] + 8.0f)) {
@@ -388,44 +442,49 @@ __global__ void __launch_bounds__(288, 1)
               for (int e = 0; e < 4; ++e) o[i][e] *= al[e >> 1];
           }
           const float ms[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
-          float p[2][4];
 #pragma unroll
-          for (int n = 0; n < 2; ++n)
+          for (int n = 0; n < 4; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              p[n][e] = fast_exp2(sc[n][e] - ms[e >> 1]);
-              l[e >> 1] += p[n][e];
+              sc[n][e] = fast_exp2(sc[n][e] - ms[e >> 1]);
+              l[e >> 1] += sc[n][e];
             }
-          // the weights as a sum of two numbers of the type (16 bits and more): the products have room
-          uint32_t ph[4], pl[4];
 #pragma unroll
-          for (int n = 0; n < 2; ++n)
+          for (int x = 0; x < 2; ++x) {
+            const int seen = vis - 16 * x;
+            if (seen <= 0) break;
+            // the weights as a sum of two numbers of the type (16 bits and more): the products have room
+            uint32_t ph[4], pl[4];
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              const uint32_t h2 = pack2<DT>(p[n][2 * r], p[n][2 * r + 1]);
-              const float2 f = unpack2<DT>(h2);
-              ph[2 * n + r] = h2;
-              pl[2 * n + r] = pack2<DT>(p[n][2 * r] - f.x, p[n][2 * r + 1] - f.y);
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+              for (int r = 0; r < 2; ++r) {
+                const float p0 = sc[2 * x + n][2 * r], p1 = sc[2 * x + n][2 * r + 1];
+                const uint32_t h2 = pack2<DT>(p0, p1);
+                const float2 f = unpack2<DT>(h2);
+                ph[2 * n + r] = h2;
+                pl[2 * n + r] = pack2<DT>(p0 - f.x, p1 - f.y);
+              }
+            const bool tail = seen < 16;
+            const uint32_t k01 = tail ? (c0 < seen ? 0xffffu : 0u) | (c0 + 1 < seen ? 0xffff0000u : 0u) : ~0u;
+            const uint32_t k89 = tail ? (c0 + 8 < seen ? 0xffffu : 0u) | (c0 + 9 < seen ? 0xffff0000u : 0u) : ~0u;
+            const int vr = key0 + 16 * x + vrow;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+              uint32_t bv[4];
+              const int ch = 2 * i + vch;
+              ldsm4<true>(bv, vt + (ch >> 3) * (TK * 128) + vr * 128 + (((ch & 7) ^ (vr & 7)) * 16));
+              if (tail) {  // what lies behind the sequence's end must not meet its zero weights
+                bv[0] &= k01;
+                bv[1] &= k89;
+                bv[2] &= k01;
+                bv[3] &= k89;
+              }
+              mma16816<DT>(o[2 * i], ph, bv[0], bv[1]);
+              mma16816<DT>(o[2 * i + 1], ph, bv[2], bv[3]);
+              mma16816<DT>(o[2 * i], pl, bv[0], bv[1]);
+              mma16816<DT>(o[2 * i + 1], pl, bv[2], bv[3]);
             }
-          const bool tail = vis < 16;
-          const uint32_t k01 = tail ? (c0 < vis ? 0xffffu : 0u) | (c0 + 1 < vis ? 0xffff0000u : 0u) : ~0u;
-          const uint32_t k89 = tail ? (c0 + 8 < vis ? 0xffffu : 0u) | (c0 + 9 < vis ? 0xffff0000u : 0u) : ~0u;
-          const int vr = key0 + vrow;
-#pragma unroll
-          for (int i = 0; i < D / 16; ++i) {
-            uint32_t bv[4];
-            const int ch = 2 * i + vch;
-            ldsm4<true>(bv, vt + (ch >> 3) * (TK * 128) + vr * 128 + (((ch & 7) ^ (vr & 7)) * 16));
-            if (tail) {  // what lies behind the sequence's end must not meet its zero weights
-              bv[0] &= k01;
-              bv[1] &= k89;
-              bv[2] &= k01;
-              bv[3] &= k89;
-            }
-            mma16816<DT>(o[2 * i], ph, bv[0], bv[1]);
-            mma16816<DT>(o[2 * i + 1], ph, bv[2], bv[3]);
-            mma16816<DT>(o[2 * i], pl, bv[0], bv[1]);
-            mma16816<DT>(o[2 * i + 1], pl, bv[2], bv[3]);
           }
         }
       }
@@ -438,53 +497,65 @@ __global__ void __launch_bounds__(288, 1)
           l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
           l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
         }
+        // a few rows of a head tile at a time (the ring needs the shared memory more); channels are
+        // exchanged in fours by the row's number, so that the rows of a store lie on different banks
         const int gr = min(a.g, 16);
-        if ((lane & 3) == 0) {
-          sm_m[warp][r0] = m[0];
-          sm_m[warp][r0 + 8] = m[1];
-          sm_l[warp][r0] = l[0];
-          sm_l[warp][r0 + 8] = l[1];
-        }
-        // in two halves of the channels: the ring needs the shared memory more
-        float* mine = merge + warp * gr * (D / 2);
+#pragma unroll 1
+        for (int at = 0; at < gr; at += C::ROWS) {
+          tc::bar_sync(1, 256);  // what the last pass wrote has been read
+          if (at == 0 && (lane & 3) == 0) {
+            sm_m[warp][r0] = m[0];
+            sm_m[warp][r0 + 8] = m[1];
+            sm_l[warp][r0] = l[0];
+            sm_l[warp][r0 + 8] = l[1];
+          }
+          const int mine = r0 + (at & 8) - at;  // this thread's row of the pass
+          if (mine >= 0 && mine < C::ROWS) {
+            float* to = merge + (warp * C::ROWS + mine) * D;
+            const int flip = (mine & 3) * 8;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-#pragma unroll
-          for (int i = 0; i < D / 16; ++i) {
-            const float(&x)[4] = o[half * (D / 16) + i];
-            if (r0 < gr) *reinterpret_cast<float2*>(mine + r0 * (D / 2) + 8 * i + c0) = make_float2(x[0], x[1]);
-            if (r0 + 8 < gr) *reinterpret_cast<float2*>(mine + (r0 + 8) * (D / 2) + 8 * i + c0) = make_float2(x[2], x[3]);
+            for (int i = 0; i < D / 8; ++i)
+              *reinterpret_cast<float2*>(to + ((8 * i + c0) ^ flip)) =
+                  at < 8 ? make_float2(o[i][0], o[i][1]) : make_float2(o[i][2], o[i][3]);
           }
           tc::bar_sync(1, 256);
-          for (int x = threadIdx.x; x < a.g * (D / 4); x += 256) {
-            const int h = x / (D / 4), dh = (x % (D / 4)) * 2, d = half * (D / 2) + dh, tile = h >> 4, r = h & 15;
+          constexpr int LANES = D == 64 ? 16 : 32;  // of a row, four channels each
+          const int d = (threadIdx.x % LANES) * 4;
+#pragma unroll 1
+          for (int x = threadIdx.x / LANES; x < MT * C::ROWS; x += 256 / LANES) {
+            const int tile = x / C::ROWS, r = at + x % C::ROWS, h = tile * 16 + r;
+            if (h >= a.g || d >= D) continue;
             float mx = -INFINITY;
 #pragma unroll
             for (int i = 0; i < PARTS; ++i) mx = fmaxf(mx, sm_m[i * MT + tile][r]);
             const float ms = mx == -INFINITY ? 0.0f : mx;
             float ls = 0.0f;
-            float2 acc = make_float2(0.0f, 0.0f);
+            float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
             for (int i = 0; i < PARTS; ++i) {
               const int wp = i * MT + tile;
               const float al = fast_exp2(sm_m[wp][r] - ms);
-              const float2 v = *reinterpret_cast<const float2*>(merge + (wp * gr + r) * (D / 2) + dh);
+              const float4 v = *reinterpret_cast<const float4*>(merge + (wp * C::ROWS + (r - at)) * D + (d ^ (((r - at) & 3) * 8)));
               ls += sm_l[wp][r] * al;
               acc.x += v.x * al;
               acc.y += v.y * al;
+              acc.z += v.z * al;
+              acc.w += v.w * al;
             }
             if (w.part < 0) {
               const int64_t row = (int64_t)w.b * a.Hq + w.hk * a.g + h;
               const float inv = 1.0f / ls;
-              *reinterpret_cast<uint32_t*>(static_cast<T*>(a.o) + row * D + d) = pack2<DT>(acc.x * inv, acc.y * inv);
+              *reinterpret_cast<uint2*>(static_cast<T*>(a.o) + row * D + d) =
+                  make_uint2(pack2<DT>(acc.x * inv, acc.y * inv), pack2<DT>(acc.z * inv, acc.w * inv));
               if (d == 0) a.lse[row] = (mx + log2f(ls)) * LN2;
             } else {
               float* to = ws_part(a, w.part, D);
-              *reinterpret_cast<float2*>(to + 2 * a.g + h * D + d) = acc;
+              float2* y = reinterpret_cast<float2*>(to + 2 * a.g + h * D + d);
+              y[0] = make_float2(acc.x, acc.y);
+              y[1] = make_float2(acc.z, acc.w);
               if (d == 0) *reinterpret_cast<float2*>(to + 2 * h) = make_float2(mx, ls);
             }
           }
-          tc::bar_sync(1, 256);
         }
         clear();
       }
@@ -599,15 +670,22 @@ int launch(const void* k, const void* v, DecodeArgs a, const int64_t* sk, const 
                             i ? v : k, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B))
       return r;
   }
-  const int merge = 8 * (a.g < 16 ? a.g : 16) * (D / 2) * 4;
-  const int budget = 227 * 1024 - 2048 - merge;  // 2 KB: the static arrays
-  a.stages = budget / C::STAGE < MAX_STAGES ? budget / C::STAGE : MAX_STAGES;
+  const int budget = 227 * 1024 - 3072 - MERGE_BYTES;  // 3 KB: the static arrays
+  const int q_bytes = MT == 1 ? a.g * C::QROW : 0;  // of a stage
+  a.stages = budget / (C::STAGE + q_bytes) < MAX_STAGES ? budget / (C::STAGE + q_bytes) : MAX_STAGES;
   a.blocks = short_table(a.W, a.page) ? 0 : block_count();
   auto kern = decode_kernel<DT, D, MT>;
-  const int smem = a.stages * C::STAGE + merge;
+  const int smem = a.stages * (C::STAGE + q_bytes) + MERGE_BYTES;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return launch_status("gqa_decode(smem attr)");
-  kern<<<a.blocks ? a.blocks : a.B * a.Hkv, 288, smem, st>>>(m[0], m[1], a);
+  // the product warps' share is drawn from what the block is launched with: less would wait for ever
+  static const int regs = [] {
+    cudaFuncAttributes x;
+    return cudaFuncGetAttributes(&x, decode_kernel<DT, D, MT>) == cudaSuccess ? x.numRegs : 0;
+  }();
+  MZB_REQUIRE(regs * THREADS >= 256 * PRODUCT_REGS + (THREADS - 256) * LOAD_REGS, MZB_ERR_LAUNCH,
+              "gqa_decode: built with %d registers a thread", regs);
+  kern<<<a.blocks ? a.blocks : a.B * a.Hkv, THREADS, smem, st>>>(m[0], m[1], a);
   if (int r = launch_status("gqa_decode")) return r;
   if (!a.blocks) return MZB_OK;
   cudaLaunchConfig_t cfg{};
@@ -663,6 +741,7 @@ extern "C" int mzb_gqa_decode(const void* q, const void* k_pages, const void* v_
   a.page_log = page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7;
   a.sl = softmax_scale * gqad::LOG2E;
   a.err = err;
+  a.q16 = reinterpret_cast<uintptr_t>(q) % 16 == 0 && sq_b % 8 == 0 && sq_h % 8 == 0;
   const int64_t sk[3] = {sk_p, sk_h, sk_t}, sv[3] = {sv_p, sv_h, sv_t};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
 #define MZB_GO(DT, DD)                                                                              \
