@@ -77,7 +77,9 @@ struct PrefillArgs {
   int* parts;         // [Tq, Hq]: parts of a row; 1: written in place
   float *plse, *po;   // [splits, Tq * Hq], [splits, Tq * Hq, D]
 };
-constexpr int MIN_PART = 6;  // key tiles of a part at least (a part costs a block's start and its share of the join)
+// key tiles of a part at least (a part costs a block's start and its share of the join): 16 tokens of 16 heads on
+// one behind 4000 keys take 32 us with parts of six, 24 of two
+constexpr int MIN_PART = 2;
 
 // One work item, in shared memory.  Of a part, k0, nk and shift are those of its keys alone.
 struct Item {
@@ -499,20 +501,30 @@ __global__ void __launch_bounds__(384, 1)
       const uint8_t* ld_at = stage + (lane >> 2) * 64 + (((lane & 3) ^ ((lane >> 3) & 3)) * 16);
       const uint64_t inv2 = pack_f32x2(inv, inv);
       constexpr int CB = D % 64 ? 1 : 2;  // blocks of 32 channels in flight
-      if (CUT && cut) {
+      if (CUT && cut) {  // the part's numbers in fp32, the same way: 128 bytes of four rows a store
+        int at[8];  // this lane's rows of a block's stores: 4 i + lane / 8
+#pragma unroll
+        for (int i = 0; i < 8; ++i) at[i] = __shfl_sync(0xffffffffu, row_ok ? int(row) : -1, 4 * i + (lane >> 3));
+        float* part = prow - row * D + 4 * (lane & 7);
 #pragma unroll 1
         for (int c0 = 0; c0 < D; c0 += 32) {
           uint32_t ov[32];
           tc::tmem_ld32(ocol + c0, ov);
           tc::tmem_wait_ld();
           tc::reg_after_wait(ov);
-          if (row_ok) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              *reinterpret_cast<float4*>(prow + c0 + e) =
-                  make_float4(__uint_as_float(ov[e]) * inv, __uint_as_float(ov[e + 1]) * inv,
-                              __uint_as_float(ov[e + 2]) * inv, __uint_as_float(ov[e + 3]) * inv);
+          for (int c = 0; c < 8; ++c)
+            *reinterpret_cast<float4*>(stage + lane * 128 + ((c ^ (lane & 7)) * 16)) =
+                make_float4(__uint_as_float(ov[4 * c]) * inv, __uint_as_float(ov[4 * c + 1]) * inv,
+                            __uint_as_float(ov[4 * c + 2]) * inv, __uint_as_float(ov[4 * c + 3]) * inv);
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int r = 4 * i + (lane >> 3);
+            const float4 x = *reinterpret_cast<const float4*>(stage + r * 128 + (((lane & 7) ^ (r & 7)) * 16));
+            if (at[i] >= 0) *reinterpret_cast<float4*>(part + (int64_t)at[i] * D + c0) = x;
           }
+          __syncwarp();
         }
       }
 #pragma unroll 1
@@ -862,38 +874,54 @@ __global__ void __launch_bounds__(384, 1)
   }
 }
 
-// A warp per row: the parts of a cut key range, in their order.
+// The parts of a cut key range, in their order: a warp per row, or eight that share a row's parts where there
+// may be 32 and more (16 tokens of 16 heads on one behind 30000 keys, 74 parts: 46 us with a warp, 30 shared; 64
+// tokens of 32 on 8 behind 16000, 9 parts: 46 and 50).
+constexpr int SHARE_FROM = 32;
 template <int DT, int D>
 __global__ void __launch_bounds__(256) prefill_join_kernel(const __grid_constant__ PrefillArgs a) {
   using T = typename Elem<DT>::T;
   constexpr int C = D / 32;
+  __shared__ float shared_acc[8][D];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int lane = threadIdx.x & 31;
-  const int64_t rows = a.Tq * a.Hq, row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (row >= rows) return;
-  const int n = a.parts[row];
-  if (n <= 1) return;
-  float top = -INFINITY;
-  bool nan = false;
-  for (int i = 0; i < n; ++i) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int share = a.splits >= SHARE_FROM ? 8 : 1, sub = warp & (share - 1);  // warps of a row, this one's place
+  const int64_t rows = a.Tq * a.Hq, row = (int64_t)blockIdx.x * (8 / share) + (share == 8 ? 0 : warp);
+  const int n = row < rows ? a.parts[row] : 0;
+  if (n <= 1) return;  // (with shared rows: the whole block)
+  float top = -INFINITY, sum = 0.0f;
+  for (int i = lane; i < n; i += 32) {
     const float x = a.plse[i * rows + row];
     top = fmaxf(top, x);
-    nan |= x != x;
+    if (x != x) sum = x;
   }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
   const float ref = top == -INFINITY ? 0.0f : top;
-  float sum = nan ? NAN : 0.0f, acc[C];
+  for (int i = lane; i < n; i += 32) sum += exp2f((a.plse[i * rows + row] - ref) * LOG2E);
+#pragma unroll
+  for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  float acc[C];
 #pragma unroll
   for (int c = 0; c < C; ++c) acc[c] = 0.0f;
 #pragma unroll 4
-  for (int i = 0; i < n; ++i) {
+  for (int i = sub; i < n; i += share) {
     const float x = a.plse[i * rows + row];
     if (x == -INFINITY) continue;  // a part without keys for this row has no output
     const float w = exp2f((x - ref) * LOG2E);
-    sum += w;
 #pragma unroll
     for (int c = 0; c < C; ++c) acc[c] += w * a.po[(i * rows + row) * D + lane + 32 * c];
   }
-  const float inv = top == -INFINITY && !nan ? 0.0f : 1.0f / sum;
+  if (share > 1) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) shared_acc[warp][lane + 32 * c] = acc[c];
+    __syncthreads();
+    if (sub) return;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      for (int w = 1; w < 8; ++w) acc[c] += shared_acc[w][lane + 32 * c];
+  }
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
   for (int c = 0; c < C; ++c) static_cast<T*>(a.o)[row * D + lane + 32 * c] = Elem<DT>::store(acc[c] * inv);
   if (lane == 0) a.lse[row] = sum == 0.0f ? -INFINITY : ref + logf(sum);
@@ -952,7 +980,7 @@ int launch(const void* q, const void* k, PrefillArgs a, int64_t sq_t, int64_t sq
   cudaLaunchAttribute at{};
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at.val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3(unsigned((a.Tq * a.Hq + 7) / 8));
+  cfg.gridDim = dim3(unsigned(a.splits >= SHARE_FROM ? a.Tq * a.Hq : (a.Tq * a.Hq + 7) / 8));
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cfg.attrs = &at;

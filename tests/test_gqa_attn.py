@@ -183,6 +183,18 @@ def test_prefill_few_rows_many_keys(cuda, hq, hkv, d, new, keys):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv,d", [(1, 1, 64), (12, 2, 96), (16, 1, 128)])
+def test_prefill_many_parts(cuda, hq, hkv, d):
+    """As many parts that several warps share a row of them; sequences of one part and of none beside."""
+    _prefill(cuda, torch.bfloat16, hq, hkv, d, [3, 17, 5, 0], [9000, 70, 2, 700])
+
+    def edit(q, k, v):
+        v[8998, :, 3] = math.nan   # seen by the last two of the three
+        v[40, :, 5] = -math.inf
+    _prefill(cuda, torch.float16, hq, hkv, d, [3], [9000], edit=edit)
+
+
+@pytest.mark.gpu
 def test_prefill_parts_keep_nan_apart(cuda):
     """In a cut key range, values that a row does not see stay out of it and those it sees arrive."""
     def edit(q, k, v):
