@@ -96,6 +96,12 @@ __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
+// An 8 x 8 matrix of 16-bit numbers, a row in four lanes, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
 template <int DT>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   if constexpr (DT == MZB_BF16) {
@@ -137,10 +143,10 @@ __device__ __forceinline__ bool wait_stage(uint64_t* bar, uint32_t parity, volat
 
 __device__ __forceinline__ int len_of(const DecodeArgs& a, int b) { return max(0, min(a.lens[b], a.W * a.page)); }
 
-// MT: head tiles of 16.  A warp has one of them and, 32 at a time, its share of the tile's keys.  With one head
+// MT: head tiles of 8 NH.  A warp has one of them and, 32 at a time, its share of the tile's keys.  With one head
 // tile four warps share a key tile and the other four have the next one: a warp's chain of products and
 // exponentials (~1 us) is spread over two tiles' time.
-template <int DT, int D, int MT>
+template <int DT, int D, int MT, int NH>
 __global__ void __launch_bounds__(THREADS, 1)
     decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                   const __grid_constant__ DecodeArgs a) {
@@ -347,21 +353,25 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
     const int mt = warp % MT, kp = warp / MT % KP, turn = warp / (8 / GROUPS);
     const int r0 = lane >> 2, c0 = (lane & 3) * 2;
-    uint32_t qf[D / 16][4];
-    float o[D / 8][4], m[2], l[2];
+    constexpr int HT = 8 * NH;  // heads of a tile
+    uint32_t qf[NH][D / 16][2];                  // (channels) x (heads)
+    float o[D / 16][NH][4], m[NH][2], l[NH][2];  // channels r0, r0 + 8 of 16 x heads c0, c0 + 1 of 8
     auto clear = [&]() {
 #pragma unroll
-      for (int i = 0; i < D / 8; ++i)
+      for (int n = 0; n < NH; ++n) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[i][e] = 0.0f;
-      m[0] = m[1] = -INFINITY;
-      l[0] = l[1] = 0.0f;
+        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[i][n][e] = 0.0f;
+        m[n][0] = m[n][1] = -INFINITY;
+        l[n][0] = l[n][1] = 0.0f;
+      }
     };
     clear();
-    // ldmatrix rows of this lane: K: matrices (keys 0-7, 8-15) x (channels 0-7, 8-15) as (b0, b1) of two key
-    // blocks; V transposed: (keys 0-7, 8-15) x (channels 0-7, 8-15) as (b0, b1) of two channel blocks
-    const int krow = (lane & 7) + ((lane >> 4) << 3), kch = (lane >> 3) & 1;
-    const int vrow = lane & 15, vch = lane >> 4;
+    // ldmatrix rows of this lane.  K: (keys 0-7, 8-15) x (channels 0-7, 8-15), the keys first; V transposed:
+    // (keys 0-7, 8-15) x (channels 0-7, 8-15), the channels first
+    const int krow = lane & 15, kch = lane >> 4;
+    const int vrow = (lane & 7) + ((lane >> 4) << 3), vch = (lane >> 3) & 1;
     int s = -1, nth = 1;
     uint32_t phase = 0;
     while (true) {
@@ -378,21 +388,30 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (w.flags & END) break;
       if (w.flags & FIRST) {  // this group's query rows
         if constexpr (MT == 1) {  // (rows behind the last repeat it: their results go nowhere)
-          const uint32_t from = smem_u32(q_rows) + (s * a.g + min(lane & 15, a.g - 1)) * C::QROW + (lane >> 4) * 16;
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) ldsm4<false>(qf[kk], from + kk * 32);
+          for (int n = 0; n < NH; ++n) {
+            const uint32_t from = smem_u32(q_rows) + (s * a.g + min(8 * n + (lane & 7), a.g - 1)) * C::QROW + (lane >> 3) * 16;
+#pragma unroll
+            for (int kk = 0; kk < D / 16; kk += 2) {
+              uint32_t x[4];
+              ldsm4<false>(x, from + kk * 32);
+              qf[n][kk][0] = x[0];
+              qf[n][kk][1] = x[1];
+              qf[n][kk + 1][0] = x[2];
+              qf[n][kk + 1][1] = x[3];
+            }
+          }
         } else {
           const T* q = static_cast<const T*>(a.q) + (int64_t)w.b * a.sq_b;
-          auto ld = [&](int row, int ch) {
-            const int h = mt * 16 + row;
-            return h < a.g ? *reinterpret_cast<const uint32_t*>(q + (int64_t)(w.hk * a.g + h) * a.sq_h + ch) : 0u;
-          };
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            qf[kk][0] = ld(r0, 16 * kk + c0);
-            qf[kk][1] = ld(r0 + 8, 16 * kk + c0);
-            qf[kk][2] = ld(r0, 16 * kk + c0 + 8);
-            qf[kk][3] = ld(r0 + 8, 16 * kk + c0 + 8);
+          for (int n = 0; n < NH; ++n) {
+            const int h = mt * HT + 8 * n + r0;
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+              for (int j = 0; j < 2; ++j)
+                qf[n][kk][j] = h < a.g ? *reinterpret_cast<const uint32_t*>(q + (int64_t)(w.hk * a.g + h) * a.sq_h + 16 * kk + 8 * j + c0)
+                                       : 0u;
           }
         }
       }
@@ -402,92 +421,106 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int st = 0; st < STEPS; ++st) {
           const int key0 = (kp * STEPS + st) * 32;
           if (key0 >= w.keys) break;
-          float sc[4][4] = {};
+          float sc[2][NH][4] = {};  // keys r0, r0 + 8 of 16 x heads c0, c0 + 1 of 8
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
             const int ch = 2 * kk + kch;  // 16-byte piece
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-              uint32_t bk[4];
+              uint32_t ak[4];
               const int kr = key0 + 16 * x + krow;
-              ldsm4<false>(bk, kt + (ch >> 3) * (TK * 128) + kr * 128 + (((ch & 7) ^ (kr & 7)) * 16));
-              mma16816<DT>(sc[2 * x], qf[kk], bk[0], bk[1]);
-              mma16816<DT>(sc[2 * x + 1], qf[kk], bk[2], bk[3]);
+              ldsm4<false>(ak, kt + (ch >> 3) * (TK * 128) + kr * 128 + (((ch & 7) ^ (kr & 7)) * 16));
+#pragma unroll
+              for (int n = 0; n < NH; ++n) mma16816<DT>(sc[x][n], ak, qf[n][kk][0], qf[n][kk][1]);
             }
           }
           const int vis = w.keys - key0;  // keys of these 32 that exist
-          float mt2[2] = {-INFINITY, -INFINITY};
+          float top[NH][2];
 #pragma unroll
-          for (int n = 0; n < 4; ++n)
+          for (int n = 0; n < NH; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              sc[n][e] *= a.sl;
-              if (8 * n + c0 + (e & 1) >= vis) sc[n][e] = -INFINITY;
-              mt2[e >> 1] = fmaxf(mt2[e >> 1], sc[n][e]);
+            for (int e = 0; e < 2; ++e) {
+              float t = -INFINITY;
+#pragma unroll
+              for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                  float& y = sc[x][n][2 * r + e];
+                  y *= a.sl;
+                  if (16 * x + 8 * r + r0 >= vis) y = -INFINITY;
+                  t = fmaxf(t, y);
+                }
+#pragma unroll
+              for (int d = 4; d < 32; d <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, d));
+              top[n][e] = t;
             }
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            mt2[r] = fmaxf(mt2[r], __shfl_xor_sync(0xffffffffu, mt2[r], 1));
-            mt2[r] = fmaxf(mt2[r], __shfl_xor_sync(0xffffffffu, mt2[r], 2));
-          }
           // O and the sums are rescaled only when a maximum has grown by more than 2^8
-          if (__any_sync(0xffffffffu, mt2[0] > m[0] + 8.0f || mt2[1] > m[1] + 8.0f)) {
-            float al[2];
+          bool grown = false;
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              const float mn = fmaxf(m[r], mt2[r]);
-              al[r] = mn == -INFINITY ? 1.0f : fast_exp2(m[r] - mn);
-              m[r] = mn;
-              l[r] *= al[r];
+          for (int n = 0; n < NH; ++n) grown |= top[n][0] > m[n][0] + 8.0f || top[n][1] > m[n][1] + 8.0f;
+          if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+            for (int n = 0; n < NH; ++n) {
+              float al[2];
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const float mn = fmaxf(m[n][e], top[n][e]);
+                al[e] = mn == -INFINITY ? 1.0f : fast_exp2(m[n][e] - mn);
+                m[n][e] = mn;
+                l[n][e] *= al[e];
+              }
+#pragma unroll
+              for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[i][n][e] *= al[e & 1];
             }
-#pragma unroll
-            for (int i = 0; i < D / 8; ++i)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) o[i][e] *= al[e >> 1];
           }
-          const float ms[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
-#pragma unroll
-          for (int n = 0; n < 4; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              sc[n][e] = fast_exp2(sc[n][e] - ms[e >> 1]);
-              l[e >> 1] += sc[n][e];
-            }
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             const int seen = vis - 16 * x;
             if (seen <= 0) break;
-            // the weights as a sum of two numbers of the type (16 bits and more): the products have room
-            uint32_t ph[4], pl[4];
+            // the weights as a sum of two numbers of the type (16 bits and more), turned to (keys) x (heads)
+            uint32_t ph[NH][2], pl[NH][2];
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
+            for (int n = 0; n < NH; ++n) {
+              const float ms[2] = {m[n][0] == -INFINITY ? 0.0f : m[n][0], m[n][1] == -INFINITY ? 0.0f : m[n][1]};
 #pragma unroll
               for (int r = 0; r < 2; ++r) {
-                const float p0 = sc[2 * x + n][2 * r], p1 = sc[2 * x + n][2 * r + 1];
+                const float p0 = fast_exp2(sc[x][n][2 * r] - ms[0]), p1 = fast_exp2(sc[x][n][2 * r + 1] - ms[1]);
+                l[n][0] += p0;
+                l[n][1] += p1;
                 const uint32_t h2 = pack2<DT>(p0, p1);
                 const float2 f = unpack2<DT>(h2);
-                ph[2 * n + r] = h2;
-                pl[2 * n + r] = pack2<DT>(p0 - f.x, p1 - f.y);
+                ph[n][r] = transpose8(h2);
+                pl[n][r] = transpose8(pack2<DT>(p0 - f.x, p1 - f.y));
               }
+            }
             const bool tail = seen < 16;
             const uint32_t k01 = tail ? (c0 < seen ? 0xffffu : 0u) | (c0 + 1 < seen ? 0xffff0000u : 0u) : ~0u;
             const uint32_t k89 = tail ? (c0 + 8 < seen ? 0xffffu : 0u) | (c0 + 9 < seen ? 0xffff0000u : 0u) : ~0u;
             const int vr = key0 + 16 * x + vrow;
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i) {
-              uint32_t bv[4];
-              const int ch = 2 * i + vch;
-              ldsm4<true>(bv, vt + (ch >> 3) * (TK * 128) + vr * 128 + (((ch & 7) ^ (vr & 7)) * 16));
-              if (tail) {  // what lies behind the sequence's end must not meet its zero weights
-                bv[0] &= k01;
-                bv[1] &= k89;
-                bv[2] &= k01;
-                bv[3] &= k89;
+            for (int i = 0; i < D / 16; i += 2) {
+              uint32_t av[2][4];
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                const int ch = 2 * (i + j) + vch;
+                ldsm4<true>(av[j], vt + (ch >> 3) * (TK * 128) + vr * 128 + (((ch & 7) ^ (vr & 7)) * 16));
+                if (tail) {  // what lies behind the sequence's end must not meet its zero weights
+                  av[j][0] &= k01;
+                  av[j][1] &= k01;
+                  av[j][2] &= k89;
+                  av[j][3] &= k89;
+                }
               }
-              mma16816<DT>(o[2 * i], ph, bv[0], bv[1]);
-              mma16816<DT>(o[2 * i + 1], ph, bv[2], bv[3]);
-              mma16816<DT>(o[2 * i], pl, bv[0], bv[1]);
-              mma16816<DT>(o[2 * i + 1], pl, bv[2], bv[3]);
+#pragma unroll
+              for (int n = 0; n < NH; ++n)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) mma16816<DT>(o[i + j][n], av[j], ph[n][0], ph[n][1]);
+#pragma unroll
+              for (int n = 0; n < NH; ++n)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) mma16816<DT>(o[i + j][n], av[j], pl[n][0], pl[n][1]);
             }
           }
         }
@@ -497,37 +530,41 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (w.flags & LAST) {
         // ------------------------------------------------------------ merge the warps' results
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-          l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-        }
-        // a few rows of a head tile at a time (the ring needs the shared memory more); channels are
-        // exchanged in fours by the row's number, so that the rows of a store lie on different banks
-        const int gr = min(a.g, 16);
+        for (int n = 0; n < NH; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], d);
+        // a few heads of a tile at a time (the ring needs the shared memory more); channels are exchanged in
+        // eights by the head's number, so that the heads of a store lie on different banks
+        const int gr = min(a.g, HT);
 #pragma unroll 1
         for (int at = 0; at < gr; at += C::ROWS) {
           tc::bar_sync(1, 256);  // what the last pass wrote has been read
-          if (at == 0 && (lane & 3) == 0) {
-            sm_m[warp][r0] = m[0];
-            sm_m[warp][r0 + 8] = m[1];
-            sm_l[warp][r0] = l[0];
-            sm_l[warp][r0 + 8] = l[1];
-          }
-          const int mine = r0 + (at & 8) - at;  // this thread's row of the pass
+          if (at == 0 && r0 == 0)
+#pragma unroll
+            for (int n = 0; n < NH; ++n)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                sm_m[warp][8 * n + c0 + e] = m[n][e];
+                sm_l[warp][8 * n + c0 + e] = l[n][e];
+              }
+          const int mine = c0 + (at & 8) - at;  // this thread's heads of the pass: this one and the next
           if (mine >= 0 && mine < C::ROWS) {
             float* to = merge + (warp * C::ROWS + mine) * D;
-            const int flip = (mine & 3) * 8;
+            const int flip = (mine >> 1 & 3) * 8;
 #pragma unroll
-            for (int i = 0; i < D / 8; ++i)
-              *reinterpret_cast<float2*>(to + ((8 * i + c0) ^ flip)) =
-                  at < 8 ? make_float2(o[i][0], o[i][1]) : make_float2(o[i][2], o[i][3]);
+            for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                to[(e & 1) * D + ((16 * i + 8 * (e >> 1) + r0) ^ flip)] = at < 8 ? o[i][0][e] : o[i][NH - 1][e];
           }
           tc::bar_sync(1, 256);
           constexpr int LANES = D == 64 ? 16 : 32;  // of a row, four channels each
           const int d = (threadIdx.x % LANES) * 4;
 #pragma unroll 1
           for (int x = threadIdx.x / LANES; x < MT * C::ROWS; x += 256 / LANES) {
-            const int tile = x / C::ROWS, r = at + x % C::ROWS, h = tile * 16 + r;
+            const int tile = x / C::ROWS, r = at + x % C::ROWS, h = tile * HT + r;
             if (h >= a.g || d >= D) continue;
             float mx = -INFINITY;
 #pragma unroll
@@ -539,7 +576,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             for (int i = 0; i < PARTS; ++i) {
               const int wp = i * MT + tile;
               const float al = fast_exp2(sm_m[wp][r] - ms);
-              const float4 v = *reinterpret_cast<const float4*>(merge + (wp * C::ROWS + (r - at)) * D + (d ^ (((r - at) & 3) * 8)));
+              const float4 v = *reinterpret_cast<const float4*>(merge + (wp * C::ROWS + (r - at)) * D + (d ^ (((r - at) >> 1 & 3) * 8)));
               ls += sm_l[wp][r] * al;
               acc.x += v.x * al;
               acc.y += v.y * al;
@@ -661,7 +698,7 @@ int block_count() { return num_sms() < MAX_BLOCKS ? num_sms() : MAX_BLOCKS; }
 // 8 heads 17.5 -> 15.4 us with the launches, 256 of 256 keys 67 -> 64.  Longer ones in runs of equal length.
 bool short_table(int W, int page) { return (int64_t)W * page <= MIN_TILES * TK; }
 
-template <int DT, int D, int MT>
+template <int DT, int D, int MT, int NH>
 int launch(const void* k, const void* v, DecodeArgs a, const int64_t* sk, const int64_t* sv, cudaStream_t st) {
   using C = DCfg<D>;
   CUtensorMap m[2];
@@ -682,14 +719,14 @@ int launch(const void* k, const void* v, DecodeArgs a, const int64_t* sk, const 
   a.whole = short_table(a.W, a.page);
   a.blocks = block_count();
   if (a.whole && (int64_t)a.B * a.Hkv < a.blocks) a.blocks = a.B * a.Hkv;
-  auto kern = decode_kernel<DT, D, MT>;
+  auto kern = decode_kernel<DT, D, MT, NH>;
   const int smem = a.stages * (C::STAGE + q_bytes) + MERGE_BYTES;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return launch_status("gqa_decode(smem attr)");
   // the product warps' share is drawn from what the block is launched with: less would wait for ever
   static const int regs = [] {
     cudaFuncAttributes x;
-    return cudaFuncGetAttributes(&x, decode_kernel<DT, D, MT>) == cudaSuccess ? x.numRegs : 0;
+    return cudaFuncGetAttributes(&x, decode_kernel<DT, D, MT, NH>) == cudaSuccess ? x.numRegs : 0;
   }();
   MZB_REQUIRE(regs * THREADS >= 256 * PRODUCT_REGS + (THREADS - 256) * LOAD_REGS, MZB_ERR_LAUNCH,
               "gqa_decode: built with %d registers a thread", regs);
@@ -753,10 +790,11 @@ extern "C" int mzb_gqa_decode(const void* q, const void* k_pages, const void* v_
   const int64_t sk[3] = {sk_p, sk_h, sk_t}, sv[3] = {sv_p, sv_h, sv_t};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
 #define MZB_GO(DT, DD)                                                                              \
-  (a.g <= 16 ? gqad::launch<DT, DD, 1>(k_pages, v_pages, a, sk, sv, st)                             \
-   : a.g <= 32 ? gqad::launch<DT, DD, 2>(k_pages, v_pages, a, sk, sv, st)                           \
-   : a.g <= 64 ? gqad::launch<DT, DD, 4>(k_pages, v_pages, a, sk, sv, st)                           \
-               : gqad::launch<DT, DD, 8>(k_pages, v_pages, a, sk, sv, st))
+  (a.g <= 8 ? gqad::launch<DT, DD, 1, 1>(k_pages, v_pages, a, sk, sv, st)                           \
+   : a.g <= 16 ? gqad::launch<DT, DD, 1, 2>(k_pages, v_pages, a, sk, sv, st)                        \
+   : a.g <= 32 ? gqad::launch<DT, DD, 2, 2>(k_pages, v_pages, a, sk, sv, st)                        \
+   : a.g <= 64 ? gqad::launch<DT, DD, 4, 2>(k_pages, v_pages, a, sk, sv, st)                        \
+               : gqad::launch<DT, DD, 8, 2>(k_pages, v_pages, a, sk, sv, st))
   if (dtype == MZB_BF16) return D == 64 ? MZB_GO(MZB_BF16, 64) : D == 96 ? MZB_GO(MZB_BF16, 96) : MZB_GO(MZB_BF16, 128);
   return D == 64 ? MZB_GO(MZB_F16, 64) : D == 96 ? MZB_GO(MZB_F16, 96) : MZB_GO(MZB_F16, 128);
 #undef MZB_GO
