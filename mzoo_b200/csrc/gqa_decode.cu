@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   __shared__ int abort_s;
   volatile int* abort_flag = &abort_s;
   float* merge = reinterpret_cast<float*>(smem + a.stages * C::STAGE);  // [8 warps][ROWS][D]
-  uint8_t* q_rows = smem + a.stages * C::STAGE + MERGE_BYTES;           // MT 1: [stages][g] rows of QROW bytes
+  uint8_t* q_rows = smem + a.stages * C::STAGE + MERGE_BYTES;           // up to 16 heads: [stages][g] rows of QROW bytes
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (smem_u32(smem) & 1023) {
     if (threadIdx.x == 0) atomicExch(a.err, MZB_ERR_ALIGN);
@@ -285,7 +285,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         ok = wait_stage(&empty[s], phase ^ 1, abort_flag, a.err, 421);
         if (!ok) break;
-        if (MT == 1 && i == 0) {  // the segment's query rows come with its first tile
+        if (MT * NH <= 2 && i == 0) {  // the segment's query rows come with its first tile
           const T* q = static_cast<const T*>(a.q) + (int64_t)b * a.sq_b + (int64_t)hk * a.g * a.sq_h;
           const uint32_t to = smem_u32(q_rows) + s * a.g * C::QROW;
           auto rows_by = [&](auto piece) {
@@ -387,10 +387,10 @@ __global__ void __launch_bounds__(THREADS, 1)
       const Meta w = meta[s];
       if (w.flags & END) break;
       if (w.flags & FIRST) {  // this group's query rows
-        if constexpr (MT == 1) {  // (rows behind the last repeat it: their results go nowhere)
+        if constexpr (MT * HT <= 16) {  // (rows behind the last repeat it: their results go nowhere)
 #pragma unroll
           for (int n = 0; n < NH; ++n) {
-            const uint32_t from = smem_u32(q_rows) + (s * a.g + min(8 * n + (lane & 7), a.g - 1)) * C::QROW + (lane >> 3) * 16;
+            const uint32_t from = smem_u32(q_rows) + (s * a.g + min(mt * HT + 8 * n + (lane & 7), a.g - 1)) * C::QROW + (lane >> 3) * 16;
 #pragma unroll
             for (int kk = 0; kk < D / 16; kk += 2) {
               uint32_t x[4];
@@ -714,7 +714,7 @@ int launch(const void* k, const void* v, DecodeArgs a, const int64_t* sk, const 
       return r;
   }
   const int budget = 227 * 1024 - 3072 - MERGE_BYTES;  // 3 KB: the static arrays
-  const int q_bytes = MT == 1 ? a.g * C::QROW : 0;  // of a stage
+  const int q_bytes = MT * NH <= 2 ? a.g * C::QROW : 0;  // of a stage
   a.stages = budget / (C::STAGE + q_bytes) < MAX_STAGES ? budget / (C::STAGE + q_bytes) : MAX_STAGES;
   a.whole = short_table(a.W, a.page);
   a.blocks = block_count();
@@ -791,7 +791,7 @@ extern "C" int mzb_gqa_decode(const void* q, const void* k_pages, const void* v_
   cudaStream_t st = static_cast<cudaStream_t>(stream);
 #define MZB_GO(DT, DD)                                                                              \
   (a.g <= 8 ? gqad::launch<DT, DD, 1, 1>(k_pages, v_pages, a, sk, sv, st)                           \
-   : a.g <= 16 ? gqad::launch<DT, DD, 1, 2>(k_pages, v_pages, a, sk, sv, st)                        \
+   : a.g <= 16 ? gqad::launch<DT, DD, 2, 1>(k_pages, v_pages, a, sk, sv, st)                        \
    : a.g <= 32 ? gqad::launch<DT, DD, 2, 2>(k_pages, v_pages, a, sk, sv, st)                        \
    : a.g <= 64 ? gqad::launch<DT, DD, 4, 2>(k_pages, v_pages, a, sk, sv, st)                        \
                : gqad::launch<DT, DD, 8, 2>(k_pages, v_pages, a, sk, sv, st))
