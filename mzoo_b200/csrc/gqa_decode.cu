@@ -620,7 +620,7 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Decod
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int first = blockIdx.x / a.g, h = blockIdx.x % a.g;
   const int of = ws_open(a)[first];  // sequence * Hkv + head
-  if (of < 0) return;
+  if (of < 0 || of >= a.B * a.Hkv) return;
   const int64_t row = (int64_t)of * a.g + h;
   const int n = max(1, min(ws_last(a)[of], a.blocks - 1) - first + 1);
   auto part = [&](int i) { return ws_part(a, i == 0 ? 2 * first + 1 : 2 * (first + i), D); };

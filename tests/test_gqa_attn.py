@@ -352,6 +352,31 @@ def test_decode_splits(cuda, lens):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv,d", [(12, 4, 64), (36, 4, 128), (16, 8, 96), (22, 2, 96)])
+@pytest.mark.parametrize("lens", [[0, 256, 1, 0, 130] * 17, [0] * 50 + [200, 255, 3] + [0] * 40, [128] * 37, [0, 300, 1, 129] * 24])
+def test_decode_short_tables(cuda, hq, hkv, d, lens):
+    """More (sequence, head)s than blocks, none of their rows cut, runs that begin in empty sequences;
+    tables just above, with cut rows; one and two head tiles, full and not."""
+    _decode(cuda, torch.bfloat16, hq, hkv, d, 16, lens, fill=None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (11, 1, 64), (40, 2, 96)])
+def test_decode_query_rows_at_any_even_offset(cuda, hq, hkv, d):
+    """Query rows that are only 4-byte aligned, as the library takes them."""
+    from mzoo_b200 import ops
+    g = torch.Generator().manual_seed(3)
+    lens = [200, 0, 33, 900]
+    kp, vp, table = _pages(g, torch.bfloat16, hkv, d, 32, lens)
+    rest = [t.to(cuda) for t in (kp, vp, table, torch.tensor(lens, dtype=torch.int32))]
+    wide = _randn(g, torch.bfloat16, 4 * (hq * (d + 2) + 6) + 2).to(cuda)
+    q = wide[2:].as_strided((4, hq, d), (hq * (d + 2) + 6, d + 2, 1), 2)
+    want = gqa_attn.decode(q.contiguous(), *rest, check=True)
+    got = ops.gqa_decode(q, *rest, d ** -0.5, True)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.gpu
 def test_decode_scale_and_wide_scores(cuda):
     _decode(cuda, torch.bfloat16, 4, 1, 128, 16, [500, 77], scale=2.0)
     _decode(cuda, torch.float16, 4, 1, 128, 16, [500, 77], scale=0.0)
