@@ -275,7 +275,7 @@ MZB_API int mzb_kv_unpack_fp4(const uint8_t* codes, const uint8_t* scales, void*
  *   cu_k[b+1] of k / v (int32 [B+1], ascending from 0).  Row i of a sequence of nq tokens and
  *   nk keys sees the keys j <= i + nk - nq (causal) or all; head h reads K / V head
  *   h / (Hq / Hkv).  o [Tq, Hq, D] and lse fp32 [Tq, Hq] (natural log) dense; a row that sees
- *   no key has o = 0 and lse = -inf.  Hq / Hkv at most 128; D in {64, 96, 128}.  ws:
+ *   no key, or lies behind cu_q[B] (padding), has o = 0 and lse = -inf.  Hq / Hkv at most 128; D in {64, 96, 128}.  ws:
  *   mzb_gqa_prefill_ws(...) floats (0 unless few rows meet many keys), 16-byte aligned.
  * mzb_gqa_decode -- one token per sequence over a paged cache.  q [B, Hq, D]; k_pages /
  *   v_pages [P, Hkv, page, D] by their page, head and token strides in elements; key t of

@@ -35,6 +35,7 @@
 // against it and was slower or no better: a thread for half a row (with an exchange of the maxima),
 // weights against the maximum of the tile before, one issuing thread for each tile (they fall into
 // step and fight for the exponential unit), more of the exponentials on the FMA pipe.
+#include "gqa_items.cuh"
 #include "tc.cuh"
 
 namespace mzb {
@@ -42,7 +43,6 @@ namespace gqa {
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
-constexpr int BN = 128;  // keys per tile
 
 template <int D>
 struct PCfg {
@@ -63,33 +63,15 @@ struct PCfg {
   static_assert(SMEM <= 232448, "shared memory budget");
 };
 
-struct PrefillArgs {
+struct PrefillArgs : ItemArgs {
   const void* v;
-  const int32_t *cu_q, *cu_k;
   void* o;
   float* lse;
-  int64_t Tq, Tk, sv_t, sv_h;
-  int B, Hq, Hkv, g, ntok, causal, neg;  // g = Hq / Hkv, ntok = 128 / g tokens per tile
-  float sl;                              // |scale| log2 e
+  int64_t sv_t, sv_h;
+  int Hq, Hkv, g, neg;  // g = Hq / Hkv
+  float sl;             // |scale| log2 e
   int* err;
-  // a call with few work items cuts the longer key ranges into up to `splits` (1: none) parts
-  int splits;
-  int* parts;         // [Tq, Hq]: parts of a row; 1: written in place
-  float *plse, *po;   // [splits, Tq * Hq], [splits, Tq * Hq, D]
-};
-// key tiles of a part at least (a part costs a block's start and its share of the join): 16 tokens of 16 heads on
-// one behind 4000 keys take 32 us with parts of six, 24 of two
-constexpr int MIN_PART = 2;
-
-// One work item, in shared memory.  Of a part, k0, nk and shift are those of its keys alone.
-struct Item {
-  int tok0, tok_end;  // first packed token, end of the sequence
-  int i0, shift;      // tok0's place in its sequence; keys seen by place i: min(nk, i + shift) (not causal: nk)
-  int k0, nk, hk;     // first packed key, keys, K / V head
-  int n0, n1;         // key tiles of the query tiles
-  int part, of;       // which part of how many
-  int lim0, jfix;     // keys that tok0 sees (the fewest); V tiles from jfix on reach past them
-  int done;
+  float *plse, *po;     // of cut key ranges: [splits, Tq * Hq], [splits, Tq * Hq, D]
 };
 
 enum PBar { P_QF = 0, P_QE = 2, P_SF = 4, P_PF = 6, P_OF = 10, P_OE = 12, P_ITF = 14, P_ITE = 16, P_CLC = 18, P_ASK = 19,
@@ -167,109 +149,6 @@ __device__ __forceinline__ uint32_t nonfinite2(uint32_t w) {
   constexpr uint32_t E = DT == MZB_BF16 ? 0x7f80u : 0x7c00u;
   return ((w & E) == E ? 0xffffu : 0u) | ((w & (E << 16)) == (E << 16) ? 0xffff0000u : 0u);
 }
-
-// ---------------------------------------------------------------- work items
-
-// Item number -> (sequence, pair within it), by the scheduler warp.  Up to 32 sequences (a lane
-// for each): by descending end of the pair's key range, so that the longest items come first and
-// the last blocks' shares are even; more: sequence after sequence, the last pair first, from a
-// cursor (a block's item numbers only grow).
-struct Finder {
-  int n, q0, nq, k0, nk;  // this lane's sequence (of 32 from cur_b)
-  int low, top, total, cur_b, cur_at;
-
-  __device__ void load(const PrefillArgs& a, int lane) {
-    const int b = cur_b + lane;
-    n = 0;
-    if (b < a.B) {
-      // (whatever the offsets hold, rows stay inside the tensors)
-      const int qa = a.cu_q[b], qb = a.cu_q[b + 1], ka = a.cu_k[b], kb = a.cu_k[b + 1];
-      q0 = max(0, min(qa, int(a.Tq)));
-      nq = max(0, min(qb, int(a.Tq)) - q0);
-      k0 = max(0, min(ka, int(a.Tk)));
-      nk = max(0, min(kb, int(a.Tk)) - k0);
-      n = nq > 0 ? (nq + 2 * a.ntok - 1) / (2 * a.ntok) : 0;
-    }
-    total = __reduce_add_sync(0xffffffffu, n);
-    low = __reduce_min_sync(0xffffffffu, n ? end_of(a, 0) : 0x7fffffff);
-    top = __reduce_max_sync(0xffffffffu, n ? end_of(a, n - 1) : -0x7fffffff);
-  }
-  // a pair's key range ends here (or at the sequence's end)
-  __device__ int end_of(const PrefillArgs& a, int pair) { return nk - nq + (pair + 1) * 2 * a.ntok; }
-  __device__ void init(const PrefillArgs& a, int lane) {
-    cur_b = cur_at = 0;
-    load(a, lane);
-  }
-  // pairs that end at x or later
-  __device__ int above(const PrefillArgs& a, int x) {
-    const int before = max(0, x - end_of(a, 0) + 2 * a.ntok - 1) / (2 * a.ntok);
-    return __reduce_add_sync(0xffffffffu, n ? max(0, n - before) : 0);
-  }
-  // -> the lane of the sequence, or -1 behind the last item
-  __device__ int find(const PrefillArgs& a, int idx, int lane, int& pair) {
-    while (idx >= cur_at + total) {
-      if (cur_b + 32 >= a.B) return -1;
-      cur_at += total;
-      cur_b += 32;
-      load(a, lane);
-    }
-    const int r = idx - cur_at;
-    if (a.B > 32) {
-      int inc = n;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, inc, d);
-        if (lane >= d) inc += y;
-      }
-      const int l = __ffs(__ballot_sync(0xffffffffu, r < inc)) - 1;
-      pair = __shfl_sync(0xffffffffu, inc, l) - 1 - r;
-      return l;
-    }
-    int lo = low, hi = top + 1;  // above(lo) > r >= above(hi)
-    while (hi - lo > 1) {
-      const int mid = lo + (hi - lo) / 2;
-      if (above(a, mid) > r) lo = mid; else hi = mid;
-    }
-    // the sequences that have a pair with this end, at most one each
-    const int off = lo - end_of(a, 0), mine = off >= 0 && off % (2 * a.ntok) == 0 ? off / (2 * a.ntok) : n;
-    const unsigned have = __ballot_sync(0xffffffffu, mine < n);
-    const int rank = r - above(a, hi);
-    const int l = __ffs(__ballot_sync(0xffffffffu, mine < n && __popc(have & ((1u << lane) - 1)) == rank)) - 1;
-    pair = __shfl_sync(0xffffffffu, mine, max(l, 0));
-    return l;
-  }
-  // by the sequence's lane: the item, or part `part` of it
-  __device__ void fill(const PrefillArgs& a, int pair, int hk, int part, int of, Item* m) {
-    const int i0 = pair * 2 * a.ntok, n = max(tiles(a, i0, 0), tiles(a, i0, 1));
-    // (an item without parts: plain numbers, no division)
-    const int j0 = of == 1 ? 0 : int((int64_t)n * part / of), j1 = of == 1 ? n : int((int64_t)n * (part + 1) / of);
-    m->tok0 = q0 + i0;
-    m->tok_end = q0 + nq;
-    m->i0 = i0;
-    m->shift = a.causal ? nk - nq + 1 - j0 * BN : 0x3fffffff;
-    m->k0 = k0 + j0 * BN;
-    m->nk = min(nk, j1 * BN) - j0 * BN;
-    m->hk = hk;
-    m->n0 = max(0, min(tiles(a, i0, 0), j1) - j0);
-    m->n1 = max(0, min(tiles(a, i0, 1), j1) - j0);
-    m->lim0 = max(0, min(m->nk, sees(a, i0) - j0 * BN));
-    m->jfix = m->lim0 / BN;
-    m->part = part;
-    m->of = of;
-    m->done = 0;
-  }
-  // keys that place i of this lane's sequence sees; key tiles of query tile t of the pair at i0
-  __device__ int sees(const PrefillArgs& a, int i) { return a.causal ? max(0, min(nk, i + nk - nq + 1)) : nk; }
-  __device__ int tiles(const PrefillArgs& a, int i0, int t) {
-    const int first = i0 + t * a.ntok, last = min(first + a.ntok, nq) - 1;
-    return last >= first ? (sees(a, last) + BN - 1) / BN : 0;
-  }
-  // parts of this lane's pair
-  __device__ int parts_of(const PrefillArgs& a, int pair) {
-    const int i0 = pair * 2 * a.ntok;
-    return max(1, min(a.splits, max(tiles(a, i0, 0), tiles(a, i0, 1)) / MIN_PART));
-  }
-};
 
 // ---------------------------------------------------------------- kernel
 
@@ -467,7 +346,6 @@ __global__ void __launch_bounds__(384, 1)
       }
       if (!ok) break;
       const int64_t row = (int64_t)tok * a.Hq + m.hk * a.g + rhead;
-      if (CUT && row_ok && m.part == 0) a.parts[row] = m.of;
       const bool cut = CUT && m.of > 1;  // into the workspace, in 32 bits
       float* prow = cut ? a.po + ((int64_t)m.part * a.Tq * a.Hq + row) * D : nullptr;
       float* lse_at = cut ? a.plse + (int64_t)m.part * a.Tq * a.Hq + row : a.lse + row;
@@ -767,14 +645,14 @@ __global__ void __launch_bounds__(384, 1)
         int who = f.find(a, int(item / uint32_t(a.Hkv)), lane, pair);
         int of = 1;
         if (CUT && who >= 0) {
-          of = __shfl_sync(0xffffffffu, f.parts_of(a, pair), who);
+          of = __shfl_sync(0xffffffffu, parts_of(a, f.of(who), pair), who % 32);
           if (int(part) >= of) who = -1;
         }
         if (who >= 0) {
           const int s = k & 1;
           if (!wait_all(P_ITE + s, ((k >> 1) & 1) ^ 1, 411)) break;
-          if (lane == who) {
-            f.fill(a, pair, int(item % uint32_t(a.Hkv)), int(part), of, &items[s]);
+          if (lane == who % 32) {
+            fill(a, f.of(who), pair, int(item % uint32_t(a.Hkv)), int(part), of, &items[s]);
             tc::mbar_arrive(&bars[P_ITF + s]);
           }
           if (!wait_all(P_ASK, k & 1, 415)) break;
@@ -883,11 +761,13 @@ __global__ void __launch_bounds__(256) prefill_join_kernel(const __grid_constant
   using T = typename Elem<DT>::T;
   constexpr int C = D / 32;
   __shared__ float shared_acc[8][D];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int share = a.splits >= SHARE_FROM ? 8 : 1, sub = warp & (share - 1);  // warps of a row, this one's place
   const int64_t rows = a.Tq * a.Hq, row = (int64_t)blockIdx.x * (8 / share) + (share == 8 ? 0 : warp);
-  const int n = row < rows ? a.parts[row] : 0;
+  // the count from the offsets, as the items have it: it needs no word of the kernel before, whose rows may be
+  // fewer than these (padding behind the last sequence) or, behind a wait that gave up, unwritten
+  const int n = row < rows ? parts_of_token(a, int(row / a.Hq), lane) : 0;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (n <= 1) return;  // (with shared rows: the whole block)
   float top = -INFINITY, sum = 0.0f;
   for (int i = lane; i < n; i += 32) {
@@ -925,6 +805,12 @@ __global__ void __launch_bounds__(256) prefill_join_kernel(const __grid_constant
 #pragma unroll
   for (int c = 0; c < C; ++c) static_cast<T*>(a.o)[row * D + lane + 32 * c] = Elem<DT>::store(acc[c] * inv);
   if (lane == 0) a.lse[row] = sum == 0.0f ? -INFINITY : ref + logf(sum);
+}
+
+// Query tile pairs that Tq tokens in `seqs` sequences have at most: all of them one token longer than whole pairs.
+int64_t most_pairs(int64_t Tq, int64_t seqs, int g) {
+  const int64_t c = 2 * (128 / g);
+  return (Tq + (seqs < Tq ? seqs : Tq) * (c - 1)) / c;
 }
 
 // Query tile pairs: at least as many as any packing of Tq tokens into B sequences has.
@@ -971,7 +857,7 @@ int launch(const void* q, const void* k, PrefillArgs a, int64_t sq_t, int64_t sq
                ? (x.numRegs < y.numRegs ? x.numRegs : y.numRegs) : 0;
   }();
   MZB_REQUIRE(regs * 384 >= 256 * 208 + 128 * 88, MZB_ERR_LAUNCH, "gqa_prefill: built with %d registers a thread", regs);
-  const int64_t blocks = pairs_bound(a.Tq, a.B, a.g) * a.Hkv * a.splits;
+  const int64_t blocks = most_pairs(a.Tq, int64_t(a.B) + 1, a.g) * a.Hkv * a.splits;  // (the padding is one more sequence)
   MZB_REQUIRE(blocks < (int64_t(1) << 31), MZB_ERR_SHAPE, "gqa_prefill: too large");
   kern<<<unsigned(blocks), 384, C::SMEM, st>>>(m[0], m[1], m[2], a);
   if (int r = launch_status("gqa_prefill")) return r;
@@ -1002,7 +888,7 @@ using namespace mzb;
 extern "C" int64_t mzb_gqa_prefill_ws(int64_t Tq, int64_t Tk, int B, int Hq, int Hkv, int D) {
   if (Tq <= 0 || Tk <= 0 || B <= 0 || Hkv <= 0 || Hq < Hkv || Hq % Hkv || Hq / Hkv > 128) return 0;
   const int n = gqa::split_count(Tq, Tk, B, Hq, Hkv);
-  return n == 1 ? 0 : ((Tq * Hq * (n + 1) + 3) & ~int64_t(3)) + n * Tq * Hq * D;
+  return n == 1 ? 0 : ((Tq * Hq * n + 3) & ~int64_t(3)) + n * Tq * Hq * D;
 }
 
 extern "C" int mzb_gqa_prefill(const void* q, const void* k, const void* v, const int32_t* cu_q, const int32_t* cu_k,
@@ -1028,9 +914,8 @@ extern "C" int mzb_gqa_prefill(const void* q, const void* k, const void* v, cons
   a.err = err;
   a.splits = gqa::split_count(Tq, Tk, B, Hq, Hkv);
   MZB_REQUIRE(a.splits == 1 || ws != nullptr, MZB_ERR_SHAPE, "gqa_prefill: needs a workspace");
-  a.parts = reinterpret_cast<int*>(ws);
-  a.plse = ws + Tq * Hq;
-  a.po = ws + ((Tq * Hq * (a.splits + 1) + 3) & ~int64_t(3));
+  a.plse = ws;
+  a.po = ws + ((Tq * Hq * a.splits + 3) & ~int64_t(3));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
 #define MZB_GO(DT, DD) gqa::launch<DT, DD>(q, k, a, sq_t, sq_h, sk_t, sk_h, st)
   if (dtype == MZB_BF16) return D == 64 ? MZB_GO(MZB_BF16, 64) : D == 96 ? MZB_GO(MZB_BF16, 96) : MZB_GO(MZB_BF16, 128);

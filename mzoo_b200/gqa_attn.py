@@ -76,7 +76,8 @@ def prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tenso
     q ``[Tq, Hq, D]``, k / v ``[Tk, Hkv, D]`` bf16 or f16 (slices of a fused projection are read in
     place); ``cu_q`` / ``cu_k`` int32 ``[B + 1]`` on the device, from 0 ascending: sequence b is
     rows ``cu_q[b] .. cu_q[b+1]`` of q and ``cu_k[b] .. cu_k[b+1]`` of k / v (``cu_k`` None: the
-    same as q's).  softmax_scale defaults to ``D ** -0.5``."""
+    same as q's).  Rows of q from ``cu_q[B]`` on (a batch padded to a fixed size) belong to no
+    sequence: output 0, lse -inf.  softmax_scale defaults to ``D ** -0.5``."""
     if cu_k is None:
         _check_types("prefill", q, k, v, cu_q)
     else:

@@ -1,0 +1,57 @@
+"""Edges of the dense serving operators: rows of no sequence, infinite scores, broken tables, error words,
+tracing."""
+
+import math
+
+import pytest
+import torch
+
+from mzoo_b200 import gqa_attn
+from test_gqa_attn import _cu, _prefill, _randn
+
+
+def _soil(dev, numbers):
+    """Free blocks of the allocator that hold large numbers, of the sizes that a call takes next."""
+    for n in numbers:
+        del_me = torch.full((max(1, n),), 0x3fffffff, dtype=torch.int32, device=dev)
+        del del_me
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv,d,new,keys", [(16, 1, 128, [16], [4000]), (16, 1, 128, [3], [30000]), (4, 2, 64, [2, 0, 5], [1600, 9, 4000]),
+                                               (8, 2, 96, [130, 1, 64], [130, 1, 64]), (2, 1, 64, [7] * 40, [9] * 40),
+                                               (3, 1, 128, [5], [0]), (4, 4, 64, [0], [700])])
+@pytest.mark.parametrize("pad", [1, 16, 300])
+def test_prefill_padded_batch(cuda, hq, hkv, d, new, keys, pad):
+    """Rows behind cu_q[B], with and without cut key ranges, as few and as many parts: 0 and -inf; the
+    rows of sequences are those of the call without padding."""
+    g = torch.Generator().manual_seed(pad)
+    n = sum(new)
+    q = _randn(g, torch.bfloat16, n + pad, hq, d).to(cuda)
+    k, v = (_randn(g, torch.bfloat16, max(1, sum(keys)) + 3, hkv, d).to(cuda) for _ in range(2))
+    cu_q, cu_k = _cu(new).to(cuda), _cu(keys).to(cuda)
+    rows = (n + pad) * hq
+    _soil(cuda, [rows * (s * (d + 1) + 1) for s in (1, 2, 4, 9, 16, 37, 74)])
+    o, lse = gqa_attn.prefill(q, k, v, cu_q, cu_k, check=True)
+    assert not o[n:].any() and bool((lse[n:] == -math.inf).all())
+    if n:
+        want = gqa_attn.prefill(q[:n], k, v, cu_q, cu_k, check=True)
+        # the number of parts may differ: each row is within a rounding of the output's type
+        assert (o[:n].float() - want[0].float()).abs().max() <= 2.0 ** -6 * v.float().abs().max()
+        assert torch.equal(torch.isinf(lse[:n]), torch.isinf(want[1]))
+        some = torch.isfinite(want[1])
+        assert (lse[:n] - want[1])[some].abs().max() <= 1e-4 if some.any() else True
+
+
+@pytest.mark.gpu
+def test_prefill_padding_beside_the_definition(cuda):
+    """A padded call against 64 bits: the keys of the padding's rows are nobody's."""
+    dt = torch.float16
+    g = torch.Generator().manual_seed(1)
+    q, k, v = (_randn(g, dt, 40, h, 64).to(cuda) for h in (4, 2, 2))
+    k[25:], v[25:] = math.nan, math.nan
+    o, lse = gqa_attn.prefill(q, k, v, _cu([9, 16]).to(cuda), check=True)
+    want = gqa_attn.prefill(q[:25], k[:25], v[:25], _cu([9, 16]).to(cuda), check=True)
+    assert torch.equal(o[:25], want[0]) and torch.equal(lse[:25], want[1])
+    assert not o[25:].any() and bool((lse[25:] == -math.inf).all())
+    _prefill(cuda, dt, 4, 2, 64, [9, 16], [9, 16], seed=1)
