@@ -753,8 +753,9 @@ __global__ void __launch_bounds__(384, 1)
 }
 
 // The parts of a cut key range, in their order: a warp per row, or eight that share a row's parts where there
-// may be 32 and more (16 tokens of 16 heads on one behind 30000 keys, 74 parts: 46 us with a warp, 30 shared; 64
-// tokens of 32 on 8 behind 16000, 9 parts: 46 and 50).
+// may be 32 and more.  With a warp a row and shared, the whole call: 16 tokens of 16 heads on one behind 30000 keys (117
+// parts) 64 us and 32; 64 tokens of 32 on 8 behind 16000 (18 parts of 2048 rows) 40 and 45; 128 of 16 on 2 behind
+// 8000 (18 of 2048) 34 and 39.  (The number of rows counts too: 18 parts of 512 rows take 50 and 45.)
 constexpr int SHARE_FROM = 32;
 template <int DT, int D>
 __global__ void __launch_bounds__(256) prefill_join_kernel(const __grid_constant__ PrefillArgs a) {
@@ -813,12 +814,9 @@ int64_t most_pairs(int64_t Tq, int64_t seqs, int g) {
   return (Tq + (seqs < Tq ? seqs : Tq) * (c - 1)) / c;
 }
 
-// Query tile pairs: at least as many as any packing of Tq tokens into B sequences has.
-int64_t pairs_bound(int64_t Tq, int B, int g) { return Tq / (2 * (128 / g)) + (B < Tq ? B : Tq); }
-
 // Parts of a key range: only where the items would leave more than half of the SMs without work.
 int split_count(int64_t Tq, int64_t Tk, int B, int Hq, int Hkv) {
-  const int64_t items = pairs_bound(Tq, B, Hq / Hkv) * Hkv, most = (Tk + BN - 1) / BN / MIN_PART;
+  const int64_t items = most_pairs(Tq, B, Hq / Hkv) * Hkv, most = (Tk + BN - 1) / BN / MIN_PART;
   const int64_t n = num_sms() / items;
   return int(n < 2 || most < 2 ? 1 : n < most ? n : most);
 }

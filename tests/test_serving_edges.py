@@ -55,3 +55,13 @@ def test_prefill_padding_beside_the_definition(cuda):
     assert torch.equal(o[:25], want[0]) and torch.equal(lse[:25], want[1])
     assert not o[25:].any() and bool((lse[25:] == -math.inf).all())
     _prefill(cuda, dt, 4, 2, 64, [9, 16], [9, 16], seed=1)
+
+
+@pytest.mark.parametrize("tokens,hq,hkv,pairs", [(16, 16, 1, 1), (64, 32, 8, 1), (128, 16, 2, 4), (32, 16, 1, 2), (17, 16, 1, 2), (1, 1, 1, 1)])
+def test_one_sequence_is_cut_for_all_sms(tokens, hq, hkv, pairs):
+    """The number of parts (from the workspace's size) is what 148 SMs can take of the sequence's items, also
+    where its tokens fill them exactly."""
+    from mzoo_b200 import _lib
+    floats = _lib.lib().mzb_gqa_prefill_ws(tokens, 60000, 1, hq, hkv, 64)
+    parts = floats // (tokens * hq * 65)
+    assert parts == 148 // (pairs * hkv)
