@@ -31,7 +31,9 @@ struct Item {
   int done;
 };
 
-__device__ __forceinline__ int clip(int x, int lo, int64_t hi) { return x < lo ? lo : x > hi ? int(hi) : x; }
+__device__ __forceinline__ int least(int x, int y) { return x < y ? x : y; }
+__device__ __forceinline__ int most(int x, int y) { return x > y ? x : y; }
+__device__ __forceinline__ int clip(int x, int lo, int hi) { return most(lo, least(x, hi)); }
 
 struct Seq {
   int q0, nq, k0, nk;
@@ -40,10 +42,10 @@ struct Seq {
 __device__ __forceinline__ Seq seq_at(const ItemArgs& a, int b) {
   const int qa = a.cu_q[b], qb = a.cu_q[b + 1], ka = a.cu_k[b], kb = a.cu_k[b + 1];
   Seq s;
-  s.q0 = clip(qa, 0, a.Tq);
-  s.nq = clip(clip(qb, 0, a.Tq) - s.q0, 0, a.Tq);
-  s.k0 = clip(ka, 0, a.Tk);
-  s.nk = clip(clip(kb, 0, a.Tk) - s.k0, 0, a.Tk);
+  s.q0 = clip(qa, 0, int(a.Tq));
+  s.nq = most(0, clip(qb, 0, int(a.Tq)) - s.q0);  // (clipped on both sides: -2^31 - q0 would wrap)
+  s.k0 = clip(ka, 0, int(a.Tk));
+  s.nk = most(0, clip(kb, 0, int(a.Tk)) - s.k0);
   return s;
 }
 // keys that place i of a sequence sees; key tiles of query tile t of the pair at i0
@@ -51,16 +53,12 @@ __device__ __forceinline__ int sees(const ItemArgs& a, const Seq& s, int i) {
   return a.causal ? clip(i + s.nk - s.nq + 1, 0, s.nk) : s.nk;
 }
 __device__ __forceinline__ int tiles(const ItemArgs& a, const Seq& s, int i0, int t) {
-  const int first = i0 + t * a.ntok, end = first + a.ntok, last = (end < s.nq ? end : s.nq) - 1;
+  const int first = i0 + t * a.ntok, last = least(first + a.ntok, s.nq) - 1;
   return last >= first ? (sees(a, s, last) + BN - 1) / BN : 0;
 }
-__device__ __forceinline__ int pair_tiles(const ItemArgs& a, const Seq& s, int i0) {
-  const int x = tiles(a, s, i0, 0), y = tiles(a, s, i0, 1);
-  return x > y ? x : y;
-}
 __device__ __forceinline__ int parts_of(const ItemArgs& a, const Seq& s, int pair) {
-  const int n = pair_tiles(a, s, pair * 2 * a.ntok) / MIN_PART;
-  return n < 1 ? 1 : n < a.splits ? n : a.splits;
+  const int i0 = pair * 2 * a.ntok;
+  return most(1, least(a.splits, most(tiles(a, s, i0, 0), tiles(a, s, i0, 1)) / MIN_PART));
 }
 
 // Parts of the key range of a packed token (the whole warp calls); 1 for a token of no sequence.
@@ -71,7 +69,7 @@ __device__ __forceinline__ int parts_of_token(const ItemArgs& a, int tok, int la
     const unsigned m = __ballot_sync(0xffffffffu, at < hi && a.cu_q[at < hi ? at : lo] <= tok);
     const int last = m ? 31 - __clz(m) : 0;
     lo = lo + last * step;
-    hi = hi < lo + step ? hi : lo + step;
+    hi = least(hi, lo + step);
   }
   const Seq s = seq_at(a, lo);
   return tok >= s.q0 && tok < s.q0 + s.nq ? parts_of(a, s, (tok - s.q0) / (2 * a.ntok)) : 1;
@@ -79,7 +77,7 @@ __device__ __forceinline__ int parts_of_token(const ItemArgs& a, int tok, int la
 
 // By one lane: the item, or part `part` of it.
 __device__ __forceinline__ void fill(const ItemArgs& a, const Seq& s, int pair, int hk, int part, int of, Item* m) {
-  const int i0 = pair * 2 * a.ntok, t0 = tiles(a, s, i0, 0), t1 = tiles(a, s, i0, 1), n = t0 > t1 ? t0 : t1;
+  const int i0 = pair * 2 * a.ntok, t0 = tiles(a, s, i0, 0), t1 = tiles(a, s, i0, 1), n = most(t0, t1);
   // (an item without parts: plain numbers, no division)
   const int j0 = of == 1 ? 0 : int((int64_t)n * part / of), j1 = of == 1 ? n : int((int64_t)n * (part + 1) / of);
   m->tok0 = s.q0 + i0;
@@ -87,10 +85,10 @@ __device__ __forceinline__ void fill(const ItemArgs& a, const Seq& s, int pair, 
   m->i0 = i0;
   m->shift = a.causal ? s.nk - s.nq + 1 - j0 * BN : 0x3fffffff;
   m->k0 = s.k0 + j0 * BN;
-  m->nk = (s.nk < j1 * BN ? s.nk : j1 * BN) - j0 * BN;
+  m->nk = least(s.nk, j1 * BN) - j0 * BN;
   m->hk = hk;
-  m->n0 = clip((t0 < j1 ? t0 : j1) - j0, 0, n);
-  m->n1 = clip((t1 < j1 ? t1 : j1) - j0, 0, n);
+  m->n0 = most(0, least(t0, j1) - j0);
+  m->n1 = most(0, least(t1, j1) - j0);
   m->lim0 = clip(sees(a, s, i0) - j0 * BN, 0, m->nk);
   m->jfix = m->lim0 / BN;
   m->part = part;
@@ -105,19 +103,23 @@ __device__ __forceinline__ void fill(const ItemArgs& a, const Seq& s, int pair, 
 // last, as the pairs of one more sequence, which has no keys.
 struct Finder {
   static constexpr int PAD = 32;
-  Seq mine, pad;  // this lane's sequence (of 32 from cur_b); the padding
-  int n;          // its pairs
+  Seq mine;    // this lane's sequence (of 32 from cur_b)
+  int n;       // its pairs
+  int behind;  // end of the last sequence
   int low, top, total, cur_b, cur_at;
 
-  __device__ const Seq& of(int who) const { return who == PAD ? pad : mine; }
-  __device__ int pairs(const ItemArgs& a, const Seq& s) const { return (s.nq + 2 * a.ntok - 1) / (2 * a.ntok); }
+  // the sequence of find's answer, in its lane (the padding: in lane 0)
+  __device__ Seq of(const ItemArgs& a, int who) const {
+    const int end = clip(behind, 0, int(a.Tq));
+    return who == PAD ? Seq{end, int(a.Tq) - end, 0, 0} : mine;
+  }
   __device__ void load(const ItemArgs& a, int lane) {
     const int b = cur_b + lane;
     mine = Seq{0, 0, 0, 0};
     n = 0;
     if (b < a.B) {
       mine = seq_at(a, b);
-      n = pairs(a, mine);
+      n = (mine.nq + 2 * a.ntok - 1) / (2 * a.ntok);
     }
     total = __reduce_add_sync(0xffffffffu, n);
     low = __reduce_min_sync(0xffffffffu, n ? end_of(a, 0) : 0x7fffffff);
@@ -126,22 +128,21 @@ struct Finder {
   // a pair's key range ends here (or at the sequence's end)
   __device__ int end_of(const ItemArgs& a, int pair) const { return mine.nk - mine.nq + (pair + 1) * 2 * a.ntok; }
   __device__ void init(const ItemArgs& a, int lane) {
-    const int end = clip(a.cu_q[a.B], 0, a.Tq);
-    pad = Seq{end, int(a.Tq) - end, 0, 0};
+    behind = a.cu_q[a.B];
     cur_b = cur_at = 0;
     load(a, lane);
   }
   // pairs that end at x or later
   __device__ int above(const ItemArgs& a, int x) const {
-    const int d = x - end_of(a, 0) + 2 * a.ntok - 1, before = d > 0 ? d / (2 * a.ntok) : 0;
-    return __reduce_add_sync(0xffffffffu, n > before ? n - before : 0);
+    const int before = most(0, x - end_of(a, 0) + 2 * a.ntok - 1) / (2 * a.ntok);
+    return __reduce_add_sync(0xffffffffu, most(0, n - before));
   }
   // -> the lane of the sequence, PAD, or -1 behind the last item
   __device__ int find(const ItemArgs& a, int idx, int lane, int& pair) {
     while (idx >= cur_at + total) {
       if (cur_b + 32 >= a.B) {
         pair = idx - cur_at - total;
-        return pair < pairs(a, pad) ? PAD : -1;
+        return pair * int64_t(2 * a.ntok) < a.Tq - clip(behind, 0, int(a.Tq)) ? PAD : -1;
       }
       cur_at += total;
       cur_b += 32;
@@ -169,7 +170,7 @@ struct Finder {
     const unsigned have = __ballot_sync(0xffffffffu, at < n);
     const int rank = r - above(a, hi);
     const int l = __ffs(__ballot_sync(0xffffffffu, at < n && __popc(have & ((1u << lane) - 1)) == rank)) - 1;
-    pair = __shfl_sync(0xffffffffu, at, l > 0 ? l : 0);
+    pair = __shfl_sync(0xffffffffu, at, most(l, 0));
     return l;
   }
 };

@@ -645,14 +645,14 @@ __global__ void __launch_bounds__(384, 1)
         int who = f.find(a, int(item / uint32_t(a.Hkv)), lane, pair);
         int of = 1;
         if (CUT && who >= 0) {
-          of = __shfl_sync(0xffffffffu, parts_of(a, f.of(who), pair), who % 32);
+          of = __shfl_sync(0xffffffffu, parts_of(a, f.of(a, who), pair), who % 32);
           if (int(part) >= of) who = -1;
         }
         if (who >= 0) {
           const int s = k & 1;
           if (!wait_all(P_ITE + s, ((k >> 1) & 1) ^ 1, 411)) break;
           if (lane == who % 32) {
-            fill(a, f.of(who), pair, int(item % uint32_t(a.Hkv)), int(part), of, &items[s]);
+            fill(a, f.of(a, who), pair, int(item % uint32_t(a.Hkv)), int(part), of, &items[s]);
             tc::mbar_arrive(&bars[P_ITF + s]);
           }
           if (!wait_all(P_ASK, k & 1, 415)) break;

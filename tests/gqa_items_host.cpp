@@ -96,10 +96,10 @@ int main() {
     for (int idx : order) {
       int pair = 0, who = f.find(a, idx / splits, lane, pair), of = 1;
       if (who < 0) continue;
-      of = __shfl_sync(~0u, parts_of(a, f.of(who), pair), who % 32);
+      of = __shfl_sync(~0u, parts_of(a, f.of(a, who), pair), who % 32);
       if (idx % splits >= of) continue;
       if (lane == who % 32) {
-        fill(a, f.of(who), pair, 0, idx % splits, of, &item);
+        fill(a, f.of(a, who), pair, 0, idx % splits, of, &item);
         printf("item %d %d %d %d %d %d %d %d %d\n", who, item.tok0, item.tok_end, item.k0, item.nk, item.n0, item.n1, item.part, item.of);
       }
     }
