@@ -99,7 +99,7 @@ __device__ __forceinline__ void fill(const ItemArgs& a, const Seq& s, int pair, 
 // Item number -> (sequence, pair within it), by the scheduler warp.  Up to 32 sequences (a lane
 // for each): by descending end of the pair's key range, so that the longest items come first and
 // the last blocks' shares are even; more: sequence after sequence, the last pair first, from a
-// cursor (a block's item numbers only grow).  Rows behind the last sequence (a padded batch) come
+// cursor, which a number behind it sets back (a block's numbers mostly grow, but nothing promises it).  Rows behind the last sequence (a padded batch) come
 // last, as the pairs of one more sequence, which has no keys.
 struct Finder {
   static constexpr int PAD = 32;
@@ -139,6 +139,10 @@ struct Finder {
   }
   // -> the lane of the sequence, PAD, or -1 behind the last item
   __device__ int find(const ItemArgs& a, int idx, int lane, int& pair) {
+    if (idx < cur_at) {
+      cur_b = cur_at = 0;
+      load(a, lane);
+    }
     while (idx >= cur_at + total) {
       if (cur_b + 32 >= a.B) {
         pair = idx - cur_at - total;

@@ -90,3 +90,12 @@ def test_parts_stay_in_bounds_whatever_the_offsets_hold(host, seed):
     assert len(parts) == Tq and all(1 <= n <= splits for n in parts)
     for who, tok0, tok_end, k0, nk, n0, n1, part, of in items:
         assert 0 <= tok0 and tok_end <= Tq and 0 <= k0 and k0 + max(nk, 0) <= Tk and 0 <= part < of <= splits
+
+
+@pytest.mark.parametrize("new,keys,ntok,splits", CASES[-2:] + [([5, 0, 300] * 25, [5, 2, 300] * 25, 8, 1), CASES[6]])
+@pytest.mark.parametrize("seed", [0, 1, 2])
+def test_block_numbers_in_any_order(host, new, keys, ntok, splits, seed):
+    """A running block takes over numbers of others, in whatever order they come."""
+    cu_q, cu_k = _cu(new), _cu(keys)
+    items, parts = host(cu_q, cu_k, ntok, True, splits, cu_q[-1] + 9, cu_k[-1], seed)
+    _check(items, parts, cu_q, cu_k, ntok, True, splits, cu_q[-1] + 9)
