@@ -144,6 +144,15 @@ __device__ __forceinline__ bool wait_stage(uint64_t* bar, uint32_t parity, volat
   return __all_sync(0xffffffffu, got);
 }
 
+// The eight product warps meet: whether one of them has given up (they leave through here only, all of them at one
+// meeting, so that none is left behind at a barrier).
+__device__ __forceinline__ bool meet(bool gave_up) {
+  uint32_t any;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+               : "=r"(any) : "r"(uint32_t(gave_up)) : "memory");
+  return any != 0;
+}
+
 __device__ __forceinline__ int len_of(const DecodeArgs& a, int b) { return max(0, min(a.lens[b], a.W * a.page)); }
 
 // MT: head tiles of 8 NH heads.  A warp has one of them and, 32 at a time, its share of the key tile.  With one head
@@ -383,12 +392,13 @@ __global__ void __launch_bounds__(THREADS, 1)
         s = 0;
         phase ^= 1;
       }
-      if (!wait_stage(&full[s], phase, abort_flag, a.err, 423)) {
-        *abort_flag = 1;
+      const bool got = wait_stage(&full[s], phase, abort_flag, a.err, 423);
+      if (!got) *abort_flag = 1;
+      const Meta w = meta[s];
+      if (!got || (w.flags & END)) {
+        meet(!got);
         break;
       }
-      const Meta w = meta[s];
-      if (w.flags & END) break;
       if (w.flags & FIRST) {  // this group's query rows
         if constexpr (MT * HT <= 16) {  // (rows behind the last repeat it: their results go nowhere)
 #pragma unroll
@@ -538,12 +548,13 @@ __global__ void __launch_bounds__(THREADS, 1)
           for (int e = 0; e < 2; ++e)
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], d);
+        if (meet(false)) break;  // (and what the last merge wrote has been read)
         // a few heads of a tile at a time (the ring needs the shared memory more); channels are exchanged in
         // eights by the head's number, so that the heads of a store lie on different banks
         const int gr = min(a.g, HT);
 #pragma unroll 1
         for (int at = 0; at < gr; at += C::ROWS) {
-          tc::bar_sync(1, 256);  // what the last pass wrote has been read
+          if (at) tc::bar_sync(1, 256);  // what the last pass wrote has been read
           if (at == 0 && r0 == 0)
 #pragma unroll
             for (int n = 0; n < NH; ++n)
