@@ -352,6 +352,9 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
     } else {
       *abort_flag = 1;
+      // no copy is left in flight when the block ends: stages below s were last filled in this round of the ring, the
+      // others in the one before (never: the barrier's phase -1, which has passed)
+      for (int x = 0; x < a.stages; ++x) tc::mbar_wait(&full[x], x < s ? phase : phase ^ 1, a.err, 424);
     }
   } else {
     // ---------------------------------------------------------------- products

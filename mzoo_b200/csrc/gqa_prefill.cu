@@ -500,6 +500,15 @@ __global__ void __launch_bounds__(384, 1)
         }
         __syncwarp();
       }
+      // a wait gave up: no copy is left in flight when the block ends (the ring's slots, from the one that is next, and
+      // the query tiles; of a barrier that was not used yet phase -1 has passed)
+      if (*abort_flag && tc::elect_one()) {
+#pragma unroll 1
+        for (uint32_t x = 0; x < C::NS + 2; ++x) {
+          const uint32_t fills = x < C::NS ? (g + x) / C::NS : x == C::NS ? nq[0] : nq[1];
+          tc::mbar_wait(&bars[x < C::NS ? P_KF + (g + x) % C::NS : P_QF + x - C::NS], (fills & 1) ^ 1, a.err, 418);
+        }
+      }
     } else if (warp == 9) {
       // ---------------------------------------------------------------- MMA issue
       const uint32_t fmt = DT == MZB_BF16 ? 1 : 0;
@@ -630,6 +639,14 @@ __global__ void __launch_bounds__(384, 1)
         if (!ok) *abort_flag = 1;
         }
         __syncwarp();
+      }
+      // nor a product when the TMEM is freed
+      if (*abort_flag && tc::elect_one()) {
+        uint64_t* last = reinterpret_cast<uint64_t*>(smem + C::TILES + 568);
+        tc::mbar_init(last, 1);
+        tc::fence_barrier_init();
+        tc::mma_commit(last);
+        tc::mbar_wait(last, 0, a.err, 419);
       }
     } else if (warp == 10) {
       // ---------------------------------------------------------------- scheduler
