@@ -280,7 +280,8 @@ MZB_API int mzb_kv_unpack_fp4(const uint8_t* codes, const uint8_t* scales, void*
  * mzb_gqa_decode -- one token per sequence over a paged cache.  q [B, Hq, D]; k_pages /
  *   v_pages [P, Hkv, page, D] by their page, head and token strides in elements; key t of
  *   sequence b is slot t % page of page page_table[b, t / page], t < min(seq_lens[b], W * page).
- *   Entries past a sequence's length are never used (ids outside [0, P) are clamped).
+ *   Entries past a sequence's length are never used; an id outside [0, P) within it sets *err =
+ *   MZB_ERR_PAGES (that sequence's output is then of no use).
  *   ws: mzb_gqa_decode_ws(...) floats.  page in {16, 32, 64, 128}.
  */
 MZB_API int64_t mzb_gqa_prefill_ws(int64_t Tq, int64_t Tk, int B, int Hq, int Hkv, int D);

@@ -283,16 +283,21 @@ __global__ void __launch_bounds__(THREADS, 1)
       const int32_t* row = a.table + (int64_t)b * a.W;
       const int box0 = t0 << tile_log, boxes = (len + rows - 1) >> rows_log;  // boxes with live keys
       auto ids = [&](int x) {  // box x of the sequence
-        int p = 0;
-        if (x < boxes) p = row[x >> (a.page_log - rows_log)];
+        return x < boxes ? row[x >> (a.page_log - rows_log)] : 0;
+      };
+      // an id outside the pool is an error, and some page is read in its place; looked at when the ids are needed, so
+      // that the next ones stay in flight
+      auto checked = [&](int p) {
+        if (p < 0 || p >= a.P) atomicExch(a.err, MZB_ERR_PAGES);
         return max(0, min(p, int(a.P - 1)));
       };
       int cur = ids(box0 + lane), nxt = ids(box0 + 32 + lane), base = box0;
+      cur = checked(cur);
       for (int i = 0; i < n; ++i) {
         const int t = t0 + i, keys = min(TK, len - t * TK), live = (keys + rows - 1) >> rows_log;
         if ((t << tile_log) - base >= 32) {
           base += 32;
-          cur = nxt;
+          cur = checked(nxt);
           nxt = ids(base + 32 + lane);
         }
         ok = wait_stage(&empty[s], phase ^ 1, abort_flag, a.err, 421);

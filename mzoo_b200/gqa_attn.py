@@ -106,7 +106,9 @@ def decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_t
     q ``[B, Hq, D]``; k_pages / v_pages ``[P, Hkv, page, D]`` of q's type, any strides over a dense
     last dimension (a ``[P, page, Hkv, D]`` pool as ``pool.transpose(1, 2)``); page_table int32
     ``[B, W]``; seq_lens int32 ``[B]`` (the new token's key included; 0 = empty slot).  Lengths past
-    ``W * page`` are cut there.  What the pages hold past a sequence's length is not used."""
+    ``W * page`` are cut there.  What the pages hold past a sequence's length is not used.  A page id
+    outside the pool within a length (-1: a sequence without all its pages) is raised by
+    ``mzoo_b200.check_errors()``, or at once with ``check=True``."""
     _check_types("decode", q, k_pages, v_pages, page_table, seq_lens)
     qs, ks = q.shape, k_pages.shape
     assert len(ks) == 4 and ks == v_pages.shape and ks[3] == qs[-1] and ks[0], \

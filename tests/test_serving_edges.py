@@ -6,8 +6,9 @@ import math
 import pytest
 import torch
 
-from mzoo_b200 import gqa_attn
-from test_gqa_attn import _cu, _prefill, _randn
+import mzoo_b200
+from mzoo_b200 import _lib, gqa_attn
+from test_gqa_attn import _cu, _pages, _prefill, _randn
 
 
 def _soil(dev, numbers):
@@ -65,3 +66,28 @@ def test_one_sequence_is_cut_for_all_sms(tokens, hq, hkv, pairs):
     floats = _lib.lib().mzb_gqa_prefill_ws(tokens, 60000, 1, hq, hkv, 64)
     parts = floats // (tokens * hq * 65)
     assert parts == 148 // (pairs * hkv)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,width,at", [([40, 0, 100], None, (2, 3)), ([40, 0, 100], None, (0, 0)), ([200, 256], 8, (1, 7)),
+                                           ([30000, 9], None, (0, 700)), ([30000, 9], None, (1, 0)), ([5000] * 70, None, (69, 156))])
+@pytest.mark.parametrize("bad", [-1, -2 ** 31, 2 ** 31 - 1, "P"])
+def test_decode_reports_ids_outside_the_pool(cuda, lens, width, at, bad):
+    """Within a sequence's length they are an error, in whichever block's run they lie; other sequences are
+    right.  Behind the length they are nobody's."""
+    g = torch.Generator().manual_seed(0)
+    q = _randn(g, torch.bfloat16, len(lens), 4, 64).to(cuda)
+    kp, vp, table = _pages(g, torch.bfloat16, 2, 64, 32, lens, width=width)
+    rest = [t.to(cuda) for t in (kp, vp)]
+    n = torch.tensor(lens, dtype=torch.int32, device=cuda)
+    want = gqa_attn.decode(q, *rest, table.to(cuda), n, check=True)
+    table[at] = kp.shape[0] if bad == "P" else bad
+    with pytest.raises(_lib.MzbError, match="id out of range"):
+        gqa_attn.decode(q, *rest, table.to(cuda), n, check=True)
+    o, lse = gqa_attn.decode(q, *rest, table.to(cuda), n)
+    with pytest.raises(_lib.MzbError, match="page"):
+        mzoo_b200.check_errors()
+    others = torch.arange(len(lens)) != at[0]
+    assert torch.equal(o[others], want[0][others]) and torch.equal(lse[others], want[1][others])
+    n[at[0]] = 32 * at[1]  # now it lies behind the length
+    gqa_attn.decode(q, *rest, table.to(cuda), n, check=True)
