@@ -24,6 +24,7 @@
 // dependent trips to memory), 5.3 us in all for 77 keys.
 #include <type_traits>
 
+#include "gqa_softmax.cuh"
 #include "tc.cuh"
 
 namespace mzb {
@@ -54,7 +55,7 @@ struct DecodeArgs {
 };
 
 // ws: int [MAX_BLOCKS] (the (sequence, head) that a block begins and leaves to others; -1: none), int [B * Hkv]
-// (the block that ends such a one), then for each of 2 * MAX_BLOCKS parts: float2 [g] (maximum, sum), float [g][D].
+// (the block that ends such a one), then for each of 2 * MAX_BLOCKS parts: float2 [g] (reference or -inf, sum), float [g][D].
 __device__ __forceinline__ int* ws_open(const DecodeArgs& a) { return reinterpret_cast<int*>(a.ws); }
 __device__ __forceinline__ int* ws_last(const DecodeArgs& a) { return reinterpret_cast<int*>(a.ws) + MAX_BLOCKS; }
 __host__ __device__ inline int64_t ws_head(int B, int Hkv) { return (MAX_BLOCKS + (int64_t)B * Hkv + 3) & ~int64_t(3); }
@@ -475,10 +476,10 @@ __global__ void __launch_bounds__(THREADS, 1)
               for (int d = 4; d < 32; d <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, d));
               top[n][e] = t;
             }
-          // O and the sums are rescaled only when a maximum has grown by more than 2^8
+          // O and the sums are rescaled only when a maximum has grown by more than 2^GROW
           bool grown = false;
 #pragma unroll
-          for (int n = 0; n < NH; ++n) grown |= top[n][0] > m[n][0] + 8.0f || top[n][1] > m[n][1] + 8.0f;
+          for (int n = 0; n < NH; ++n) grown |= top[n][0] > m[n][0] + Running<DT>::GROW || top[n][1] > m[n][1] + Running<DT>::GROW;
           if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
             for (int n = 0; n < NH; ++n) {
@@ -486,7 +487,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
                 const float mn = fmaxf(m[n][e], top[n][e]);
-                al[e] = mn == -INFINITY ? 1.0f : fast_exp2(m[n][e] - mn);
+                al[e] = mn == -INFINITY ? 1.0f : fast_exp2(Running<DT>::relative(m[n][e]) - Running<DT>::relative(mn));
                 m[n][e] = mn;
                 l[n][e] *= al[e];
               }
@@ -504,7 +505,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             uint32_t ph[NH][2], pl[NH][2];
 #pragma unroll
             for (int n = 0; n < NH; ++n) {
-              const float ms[2] = {m[n][0] == -INFINITY ? 0.0f : m[n][0], m[n][1] == -INFINITY ? 0.0f : m[n][1]};
+              const float ms[2] = {Running<DT>::reference(m[n][0]), Running<DT>::reference(m[n][1])};
 #pragma unroll
               for (int r = 0; r < 2; ++r) {
                 const float p0 = fast_exp2(sc[x][n][2 * r] - ms[0]), p1 = fast_exp2(sc[x][n][2 * r + 1] - ms[1]);
@@ -568,7 +569,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             for (int n = 0; n < NH; ++n)
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
-                sm_m[warp][8 * n + c0 + e] = m[n][e];
+                sm_m[warp][8 * n + c0 + e] = Running<DT>::relative(m[n][e]);
                 sm_l[warp][8 * n + c0 + e] = l[n][e];
               }
           const int mine = c0 + (at & 8) - at;  // this thread's heads of the pass: this one and the next

@@ -22,7 +22,10 @@
 // The two query tiles take turns on the tensor cores: QK_0(j+1) is issued behind PV_0(j), so
 // one tile's products run while the other's exponentials do.  S and P of a tile share 128 TMEM
 // columns (P overwrites S), O takes D; a row's O is rescaled only when its maximum has grown
-// by more than 2^8 (fp32 sums and weights of at most 2^8 lose nothing by waiting).
+// by more than 2^8 (2^7 for f16; fp32 sums lose nothing by waiting).  A weight is rounded once, to V's type, for
+// the product (both operands of an MMA have one type, and a second product with what is left would add
+// half of the step's tensor time, which bounds it); the row's sum takes the unrounded ones.  o is within
+// u sum_j p_j |v_j| of the 32-bit form, u = 2^-8 or 2^-11.
 // Where few rows meet many keys, an item's key range is cut into parts that a second kernel joins
 // (16 tokens on 30000 keys, 32 heads on 8: 345 us in one part, 48 us in 18).
 //
@@ -36,6 +39,7 @@
 // weights against the maximum of the tile before, one issuing thread for each tile (they fall into
 // step and fight for the exponential unit), more of the exponentials on the FMA pipe.
 #include "gqa_items.cuh"
+#include "gqa_softmax.cuh"
 #include "tc.cuh"
 
 namespace mzb {
@@ -234,7 +238,7 @@ __global__ void __launch_bounds__(384, 1)
       const bool row_ok = rtok < a.ntok && tok < m.tok_end;
       const int lim = row_ok ? max(0, min(m.nk, i + m.shift)) : 0x3fffffff;  // keys that this row sees
       const int n = t ? m.n1 : m.n0;
-      float ms = 0.0f, mx = -INFINITY, lsum = 0.0f;  // running maximum (log2 domain) and sum
+      float ms = 0.0f, mx = -INFINITY, lsum = 0.0f;  // the weights' reference, running maximum (log2 domain), sum
       bool ok = true;
       for (int j = 0; j < n; ++j, ++ns) {
         if (!__all_sync(0xffffffffu, tc::mbar_wait(&bars[P_SF + t], ns & 1, a.err, 409))) {
@@ -284,7 +288,7 @@ __global__ void __launch_bounds__(384, 1)
         // exponential does not carry one
         float mt = max2(max2(m4[0], m4[1]), max2(m4[2], m4[3])) * a.sl;
         mt = mt < INFINITY ? mt : NAN;
-        const bool need = !(mt <= mx + 8.0f);
+        const bool need = !(mt <= mx + Running<DT>::GROW);
         bool behind = C::SEP && j > 0;  // the previous PV may still read P and add to O
         auto after_pv = [&]() {
           if (!behind) return true;
@@ -296,10 +300,10 @@ __global__ void __launch_bounds__(384, 1)
         if (__any_sync(0xffffffffu, need)) {
           if (!after_pv()) { ok = false; break; }
           const float mn = need ? mt : mx;
-          const float alpha = need ? fast_exp2(mx - mn) : 1.0f;
+          const float alpha = need ? fast_exp2(Running<DT>::relative(mx) - Running<DT>::relative(mn)) : 1.0f;
           mx = mn;
           lsum *= alpha;
-          ms = mx == -INFINITY ? 0.0f : mx;
+          ms = Running<DT>::reference(mx);
           if (j > 0) {  // (not SEP: S_FULL was committed behind the previous PV, so O is complete)
 #pragma unroll 1
             for (int c0 = 0; c0 < D; c0 += 32) {
@@ -453,7 +457,7 @@ __global__ void __launch_bounds__(384, 1)
           }
         }
       }
-      if (row_ok) *lse_at = lim > 0 ? (mx + log2f(lsum)) * LN2 : -INFINITY;
+      if (row_ok) *lse_at = lim > 0 ? (Running<DT>::relative(mx) + log2f(lsum)) * LN2 : -INFINITY;
       tc::fence_before_sync();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&bars[P_OE + t]);

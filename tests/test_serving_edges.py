@@ -91,3 +91,74 @@ def test_decode_reports_ids_outside_the_pool(cuda, lens, width, at, bad):
     assert torch.equal(o[others], want[0][others]) and torch.equal(lse[others], want[1][others])
     n[at[0]] = 32 * at[1]  # now it lies behind the length
     gqa_attn.decode(q, *rest, table.to(cuda), n, check=True)
+
+
+def _sink(g, nq, n, at, bits):
+    """q rows and n keys whose scores (scale 1) lie around 0 but for key `at`, `bits` bits above; its value is 0."""
+    q, k = torch.zeros(nq, 1, 64), torch.zeros(n, 1, 64)
+    q[:, :, 0], q[:, :, 1] = 1.0, torch.rand(nq, 1, generator=g) + 0.5
+    k[:, :, 1] = torch.randn(n, 1, generator=g) * 0.5
+    k[at, :, 0], k[at, :, 1] = bits * math.log(2.0), 0.0
+    v = torch.rand(n, 1, 64, generator=g) + 0.5
+    v[at] = 0.0
+    return q.half(), k.half(), v.half()
+
+
+def _near(o, lse, q, k, v, seen):
+    """f16 results against 64 bits: each weight and the output are rounded to 11 bits once, weights below 2^-14 of
+    2^8 times the largest to multiples of 2^-32 of it, and fp32 arithmetic adds 2^-14."""
+    q, k, v = q[:, 0].double(), k[:, 0].double(), v[:, 0].double()
+    x = (q @ k.T).masked_fill(~seen, -math.inf)
+    rl = torch.logsumexp(x, 1)
+    p = torch.exp(x - rl[:, None])
+    ro, mag, tiny = p @ v, p @ v.abs(), seen.double() @ v.abs()
+    bound = 2.0 ** -11 * (mag + ro.abs()) * 1.01 + 2.0 ** -14 * mag + 2.0 ** -33 * tiny + 2.0 ** -25
+    assert ((o.double().cpu()[:, 0] - ro).abs() / bound).max() <= 1
+    assert ((lse.double().cpu()[:, 0] - rl).abs() <= 2e-5 + 2e-6 * rl.abs()).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [10, 20, 26, 30])
+@pytest.mark.parametrize("at", [0, 30000, 59990])
+def test_f16_weights_beside_a_sink(cuda, bits, at):
+    """One key takes nearly all of the weight and has no value: the rest of a long context, some 2^-26 each, is
+    the output.  Prefill with few rows (cut key ranges) and with many, and decode."""
+    n = 60000
+    g = torch.Generator().manual_seed(bits)
+    for nq in (3, 300):
+        q, k, v = _sink(g, nq, n, at, bits)
+        qs = q.expand(-1, 1 if nq == 3 else 64, -1).contiguous()  # 64 heads of the same rows: no cuts
+        o, lse = gqa_attn.prefill(qs.to(cuda), k.to(cuda), v.to(cuda), _cu([nq]).to(cuda), _cu([n]).to(cuda),
+                                  softmax_scale=1.0, check=True)
+        seen = torch.arange(n)[None] <= torch.arange(nq)[:, None] + n - nq
+        _near(o[:, -1:], lse[:, -1:], q, k, v, seen)
+    pools = [t.view(n // 32, 32, 1, 64).transpose(1, 2).to(cuda) for t in (k, v)]
+    o, lse = gqa_attn.decode(qs[:2].to(cuda), *pools, torch.arange(n // 32, dtype=torch.int32, device=cuda).expand(2, -1),
+                             torch.tensor([n, n - 7], dtype=torch.int32, device=cuda), softmax_scale=1.0, check=True)
+    seen = torch.arange(n)[None] < torch.tensor([[n], [n - 7]])
+    _near(o[:, -1:], lse[:, -1:], q[:2], k, v, seen)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("step", [0.0, 4.0, 5.5, 8.0, 11.0])
+@pytest.mark.parametrize("base", [0.0, 3000.0, -8.4e6, 5.0e7, 3.0e8])
+def test_scores_that_grow_by_a_few_bits_a_tile(cuda, dt, step, base):
+    """Maxima that grow by about as much as a reference waits for, at small and very large scores: weights stay
+    in the type's range and every part of the sum has its share."""
+    n, tile = 1024, 128
+    q, k, v = torch.zeros(1, 1, 64), torch.zeros(n, 1, 64), torch.ones(n, 1, 64)
+    q[:, :, 0], k[:, :, 0] = 1.0, (torch.arange(n) // tile).float()[:, None] * step
+    q[:, :, 1], k[:, :, 1] = 2.0 ** 12, base / 2 ** 12 if abs(base) < 1e8 else math.copysign(2.0 ** 14, base)
+    q, k, v = (t.to(dt) for t in (q, k, v))
+    scale = math.log(2.0)
+    x = q[:, 0].double() @ k[:, 0].double().T * scale
+    o, lse = gqa_attn.prefill(q.to(cuda), k.to(cuda), v.to(cuda), _cu([1]).to(cuda), _cu([n]).to(cuda), softmax_scale=scale, check=True)
+    pools = [t.view(n // 64, 64, 1, 64).transpose(1, 2).to(cuda) for t in (k, v)]
+    od, ld = gqa_attn.decode(q.to(cuda), *pools, torch.arange(n // 64, dtype=torch.int32, device=cuda)[None],
+                             torch.tensor([n], dtype=torch.int32, device=cuda), softmax_scale=scale, check=True)
+    want = torch.logsumexp(x, 1)
+    # all values are 1, so the output is whatever the weights are; the scores are fp32 sums, off by some 2^-23 of the base
+    for a, b in ((o, lse), (od, ld)):
+        assert torch.isfinite(a).all() and (a.float() - 1).abs().max() <= 2.0 ** -6
+        assert abs(float(b) - float(want)) <= 1e-3 + 2.0 ** -21 * abs(float(want))
