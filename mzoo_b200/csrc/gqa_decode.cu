@@ -608,7 +608,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
             if (w.part < 0) {
               const int64_t row = (int64_t)w.b * a.Hq + w.hk * a.g + h;
-              const float inv = 1.0f / ls;
+              const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;  // 0: scores of -inf alone
               *reinterpret_cast<uint2*>(static_cast<T*>(a.o) + row * D + d) =
                   make_uint2(pack2<DT>(acc.x * inv, acc.y * inv), pack2<DT>(acc.z * inv, acc.w * inv));
               if (d == 0) a.lse[row] = (mx + log2f(ls)) * LN2;
@@ -700,7 +700,7 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Decod
   }
   __syncthreads();
   if (threadIdx.x < C4) {
-    const float inv = 1.0f / ls;
+    const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
     float4 t = sum[0][lane];
 #pragma unroll
     for (int w = 1; w < 4; ++w) {

@@ -368,7 +368,7 @@ __global__ void __launch_bounds__(384, 1)
       ++no;
       tc::fence_after_sync();
       const bool bad = bad_v[par] != 0;
-      const float inv = lim > 0 ? 1.0f / lsum : 0.0f;  // a row without keys in a tile with some: O is 0
+      const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;  // a row without keys or with scores of -inf alone: O is 0
       // through shared memory, 32 channels at a time, so that a store covers 64 bytes of each of eight
       // rows (a thread storing its own row touches 32 lines an instruction: ~4000 cycles an item);
       // the 16-byte pieces of a row at its place mod 8 keep both directions free of conflicts

@@ -162,3 +162,35 @@ def test_scores_that_grow_by_a_few_bits_a_tile(cuda, dt, step, base):
     for a, b in ((o, lse), (od, ld)):
         assert torch.isfinite(a).all() and (a.float() - 1).abs().max() <= 2.0 ** -6
         assert abs(float(b) - float(want)) <= 1e-3 + 2.0 ** -21 * abs(float(want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d,hq,n", [(64, 4, 200), (128, 2, 5), (96, 2, 200), (64, 1, 6000), (128, 40, 6000)])
+def test_scores_of_minus_infinity(cuda, dt, d, hq, n):
+    """Keys whose scores are -inf have no weight; rows that see no others are 0 and -inf, whether the key range
+    is cut or not."""
+    g = torch.Generator().manual_seed(n)
+    q, k, v = _randn(g, dt, 3, hq, d), _randn(g, dt, n, 1, d), _randn(g, dt, n, 1, d)
+    q[:, :, 0] = 1.0
+    cu = [_cu([3]).to(cuda), _cu([n]).to(cuda)]
+    pools = lambda x: torch.cat([x, torch.zeros(-n % 16, 1, d, dtype=dt)]).view(-1, 16, 1, d).transpose(1, 2).to(cuda)  # noqa: E731
+    table = torch.arange(-(-n // 16), dtype=torch.int32, device=cuda).expand(3, -1)
+    lens = torch.tensor([n, n, 0], dtype=torch.int32, device=cuda)
+
+    def both(k):
+        return (gqa_attn.prefill(q.to(cuda), k.to(cuda), v.to(cuda), *cu, causal=False, check=True),
+                gqa_attn.decode(q.to(cuda), pools(k), pools(v), table, lens, check=True))
+    some, kept = k.clone(), torch.rand(n, generator=g) < 0.3
+    kept[n // 2] = True
+    some[~kept, :, 0] = -math.inf
+    (o, lse), (od, ld) = both(some)
+    x = torch.einsum("qhd,kd->qhk", q.double(), k[:, 0].double()) * d ** -0.5
+    p = torch.softmax(x.masked_fill(~kept, -math.inf), -1)
+    want, mag = p @ v[:, 0].double(), p @ v[:, 0].double().abs()
+    # a rounding of each weight, one of the output, fp32 arithmetic (as in test_gqa_attn.py)
+    bound = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}[dt] * (mag + want.abs()) * 1.01 + 2.0 ** -14 * mag
+    assert ((o.double().cpu() - want).abs() <= bound).all() and ((od.double().cpu() - want)[:2].abs() <= bound[:2]).all()
+    k[:, :, 0] = -math.inf
+    for a, b in both(k):
+        assert not a.any() and bool((b == -math.inf).all())
