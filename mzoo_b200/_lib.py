@@ -103,6 +103,13 @@ def lib() -> ctypes.CDLL:
 torch_ops_loaded = False
 
 
+@ctypes.CFUNCTYPE(_I64, _I32)
+def _word_address(index: int) -> int:
+    """Address of the persistent error word of a device (called once for each, from the C++ ops)."""
+    from . import ops
+    return ops._err(torch.device("cuda", index), False).data_ptr()
+
+
 def load_torch_ops() -> None:
     """Register the C++ kernels of the serving ops with torch (once)."""
     global torch_ops_loaded
@@ -112,7 +119,7 @@ def load_torch_ops() -> None:
                               "(mzoo_b200 has no CPU or eager fallback)")
         lib()  # libmzb200.so, which it is linked to
         msg = ctypes.create_string_buffer(2000)
-        if ctypes.CDLL(TORCH_LIB_PATH).mzb_torch_register(msg, ctypes.c_size_t(len(msg))):
+        if ctypes.CDLL(TORCH_LIB_PATH).mzb_torch_register(_word_address, msg, ctypes.c_size_t(len(msg))):
             raise ImportError(f"{TORCH_LIB_PATH} does not fit this package (build it with `python -m mzoo_b200.build "
                               f"--force`): {msg.value.decode(errors='replace').splitlines()[0]}")
         torch_ops_loaded = True

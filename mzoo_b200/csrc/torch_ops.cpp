@@ -10,6 +10,9 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
 
+#include <array>
+#include <atomic>
+
 #include "../../include/mzb200.h"
 
 namespace {
@@ -42,10 +45,23 @@ T* ptr(const Tensor& t) {
   return static_cast<T*>(t.data_ptr());
 }
 
-using Err = std::optional<Tensor>;  // (None only where nothing is launched: fake tensors, tracing)
-int* word(const Err& err) {
-  TORCH_CHECK(err.has_value(), "a launch needs its error word");
-  return static_cast<int*>(err->data_ptr());
+// The error word of a launch: the given one, or (none given: the usual case, and graphs that were traced) the
+// device's persistent one, which Python keeps and check_errors() reads.
+using Err = std::optional<Tensor>;
+using WordOf = int64_t (*)(int);  // address of a device's persistent error word
+WordOf word_of = nullptr;
+int* word(const Err& err, const Tensor& on) {
+  if (err.has_value()) return static_cast<int*>(err->data_ptr());
+  static std::array<std::atomic<int*>, 64> known{};
+  const int i = int(on.get_device());
+  TORCH_CHECK(i >= 0 && i < int(known.size()) && word_of, "no error word for device ", i);
+  int* w = known[i].load(std::memory_order_acquire);
+  if (!w) {
+    w = reinterpret_cast<int*>(word_of(i));
+    TORCH_CHECK(w, "no error word for device ", i);
+    known[i].store(w, std::memory_order_release);
+  }
+  return w;
 }
 
 Tensor floats(int64_t n, const Tensor& like) { return at::empty({n}, like.options().dtype(at::kFloat)); }
@@ -72,7 +88,7 @@ std::tuple<Tensor, Tensor> gqa_prefill(const Tensor& q, const Tensor& k, const T
   if (n) ws = floats(n, q);
   ok(mzb_gqa_prefill(q.data_ptr(), k.data_ptr(), v.data_ptr(), ptr(cu_q), ptr(cu_k), o.data_ptr(), ptr<float>(lse),
                      n ? ptr<float>(ws) : nullptr, Tq, Tk, int(B), int(Hq), int(Hkv), int(D), code_of(q), q.stride(0),
-                     q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), causal, float(scale), word(err),
+                     q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), causal, float(scale), word(err, q),
                      c.stream),
      "mzb_gqa_prefill");
   return {o, lse};
@@ -90,7 +106,7 @@ std::tuple<Tensor, Tensor> gqa_decode(const Tensor& q, const Tensor& k_pages, co
   ok(mzb_gqa_decode(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), ptr(page_table), ptr(seq_lens), o.data_ptr(),
                     ptr<float>(lse), n ? ptr<float>(ws) : nullptr, int(B), int(Hq), int(Hkv), int(D), code_of(q),
                     int(page), P, int(W), q.stride(0), q.stride(1), k_pages.stride(0), k_pages.stride(1),
-                    k_pages.stride(2), v_pages.stride(0), v_pages.stride(1), v_pages.stride(2), float(scale), word(err),
+                    k_pages.stride(2), v_pages.stride(0), v_pages.stride(1), v_pages.stride(2), float(scale), word(err, q),
                     c.stream),
      "mzb_gqa_decode");
   return {o, lse};
@@ -106,7 +122,7 @@ void kv_append(const Tensor& k, const Tensor& v, Tensor k_pages, Tensor v_pages,
                                k_pages.stride(1), k_pages.stride(2), v_pages.stride(0), v_pages.stride(1), v_pages.stride(2)};
   ok(mzb_kv_append(k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), ptr(page_table), ptr(starts),
                    cu ? ptr(*cu) : nullptr, k.size(0), int(starts.numel()), int(k.size(1)), int(k.size(2)) * size,
-                   int(k_pages.size(2)), k_pages.size(0), int(page_table.size(1)), size, strides, word(err), c.stream),
+                   int(k_pages.size(2)), k_pages.size(0), int(page_table.size(1)), size, strides, word(err, k), c.stream),
      "mzb_kv_append");
 }
 
@@ -114,7 +130,7 @@ Tensor kv_reserve(Tensor page_table, Tensor seq_lens, Tensor refs, const Tensor&
   Call c(page_table);
   Tensor starts = at::empty_like(seq_lens), ws = ints(refs.numel(), refs);
   ok(mzb_kv_reserve(ptr(page_table), ptr(seq_lens), ptr(refs), ptr(n_new), ptr(starts), ptr(ws), int(page_table.size(0)),
-                    int(page_table.size(1)), refs.numel(), int(page), word(err), c.stream),
+                    int(page_table.size(1)), refs.numel(), int(page), word(err, page_table), c.stream),
      "mzb_kv_reserve");
   return starts;
 }
@@ -122,7 +138,7 @@ Tensor kv_reserve(Tensor page_table, Tensor seq_lens, Tensor refs, const Tensor&
 void kv_free(Tensor page_table, Tensor seq_lens, Tensor refs, const Tensor& seqs, const Err& err) {
   Call c(page_table);
   ok(mzb_kv_free(ptr(page_table), ptr(seq_lens), ptr(refs), ptr(seqs), seqs.numel(), page_table.size(0),
-                 int(page_table.size(1)), refs.numel(), word(err), c.stream),
+                 int(page_table.size(1)), refs.numel(), word(err, page_table), c.stream),
      "mzb_kv_free");
 }
 
@@ -130,7 +146,7 @@ void kv_copy_pages(at::TensorList pools, const Tensor& src, const Tensor& dst, c
   TORCH_CHECK(!pools.empty(), "kv_copy_pages: no pool");
   Call c(src);
   const std::vector<int64_t> x = pool_array(pools);
-  ok(mzb_kv_copy_pages(x.data(), int(pools.size()), ptr(src), ptr(dst), src.numel(), pools[0].size(0), word(err), c.stream),
+  ok(mzb_kv_copy_pages(x.data(), int(pools.size()), ptr(src), ptr(dst), src.numel(), pools[0].size(0), word(err, src), c.stream),
      "mzb_kv_copy_pages");
 }
 
@@ -141,7 +157,7 @@ void kv_fork(at::TensorList pools, Tensor page_table, Tensor seq_lens, Tensor re
   Tensor ws = ints(3 * n + S, refs);
   const std::vector<int64_t> x = pool_array(pools);
   ok(mzb_kv_fork(ptr(page_table), ptr(seq_lens), ptr(refs), ptr(src), ptr(dst), int(n), ptr(ws), S,
-                 int(page_table.size(1)), refs.numel(), int(page), x.data(), int(pools.size()), word(err), c.stream),
+                 int(page_table.size(1)), refs.numel(), int(page), x.data(), int(pools.size()), word(err, page_table), c.stream),
      "mzb_kv_fork");
 }
 
@@ -151,17 +167,18 @@ std::tuple<Tensor, Tensor> kv_compact(at::TensorList pools, const Tensor& page_t
   Tensor ws = ints(3 * P + 1, refs), table = at::empty_like(page_table), new_refs = at::empty_like(refs);
   const std::vector<int64_t> x = pool_array(pools);
   ok(mzb_kv_compact(ptr(page_table), ptr(refs), ptr(table), ptr(new_refs), ptr(ws), page_table.numel(), P, x.data(),
-                    int(pools.size()), word(err), c.stream),
+                    int(pools.size()), word(err, page_table), c.stream),
      "mzb_kv_compact");
   return {table, new_refs};
 }
 
 }  // namespace
 
-// Called once by the Python side (not a static initialiser, whose exception at a stale build's
+// Called once by the Python side with its keeper of error words (not a static initialiser, whose exception at a stale build's
 // other schema would end the process): 0, or -1 with the reason in msg.
-extern "C" __attribute__((visibility("default"))) int mzb_torch_register(char* msg, size_t size) {
+extern "C" __attribute__((visibility("default"))) int mzb_torch_register(int64_t (*word)(int), char* msg, size_t size) {
   try {
+    word_of = word;
     static torch::Library m(torch::Library::IMPL, "mzb", c10::DispatchKey::CUDA, __FILE__, __LINE__);
     m.impl("gqa_prefill", &gqa_prefill);
     m.impl("gqa_decode", &gqa_decode);

@@ -9,6 +9,8 @@ implementation so it traces under ``torch.compile`` / ``FakeTensor`` without run
 import os
 
 import torch
+from torch._subclasses.fake_tensor import FakeTensor
+from torch._subclasses.functional_tensor import FunctionalTensor
 
 from . import _lib
 from ._lib import call, ptr, require_cuda, stream_ptr
@@ -485,16 +487,22 @@ _kv_compact = _declare("kv_compact(Tensor(a!)[] pools, Tensor page_table, Tensor
                        lambda pools, page_table, refs, err: (torch.empty_like(page_table), torch.empty_like(refs)))
 
 
-def _word(t, check: bool):
-    """The error word of a launch on t's device; none where t is not real (fake, traced)."""
-    if type(t) is not torch.Tensor:
-        return None
-    if not _lib.torch_ops_loaded:
-        _lib.load_torch_ops()
+def _launch(what: str, first: torch.Tensor, check: bool, op):
+    """``op(err)`` on first's device.  Without ``check`` (and where first is traced: nothing runs there) err is None,
+    and the launch, or the traced graph's launches, use the device's word that ``check_errors`` reads."""
+    if check or not _lib.torch_ops_loaded:
+        traced = isinstance(first, (FakeTensor, FunctionalTensor))
+        if not (traced or _lib.torch_ops_loaded):
+            _lib.load_torch_ops()
+        check = check and not traced
+    err = _err(first.device, True) if check else None
+    try:
+        out = op(err)
+    except RuntimeError as e:
+        _failed(e)
     if check:
-        return _err(t.device, True)
-    w = _ERR_WORDS.get(t.get_device())
-    return _err(t.device, False) if w is None else w
+        _raise_on(err, what)
+    return out
 
 
 def _failed(e: RuntimeError):
@@ -510,94 +518,42 @@ def _failed(e: RuntimeError):
 
 def gqa_prefill(q, k, v, cu_q, cu_k, causal, scale, check):
     """(o like q, lse fp32 [Tq, Hq]) of ``mzb_gqa_prefill`` (q / k / v with a dense last dimension)."""
-    err = _word(q, check)
-    try:
-        out = _gqa_prefill(q, k, v, cu_q, cu_k, err, causal, scale)
-    except RuntimeError as e:
-        _failed(e)
-    if check:
-        _raise_on(err, "gqa prefill")
-    return out
+    return _launch("gqa prefill", q, check, lambda err: _gqa_prefill(q, k, v, cu_q, cu_k, err, causal, scale))
 
 
 def gqa_decode(q, k_pages, v_pages, page_table, seq_lens, scale, check):
     """(o like q, lse fp32 [B, Hq]) of ``mzb_gqa_decode``."""
-    err = _word(q, check)
-    try:
-        out = _gqa_decode(q, k_pages, v_pages, page_table, seq_lens, err, scale)
-    except RuntimeError as e:
-        _failed(e)
-    if check:
-        _raise_on(err, "gqa decode")
-    return out
+    return _launch("gqa decode", q, check, lambda err: _gqa_decode(q, k_pages, v_pages, page_table, seq_lens, err, scale))
 
 
 def kv_append(k, v, k_pages, v_pages, page_table, starts, cu, check):
     """``mzb_kv_append``: rows of k / v [T, Hkv, D] into k_pages / v_pages [P, Hkv, page, D]."""
-    err = _word(k, check)
-    try:
-        _kv_append(k, v, k_pages, v_pages, page_table, starts, cu, err)
-    except RuntimeError as e:
-        _failed(e)
-    if check:
-        _raise_on(err, "kv append")
+    _launch("kv append", k, check, lambda err: _kv_append(k, v, k_pages, v_pages, page_table, starts, cu, err))
 
 
 def kv_reserve(page_table, seq_lens, refs, n_new, page, check):
     """``mzb_kv_reserve``; returns the lengths before it."""
-    err = _word(page_table, check)
-    try:
-        starts = _kv_reserve(page_table, seq_lens, refs, n_new, err, page)
-    except RuntimeError as e:
-        _failed(e)
-    if check:
-        _raise_on(err, "kv reserve")
-    return starts
+    return _launch("kv reserve", page_table, check, lambda err: _kv_reserve(page_table, seq_lens, refs, n_new, err, page))
 
 
 def kv_free(page_table, seq_lens, refs, seqs, check):
     """``mzb_kv_free``."""
-    err = _word(page_table, check)
-    try:
-        _kv_free(page_table, seq_lens, refs, seqs, err)
-    except RuntimeError as e:
-        _failed(e)
-    if check:
-        _raise_on(err, "kv free")
+    _launch("kv free", page_table, check, lambda err: _kv_free(page_table, seq_lens, refs, seqs, err))
 
 
 def kv_copy_pages(pools, src, dst, check):
     """``mzb_kv_copy_pages``: page src[i] to page dst[i] of every pool."""
-    err = _word(src, check)
-    try:
-        _kv_copy_pages(pools, src, dst, err)
-    except RuntimeError as e:
-        _failed(e)
-    if check:
-        _raise_on(err, "kv copy pages")
+    _launch("kv copy pages", src, check, lambda err: _kv_copy_pages(pools, src, dst, err))
 
 
 def kv_fork(pools, page_table, seq_lens, refs, src, dst, page, check):
     """``mzb_kv_fork``."""
-    err = _word(page_table, check)
-    try:
-        _kv_fork(pools, page_table, seq_lens, refs, src, dst, err, page)
-    except RuntimeError as e:
-        _failed(e)
-    if check:
-        _raise_on(err, "kv fork")
+    _launch("kv fork", page_table, check, lambda err: _kv_fork(pools, page_table, seq_lens, refs, src, dst, err, page))
 
 
 def kv_compact(pools, page_table, refs, check):
     """``mzb_kv_compact``; returns the new (page_table, refs)."""
-    err = _word(page_table, check)
-    try:
-        out = _kv_compact(pools, page_table, refs, err)
-    except RuntimeError as e:
-        _failed(e)
-    if check:
-        _raise_on(err, "kv compact")
-    return out
+    return _launch("kv compact", page_table, check, lambda err: _kv_compact(pools, page_table, refs, err))
 
 
 if os.path.exists(_lib.TORCH_LIB_PATH):

@@ -194,3 +194,104 @@ def test_scores_of_minus_infinity(cuda, dt, d, hq, n):
     k[:, :, 0] = -math.inf
     for a, b in both(k):
         assert not a.any() and bool((b == -math.inf).all())
+
+
+# ------------------------------------------------------------------ error words, tracing, types of tensors
+
+def _traced(fn, *args, **more):
+    """fn as a graph made on fake tensors."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    mode = FakeTensorMode()
+    with mode:
+        fakes = [torch.empty(a, dtype=d, device="cuda:0") for a, d in args]
+        graph = make_fx(fn, **more)(*fakes)
+    return graph
+
+
+_BF, _I32 = torch.bfloat16, torch.int32
+
+
+def _step(q, k, v, kp, vp, table, lens, refs, ones):
+    """A step through five of the operators."""
+    from mzoo_b200 import kv_pages
+    starts = kv_pages.reserve(table, lens, refs, ones, page_size=16)
+    kv_pages.append(k, v, kp, vp, table, starts)
+    o, lse = gqa_attn.decode(q, kp, vp, table, lens)
+    table, refs = kv_pages.compact([kp, vp], table, refs)
+    return o, lse, table, refs, gqa_attn.decode(q, kp, vp, table, lens)[0]
+
+
+_STEP = [((3, 4, 64), _BF), ((3, 2, 64), _BF), ((3, 2, 64), _BF), ((20, 2, 16, 64), _BF), ((20, 2, 16, 64), _BF), ((3, 5), _I32),
+         ((3,), _I32), ((20,), _I32), ((3,), _I32)]
+
+
+def test_traced_graphs_hold_no_tensor_of_the_trace():
+    """Neither a fake error word nor any other constant; also where the checks are asked for."""
+    for fn in (_step, lambda q, k, v, *rest: gqa_attn.prefill(q, k, v, torch.ops.aten.cumsum(rest[-1], 0, dtype=_I32), check=True)):
+        args = _STEP if fn is _step else [((3, 4, 64), _BF), ((3, 2, 64), _BF), ((3, 2, 64), _BF), ((2,), _I32)]
+        graph = _traced(fn, *args)
+        assert any("gqa" in str(n.target) for n in graph.graph.nodes)
+        assert not [n for n in graph.graph.nodes if n.op == "get_attr"]
+
+
+def _state(dev):
+    g = torch.Generator().manual_seed(0)
+    x = [_randn(g, dt, *shape).to(dev) if dt == _BF else torch.zeros(*shape, dtype=dt, device=dev) for shape, dt in _STEP]
+    x[5].fill_(-1)
+    x[8].copy_(torch.tensor([1, 30, 16]))
+    return x
+
+
+@pytest.mark.gpu
+def test_traced_graph_runs_and_reports(cuda):
+    """A graph traced on fake tensors is the eager call, and its errors reach check_errors()."""
+    graph = _traced(_step, *_STEP)
+    a, b = _state(cuda), _state(cuda)
+    for x, y in zip(_step(*a), graph(*b)):
+        assert torch.equal(x, y)
+    for x, y in zip(a, b):
+        assert torch.equal(x, y)
+    mzoo_b200.check_errors()
+    b = _state(cuda)
+    b[8].fill_(1000)  # past the table
+    graph(*b)
+    with pytest.raises(_lib.MzbError, match="past its page table"):
+        mzoo_b200.check_errors()
+
+
+@pytest.mark.gpu
+def test_exported_program_runs(cuda):
+    class Attend(torch.nn.Module):
+        def forward(self, q, k, v, cu):
+            return gqa_attn.prefill(q, k, v, cu)
+
+    g = torch.Generator().manual_seed(0)
+    q, k, v = (_randn(g, _BF, 30, h, 64).to(cuda) for h in (4, 2, 2))
+    args = (q, k, v, _cu([13, 17]).to(cuda))
+    with torch.no_grad():
+        program = torch.export.export(Attend(), args, strict=False)
+        for x, y in zip(program.module()(*args), gqa_attn.prefill(*args)):
+            assert torch.equal(x, y)
+
+
+@pytest.mark.gpu
+def test_parameters_and_subclasses_are_tensors(cuda):
+    class Named(torch.Tensor):
+        pass
+
+    from mzoo_b200 import kv_pages
+    want = _step(*_state(cuda))
+    for kind in (lambda t: torch.nn.Parameter(t, requires_grad=False), lambda t: t.as_subclass(Named)):
+        x = [kind(t) for t in _state(cuda)]
+        got = _step(*x)
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+        q, k, v = x[:3]
+        gqa_attn.prefill(q, k, v, kind(_cu([1, 2]).to(cuda)), check=True)
+        ids = kind(torch.tensor([0], dtype=_I32, device=cuda))
+        kv_pages.copy_pages([x[3]], ids, ids + 1, check=True)
+        kv_pages.fork([x[3]], x[5], x[6], x[7], ids, ids + 1, page_size=16, check=True)
+        kv_pages.free(x[5], x[6], x[7], ids, check=True)
+    with pytest.raises(_lib.MzbError, match="out of range"):
+        kv_pages.free(x[5], x[6], x[7], ids + 99, check=True)
+    mzoo_b200.check_errors()  # a checked call's error is its own
