@@ -117,11 +117,15 @@ def load_torch_ops() -> None:
         if not os.path.exists(TORCH_LIB_PATH):
             raise ImportError(f"{TORCH_LIB_PATH} is missing: build it with `python -m mzoo_b200.build` "
                               "(mzoo_b200 has no CPU or eager fallback)")
-        lib()  # libmzb200.so, which it is linked to
-        msg = ctypes.create_string_buffer(2000)
-        if ctypes.CDLL(TORCH_LIB_PATH).mzb_torch_register(_word_address, msg, ctypes.c_size_t(len(msg))):
-            raise ImportError(f"{TORCH_LIB_PATH} does not fit this package (build it with `python -m mzoo_b200.build "
-                              f"--force`): {msg.value.decode(errors='replace').splitlines()[0]}")
+        msg, stale = ctypes.create_string_buffer(2000), f"{TORCH_LIB_PATH} does not fit this package (build it with " \
+            "`python -m mzoo_b200.build --force`)"
+        try:
+            lib()  # libmzb200.so, which it is linked to
+            init = ctypes.CDLL(TORCH_LIB_PATH).mzb_torch_init
+        except (OSError, AttributeError) as e:  # built against another torch or other sources
+            raise ImportError(f"{stale}: {e}") from e
+        if init(_word_address, msg, ctypes.c_size_t(len(msg))):
+            raise ImportError(f"{stale}: {msg.value.decode(errors='replace').splitlines()[0]}")
         torch_ops_loaded = True
 
 

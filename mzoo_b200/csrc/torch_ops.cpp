@@ -176,7 +176,7 @@ std::tuple<Tensor, Tensor> kv_compact(at::TensorList pools, const Tensor& page_t
 
 // Called once by the Python side with its keeper of error words (not a static initialiser, whose exception at a stale build's
 // other schema would end the process): 0, or -1 with the reason in msg.
-extern "C" __attribute__((visibility("default"))) int mzb_torch_register(int64_t (*word)(int), char* msg, size_t size) {
+extern "C" __attribute__((visibility("default"))) int mzb_torch_init(int64_t (*word)(int), char* msg, size_t size) {
   try {
     word_of = word;
     static torch::Library m(torch::Library::IMPL, "mzb", c10::DispatchKey::CUDA, __FILE__, __LINE__);

@@ -557,4 +557,7 @@ def kv_compact(pools, page_table, refs, check):
 
 
 if os.path.exists(_lib.TORCH_LIB_PATH):
-    _lib.load_torch_ops()
+    try:
+        _lib.load_torch_ops()
+    except ImportError:
+        pass  # the other modules work without it; a serving op's first call raises this again
