@@ -295,3 +295,51 @@ def test_parameters_and_subclasses_are_tensors(cuda):
     with pytest.raises(_lib.MzbError, match="out of range"):
         kv_pages.free(x[5], x[6], x[7], ids + 99, check=True)
     mzoo_b200.check_errors()  # a checked call's error is its own
+
+
+@pytest.mark.gpu
+def test_ops_refuse_what_a_kernel_would_misread(cuda):
+    """The ops themselves, without the wrappers' checks: tensors of another device or type, other shapes and
+    strides are refused before a launch."""
+    from mzoo_b200 import ops
+    z = lambda *shape, dt=_BF, dev=cuda: torch.zeros(*shape, dtype=dt, device=dev)  # noqa: E731
+    i = lambda *shape, dt=_I32, dev=cuda: torch.zeros(*shape, dtype=dt, device=dev)  # noqa: E731
+    q, k, cu, pool, table, lens, refs = z(4, 4, 64), z(4, 2, 64), i(2), z(9, 2, 16, 64), i(4, 3) - 1, i(4), i(9)
+    half = lambda t: t.to(torch.float16)  # noqa: E731
+    good = {"gqa_prefill": (q, k, k, cu, cu, True, 1.0), "gqa_decode": (q, pool, pool, table, lens, 1.0),
+            "kv_append": (k, k, pool, pool, i(4, 3), lens, None), "kv_reserve": (table, lens, refs, lens, 16), "kv_free": (table, lens, refs, cu),
+            "kv_copy_pages": ([pool], cu - 1, cu - 1), "kv_fork": ([pool], table, lens, refs, cu[:0], cu[:0], 16),
+            "kv_compact": ([pool], table, refs)}
+
+    def others(name, t, at):  # what may stand in the place of t, and must not
+        if isinstance(t, list):
+            yield from ([x] for x in (t[0].cpu(), t[0].transpose(1, 2)))
+            if name != "kv_copy_pages":  # (there any number of pages will do)
+                yield from ([x] for x in (t[0][:5], t[0][0]))
+        elif t.dtype == _I32:
+            yield from (x for x in (t.cpu(), t.long(), t[None], t[..., None].expand(*t.shape, 2)[..., 0].transpose(0, -1)) if x is not t)
+            if t.numel() > 1 and t.dim() == 1:
+                yield t.repeat_interleave(2)[::2]
+        else:
+            yield from (t.cpu(), t[..., :32], t[0], t.transpose(-1, -2))
+            if at:
+                yield half(t)
+    for name, args in good.items():
+        getattr(ops, name)(*args, True)
+        tried = 0
+        for at, t in enumerate(args):
+            if not isinstance(t, (torch.Tensor, list)):
+                continue
+            for x in others(name, t, at):
+                if isinstance(x, torch.Tensor) and x.shape == t.shape and x.dtype == t.dtype and x.device == t.device and \
+                        (x.is_contiguous() or (t.dtype != _I32 and x.stride(-1) == 1)):
+                    continue  # as good as t
+                tried += 1
+                with pytest.raises((AssertionError, NotImplementedError)):  # (no CUDA tensor first: no such kernel)
+                    getattr(ops, name)(*args[:at], x, *args[at + 1:], True)
+        assert tried >= 4
+    with pytest.raises(AssertionError, match="int32"):
+        ops.gqa_prefill(q, k, k, cu, i(3), True, 1.0, True)
+    with pytest.raises(AssertionError, match="apart"):
+        ops.kv_copy_pages([pool[:1].expand(9, -1, -1, -1)], cu, cu, True)
+    torch.cuda.synchronize()
