@@ -11,7 +11,8 @@ position past the table, an id out of range, no free page) is left out and raise
 ``mzoo_b200.check_errors()``, or at once with ``check=True``.
 
 ``pools`` is a list of tensors ``[P, ...]`` whose pages ``pool[p]`` are dense (the K and V pools of
-every layer, say); each is changed in place.  Kernels: ``csrc/kv_pages.cu``.
+every layer, say); each is changed in place.  Tensors that need gradients are refused outside
+``torch.no_grad()``.  Kernels: ``csrc/kv_pages.cu``.
 """
 
 import torch
@@ -32,14 +33,20 @@ def _state(**tensors):
         assert t.dim() == (2 if name == "page_table" else 1), f"{name} has {t.dim()} dimensions: {tuple(t.shape)}"
 
 
+def _no_grad(what, *tensors):
+    assert not (torch.is_grad_enabled() and any([t.requires_grad for t in tensors])), \
+        f"{what} has no backward: call it under torch.no_grad()"
+
+
 def _table(page_table, seq_lens, refs):
     assert seq_lens.shape[0] == page_table.shape[0], \
         f"page_table {tuple(page_table.shape)} and seq_lens {tuple(seq_lens.shape)} name different sequences"
     assert page_table.shape[1] >= 1 and refs.shape[0] >= 1, "the page table and the pool must not be empty"
 
 
-def _pools(pools, pages, dev):
+def _pools(what, pools, pages, dev):
     pools = list(pools)
+    _no_grad(what, *pools)
     i = dev.index
     for p in pools:
         shape, step = p.shape, p.stride(0)
@@ -82,6 +89,7 @@ def append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     for t in (k, v, k_pages, v_pages):
         assert t.dtype == dt and t.get_device() == i, \
             f"k, v and the pools must be {dt} on cuda:{i}, got {t.dtype} on {t.device}"
+    _no_grad("append", k, v, k_pages, v_pages)
     assert len(ks) == 3 and ks == v.shape, f"k and v must be [tokens, heads, D], got {tuple(ks)}, {tuple(v.shape)}"
     assert len(ps) == 4 and ps == v_pages.shape and ps[1] == ks[1] and ps[3] == ks[2] and ps[0] and ps[2], \
         f"the pools must be [pages, {ks[1]}, page, {ks[2]}], got {tuple(ps)}, {tuple(v_pages.shape)}"
@@ -127,7 +135,7 @@ def fork(pools, page_table: torch.Tensor, seq_lens: torch.Tensor, refs: torch.Te
     _table(page_table, seq_lens, refs)
     assert src.shape == dst.shape, f"src and dst must have one length, got {src.shape[0]} and {dst.shape[0]}"
     assert page_size >= 1, f"page_size must be positive, got {page_size}"
-    ops.kv_fork(_pools(pools, refs.shape[0], refs.device), page_table, seq_lens, refs, src, dst, int(page_size), check)
+    ops.kv_fork(_pools("fork", pools, refs.shape[0], refs.device), page_table, seq_lens, refs, src, dst, int(page_size), check)
 
 
 def compact(pools, page_table: torch.Tensor, refs: torch.Tensor, *, check: bool = False):
@@ -136,7 +144,7 @@ def compact(pools, page_table: torch.Tensor, refs: torch.Tensor, *, check: bool 
     the tables passed in are out of date afterwards."""
     _state(page_table=page_table, refs=refs)
     assert refs.shape[0] >= 1, "the pool must not be empty"
-    return ops.kv_compact(_pools(pools, refs.shape[0], refs.device), page_table, refs, check)
+    return ops.kv_compact(_pools("compact", pools, refs.shape[0], refs.device), page_table, refs, check)
 
 
 def copy_pages(pools, src: torch.Tensor, dst: torch.Tensor, *, check: bool = False) -> None:
@@ -147,4 +155,4 @@ def copy_pages(pools, src: torch.Tensor, dst: torch.Tensor, *, check: bool = Fal
     assert pools, "copy_pages needs at least one pool"
     assert src.shape == dst.shape, f"src and dst must have one length, got {src.shape[0]} and {dst.shape[0]}"
     assert pools[0].dim() and pools[0].shape[0], "the pools must not be empty"
-    ops.kv_copy_pages(_pools(pools, pools[0].shape[0], src.device), src, dst, check)
+    ops.kv_copy_pages(_pools("copy_pages", pools, pools[0].shape[0], src.device), src, dst, check)

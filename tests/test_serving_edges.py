@@ -343,3 +343,26 @@ def test_ops_refuse_what_a_kernel_would_misread(cuda):
     with pytest.raises(AssertionError, match="apart"):
         ops.kv_copy_pages([pool[:1].expand(9, -1, -1, -1)], cu, cu, True)
     torch.cuda.synchronize()
+
+
+def test_cache_writes_refuse_tensors_that_need_gradients():
+    """As the attention does: a gradient would be lost without a word."""
+    from mzoo_b200 import kv_pages
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        t = lambda *shape, dt=_BF: torch.empty(*shape, dtype=dt, device="cuda:0")  # noqa: E731
+        table, lens, refs, ids = t(3, 4, dt=_I32), t(3, dt=_I32), t(9, dt=_I32), t(2, dt=_I32)
+        for at in range(4):
+            args = [t(3, 2, 64), t(3, 2, 64), t(9, 2, 16, 64), t(9, 2, 16, 64)]
+            args[at].requires_grad_()
+            with pytest.raises(AssertionError, match="append has no backward"):
+                kv_pages.append(*args, table, lens)
+            with torch.no_grad():
+                kv_pages.append(*args, table, lens)
+        pools = [t(9, 2, 16, 64), t(9, 2, 16, 64).requires_grad_()]
+        for name, rest in (("fork", (table, lens, refs, ids, ids)), ("compact", (table, refs)), ("copy_pages", (ids, ids))):
+            more = {"page_size": 16} if name == "fork" else {}
+            with pytest.raises(AssertionError, match=f"{name} has no backward"):
+                getattr(kv_pages, name)(pools, *rest, **more)
+            with torch.no_grad():
+                getattr(kv_pages, name)(pools, *rest, **more)
