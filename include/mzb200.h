@@ -304,7 +304,8 @@ MZB_API int mzb_gqa_decode(const void* q, const void* k_pages, const void* v_pag
  *   position starts[b] + i.  strides: 10 element strides: k token, head; v token, head; k_pages page,
  *   head, token; v_pages page, head, token.  Rows of row_bytes (a multiple of 16) bytes.
  * mzb_kv_reserve -- sequence b grows by n_new[b] tokens (all or none): pages are taken in
- *   (sequence, position) order, seq_lens is raised, starts[b] is the old length.  ws: P ints.
+ *   (sequence, position) order, seq_lens is raised, starts[b] is the old length.  Behind the first
+ *   sequence that the free pages do not suffice for, none that needs a page gets one.  ws: P ints.
  * mzb_kv_free    -- the sequences seqs[0..n): refs - 1 for their pages, entries -1, length 0.
  * mzb_kv_fork    -- dst[i] becomes a copy of src[i]: what dst held is released, full pages are
  *   shared (refs + 1), a partly filled last page is copied to a page of its own in every pool.

@@ -176,7 +176,8 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
 
 // ---------------------------------------------------------------- reserve
 
-// One block: needs per sequence, their prefix sum, the lowest free pages, the table entries.
+// One block: needs per sequence, their prefix sum, the lowest free pages, the table entries.  A sequence whose sum
+// passes the number of free pages gets none, and so does every one behind it: no one is passed over.
 __global__ void __launch_bounds__(NT) reserve_kernel(int32_t* table, int32_t* lens, int32_t* refs,
                                                      const int32_t* n_new, int32_t* starts, int32_t* list, int B,
                                                      int W, int64_t P, int page, int* err) {

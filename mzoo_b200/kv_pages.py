@@ -108,7 +108,9 @@ def reserve(page_table: torch.Tensor, seq_lens: torch.Tensor, refs: torch.Tensor
             check: bool = False) -> torch.Tensor:
     """Room for ``n_new[b]`` more tokens of each sequence: takes the pages, raises seq_lens and returns
     the lengths before (``append``'s ``starts``).  A sequence that cannot have all of them (the
-    table is too narrow, no free page) gets none and keeps its length."""
+    table is too narrow, no free page) gets none and keeps its length.  Pages are given out in the order of
+    the sequences, and none is passed over: behind the first one that the free pages do not
+    suffice for, no sequence that needs a page gets one in this call."""
     _state(page_table=page_table, seq_lens=seq_lens, refs=refs, n_new=n_new)
     _table(page_table, seq_lens, refs)
     assert n_new.shape == seq_lens.shape, f"n_new must be {tuple(seq_lens.shape)}, got {tuple(n_new.shape)}"
