@@ -38,7 +38,9 @@ extern "C" {
 #define MZB_ERR_TIMEOUT (-4)     /* a bounded device-side wait gave up */
 #define MZB_ERR_ALIGN (-5)       /* pointer not 16-byte aligned where required */
 #define MZB_ERR_BOUND (-6)       /* a device-side error-bound check failed */
-#define MZB_ERR_PAGES (-7)       /* a position past its page table, a page id outside the pool, no free page */
+#define MZB_ERR_PAGES (-7)       /* a page or sequence id out of range */
+#define MZB_ERR_TABLE (-8)       /* a position past its page table */
+#define MZB_ERR_NO_PAGE (-9)     /* no free page */
 
 /* element type codes */
 #define MZB_F32 0
@@ -299,7 +301,8 @@ MZB_API int mzb_gqa_decode(const void* q, const void* k_pages, const void* v_pag
 /* ------------------------------------------------------------------ pages of a K / V cache
  * No counterpart in the reference.  State: page_table int32 [S, W] (-1 = no page), seq_lens
  * int32 [S], refs int32 [P] (tables that name the page; 0 = free).  What cannot be done is left
- * out and sets *err = MZB_ERR_PAGES; new pages are the lowest free ids.
+ * out and sets *err (if it is 0) to MZB_ERR_TABLE (a position past its page table), MZB_ERR_PAGES (an id out of
+ * range, a pair that fork cannot take) or MZB_ERR_NO_PAGE; new pages are the lowest free ids.
  * mzb_kv_append  -- row i of sequence b (rows cu[b] .. cu[b+1]; cu NULL: row b) of k, v goes to
  *   position starts[b] + i.  strides: 10 element strides: k token, head; v token, head; k_pages page,
  *   head, token; v_pages page, head, token.  Rows of row_bytes (a multiple of 16) bytes.

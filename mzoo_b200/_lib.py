@@ -23,6 +23,8 @@ MZB_ERR_TIMEOUT = -4
 MZB_ERR_ALIGN = -5
 MZB_ERR_BOUND = -6
 MZB_ERR_PAGES = -7
+MZB_ERR_TABLE = -8
+MZB_ERR_NO_PAGE = -9
 
 DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
@@ -81,7 +83,12 @@ _lib = None
 
 
 class MzbError(RuntimeError):
-    """A kernel-side failure reported through the C ABI (launch error, timeout, bound check)."""
+    """A kernel-side failure reported through the C ABI (launch error, timeout, bound check).  ``code`` is the error
+    word's value for what a kernel recorded (``MZB_ERR_NO_PAGE``, say), 0 for other failures."""
+
+    def __init__(self, text: str, code: int = 0):
+        super().__init__(text)
+        self.code = code
 
 
 def lib() -> ctypes.CDLL:

@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       // an id outside the pool is an error, and some page is read in its place; looked at when the ids are needed, so
       // that the next ones stay in flight
       auto checked = [&](int p) {
-        if (p < 0 || p >= a.P) atomicExch(a.err, MZB_ERR_PAGES);
+        if (p < 0 || p >= a.P) atomicCAS(a.err, 0, MZB_ERR_PAGES);
         return max(0, min(p, int(a.P - 1)));
       };
       int cur = ids(box0 + lane), nxt = ids(box0 + 32 + lane), base = box0;

@@ -6,7 +6,7 @@
 // (how many tables name the page; 0 = free).  New pages are always the lowest free ids, in
 // the order of the sequences that ask, so equal inputs give equal tables.  What cannot be
 // done (a position past the table, a page id outside the pool, no free page) is left out and
-// recorded as MZB_ERR_PAGES in the error word.
+// recorded in the error word, the first cause staying: MZB_ERR_TABLE, MZB_ERR_PAGES, MZB_ERR_NO_PAGE.
 //
 // Rows and pages move at HBM's rate (B200: 19700 rows of 2 x 2 KB written in 30 us = 5.4 TB/s of reads
 // and writes, 2048 moves of 2 x 64 KB in 86 us = 6.2 TB/s); the planning kernels are chains of dependent
@@ -85,7 +85,7 @@ __device__ int lowest_free(const int32_t* refs, int64_t P, int want, int32_t* li
   return min(found, want);
 }
 
-__device__ __forceinline__ void report(int* err) { atomicExch(err, MZB_ERR_PAGES); }
+__device__ __forceinline__ void report(int* err, int code) { atomicCAS(err, 0, code); }
 
 // ---------------------------------------------------------------- append
 
@@ -144,14 +144,15 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
       int64_t d = -1, e = -1;
       if (ok) {
         const int64_t pos = (int64_t)a.starts[b] + i, j = pos / a.page;
-        if (pos >= 0 && j < a.W) {
+        const bool there = pos >= 0 && j < a.W;
+        if (there) {
           const int64_t p = a.table[(int64_t)b * a.W + j];
           if (p >= 0 && p < a.P) {
             d = p * a.kp_p + (pos % a.page) * a.kp_t;
             e = p * a.vp_p + (pos % a.page) * a.vp_t;
           }
         }
-        if (d < 0) report(a.err);
+        if (d < 0) report(a.err, there ? MZB_ERR_PAGES : MZB_ERR_TABLE);
       }
       kdst[warp] = d;
       vdst[warp] = e;
@@ -217,7 +218,7 @@ __global__ void __launch_bounds__(NT) reserve_kernel(int32_t* table, int32_t* le
             }
           lens[b] = int32_t(to);
         } else {
-          report(err);
+          report(err, ok ? MZB_ERR_NO_PAGE : MZB_ERR_TABLE);
         }
       }
       __syncthreads();
@@ -238,7 +239,7 @@ __global__ void __launch_bounds__(256) free_kernel(int32_t* table, int32_t* lens
   if (i >= n) return;
   const int64_t s = seqs[i];
   if (s < 0 || s >= S) {
-    if (threadIdx.x == 0 && blockIdx.x == 0) report(err);
+    if (threadIdx.x == 0 && blockIdx.x == 0) report(err, MZB_ERR_PAGES);
     return;
   }
   const int j = blockIdx.x * 256 + threadIdx.x;
@@ -302,7 +303,7 @@ __global__ void __cluster_dims__(FORK_CTAS, 1, 1) __launch_bounds__(NT)
         const int j = j0 + 32 * e;
         if (j >= W) continue;
         const bool share = now[e] >= 0 && now[e] < P;
-        if (j < full && !share) report(err);
+        if (j < full && !share) report(err, MZB_ERR_PAGES);
         if (was[e] != -1 || share) to[j] = share ? now[e] : -1;
         if (was[e] >= 0 && was[e] < P) atomicSub(&refs[was[e]], 1);
         if (share) atomicAdd(&refs[now[e]], 1);
@@ -319,14 +320,14 @@ __global__ void __cluster_dims__(FORK_CTAS, 1, 1) __launch_bounds__(NT)
       ps[i] = pd[i] = -1;
       const int full = full_of(i);
       if (full < 0) {
-        report(err);
+        report(err, MZB_ERR_PAGES);
       } else if (lens[src[i]] % page) {
         const int p = table[(int64_t)src[i] * W + full];
         if (p >= 0 && p < P) {
           need = 1;
           ps[i] = p;
         } else {
-          report(err);
+          report(err, MZB_ERR_PAGES);
         }
       }
     }
@@ -349,7 +350,7 @@ __global__ void __cluster_dims__(FORK_CTAS, 1, 1) __launch_bounds__(NT)
         table[d * W + full] = p;
         refs[p] = 1;
       } else {  // no page for the last tokens: the copy ends at its last full page
-        if (pd[i] >= 0) report(err);
+        if (pd[i] >= 0) report(err, MZB_ERR_NO_PAGE);
         got = full * page;
         ps[i] = -1;
       }
@@ -459,7 +460,7 @@ __global__ void __launch_bounds__(256) copy_kernel(const __grid_constant__ CopyA
     int q = -1;
     if (p >= 0) {
       q = p < a.P ? a.to[p] : -1;
-      if (q < 0) report(a.err);  // a table names a free page or none of the pool's
+      if (q < 0) report(a.err, MZB_ERR_PAGES);  // a table names a free page or none of the pool's
     }
     a.new_table[i] = q;
   }
@@ -471,7 +472,7 @@ __global__ void __launch_bounds__(256) copy_kernel(const __grid_constant__ CopyA
     const int64_t s = a.src[i], d = a.dst[i];
     if (s < 0 && d < 0) continue;
     if (s < 0 || d < 0 || s >= a.P || d >= a.P) {
-      if (threadIdx.x == 0) report(a.err);
+      if (threadIdx.x == 0) report(a.err, MZB_ERR_PAGES);
       continue;
     }
     const int64_t off = (int64_t)c * CHUNK, left = a.bytes[pool] - off;

@@ -8,7 +8,8 @@ sequence's positions ``j * page .. (j + 1) * page`` (-1 = none), ``seq_lens [S]`
 counts the tables that name a page (0 = free).  A new page is always the lowest free id, in
 the order of the sequences that ask.  Nothing here reads from the host: what cannot be done (a
 position past the table, an id out of range, no free page) is left out and raised by
-``mzoo_b200.check_errors()``, or at once with ``check=True``.
+``mzoo_b200.check_errors()``, or at once with ``check=True``, as an ``MzbError`` whose ``code`` is
+``_lib.MZB_ERR_TABLE``, ``MZB_ERR_PAGES`` or ``MZB_ERR_NO_PAGE`` (of several, the first).
 
 ``pools`` is a list of tensors ``[P, ...]`` whose pages ``pool[p]`` are dense (the K and V pools of
 every layer, say); each is changed in place.  Tensors that need gradients are refused outside

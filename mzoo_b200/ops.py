@@ -74,13 +74,17 @@ def _err(dev, check: bool) -> torch.Tensor:
     return w
 
 
+_PAGE_ERRORS = {_lib.MZB_ERR_TABLE: "a position past its page table", _lib.MZB_ERR_PAGES: "a page or sequence id out of range",
+                _lib.MZB_ERR_NO_PAGE: "no free page"}
+
+
 def _raise_code(code: int, what: str) -> None:
     if code == _lib.MZB_ERR_BOUND:
-        raise _lib.MzbError(f"{what}: error bound left too many top-k candidates")
-    if code == _lib.MZB_ERR_PAGES:
-        raise _lib.MzbError(f"{what}: a position past its page table, a page or sequence id out of range, or no free page")
+        raise _lib.MzbError(f"{what}: error bound left too many top-k candidates", code)
+    if code in _PAGE_ERRORS:
+        raise _lib.MzbError(f"{what}: {_PAGE_ERRORS[code]} (of the page errors: {'; '.join(_PAGE_ERRORS.values())})", code)
     if code:
-        raise _lib.MzbError(f"{what}: device error code {code} (a bounded device wait gave up)")
+        raise _lib.MzbError(f"{what}: device error code {code} (a bounded device wait gave up)", code)
 
 
 def _raise_on(err: torch.Tensor, what: str) -> None:
