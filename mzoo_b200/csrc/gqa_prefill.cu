@@ -326,7 +326,9 @@ __global__ void __launch_bounds__(384, 1)
           for (int e = 0; e < 16; ++e) {
             const uint64_t x = ffma_f32x2(pack_f32x2(__uint_as_float(sv[q][2 * e]), __uint_as_float(sv[q][2 * e + 1])), sl2, nm2);
             float2 p;
-            if (e % 8 == 7) {  // one pair in eight on the FMA pipe: measured best of 0, 1/8, 1/4, 3/8, 1/2
+            // one pair in eight on the FMA pipe.  With 0, 1/8, 1/4, 3/8, 1/2 of them: a prompt of 16384, 16 heads on 2, D = 128
+            // 814, 803, 818, 818, 877 us; D = 96 746, 745, 790, 746, 806; two f16 chunks, 24 on 4, D = 64 100, 97, 100, 103, 110
+            if (e % 8 == 7) {
               p = poly_exp2(x);
             } else {
               const float2 xf = unpack_f32x2(x);
