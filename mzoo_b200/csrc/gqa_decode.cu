@@ -10,18 +10,18 @@
 // it, whatever the lengths: a warp walks the page tables and feeds a ring of shared-memory
 // stages (K and V of one tile each, ~200 KB in flight per SM) by TMA, eight warps do the
 // products, S^T = K Q^T and O^T = V^T P^T: keys and channels are the 16 rows of mma.sync tiles, the query heads
-// of a group their 8 columns, so that a small group wastes little (heads as rows: 322 us in the place of 317 below,
-// and 349 in the place of 323 back to back, where the power cap bound it).  The tensor pipe is 15 % busy
+// of a group their 8 columns, so that a small group wastes little (heads as rows: 349 us in the place of the
+// batch's 323 when they were compared, back to back, where the power cap bound it).  The tensor pipe is 15 % busy
 // while the bytes come: larger tensor instructions would gain nothing up to 16 heads a group.
 // A (sequence, head) that lies in several blocks' runs leaves its (maximum, sum, output) parts in
 // a workspace; a second kernel, started early and waiting, joins them in a fixed order.
 //
-// Measured (B200, 32 heads on 8, D = 128, bf16): 64 sequences of 512 to 16384 keys (2.2 GB) in 318 us
-// (7.0 TB/s; a copy's rate is 6.54); one of 131001 keys (0.54 GB) in 82 us + 5 us of join; 256 of 300 keys, where
-// merging a sequence's results costs half as much as its bytes, 75 us (4.2 TB/s).  64 heads on one K / V head are
-// bound by products and exponentials (189 us for 0.54 GB).  Small calls are
+// Measured (B200, 32 heads on 8, D = 128, bf16): 64 sequences of 512 to 16384 keys (2.2 GB) in 329 us
+// a pass (6.8 TB/s; a copy's rate is 6.54); one of 131001 keys (0.54 GB) in 88 us with 5 of join; 256 of 300 keys, where
+// merging a sequence's results costs half as much as its bytes, 73 us (4.4 TB/s).  64 heads on one K / V head are
+// bound by products and exponentials (183 us for 0.54 GB).  Small calls are
 // bound by latency: ~4 us from the start to the first tile (lengths, page ids, the copy: three
-// dependent trips to memory), 5.3 us in all for 77 keys.
+// dependent trips to memory), 6.1 us in all for 77 keys.
 #include <type_traits>
 
 #include "gqa_softmax.cuh"
@@ -718,7 +718,7 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Decod
 int block_count() { return num_sms() < MAX_BLOCKS ? num_sms() : MAX_BLOCKS; }
 
 // Tables of at most MIN_TILES tiles: whole (sequence, head)s to a block, nothing to join: 64 sequences of one key on
-// 8 heads 17.5 -> 15.4 us with the launches, 256 of 256 keys 67 -> 64.  Longer ones in runs of equal length.
+// 8 heads 17.5 -> 15.4 us with the launches, 256 of 256 keys 66.6 -> 65.5.  Longer ones in runs of equal length.
 bool short_table(int W, int page) { return (int64_t)W * page <= MIN_TILES * TK; }
 
 template <int DT, int D, int MT, int NH>
@@ -813,7 +813,7 @@ extern "C" int mzb_gqa_decode(const void* q, const void* k_pages, const void* v_
   const int64_t sk[3] = {sk_p, sk_h, sk_t}, sv[3] = {sv_p, sv_h, sv_t};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   // up to 16 heads in tiles of 8 (9 to 16 as one of 16: 200 sequences of 500 keys, 64 heads on 4, 68.6 us against
-  // 62.5), more in tiles of 16, which read K and V half as often (64 on 1: 189 us against 222)
+  // 62.3), more in tiles of 16, which read K and V half as often (64 on 1: 189 us against 222)
 #define MZB_GO(DT, DD)                                                                              \
   (a.g <= 8 ? gqad::launch<DT, DD, 1, 1>(k_pages, v_pages, a, sk, sv, st)                           \
    : a.g <= 16 ? gqad::launch<DT, DD, 2, 1>(k_pages, v_pages, a, sk, sv, st)                        \

@@ -31,7 +31,8 @@
 //
 // Measured (B200): one prompt of 16384 tokens, 16 heads on 2, D = 128, in 0.79-0.81 ms = 1360-1390
 // TFLOP/s alone (1690 is a cuBLAS burst), 0.94 ms = 1170 TFLOP/s back to back at the 1 kW power cap
-// (1410 is cuBLAS there); nine prompts of 1 to 2047 tokens, 32 heads on 8, in 132 us = 955 TFLOP/s.  A
+// (1410 is cuBLAS there); nine prompts of 1 to 2047 tokens, 32 heads on 8, in 128-132 us = 960-990
+// TFLOP/s.  A
 // step (two 128 x 128 tiles) takes ~3100 cycles: 2048 are the tensor cores' (66 % active), 1792 the
 // exponential unit's (58 %); the rest is the chain of a tile, scores -> maximum -> exponentials ->
 // weights -> product -> next scores, which two tiles in turns do not hide in full.  What was tried
