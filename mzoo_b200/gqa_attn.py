@@ -7,7 +7,8 @@ model mixes with the window and sparse ones.
 ``j <= i + nk - nq`` (the last token sees all of them, so a prompt can be run in chunks over
 keys that grow); head h reads K / V head ``h // (Hq // Hkv)``.  Both return the output in q's
 type and the natural-log-sum-exp in fp32; a row that sees no key, or only keys whose scores are
--inf, has output 0 and lse -inf.
+-inf, has output 0 and lse -inf.  An infinite value of v that a row sees makes that channel of its
+output infinite in ``prefill``, infinite or NaN in ``decode`` (weights in two parts).
 fp32 softmax statistics and accumulation; ``prefill`` rounds each softmax weight to v's type for the
 product with v (an error of at most 2^-8 (bf16) or 2^-11 (f16) of sum_j p_j |v_j|), ``decode`` keeps the
 weights as two numbers of it; forward only.  The cache's pages are written,

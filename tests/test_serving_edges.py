@@ -366,3 +366,31 @@ def test_cache_writes_refuse_tensors_that_need_gradients():
                 getattr(kv_pages, name)(pools, *rest, **more)
             with torch.no_grad():
                 getattr(kv_pages, name)(pools, *rest, **more)
+
+
+@pytest.mark.gpu
+def test_compiled_step_is_the_eager_one(cuda):
+    """torch.compile around the wrappers (the eager backend behind AOT autograd: no kernels of its own)."""
+    a, b = _state(cuda), _state(cuda)
+    with torch.no_grad():
+        want = _step(*a)
+        got = torch.compile(_step, backend="aot_eager")(*b)
+    assert all(torch.equal(x, y) for x, y in zip(want, got)) and all(torch.equal(x, y) for x, y in zip(a, b))
+    mzoo_b200.check_errors()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seed", range(6))
+def test_prefill_wild_offsets_of_cut_key_ranges(cuda, seed):
+    """Offsets that do not ascend or leave the tensors, where key ranges are cut (test_gqa_items.py shows that
+    rows, keys and parts stay inside): no error, and a sequence that overlaps no other is right."""
+    g = torch.Generator().manual_seed(seed)
+    q, k, v = (_randn(g, torch.bfloat16, *shape).to(cuda) for shape in ((32, 16, 64), (4000, 1, 64), (4000, 1, 64)))
+    wild = [int(x) for x in torch.randint(-50, 4100, (3,), generator=g)] + [2 ** 31 - 1, -2 ** 31, 0]
+    cu_k = torch.tensor([0, 3000, *wild], dtype=torch.int32, device=cuda)
+    cu_q = torch.tensor([0, 16, 32, *wild[::-1][:-1]], dtype=torch.int32, device=cuda)
+    cu_q[3:] = cu_q[3:].masked_fill(cu_q[3:].abs() < 32, 40)  # (none comes back to the first sequence's rows)
+    o, lse = gqa_attn.prefill(q, k, v, cu_q, cu_k, check=True)
+    want = gqa_attn.prefill(q[:16], k[:3000], v[:3000], _cu([16]).to(cuda), _cu([3000]).to(cuda), check=True)
+    # the number of parts may differ: two results within 2^-8 (mag + |o|) of the value, both at most max |v|
+    assert (o[:16].float() - want[0].float()).abs().max() <= 2.0 ** -6 * v.float().abs().max()
